@@ -987,6 +987,100 @@ int32_t sgl_rocm_kv_paged_attention_async_noalloc(sgl_rocm_kv_ctx *ctx, const sg
                                                   const sgl_kv_attention_buffers *buffers,
                                                   uint64_t max_sequence_length, void *stream);
 
+/* ---- Page selection: attention over the pages of a long context that matter ----
+ * No counterpart in the reference, whose attention reads every token. For a
+ * decode step over a long sequence three calls replace
+ * sgl_rocm_kv_paged_attention_async: page_bounds keeps each page's smallest and
+ * largest key per channel as pages are written, select_pages takes the pages
+ * with the largest upper bound of q.k for each (query, KV head), and
+ * selected_attention attends these alone. All are asynchronous: nothing waits,
+ * nothing is allocated, and errors found on the device surface at
+ * sgl_rocm_kv_check_errors. They can be captured into a graph.
+ *
+ * Pages: logical page j of a request is tokens [j page_size, (j + 1)
+ * page_size) of its sequence, and its slots are one pool page's, in order (as
+ * sgl_kv_page_allocator hands them out): only the slot of its first token is
+ * read, and must be a multiple of page_size. The pools are bf16. */
+
+/* Bounds of `count` pages of one layer: `keys` describes the layer (tensor 0 is
+ * the keys; sgl_kv_pool_view_for_layer), pages[i] (u32) is a page of the pool
+ * and counts[i] (u32) its tokens so far: its first counts[i] key rows are read.
+ * bounds is bf16 [page_count][heads][2][dims]: row page is pages[i]'s smallest
+ * and then largest key per channel; rows of other pages stay as they are, and a
+ * page of no tokens is left alone. A NaN key makes both bounds of its channel
+ * NaN. A decode step lists each request's last page; a prompt all of its own.
+ * List a page once: two entries of it race. A page past the pool raises PAGE
+ * (SGL_KV_DEVICE_PAGE_INDEX_OUT_OF_RANGE), a count past page_size SPAN
+ * (SGL_KV_DEVICE_SPAN_OUT_OF_RANGE), and the entry is skipped. count 0 is a
+ * no-op. Errors: those of a pool view (DimensionTooLarge past 1,024 dims;
+ * InvalidArgument "heads" where a row does not split into bf16 heads),
+ * AllocationOutOfBounds, DeviceMismatch. */
+int32_t sgl_rocm_kv_page_bounds(sgl_rocm_kv_ctx *ctx, const sgl_kv_pool_view *keys,
+                                const sgl_kv_device_buffer *pages, const sgl_kv_device_buffer *counts,
+                                uint64_t count, const sgl_kv_device_buffer *bounds, void *stream);
+
+typedef struct sgl_kv_page_selection_config {
+    uint64_t max_pages;           /* entries of a (query, KV head)'s list */
+    uint64_t first_pages;         /* pages at the sequence's start that are always listed ... */
+    uint64_t last_pages;          /* ... and at its end (together at most max_pages) */
+    uint64_t max_sequence_length; /* longest query length; 0: sequence_slot_count */
+} sgl_kv_page_selection_config;
+
+typedef struct sgl_kv_page_selection_plan {
+    sgl_kv_attention_plan attention;
+    sgl_kv_page_selection_config config;
+    uint64_t bounds_required_bytes;    /* every page of the pool */
+    uint64_t selected_required_bytes;  /* u32 [query][KV head][max_pages] */
+    uint64_t workspace_required_bytes; /* for either call; 0: none is needed */
+} sgl_kv_page_selection_plan;
+
+/* The plan of select_pages and selected_attention for the calls that
+ * `attention` describes. Errors: attention_plan_new's; ZeroDimension
+ * ("max_pages"); InvalidArgument ("first_pages" where first_pages + last_pages
+ * pass max_pages); DimensionTooLarge: "page_size" past 2^24, "max_pages" or
+ * "sequence_pages" past 2^31, "query_key_head_dim" past 1,024,
+ * "query_heads_per_kv_head" where the query heads of one KV head pass 76 Ki
+ * elements (they lie in LDS). A sequence longer than max_sequence_length is
+ * reported (SEQUENCE) and treated as empty. */
+int32_t sgl_kv_page_selection_plan_new(const sgl_kv_attention_plan *attention,
+                                       const sgl_kv_page_selection_config *config,
+                                       sgl_kv_page_selection_plan *out);
+
+/* `attention` as for sgl_rocm_kv_paged_attention; select_pages reads no pool and
+ * writes no output (these may be null), selected_attention reads no bounds. The
+ * workspace is scratch for one call: calls that may run at the same time (on
+ * two streams, in two graphs) need one each. Its address is a multiple of 16. */
+typedef struct sgl_kv_page_selection_buffers {
+    sgl_kv_attention_buffers attention;
+    sgl_kv_device_buffer bounds;    uint64_t bounds_offset;
+    sgl_kv_device_buffer selected;  uint64_t selected_offset;
+    sgl_kv_device_buffer workspace; uint64_t workspace_offset;
+} sgl_kv_page_selection_buffers;
+
+/* The lists: for query q and KV head h the max_pages logical pages of q's
+ * sequence with the largest score
+ *   max over the query heads i of h of
+ *     sum_d max(q_id, 0) high_d + min(q_id, 0) low_d
+ * (an upper bound of q_i . k over the page, scale aside), summed in 64 bits;
+ * equal scores go to the lower page, a NaN score ranks above every number, and
+ * the first_pages and last_pages rank above all. Ascending, followed by
+ * UINT32_MAX; a sequence of at most max_pages pages has them all. A query of
+ * length 0 (padding) has none, and so has one whose metadata does not hold
+ * (reported as paged attention does). */
+int32_t sgl_rocm_kv_select_pages(sgl_rocm_kv_ctx *ctx, const sgl_kv_page_selection_plan *plan,
+                                 const sgl_kv_page_selection_buffers *buffers, void *stream);
+
+/* Softmax attention of each query head over the tokens of its KV head's listed
+ * pages that lie before the query's length; with lists of all pages the result
+ * is paged attention's. The lists may come from anywhere: they ascend, without
+ * repeats, UINT32_MAX behind the last; a list that does not, or that names a
+ * page past the sequence, is reported (SEQUENCE) and its output unspecified. A
+ * (query, KV head) of no pages gives zeros. Softmax statistics and sums are held
+ * in 32 bits, the weights enter the products as hi + lo bf16 pairs, and the
+ * output is rounded to bf16. */
+int32_t sgl_rocm_kv_selected_attention(sgl_rocm_kv_ctx *ctx, const sgl_kv_page_selection_plan *plan,
+                                       const sgl_kv_page_selection_buffers *buffers, void *stream);
+
 /* ---- Bootstrap wire format: the decode side's page table and layout ----
  * The multipart frames a decode worker sends a prefill worker's bootstrap
  * listener (Mooncake protocol, crates/sglang-srt/src/pd_bootstrap.rs):

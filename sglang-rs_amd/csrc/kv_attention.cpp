@@ -231,9 +231,7 @@ extern "C" int32_t sgl_kv_attention_plan_for_layer(const sgl_kv_paged_layout *la
     return sgl_kv_attention_plan_new(&c, out);
 }
 
-namespace {
-
-int32_t attn_ptr(const char *name, const sgl_kv_device_buffer &b, uint64_t offset, uint64_t need,
+int32_t sglkv::attention_ptr(const char *name, const sgl_kv_device_buffer &b, uint64_t offset, uint64_t need,
                  uint64_t *addr) {
     if (!b.ptr) return fail(SGL_KV_INVALID_ARGUMENT, name, 0, 0, 0, "null buffer %s", name);
     uint64_t end;
@@ -245,6 +243,48 @@ int32_t attn_ptr(const char *name, const sgl_kv_device_buffer &b, uint64_t offse
     *addr = (uint64_t)(uintptr_t)b.ptr + offset;
     return SGL_KV_OK;
 }
+
+// The kernels' sizes and strides of a plan.
+void sglkv::attention_geometry(const sgl_kv_attention_plan_config &c, sglkv_attn_params *params) {
+    sglkv_attn_params &p = *params;
+    const sgl_kv_attention_layout &lay = c.layout;
+    p.query_count = c.query_count;
+    p.request_count = c.request_count;
+    p.sequence_slot_count = c.sequence_slot_count;
+    p.slot_count = c.slot_count;
+    p.page_size = lay.page_size;
+    p.page_stride = lay.page_stride_bytes;
+    p.key_offset = lay.key_in_page_offset;
+    p.value_offset = lay.value_in_page_offset;
+    const uint64_t kh = c.query_key_head_dim * 2, vh = c.value_head_dim * 2;
+    if (lay.head_layout == SGL_KV_HND) {
+        p.key_head_stride = lay.page_size * kh;
+        p.key_token_stride = kh;
+        p.value_head_stride = lay.page_size * vh;
+        p.value_token_stride = vh;
+    } else {
+        p.key_head_stride = kh;
+        p.key_token_stride = lay.key_row_bytes;
+        p.value_head_stride = vh;
+        p.value_token_stride = lay.value_row_bytes;
+    }
+    p.query_heads = (uint32_t)c.query_head_count;
+    p.kv_heads = (uint32_t)c.kv_head_count;
+    p.group = (uint32_t)(c.query_head_count / c.kv_head_count);
+    p.head_groups = (uint32_t)(((uint64_t)p.group + SGLKV_ATTN_HEADS - 1) / SGLKV_ATTN_HEADS);
+    p.dk = (uint32_t)c.query_key_head_dim;
+    p.dk_pad = (p.dk + 31) / 32 * 32;
+    p.dv = (uint32_t)c.value_head_dim;
+    p.dv_blocks = (p.dv + SGLKV_ATTN_DV - 1) / SGLKV_ATTN_DV;
+    p.scale_log2 = c.scale * 1.4426950408889634f;
+    p.page_shift = 32;
+    if ((lay.page_size & (lay.page_size - 1)) == 0) {
+        p.page_shift = 0;
+        while ((1ull << p.page_shift) < lay.page_size) ++p.page_shift;
+    }
+}
+
+namespace {
 
 uint64_t ceil_div(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
 
@@ -323,18 +363,18 @@ int32_t attention_params(sgl_rocm_kv_ctx *ctx, const sgl_kv_attention_plan *plan
     // A plan is a plain struct the caller may have edited since plan_new.
     if ((rc = check_flags(c.flags))) return rc;
     uint64_t qp, rip, slp, rop, ssp, poolp, outp;
-    if ((rc = attn_ptr("queries", b->queries, b->queries_offset, plan->query_required_bytes, &qp)) ||
-        (rc = attn_ptr("query_request_indices", b->query_request_indices, b->query_request_indices_offset,
+    if ((rc = attention_ptr("queries", b->queries, b->queries_offset, plan->query_required_bytes, &qp)) ||
+        (rc = attention_ptr("query_request_indices", b->query_request_indices, b->query_request_indices_offset,
                        plan->query_request_indices_required_bytes, &rip)) ||
-        (rc = attn_ptr("query_sequence_lengths", b->query_sequence_lengths,
+        (rc = attention_ptr("query_sequence_lengths", b->query_sequence_lengths,
                        b->query_sequence_lengths_offset, plan->query_sequence_lengths_required_bytes,
                        &slp)) ||
-        (rc = attn_ptr("request_slot_offsets", b->request_slot_offsets, b->request_slot_offsets_offset,
+        (rc = attention_ptr("request_slot_offsets", b->request_slot_offsets, b->request_slot_offsets_offset,
                        plan->request_slot_offsets_required_bytes, &rop)) ||
-        (rc = attn_ptr("sequence_slots", b->sequence_slots, b->sequence_slots_offset,
+        (rc = attention_ptr("sequence_slots", b->sequence_slots, b->sequence_slots_offset,
                        plan->sequence_slots_required_bytes, &ssp)) ||
-        (rc = attn_ptr("pool", b->pool, b->pool_offset, plan->pool_required_bytes, &poolp)) ||
-        (rc = attn_ptr("output", b->output, b->output_offset, plan->output_required_bytes, &outp)))
+        (rc = attention_ptr("pool", b->pool, b->pool_offset, plan->pool_required_bytes, &poolp)) ||
+        (rc = attention_ptr("output", b->output, b->output_offset, plan->output_required_bytes, &outp)))
         return rc;
     if (c.query_key_head_dim > SGLKV_ATTN_MAX_DK)
         return too_large_dim("query_key_head_dim", c.query_key_head_dim, SGLKV_ATTN_MAX_DK);
@@ -357,40 +397,7 @@ int32_t attention_params(sgl_rocm_kv_ctx *ctx, const sgl_kv_attention_plan *plan
     p.pool = reinterpret_cast<const uint8_t *>(poolp);
     p.output = reinterpret_cast<uint16_t *>(outp);
     p.flag = flag_word;
-    p.query_count = c.query_count;
-    p.request_count = c.request_count;
-    p.sequence_slot_count = c.sequence_slot_count;
-    p.slot_count = c.slot_count;
-    p.page_size = lay.page_size;
-    p.page_stride = lay.page_stride_bytes;
-    p.key_offset = lay.key_in_page_offset;
-    p.value_offset = lay.value_in_page_offset;
-    const uint64_t kh = c.query_key_head_dim * 2, vh = c.value_head_dim * 2;
-    if (lay.head_layout == SGL_KV_HND) {
-        p.key_head_stride = lay.page_size * kh;
-        p.key_token_stride = kh;
-        p.value_head_stride = lay.page_size * vh;
-        p.value_token_stride = vh;
-    } else {
-        p.key_head_stride = kh;
-        p.key_token_stride = lay.key_row_bytes;
-        p.value_head_stride = vh;
-        p.value_token_stride = lay.value_row_bytes;
-    }
-    p.query_heads = (uint32_t)c.query_head_count;
-    p.kv_heads = (uint32_t)c.kv_head_count;
-    p.group = (uint32_t)(c.query_head_count / c.kv_head_count);
-    p.head_groups = (uint32_t)(((uint64_t)p.group + SGLKV_ATTN_HEADS - 1) / SGLKV_ATTN_HEADS);
-    p.dk = (uint32_t)c.query_key_head_dim;
-    p.dk_pad = (p.dk + 31) / 32 * 32;
-    p.dv = (uint32_t)c.value_head_dim;
-    p.dv_blocks = (p.dv + SGLKV_ATTN_DV - 1) / SGLKV_ATTN_DV;
-    p.scale_log2 = c.scale * 1.4426950408889634f;
-    p.page_shift = 32;
-    if ((lay.page_size & (lay.page_size - 1)) == 0) {
-        p.page_shift = 0;
-        while ((1ull << p.page_shift) < lay.page_size) ++p.page_shift;
-    }
+    attention_geometry(c, &p);
     p.zero_row = ctx->zero_row;
     return SGL_KV_OK;
 }

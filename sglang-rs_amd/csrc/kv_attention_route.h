@@ -50,6 +50,10 @@ struct AttentionRoute {
     unsigned combine_threads;
 };
 
+// A buffer's address at `offset`, checked to hold `need` bytes there.
+int32_t attention_ptr(const char *name, const sgl_kv_device_buffer &b, uint64_t offset, uint64_t need, uint64_t *addr);
+// The kernels' sizes and strides of a plan (no pointers, no launch fields).
+void attention_geometry(const sgl_kv_attention_plan_config &c, sglkv_attn_params *p);
 // The reference's overflow error.
 int32_t attention_overflow();
 

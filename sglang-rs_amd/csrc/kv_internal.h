@@ -114,6 +114,9 @@ inline int32_t too_large_rows(uint64_t rows, uint64_t maximum) {
 // DeviceMismatch unless `b` lives on the context's device.
 int32_t check_device(const sgl_rocm_kv_ctx *ctx, const char *name, const sgl_kv_device_buffer &b);
 
+// A pool view by itself: its dimensions, regions and allocation.
+int32_t check_pool_view(const sgl_kv_pool_view *view);
+
 #define SGLKV_CHECK_HIP(call)                                              \
     do {                                                                   \
         hipError_t e_ = (call);                                            \
@@ -147,6 +150,12 @@ struct sgl_rocm_kv_ctx {
     hipFunction_t attention_live[15];     // the same for ragged batches, live splits first (staged and latent only)
     hipFunction_t attention_combine;
     hipFunction_t attention_combine_h;    // the latent body's scaled fp16 records
+    // 8, 16, 32, 64 lanes to a row of 16-byte vectors; any row
+    hipFunction_t page_bounds[5];
+    hipFunction_t page_scores[5];
+    hipFunction_t pick_pages;
+    hipFunction_t selected_attention[2];  // 16-byte vectors, elements
+    hipFunction_t selected_combine;
     uint32_t attention_occupancy[15];     // resident workgroups per CU of attention[i] ...
     uint32_t attention_occupancy_lds[15]; // ... at this LDS size (0 = not yet queried)
     int max_lds_per_block;                // device limit on a workgroup's LDS bytes

@@ -372,6 +372,47 @@ typedef struct sglkv_pair_slots_params {
     uint32_t reserved;
 } sglkv_pair_slots_params;
 
+/* Page key bounds: page `pages[i]`'s minimum and maximum key per channel over
+ * its first counts[i] tokens, of one layer: bf16 [page][head][low, high][dk]. */
+typedef struct sglkv_bounds_params {
+    const uint8_t *pool;      /* byte 0 of the pool */
+    const uint32_t *pages;
+    const uint32_t *counts;
+    uint16_t *bounds;
+    uint32_t *flag;
+    uint64_t count;           /* entries of pages and counts */
+    uint64_t page_count;
+    uint64_t page_stride;
+    uint64_t key_offset;
+    uint64_t key_head_stride, key_token_stride;
+    uint32_t page_size;
+    uint32_t heads;
+    uint32_t dk;
+    uint32_t reserved;
+} sglkv_bounds_params;
+
+/* Page selection and the attention over selected pages. `a` holds what both
+ * share with paged attention: queries, metadata, geometry, split records.
+ * Logical page j of a request is the pool page of its slot number j *
+ * page_size, whose tokens are the page's first ones in order. */
+#define SGLKV_SELECT_NONE 0xFFFFFFFFu   /* past the end of a page list */
+#define SGLKV_SELECT_THREADS 256u
+#define SGLKV_SELECT_LDS_PAGES 8192u    /* keys a picking workgroup keeps in LDS (8 bytes each) */
+#define SGLKV_SELECT_CHUNK_PAGES 64u    /* most pages of a split of the attention: one lane's each */
+#define SGLKV_SELECT_QSTRIDE(dk) (((dk) + 7u) & ~7u) /* dims of a query head in a scoring workgroup's LDS */
+typedef struct sglkv_select_params {
+    sglkv_attn_params a;
+    const uint16_t *bounds;   /* bf16 [page][kv head][low, high][dk] */
+    uint32_t *selected;       /* [query][kv head][max_pages] logical pages, ascending */
+    uint64_t *keys;           /* [query][kv head][sequence_pages] ordered scores, or null */
+    uint64_t max_length;      /* the longest query length that the launch covers */
+    uint32_t max_pages;
+    uint32_t first_pages, last_pages;
+    uint32_t sequence_pages;  /* pages of a sequence of max_length tokens */
+    uint32_t chunk_pages;     /* attention: pages per split; scores: pages per workgroup */
+    uint32_t heads;           /* select: KV heads * chunks of a query (scores), or KV heads */
+} sglkv_select_params;
+
 /* Bytes of zeros the context keeps for reads that must contribute nothing
  * (>= the widest row piece a pipelined attention lane reads, 256 B). */
 #define SGLKV_ZERO_ROW_BYTES 1024u

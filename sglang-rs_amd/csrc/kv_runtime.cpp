@@ -353,6 +353,16 @@ int32_t validate_device(const sgl_rocm_kv_ctx *ctx, const char *name, const sgl_
 
 }  // namespace
 
+int32_t sglkv::check_pool_view(const sgl_kv_pool_view *view) {
+    int32_t rc = check_pool_shape(view);
+    if (rc) return rc;
+    // (The rules of a copy's pool side, for a copy of no rows.)
+    static const uint64_t none = 0;
+    const sgl_kv_device_buffer slots = {const_cast<uint64_t *>(&none), sizeof none};
+    sglkv_side side;
+    return pool_side(view, &slots, 0, shape_of(*view, view->head_layout == SGL_KV_HND, view->heads), &side);
+}
+
 int32_t sglkv::check_device(const sgl_rocm_kv_ctx *ctx, const char *name, const sgl_kv_device_buffer &b) {
     return validate_device(ctx, name, b);
 }
@@ -526,6 +536,25 @@ extern "C" int32_t sgl_rocm_kv_init(int32_t device, const char *code_object_path
         err = hipModuleGetFunction(&ctx->attention_combine, ctx->module, "sglkv_paged_attention_combine");
     if (err == hipSuccess)
         err = hipModuleGetFunction(&ctx->attention_combine_h, ctx->module, "sglkv_paged_attention_combine_h");
+    const struct {
+        const char *name;
+        hipFunction_t *function;
+    } selection[] = {{"sglkv_page_bounds_8", &ctx->page_bounds[0]},
+                     {"sglkv_page_bounds_16", &ctx->page_bounds[1]},
+                     {"sglkv_page_bounds_32", &ctx->page_bounds[2]},
+                     {"sglkv_page_bounds_64", &ctx->page_bounds[3]},
+                     {"sglkv_page_bounds_element", &ctx->page_bounds[4]},
+                     {"sglkv_page_scores_8", &ctx->page_scores[0]},
+                     {"sglkv_page_scores_16", &ctx->page_scores[1]},
+                     {"sglkv_page_scores_32", &ctx->page_scores[2]},
+                     {"sglkv_page_scores_64", &ctx->page_scores[3]},
+                     {"sglkv_page_scores_element", &ctx->page_scores[4]},
+                     {"sglkv_pick_pages", &ctx->pick_pages},
+                     {"sglkv_selected_attention_v16", &ctx->selected_attention[0]},
+                     {"sglkv_selected_attention_v2", &ctx->selected_attention[1]},
+                     {"sglkv_selected_attention_combine", &ctx->selected_combine}};
+    for (const auto &f : selection)
+        if (err == hipSuccess) err = hipModuleGetFunction(f.function, ctx->module, f.name);
     if (err == hipSuccess) err = hipDeviceGetAttribute(&ctx->cu_count, hipDeviceAttributeMultiprocessorCount, device);
     // The tile constants the kernels were compiled with.
     const char *const constants[3] = {"sglkv_rows_per_thread", "sglkv_max_tile_rows",

@@ -1,0 +1,635 @@
+// kv_select.hip -- attention over the pages of a long context that matter,
+// for gfx950: each page's key bounds, the choice of pages for each (query, KV
+// head), and softmax attention over the chosen pages alone. It reads the pools,
+// slot lists and query metadata that kv_attention.hip reads.
+//
+// For a page with keys k_t, low_d = min_t k_td and high_d = max_t k_td, any
+// query q has
+//     q . k_t <= sum_d max(q_d, 0) high_d + min(q_d, 0) low_d
+// for every token t of the page: the page's score, which takes 2 dk values
+// instead of page_size * dk to compute.
+
+namespace {
+
+typedef __attribute__((address_space(1))) const sglkv_u16x8 sel_vec_t;
+
+__device__ __forceinline__ sglkv_u16x8 sel_load(uint64_t at) { return *reinterpret_cast<sel_vec_t *>(at); }
+
+__device__ __forceinline__ float sel_f32(uint16_t bits) { return __uint_as_float(static_cast<uint32_t>(bits) << 16); }
+
+// A value from lane `lane ^ MASK`, MASK a power of two: within a row of 16
+// lanes (permutes and mirrors of the vector unit; mirrors reverse 8 or 16
+// lanes, which serves sums and extremes whose lower bits are already joined),
+// then across rows.
+template <uint32_t MASK>
+__device__ __forceinline__ uint32_t sel_join(uint32_t x) {
+    if constexpr (MASK == 1) return __builtin_amdgcn_update_dpp(x, x, 0xB1, 0xF, 0xF, true);   // quad 1 0 3 2
+    if constexpr (MASK == 2) return __builtin_amdgcn_update_dpp(x, x, 0x4E, 0xF, 0xF, true);   // quad 2 3 0 1
+    if constexpr (MASK == 4) return __builtin_amdgcn_update_dpp(x, x, 0x141, 0xF, 0xF, true);  // mirror of 8
+    if constexpr (MASK == 8) return __builtin_amdgcn_update_dpp(x, x, 0x140, 0xF, 0xF, true);  // mirror of 16
+    if constexpr (MASK == 16) return __float_as_uint(attn_xor16(__uint_as_float(x)));
+    return __float_as_uint(attn_xor32(__uint_as_float(x)));
+}
+
+template <uint32_t MASK>
+__device__ __forceinline__ double sel_join(double x) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = sel_join<MASK>(static_cast<uint32_t>(b)), hi = sel_join<MASK>(static_cast<uint32_t>(b >> 32));
+    return __builtin_bit_cast(double, (static_cast<uint64_t>(hi) << 32) | lo);
+}
+
+// The sum over each group of LANES (a power of two) adjacent lanes, in all of
+// them, by the same tree for every group.
+template <uint32_t LANES>
+__device__ __forceinline__ double sel_sum(double x) {
+    if constexpr (LANES > 1) x += sel_join<1>(x);
+    if constexpr (LANES > 2) x += sel_join<2>(x);
+    if constexpr (LANES > 4) x += sel_join<4>(x);
+    if constexpr (LANES > 8) x += sel_join<8>(x);
+    if constexpr (LANES > 16) x += sel_join<16>(x);
+    if constexpr (LANES > 32) x += sel_join<32>(x);
+    return x;
+}
+
+// ---- Page key bounds ------------------------------------------------------
+//
+// One wave per (page, KV head). NaN carries into both bounds (minimum and
+// maximum of IEEE 754-2019), so that a page with one is not passed over.
+
+__device__ __forceinline__ bool bounds_item(const sglkv_bounds_params &p, uint64_t *page, uint32_t *head,
+                                            uint32_t *tokens) {
+    const uint64_t item = static_cast<uint64_t>(blockIdx.x) * (blockDim.x / 64) +
+                          __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    if (item >= p.count * p.heads) return false;
+    const uint64_t i = item / p.heads;
+    *head = static_cast<uint32_t>(item - i * p.heads);
+    *page = p.pages[i];
+    *tokens = p.counts[i];
+    const bool ok = *page < p.page_count && *tokens <= p.page_size;
+    if (!ok && *head == 0 && (threadIdx.x & 63) == 0)
+        atomicOr(p.flag, *page < p.page_count ? SGLKV_FLAG_SPAN : SGLKV_FLAG_PAGE);
+    return ok && *tokens > 0;
+}
+
+// LANES lanes to a token's row, 8 dims each; 64 / LANES tokens side by side.
+template <uint32_t LANES>
+__device__ __forceinline__ void bounds_body(const sglkv_bounds_params &p) {
+    uint64_t page;
+    uint32_t head, tokens;
+    if (!bounds_item(p, &page, &head, &tokens)) return;
+    constexpr uint32_t GROUPS = 64 / LANES, U = 8;
+    const uint32_t lane = threadIdx.x & 63, v = lane % LANES, group = lane / LANES;
+    const uint64_t rows = reinterpret_cast<uint64_t>(p.pool) + page * p.page_stride + p.key_offset +
+                          head * p.key_head_stride;
+    uint16_t *const out = p.bounds + (page * p.heads + head) * 2 * p.dk;
+    for (uint32_t d = 8 * v; d < p.dk; d += 8 * LANES) {  // (the lanes of one row alike, up to the row's end)
+        float low[8], high[8];
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e) {
+            low[e] = INFINITY;
+            high[e] = -INFINITY;
+        }
+        // U tokens' loads in flight; past the last token, the last again.
+        for (uint32_t t0 = group; t0 < tokens + group; t0 += GROUPS * U) {
+            sglkv_u16x8 r[U];
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u) {
+                const uint32_t t = t0 + GROUPS * u < tokens ? t0 + GROUPS * u : tokens - 1;
+                r[u] = sel_load(rows + static_cast<uint64_t>(t) * p.key_token_stride + 2 * d);
+            }
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u)
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e) {
+                    low[e] = __builtin_elementwise_minimum(low[e], sel_f32(r[u][e]));
+                    high[e] = __builtin_elementwise_maximum(high[e], sel_f32(r[u][e]));
+                }
+        }
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e) {
+#pragma unroll
+            for (uint32_t m = LANES; m < 64; m <<= 1) {
+                low[e] = __builtin_elementwise_minimum(low[e], __shfl_xor(low[e], m));
+                high[e] = __builtin_elementwise_maximum(high[e], __shfl_xor(high[e], m));
+            }
+        }
+        if (group == 0) {
+            sglkv_u16x8 lo, hi;
+#pragma unroll
+            for (uint32_t e = 0; e < 8; ++e) {
+                lo[e] = static_cast<uint16_t>(__float_as_uint(low[e]) >> 16);  // (a bf16 value: exact)
+                hi[e] = static_cast<uint16_t>(__float_as_uint(high[e]) >> 16);
+            }
+            *reinterpret_cast<sglkv_u16x8 *>(out + d) = lo;
+            *reinterpret_cast<sglkv_u16x8 *>(out + p.dk + d) = hi;
+        }
+    }
+}
+
+// Rows of any width and alignment: a lane takes a dim of every token.
+__device__ __forceinline__ void bounds_body_element(const sglkv_bounds_params &p) {
+    uint64_t page;
+    uint32_t head, tokens;
+    if (!bounds_item(p, &page, &head, &tokens)) return;
+    const uint64_t rows = reinterpret_cast<uint64_t>(p.pool) + page * p.page_stride + p.key_offset +
+                          head * p.key_head_stride;
+    uint16_t *const out = p.bounds + (page * p.heads + head) * 2 * p.dk;
+    for (uint32_t d = threadIdx.x & 63; d < p.dk; d += 64) {
+        float low = INFINITY, high = -INFINITY;
+        for (uint32_t t = 0; t < tokens; ++t) {
+            const float x = sel_f32(*reinterpret_cast<__attribute__((address_space(1))) const uint16_t *>(
+                rows + static_cast<uint64_t>(t) * p.key_token_stride + 2 * d));
+            low = __builtin_elementwise_minimum(low, x);
+            high = __builtin_elementwise_maximum(high, x);
+        }
+        out[d] = static_cast<uint16_t>(__float_as_uint(low) >> 16);
+        out[p.dk + d] = static_cast<uint16_t>(__float_as_uint(high) >> 16);
+    }
+}
+
+// ---- The pages of a (query, KV head) ---------------------------------------
+//
+// Scores are summed in 64 bits: a product of two bf16 values has 16 bits, so
+// the sums of up to 1,024 of them are exact unless they span over 2^27 in
+// magnitude, and the choice does not depend on the order of summation. They are
+// kept as keys that order like them: unsigned, NaN above every number, and
+// pages that are always in above that.
+
+constexpr uint64_t kSelForced = ~0ull, kSelNaN = ~0ull - 1;
+
+__device__ __forceinline__ uint64_t sel_key(double score) {
+    if (score != score) return kSelNaN;
+    const uint64_t b = __builtin_bit_cast(uint64_t, score + 0.0);  // (-0 is 0)
+    return b ^ (static_cast<uint64_t>(static_cast<int64_t>(b) >> 63) | (1ull << 63));
+}
+
+// A query's sequence: where its slots start and its length (0: none, or its
+// metadata does not hold, which sets the error word when `report`).
+__device__ __forceinline__ void sel_sequence(const sglkv_attn_params &p, uint64_t max_length, uint64_t q, bool report,
+                                             uint64_t *start, uint64_t *len) {
+    *start = *len = 0;
+    const uint64_t n = p.query_sequence_lengths[q];
+    if (n == 0) return;
+    const uint32_t r = p.query_request_indices[q];
+    if (r >= p.request_count) {
+        if (report) atomicOr(p.flag, SGLKV_FLAG_ATTN_REQUEST);
+        return;
+    }
+    const uint64_t s = p.request_slot_offsets[r], e = p.request_slot_offsets[r + 1];
+    if (s > e || e > p.sequence_slot_count || n > e - s || n > max_length) {
+        if (report) atomicOr(p.flag, SGLKV_FLAG_ATTN_SEQUENCE);
+        return;
+    }
+    *start = s;
+    *len = n;
+}
+
+// Pool page of logical page j (whose slots start at sequence_slots[start]),
+// of which `tokens` are read; false (and the error word) where the slot is no
+// page's first or the tokens pass the pool's slots.
+__device__ __forceinline__ bool sel_page(const sglkv_attn_params &p, uint64_t start, uint64_t j, uint64_t tokens,
+                                         uint64_t *page) {
+    const uint64_t slot = p.sequence_slots[start + j * p.page_size];
+    uint64_t in_page;
+    attn_split_slot(p, slot, page, &in_page);
+    if (slot < p.slot_count && tokens <= p.slot_count - slot && in_page == 0) return true;
+    atomicOr(p.flag, SGLKV_FLAG_ATTN_SLOT);
+    return false;
+}
+
+// The q.k bound of `pages` logical pages from `first` for one (query, KV
+// head), as keys handed to store(i, key). A page takes LANES lanes, 8 dims
+// each (NV times, past 8 LANES dims); a workgroup of SGLKV_SELECT_THREADS
+// threads; the query heads' vectors lie in LDS (qs, 64 bits each).
+template <uint32_t LANES, uint32_t NV, bool VEC, class Store>
+__device__ __forceinline__ void sel_scores(const sglkv_select_params &p, uint32_t head, uint64_t start, uint64_t len,
+                                           uint64_t first, uint64_t last, const uint16_t *qs, Store store) {
+    constexpr uint32_t SIDE = SGLKV_SELECT_THREADS / LANES;  // pages side by side
+    const uint32_t v = threadIdx.x % LANES, mine = threadIdx.x / LANES, dk = p.a.dk, qstride = SGLKV_SELECT_QSTRIDE(dk);
+    const uint64_t count = (len + p.a.page_size - 1) / p.a.page_size;
+    for (uint64_t j0 = first; j0 < last; j0 += SIDE) {
+        const uint64_t j = j0 + mine;
+        const bool live = j < last;
+        const uint64_t left = len - j * p.a.page_size;
+        uint64_t page = 0;
+        bool ok = false;
+        if (live) ok = sel_page(p.a, start, j, left < p.a.page_size ? left : p.a.page_size, &page);
+        const uint64_t row = reinterpret_cast<uint64_t>(p.bounds) + (page * p.a.kv_heads + head) * 4 * dk;
+        sglkv_u16x8 low[NV], high[NV];
+#pragma unroll
+        for (uint32_t n = 0; n < NV; ++n) {
+            const uint32_t d = 8 * (v + LANES * n);
+            low[n] = attn_load8<VEC>(row, d, dk, ok);
+            high[n] = attn_load8<VEC>(row + 2 * dk, d, dk, ok);
+        }
+        double best = -INFINITY;
+        for (uint32_t g = 0; g < p.a.group; ++g) {
+            double sum = 0.0;
+#pragma unroll
+            for (uint32_t n = 0; n < NV; ++n) {
+                const uint32_t d = 8 * (v + LANES * n);
+                if (d < dk)
+#pragma unroll
+                    for (uint32_t e = 0; e < 8; ++e) {
+                        const float q = sel_f32(qs[g * qstride + d + e]);  // (a NaN stays in the second product)
+                        sum += static_cast<double>(q > 0.0f ? q : 0.0f) * static_cast<double>(sel_f32(high[n][e]));
+                        sum += static_cast<double>(q > 0.0f ? 0.0f : q) * static_cast<double>(sel_f32(low[n][e]));
+                    }
+            }
+            sum = sel_sum<LANES>(sum);
+            best = !(sum <= best) && best == best ? sum : best;  // (NaN stays)
+        }
+        if (live && v == 0)
+            store(j, j < p.first_pages || j + p.last_pages >= count ? kSelForced : ok ? sel_key(best) : 0);
+    }
+}
+
+// The query heads of KV head `head` into LDS, zeros behind their dims.
+__device__ __forceinline__ void sel_stage_queries(const sglkv_attn_params &p, uint64_t q, uint32_t head, uint16_t *qs) {
+    const uint16_t *from = p.queries + (q * p.query_heads + static_cast<uint64_t>(head) * p.group) * p.dk;
+    const uint32_t stride = SGLKV_SELECT_QSTRIDE(p.dk);
+    for (uint32_t i = threadIdx.x; i < p.group * stride; i += SGLKV_SELECT_THREADS) {
+        const uint32_t g = i / stride, d = i - g * stride;
+        qs[i] = d < p.dk ? from[g * p.dk + d] : 0;
+    }
+}
+
+struct sel_pick_state {
+    uint32_t histogram[256];
+    uint64_t ors[16], ands[16];
+    uint32_t above[16], equal[16];
+    uint64_t prefix;
+    uint32_t shift, need, done;
+};
+
+// Writes the indices of the `keep` largest of keys load(0..n), ties to the
+// lowest index, ascending, to out[0..keep), SGLKV_SELECT_NONE behind them.
+// A workgroup of WAVES waves. Radix selection from the first bit in which the
+// keys differ, 8 bits a round, until a bucket is taken whole: about two rounds
+// on scores, at most one per 8 bits. Counting uses LDS atomics, whose order
+// does not show.
+template <typename Key, uint32_t WAVES, class Load>
+__device__ __forceinline__ void sel_pick(uint64_t n, uint64_t keep, Load load, uint32_t *out, sel_pick_state &s) {
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid / 64;
+    constexpr uint32_t THREADS = 64 * WAVES;
+    if (n <= keep) {
+        for (uint64_t i = tid; i < keep; i += THREADS) out[i] = i < n ? static_cast<uint32_t>(i) : SGLKV_SELECT_NONE;
+        return;
+    }
+    Key ors = 0, ands = static_cast<Key>(~static_cast<Key>(0));
+    for (uint64_t i = tid; i < n; i += THREADS) {
+        const Key k = load(i);
+        ors |= k;
+        ands &= k;
+    }
+#pragma unroll
+    for (uint32_t m = 1; m < 64; m <<= 1) {
+        ors |= __shfl_xor(ors, m);
+        ands &= __shfl_xor(ands, m);
+    }
+    if (lane == 0) {
+        s.ors[wave] = ors;
+        s.ands[wave] = ands;
+    }
+    __syncthreads();
+    if (tid == 0) {
+        Key o = 0, a = static_cast<Key>(~static_cast<Key>(0));
+        for (uint32_t w = 0; w < WAVES; ++w) {
+            o |= static_cast<Key>(s.ors[w]);
+            a &= static_cast<Key>(s.ands[w]);
+        }
+        const uint64_t differ = static_cast<uint64_t>(static_cast<Key>(o ^ a));
+        const uint32_t bits = differ ? 64 - __builtin_clzll(differ) : 0;  // the bits below which keys differ
+        s.shift = bits;
+        s.prefix = bits < 64 ? static_cast<uint64_t>(o) >> bits : 0;
+        s.need = static_cast<uint32_t>(keep);
+        s.done = bits == 0;
+    }
+    __syncthreads();
+    // Keys are `prefix` above bit `shift`; `need` of those that are, are taken.
+    while (!s.done) {
+        const uint32_t shift = s.shift, next = shift > 8 ? shift - 8 : 0;
+        const uint64_t prefix = s.prefix;
+        for (uint32_t b = tid; b < 256; b += THREADS) s.histogram[b] = 0;
+        __syncthreads();
+        for (uint64_t i = tid; i < n; i += THREADS) {
+            const uint64_t k = static_cast<uint64_t>(load(i));
+            const uint64_t top = shift < 64 ? k >> shift : 0;
+            if (top == prefix) atomicAdd(&s.histogram[(k >> next) & ((1u << (shift - next)) - 1)], 1u);
+        }
+        __syncthreads();
+        if (wave == 0) {
+            // Lane l holds buckets 4 (63 - l) .. + 3: sums from the top down.
+            const uint32_t b0 = 4 * (63 - lane);
+            const uint32_t c[4] = {s.histogram[b0 + 3], s.histogram[b0 + 2], s.histogram[b0 + 1], s.histogram[b0]};
+            const uint32_t sum = c[0] + c[1] + c[2] + c[3];
+            uint32_t upto = sum;
+#pragma unroll
+            for (uint32_t m = 1; m < 64; m <<= 1) {
+                const uint32_t x = __shfl_up(upto, m);
+                if (lane >= m) upto += x;
+            }
+            const uint32_t need = s.need;
+            uint32_t before = upto - sum;
+            if (before < need && upto >= need) {  // (one lane: the counts reach `need`)
+                uint32_t j = 0;
+                while (j < 3 && before + c[j] < need) before += c[j++];
+                s.need = need - before;
+                s.prefix = (shift < 64 ? prefix << (shift - next) : 0) | (b0 + 3 - j);
+                s.shift = next;
+                s.done = c[j] == need - before || next == 0;
+            }
+        }
+        __syncthreads();
+    }
+    const uint32_t shift = s.shift, need = s.need;
+    const uint64_t prefix = s.prefix;
+    auto top = [&](uint64_t i) {
+        const uint64_t k = static_cast<uint64_t>(load(i));
+        return shift < 64 ? k >> shift : 0;
+    };
+    // Each wave a run of indices: count, then write in order.
+    const uint64_t run = (n + WAVES - 1) / WAVES, i0 = wave * run, i1 = i0 + run < n ? i0 + run : n;
+    uint32_t above = 0, equal = 0;
+    for (uint64_t i = i0; i < i1; i += 64) {
+        const uint64_t t = i + lane < i1 ? top(i + lane) : 0;
+        above += __popcll(__ballot(i + lane < i1 && t > prefix));
+        equal += __popcll(__ballot(i + lane < i1 && t == prefix));
+    }
+    if (lane == 0) {
+        s.above[wave] = above;
+        s.equal[wave] = equal;
+    }
+    __syncthreads();
+    uint32_t at = 0, ties = 0;
+    for (uint32_t w = 0; w < wave; ++w) {
+        at += s.above[w];
+        ties += s.equal[w];
+    }
+    at += ties < need ? ties : need;
+    for (uint64_t i = i0; i < i1; i += 64) {
+        const bool in = i + lane < i1;
+        const uint64_t t = in ? top(i + lane) : 0;
+        const uint64_t eq = __ballot(in && t == prefix);
+        const uint32_t rank = ties + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(eq >> 32),
+                                                               __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(eq), 0));
+        const bool take = in && (t > prefix || (t == prefix && rank < need));
+        const uint64_t taken = __ballot(take);
+        if (take)
+            out[at + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(taken >> 32),
+                                               __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(taken), 0))] =
+                static_cast<uint32_t>(i + lane);
+        at += __popcll(taken);
+        ties += __popcll(eq);
+    }
+}
+
+// Scores of a chunk of a (query, KV head)'s pages into the workspace.
+template <uint32_t LANES, uint32_t NV, bool VEC>
+__device__ __forceinline__ void sel_scores_body(const sglkv_select_params &p) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t sel_lds[];
+    uint16_t *qs = reinterpret_cast<uint16_t *>(sel_lds);
+    const uint32_t chunks = p.heads / p.a.kv_heads;
+    const uint32_t chunk = blockIdx.x % chunks, item = blockIdx.x / chunks;
+    const uint32_t head = item % p.a.kv_heads;
+    const uint64_t q = item / p.a.kv_heads;
+    uint64_t start, len;
+    sel_sequence(p.a, p.max_length, q, false, &start, &len);
+    const uint64_t count = (len + p.a.page_size - 1) / p.a.page_size;
+    const uint64_t first = static_cast<uint64_t>(chunk) * p.chunk_pages;
+    if (first >= count || count <= p.max_pages) return;  // (nothing to choose from)
+    sel_stage_queries(p.a, q, head, qs);
+    __syncthreads();
+    uint64_t *keys = p.keys + (q * p.a.kv_heads + head) * p.sequence_pages;
+    sel_scores<LANES, NV, VEC>(p, head, start, len, first, first + p.chunk_pages < count ? first + p.chunk_pages : count, qs,
+                          [&](uint64_t j, uint64_t key) { keys[j] = key; });
+}
+
+// The pages of a (query, KV head) from the workspace's keys.
+__device__ __forceinline__ void sel_pick_body(const sglkv_select_params &p) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t sel_lds[];
+    __shared__ sel_pick_state state;
+    uint64_t *kept = reinterpret_cast<uint64_t *>(sel_lds);
+    const uint32_t head = blockIdx.x % p.a.kv_heads;
+    const uint64_t q = blockIdx.x / p.a.kv_heads;
+    uint64_t start, len;
+    sel_sequence(p.a, p.max_length, q, head == 0 && threadIdx.x == 0, &start, &len);
+    const uint64_t count = (len + p.a.page_size - 1) / p.a.page_size;
+    const uint64_t *keys = p.keys + (q * p.a.kv_heads + head) * p.sequence_pages;
+    uint32_t *out = p.selected + (q * p.a.kv_heads + head) * p.max_pages;
+    if (count <= SGLKV_SELECT_LDS_PAGES) {
+        if (count > p.max_pages)
+            for (uint64_t i = threadIdx.x; i < count; i += SGLKV_SELECT_THREADS) kept[i] = keys[i];
+        __syncthreads();
+        sel_pick<uint64_t, SGLKV_SELECT_THREADS / 64>(count, p.max_pages, [&](uint64_t i) { return kept[i]; }, out, state);
+    } else {
+        sel_pick<uint64_t, SGLKV_SELECT_THREADS / 64>(count, p.max_pages, [&](uint64_t i) { return keys[i]; }, out, state);
+    }
+}
+
+// ---- Attention over the selected pages --------------------------------------
+
+// The work of this workgroup: `pages` entries of its list from entry e0, in
+// the order of the list, `tokens` tokens in all.
+struct sel_work {
+    attn_work w;
+    uint64_t start, len;
+    uint32_t e0, pages, tokens;
+};
+
+// Lane l's entry e0 + l of the list as its pool page, for this split of the
+// list; the lists ascend, so only the sequence's last page, the last entry,
+// holds fewer than page_size tokens. An entry that is no page of the sequence
+// or does not ascend sets the error word, and the split counts as empty.
+__device__ __forceinline__ uint64_t sel_decode(const sglkv_select_params &p, uint32_t lane, sel_work *s) {
+    // (The head groups and value blocks of a (query, KV head) side by side: they read the same rows.)
+    uint32_t bx = blockIdx.x;
+    const uint32_t dblk = bx % p.a.dv_blocks;
+    bx /= p.a.dv_blocks;
+    const uint32_t hg = bx % p.a.head_groups;
+    bx /= p.a.head_groups;
+    const uint32_t kvh = bx % p.a.kv_heads;
+    const uint64_t q = bx / p.a.kv_heads;
+    const uint32_t split = blockIdx.y;
+    s->w.q = q;
+    s->w.kvh = kvh;
+    s->w.h0 = kvh * p.a.group + hg * SGLKV_ATTN_HEADS;
+    const uint32_t heads = p.a.group - hg * SGLKV_ATTN_HEADS;
+    s->w.nh = heads < SGLKV_ATTN_HEADS ? heads : SGLKV_ATTN_HEADS;
+    s->w.d0 = dblk * SGLKV_ATTN_DV;
+    s->w.dblk = dblk;
+    s->w.split = split;
+    sel_sequence(p.a, p.max_length, q, lane == 0 && split == 0 && hg == 0 && dblk == 0 && kvh == 0, &s->start, &s->len);
+    s->e0 = split * p.chunk_pages;
+    s->pages = s->tokens = 0;
+    const uint32_t e = s->e0 + lane;
+    const uint32_t *list = p.selected + (q * p.a.kv_heads + kvh) * p.max_pages;
+    const bool inside = s->len > 0 && lane < p.chunk_pages && e < p.max_pages;
+    const uint32_t j = inside ? list[e] : SGLKV_SELECT_NONE;
+    const uint32_t before = inside && e > 0 ? list[e - 1] : 0;
+    const uint64_t listed = __ballot(j != SGLKV_SELECT_NONE);
+    const uint64_t count = (s->len + p.a.page_size - 1) / p.a.page_size;
+    uint64_t page = 0;
+    bool bad = false;
+    if (j != SGLKV_SELECT_NONE) {
+        bad = j >= count || (e > 0 && before >= j);
+        if (bad) {
+            atomicOr(p.a.flag, SGLKV_FLAG_ATTN_SEQUENCE);
+        } else {
+            const uint64_t left = s->len - static_cast<uint64_t>(j) * p.a.page_size;
+            bad = !sel_page(p.a, s->start, j, left < p.a.page_size ? left : p.a.page_size, &page);
+        }
+    }
+    if (__ballot(bad) != 0 || listed == 0) return page;
+    // (The listed ones are the first: NONE before a page does not ascend.)
+    s->pages = __popcll(listed);
+    const uint32_t last = __shfl(j, s->pages - 1);
+    const uint64_t left = s->len - static_cast<uint64_t>(last) * p.a.page_size;
+    s->tokens = static_cast<uint32_t>((s->pages - 1) * p.a.page_size + (left < p.a.page_size ? left : p.a.page_size));
+    return page;
+}
+
+// A split without tokens: zeros where it is the only one, else a record that
+// the merge leaves out (a maximum of -inf, which no split with tokens has).
+__device__ __forceinline__ void sel_empty(const sglkv_select_params &p, const sel_work &s, uint32_t lane, uint32_t dims) {
+    const sglkv_attn_params &a = p.a;
+    if (a.splits == 1) {
+        for (uint32_t i = lane; i < s.w.nh * dims; i += 64) {
+            const uint32_t h = i / dims, d = s.w.d0 + i % dims;
+            if (d < a.dv) a.output[(s.w.q * a.query_heads + s.w.h0 + h) * a.dv + d] = 0;
+        }
+    } else if (s.w.dblk == 0 && lane < s.w.nh) {
+        float *ml = attn_rec_ml(a, (s.w.q * a.query_heads + s.w.h0 + lane) * a.splits + s.w.split);
+        ml[0] = -INFINITY;
+        ml[1] = 0.0f;
+    }
+}
+
+// Any head dims, page size and alignment: a wave to 16 query heads and
+// SGLKV_ATTN_DV value dims, 32 tokens a step, as the generic body of paged
+// attention (attn_body), whose layouts of the matrix products it shares.
+template <bool VEC>
+__device__ __forceinline__ void sel_attend_body(const sglkv_select_params &p) {
+    extern __shared__ __attribute__((aligned(16))) uint16_t sel_attend_lds[];
+    __shared__ uint64_t pages[SGLKV_SELECT_CHUNK_PAGES];
+    const sglkv_attn_params &a = p.a;
+    const uint32_t lane = threadIdx.x, g = lane >> 4, r = lane & 15;
+    sel_work s;
+    pages[lane] = sel_decode(p, lane, &s);
+    if (s.tokens == 0) {
+        sel_empty(p, s, lane, SGLKV_ATTN_DV);
+        return;
+    }
+    const attn_work &w = s.w;
+    const uint32_t qstride = a.dk_pad + 8;
+    uint16_t *qs = sel_attend_lds, *vt = sel_attend_lds + SGLKV_ATTN_HEADS * qstride;
+    attn_stage_queries(a, w, lane, qs, qstride);  // (and a barrier: pages[] too)
+    const uint64_t pool = reinterpret_cast<uint64_t>(a.pool);
+    const uint64_t kbase = pool + a.key_offset + w.kvh * a.key_head_stride;
+    const uint64_t vbase = pool + a.value_offset + w.kvh * a.value_head_stride;
+    attn_state st;
+    attn_state_init(st);
+    for (uint32_t tb = 0; tb < s.tokens; tb += SGLKV_ATTN_TOKENS) {
+        uint64_t krow[2], vrow[2];
+        bool valid[2];
+#pragma unroll
+        for (uint32_t b = 0; b < 2; ++b) {
+            const uint32_t tok = tb + 8 * (r >> 2) + 4 * b + (r & 3);
+            valid[b] = tok < s.tokens;
+            uint64_t e, pos;
+            attn_split_slot(a, valid[b] ? tok : 0, &e, &pos);
+            const uint64_t page = pages[e] * a.page_stride;
+            krow[b] = kbase + page + pos * a.key_token_stride;
+            vrow[b] = vbase + page + pos * a.value_token_stride;
+        }
+        sglkv_f32x4 sc[2] = {sglkv_f32x4{0.f, 0.f, 0.f, 0.f}, sglkv_f32x4{0.f, 0.f, 0.f, 0.f}};
+        for (uint32_t kk = 0; kk < a.dk_pad; kk += 32) {
+            const sglkv_u16x8 qv = *reinterpret_cast<const sglkv_u16x8 *>(qs + r * qstride + kk + 8 * g);
+#pragma unroll
+            for (uint32_t b = 0; b < 2; ++b)
+                sc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                    attn_as_bf16(attn_load8<VEC>(krow[b], kk + 8 * g, a.dk, valid[b])), attn_as_bf16(qv), sc[b], 0, 0, 0);
+        }
+#pragma unroll
+        for (uint32_t b = 0; b < 2; ++b) {
+            const uint32_t tl = 8 * (r >> 2) + 4 * b + (r & 3);
+#pragma unroll
+            for (uint32_t n = 0; n < 4; ++n) {
+                const sglkv_u16x8 v = attn_load8<VEC>(vrow[b], w.d0 + 8 * (g + 4 * n), a.dv, valid[b]);
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e) vt[(8 * (g + 4 * n) + e) * SGLKV_ATTN_VT_STRIDE + tl] = v[e];
+            }
+        }
+        attn_softmax_pv(a, g, sc, __ballot(valid[0]), __ballot(valid[1]), vt, r, st);
+    }
+    attn_finish(a, w, g, r, st);
+}
+
+}  // namespace
+
+extern "C" __global__ __launch_bounds__(256) void sglkv_page_bounds_8(sglkv_bounds_params p) { bounds_body<8>(p); }
+extern "C" __global__ __launch_bounds__(256) void sglkv_page_bounds_16(sglkv_bounds_params p) { bounds_body<16>(p); }
+extern "C" __global__ __launch_bounds__(256) void sglkv_page_bounds_32(sglkv_bounds_params p) { bounds_body<32>(p); }
+extern "C" __global__ __launch_bounds__(256) void sglkv_page_bounds_64(sglkv_bounds_params p) { bounds_body<64>(p); }
+extern "C" __global__ __launch_bounds__(256) void sglkv_page_bounds_element(sglkv_bounds_params p) {
+    bounds_body_element(p);
+}
+
+extern "C" __global__ __launch_bounds__(SGLKV_SELECT_THREADS) void sglkv_page_scores_8(sglkv_select_params p) {
+    sel_scores_body<8, 1, true>(p);
+}
+extern "C" __global__ __launch_bounds__(SGLKV_SELECT_THREADS) void sglkv_page_scores_16(sglkv_select_params p) {
+    sel_scores_body<16, 1, true>(p);
+}
+extern "C" __global__ __launch_bounds__(SGLKV_SELECT_THREADS) void sglkv_page_scores_32(sglkv_select_params p) {
+    sel_scores_body<32, 1, true>(p);
+}
+extern "C" __global__ __launch_bounds__(SGLKV_SELECT_THREADS) void sglkv_page_scores_64(sglkv_select_params p) {
+    sel_scores_body<64, 2, true>(p);
+}
+extern "C" __global__ __launch_bounds__(SGLKV_SELECT_THREADS) void sglkv_page_scores_element(sglkv_select_params p) {
+    sel_scores_body<64, 2, false>(p);
+}
+extern "C" __global__ __launch_bounds__(SGLKV_SELECT_THREADS) void sglkv_pick_pages(sglkv_select_params p) {
+    sel_pick_body(p);
+}
+
+extern "C" __global__ __launch_bounds__(64) void sglkv_selected_attention_v16(sglkv_select_params p) {
+    sel_attend_body<true>(p);
+}
+extern "C" __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void
+sglkv_selected_attention_v2(sglkv_select_params p) {
+    sel_attend_body<false>(p);
+}
+
+// Merges the split records of a (query, head), one wave each: lane l takes
+// dims 4l .. 4l+3 (+256 ...). Empty splits' records are not read; a (query,
+// head) of nothing else is zeros.
+extern "C" __global__ __launch_bounds__(64) void sglkv_selected_attention_combine(sglkv_select_params p) {
+    const sglkv_attn_params &a = p.a;
+    const uint64_t item = blockIdx.x;
+    const uint32_t lane = threadIdx.x;
+    const float2 *ml = reinterpret_cast<const float2 *>(attn_rec_ml(a, item * a.splits));
+    float m = -INFINITY;
+    for (uint32_t s = lane; s < a.splits; s += 64) m = fmaxf(m, ml[s].x);
+#pragma unroll
+    for (uint32_t x = 1; x < 64; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
+    for (uint32_t d = 4 * lane; d < a.dv; d += 256) {
+        float l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (uint32_t s = 0; s < a.splits; ++s) {
+            const float2 r = ml[s];
+            if (r.x == -INFINITY) continue;
+            const float w = exp2f(r.x - m);
+            const float4 v = *reinterpret_cast<const float4 *>(attn_rec_o(a, item * a.splits + s) + d);
+            l += w * r.y;
+            o[0] += w * v.x;
+            o[1] += w * v.y;
+            o[2] += w * v.z;
+            o[3] += w * v.w;
+        }
+        const float linv = m == -INFINITY ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e)
+            if (d + e < a.dv) a.output[item * a.dv + d + e] = attn_to_bf16(o[e] * linv);
+    }
+}

@@ -325,6 +325,20 @@ class _AttentionRoute(ctypes.Structure):
                 ("chunk_tokens", _u64), ("workgroups", _u64), ("record_bytes", _u64), ("records_apart", _u64)]
 
 
+class _PageSelectionConfig(ctypes.Structure):
+    _fields_ = [(n, _u64) for n in ("max_pages", "first_pages", "last_pages", "max_sequence_length")]
+
+
+class _PageSelectionPlan(ctypes.Structure):
+    _fields_ = [("attention", _AttentionPlan), ("config", _PageSelectionConfig)] + [
+        (n, _u64) for n in ("bounds_required_bytes", "selected_required_bytes", "workspace_required_bytes")]
+
+
+class _PageSelectionBuffers(ctypes.Structure):
+    _fields_ = [("attention", _AttentionBuffers)] + [f for n in ("bounds", "selected", "workspace")
+                                                     for f in ((n, _DeviceBuffer), (n + "_offset", _u64))]
+
+
 # SGL_KV_ATTN_BODY_*, by value
 ATTENTION_BODIES = ("vector", "element", "pipe128", "pipe", "wide576", "wide128", "latent", "staged128", "staged64",
                     "latent_exact", "staged256", "staged128k", "tile128", "tile64", "tile256")
@@ -535,6 +549,16 @@ _EXPORTS = {
                                                                    ctypes.POINTER(_AttentionPlan),
                                                                    ctypes.POINTER(_AttentionBuffers), _u64,
                                                                    ctypes.c_void_p]),
+    "sgl_kv_page_selection_plan_new": (ctypes.c_int32, [ctypes.POINTER(_AttentionPlan),
+                                                        ctypes.POINTER(_PageSelectionConfig),
+                                                        ctypes.POINTER(_PageSelectionPlan)]),
+    "sgl_rocm_kv_page_bounds": (ctypes.c_int32, [ctypes.c_void_p, ctypes.POINTER(PoolView),
+                                                 ctypes.POINTER(_DeviceBuffer), ctypes.POINTER(_DeviceBuffer), _u64,
+                                                 ctypes.POINTER(_DeviceBuffer), ctypes.c_void_p]),
+    "sgl_rocm_kv_select_pages": (ctypes.c_int32, [ctypes.c_void_p, ctypes.POINTER(_PageSelectionPlan),
+                                                  ctypes.POINTER(_PageSelectionBuffers), ctypes.c_void_p]),
+    "sgl_rocm_kv_selected_attention": (ctypes.c_int32, [ctypes.c_void_p, ctypes.POINTER(_PageSelectionPlan),
+                                                        ctypes.POINTER(_PageSelectionBuffers), ctypes.c_void_p]),
     "sgl_rocm_kv_execute_page_requests": (ctypes.c_int32, [ctypes.c_void_p,
                                                            ctypes.POINTER(_DeviceBuffer), _u64, _u64,
                                                            ctypes.POINTER(_DeviceBuffer),
@@ -1332,6 +1356,28 @@ class RocmKvPairCopyKernels:
         _paged_attention(lib().sgl_rocm_kv_paged_attention_async_noalloc, self, plan, buffers,
                          max_sequence_length, stream)
 
+    def page_bounds(self, keys: PoolView, *, pages, counts, page_count: int, bounds, stream=None):
+        """Smallest and largest key per channel of `page_count` pages (u32
+        `pages`, with u32 `counts` tokens each) of the layer that `keys`
+        describes, into `bounds` (bf16 [page][head][2][dims], every page of the
+        pool). Asynchronous; a page past the pool or a count past the page
+        surfaces at the next check_errors."""
+        _call(lib().sgl_rocm_kv_page_bounds, self._h, ctypes.byref(keys), ctypes.byref(_as_db(pages)),
+              ctypes.byref(_as_db(counts)), page_count, ctypes.byref(_as_db(bounds)), _stream(stream))
+
+    def select_pages(self, plan: "PageSelectionPlan", buffers: "PageSelectionBuffers", *, stream=None):
+        """The max_pages pages of each (query, KV head) with the largest upper
+        bound of q.k, into `selected` (u32 [query][KV head][max_pages],
+        ascending, UINT32_MAX behind them). Asynchronous."""
+        _call(lib().sgl_rocm_kv_select_pages, self._h, ctypes.byref(plan._c), ctypes.byref(buffers._c),
+              _stream(stream))
+
+    def selected_attention(self, plan: "PageSelectionPlan", buffers: "PageSelectionBuffers", *, stream=None):
+        """Attention of each query over its KV heads' `selected` pages, into
+        `output`. Asynchronous."""
+        _call(lib().sgl_rocm_kv_selected_attention, self._h, ctypes.byref(plan._c), ctypes.byref(buffers._c),
+              _stream(stream))
+
     def check_errors(self, stream=None):
         _call(lib().sgl_rocm_kv_check_errors, self._h, _stream(stream))
 
@@ -1896,6 +1942,61 @@ class PagedAttentionPlan:
         lay = self._c.config.layout
         return (lay.page_size, lay.page_stride_bytes, lay.key_in_page_offset,
                 lay.value_in_page_offset, lay.key_row_bytes, lay.value_row_bytes)
+
+
+class PageSelectionPlan:
+    """What select_pages and selected_attention need to know: the attention
+    plan of the step, lists of `max_pages` pages, of which the sequence's
+    `first_pages` and `last_pages` are always members, and the longest query
+    length (0: as many as the plan's slots)."""
+
+    def __init__(self, c: _PageSelectionPlan):
+        self._c = c
+
+    @classmethod
+    def new(cls, attention: PagedAttentionPlan, *, max_pages: int, first_pages: int = 0, last_pages: int = 0,
+            max_sequence_length: int = 0) -> "PageSelectionPlan":
+        config, out = _PageSelectionConfig(max_pages, first_pages, last_pages, max_sequence_length), _PageSelectionPlan()
+        _call(lib().sgl_kv_page_selection_plan_new, ctypes.byref(attention._c), ctypes.byref(config), ctypes.byref(out))
+        return cls(out)
+
+    @property
+    def attention(self) -> PagedAttentionPlan:
+        return PagedAttentionPlan(self._c.attention)
+
+    def __getattr__(self, name):
+        c = self.__dict__["_c"]
+        for part in (c, c.config):
+            if hasattr(part, name) and name not in ("attention", "config"):
+                return getattr(part, name)
+        raise AttributeError(name)
+
+
+def _fill_buffers(struct, names, given: dict):
+    """Sets the named buffers (objects with .ptr/.nbytes, or device_buffer(...))
+    and their <name>_offset; returns the names left over."""
+    rest = dict(given)
+    for n in names:
+        if n in rest:
+            setattr(struct, n, _as_db(rest.pop(n)))
+        if n + "_offset" in rest:
+            setattr(struct, n + "_offset", rest.pop(n + "_offset"))
+    return rest
+
+
+class PageSelectionBuffers:
+    """The buffers of select_pages and selected_attention by name, each with an
+    optional <name>_offset: those of paged_attention, and `bounds`, `selected`
+    and `workspace`. A call reads only its own; a decode loop keeps one of these,
+    which keeps the given objects."""
+
+    def __init__(self, **buffers):
+        self._c = _PageSelectionBuffers()
+        self._given = buffers
+        rest = _fill_buffers(self._c.attention, _ATTENTION_BUFFERS, buffers)
+        rest = _fill_buffers(self._c, ("bounds", "selected", "workspace"), rest)
+        if rest:
+            raise TypeError(f"unknown buffers: {', '.join(sorted(rest))}")
 
 
 def _attention_buffers(buffers: dict) -> _AttentionBuffers:
