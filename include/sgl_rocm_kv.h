@@ -1081,6 +1081,128 @@ int32_t sgl_rocm_kv_select_pages(sgl_rocm_kv_ctx *ctx, const sgl_kv_page_selecti
 int32_t sgl_rocm_kv_selected_attention(sgl_rocm_kv_ctx *ctx, const sgl_kv_page_selection_plan *plan,
                                        const sgl_kv_page_selection_buffers *buffers, void *stream);
 
+/* ---- Eviction by accumulated attention weight ----
+ * No counterpart in the reference, whose caches grow until a request ends. To
+ * hold a sequence in a budget of tokens, a caller adds up the attention that
+ * each position gets (accumulate_weights, for the queries it runs anyway),
+ * takes the positions of each KV head that got the most (select_tokens), and
+ * copies their rows to slots of their own (compact_tokens), after which the old
+ * slots can be released and the request goes on at its new length. Keys that
+ * were rotated by their position stay valid, since rows move unchanged. All
+ * calls are asynchronous: nothing waits, nothing is allocated, errors found on
+ * the device surface at sgl_rocm_kv_check_errors. They can be captured. */
+
+typedef struct sgl_kv_weight_plan {
+    sgl_kv_attention_plan attention;
+    uint64_t max_sequence_length;      /* longest query length; 0: sequence_slot_count */
+    uint64_t weights_required_bytes;   /* f32 [KV head][sequence_slot_count] */
+    uint64_t workspace_required_bytes;
+} sgl_kv_weight_plan;
+
+/* The plan of accumulate_weights for the queries that `attention` describes (the
+ * values and the output are not touched). Errors: attention_plan_new's;
+ * DimensionTooLarge: "query_key_head_dim" past 1,024, "workgroups" past one
+ * dispatch. */
+int32_t sgl_kv_weight_plan_new(const sgl_kv_attention_plan *attention, uint64_t max_sequence_length,
+                               sgl_kv_weight_plan *out);
+
+/* `attention` as for sgl_rocm_kv_paged_attention (its output is not used and may
+ * be null). weights: f32 [KV head][sequence_slot_count], position t of request r
+ * at request_slot_offsets[r] + t. The workspace is scratch for one call: calls
+ * that may run at the same time need one each. Its address is a multiple of 16. */
+typedef struct sgl_kv_weight_buffers {
+    sgl_kv_attention_buffers attention;
+    sgl_kv_device_buffer weights;   uint64_t weights_offset;
+    sgl_kv_device_buffer workspace; uint64_t workspace_offset;
+} sgl_kv_weight_buffers;
+
+/* weights[h][t] += the softmax weight of token t, summed over the query heads of
+ * KV head h and over the queries of t's request whose length passes t. Scores,
+ * statistics and sums are held in 32 bits; positions that no query attends stay
+ * as they are. The result does not depend on the order in which workgroups run.
+ * The queries come request by request: query_request_indices never fall
+ * (otherwise REQUEST is reported and the sums are unspecified). A query of
+ * length 0 (padding) adds nothing, nor does one whose metadata does not hold
+ * (reported as paged attention does). */
+int32_t sgl_rocm_kv_accumulate_weights(sgl_rocm_kv_ctx *ctx, const sgl_kv_weight_plan *plan,
+                                       const sgl_kv_weight_buffers *buffers, void *stream);
+
+typedef struct sgl_kv_eviction_config {
+    uint64_t request_count;
+    uint64_t kv_head_count;
+    uint64_t sequence_slot_count;     /* entries of sequence_slots, columns of weights */
+    uint64_t destination_slot_count;  /* entries of destination_slots, columns of destination_weights */
+    uint64_t max_kept;                /* entries of a (request, KV head)'s list */
+    uint64_t first_tokens;            /* positions at the start that are always kept ... */
+    uint64_t last_tokens;             /* ... and at the end (together at most max_kept) */
+    uint64_t max_sequence_length;     /* longest request length; 0: sequence_slot_count */
+} sgl_kv_eviction_config;
+
+typedef struct sgl_kv_eviction_plan {
+    sgl_kv_eviction_config config;
+    uint64_t request_lengths_required_bytes;
+    uint64_t request_slot_offsets_required_bytes;   /* destination_slot_offsets alike */
+    uint64_t sequence_slots_required_bytes;
+    uint64_t weights_required_bytes;
+    uint64_t kept_required_bytes;                   /* u32 [request][KV head][max_kept] */
+    uint64_t destination_slots_required_bytes;
+    uint64_t destination_weights_required_bytes;
+    uint64_t workspace_required_bytes;              /* select_tokens; 0: none is needed */
+} sgl_kv_eviction_plan;
+
+/* Errors: ZeroDimension (request_count, kv_head_count, sequence_slot_count,
+ * max_kept); InvalidArgument ("first_tokens" where first_tokens + last_tokens
+ * pass max_kept); DimensionTooLarge: "max_kept" or "max_sequence_length" past
+ * 2^31, "workgroups" past one dispatch. */
+int32_t sgl_kv_eviction_plan_new(const sgl_kv_eviction_config *config, sgl_kv_eviction_plan *out);
+
+/* request_lengths u64 per request (0: nothing is kept); request_slot_offsets and
+ * sequence_slots as for paged attention; weights f32 [KV
+ * head][sequence_slot_count]; kept u32 [request][KV head][max_kept];
+ * destination_slot_offsets u64 (request_count + 1) into destination_slots (u64)
+ * and the columns of destination_weights (f32 [KV
+ * head][destination_slot_count]). select_tokens reads request_lengths,
+ * request_slot_offsets and weights and writes kept; compact_tokens reads all but
+ * the workspace, and weights and destination_weights may both be null. */
+typedef struct sgl_kv_eviction_buffers {
+    sgl_kv_device_buffer request_lengths;          uint64_t request_lengths_offset;
+    sgl_kv_device_buffer request_slot_offsets;     uint64_t request_slot_offsets_offset;
+    sgl_kv_device_buffer sequence_slots;           uint64_t sequence_slots_offset;
+    sgl_kv_device_buffer weights;                  uint64_t weights_offset;
+    sgl_kv_device_buffer kept;                     uint64_t kept_offset;
+    sgl_kv_device_buffer destination_slot_offsets; uint64_t destination_slot_offsets_offset;
+    sgl_kv_device_buffer destination_slots;        uint64_t destination_slots_offset;
+    sgl_kv_device_buffer destination_weights;      uint64_t destination_weights_offset;
+    sgl_kv_device_buffer workspace;                uint64_t workspace_offset;
+} sgl_kv_eviction_buffers;
+
+/* The lists: of each (request, KV head) the max_kept positions below the
+ * request's length with the largest weights; equal ones go to the lower
+ * position, NaN ranks above every number, and the first_tokens and last_tokens
+ * rank above all. Ascending, followed by UINT32_MAX; a request of at most
+ * max_kept tokens keeps all. A request whose range or length does not hold is
+ * reported (SEQUENCE) and keeps nothing. */
+int32_t sgl_rocm_kv_select_tokens(sgl_rocm_kv_ctx *ctx, const sgl_kv_eviction_plan *plan,
+                                  const sgl_kv_eviction_buffers *buffers, void *stream);
+
+/* Row i of KV head h of request r's destination <- that head's row of its i-th
+ * kept position: the head's chunk of each tensor from `source`'s slot
+ * sequence_slots[request_slot_offsets[r] + kept[i]] to `destination`'s slot
+ * destination_slots[destination_slot_offsets[r] + i]. The views describe one
+ * layer of one or two pools, of any element type, with their own page sizes and
+ * head layouts; heads = kv_head_count and row widths agree (InvalidArgument
+ * "views"), and scales are copied when both carry a pointer. Sums move along:
+ * destination_weights[h][offset + i] = weights[h][kept[i]], and 0 for the
+ * destination's further positions, whose rows are left as they are. A request
+ * may keep fewer positions than its destination has slots, not more (SEQUENCE,
+ * also for a position past the length); a slot past its pool is reported
+ * (SLOT); such rows are skipped. No destination slot may be a source slot of
+ * the call: a row could be overwritten before it is read. Passing one buffer as
+ * both slot lists of the same layer is refused (InvalidArgument "in place"). */
+int32_t sgl_rocm_kv_compact_tokens(sgl_rocm_kv_ctx *ctx, const sgl_kv_eviction_plan *plan,
+                                   const sgl_kv_eviction_buffers *buffers, const sgl_kv_pool_view *source,
+                                   const sgl_kv_pool_view *destination, void *stream);
+
 /* ---- Bootstrap wire format: the decode side's page table and layout ----
  * The multipart frames a decode worker sends a prefill worker's bootstrap
  * listener (Mooncake protocol, crates/sglang-srt/src/pd_bootstrap.rs):

@@ -1,0 +1,368 @@
+// kv_evict.hip -- eviction from a paged KV cache by accumulated attention
+// weight, for gfx950: the softmax weights that each position of a sequence gets
+// from the queries, added to a running sum per KV head; the positions with the
+// largest sums; and the copy of their K/V rows (and sums) to other slots.
+//
+// For query head i of KV head h at query q, with scores s_t = scale q_i . k_t
+// over the query's first len tokens,
+//     weights[h][t] += sum_{q, i} exp(s_t - m) / l,  m = max s, l = sum exp(s - m).
+// The values are not read. The first kernel finds (m, l) of each (query, head);
+// the second computes the scores again, with the tokens as the outer loop, so
+// that each position's sum is added up by one wave in one order: no atomics,
+// and the same result every time.
+
+namespace {
+
+// A query's metadata; false, and nothing to weigh, for a query of no tokens or
+// whose metadata does not hold (which sets the error word when `report`).
+__device__ __forceinline__ bool wgt_query(const sglkv_weights_params &p, uint64_t q, bool report, uint64_t *start,
+                                          uint64_t *len) {
+    sel_sequence(p.a, p.max_length, q, report, start, len);
+    // The second kernel finds a request's queries by halving: they come request by request.
+    if (report && q > 0 && p.a.query_request_indices[q - 1] > p.a.query_request_indices[q])
+        atomicOr(p.a.flag, SGLKV_FLAG_ATTN_REQUEST);
+    return *len > 0;
+}
+
+// The (maximum, sum) pair of (query, head, split). A split without tokens
+// leaves (-inf, 0); one with tokens has a finite maximum.
+__device__ __forceinline__ float2 *wgt_stats(const sglkv_weights_params &p, uint64_t q, uint64_t head) {
+    return reinterpret_cast<float2 *>(p.a.partial) + (q * p.a.query_heads + head) * p.a.splits;
+}
+
+// K row address of a sequence's token; false where its slot lies outside the
+// pool (the address is slot 0's).
+__device__ __forceinline__ bool wgt_row(const sglkv_attn_params &p, uint64_t kbase, uint64_t start, uint64_t tok,
+                                        bool inside, bool report, uint64_t *row) {
+    uint64_t slot = inside ? p.sequence_slots[start + tok] : 0;
+    const bool ok = inside && slot < p.slot_count;
+    if (inside && !ok) {
+        if (report) atomicOr(p.flag, SGLKV_FLAG_ATTN_SLOT);
+        slot = 0;
+    }
+    uint64_t page, pos;
+    attn_split_slot(p, slot, &page, &pos);
+    *row = kbase + page * p.page_stride + pos * p.key_token_stride;
+    return ok;
+}
+
+// ---- Statistics -------------------------------------------------------------
+//
+// One wave per (query, KV head, 16 query heads, split); 32 tokens a step, K
+// rows as the A operand of the matrix product, queries (from LDS) as B, so lane
+// (g, r) gets tokens 4g .. 4g+3 of each 16 for head r and keeps a running
+// (maximum, sum) of its own; the four lanes of a head join at the end.
+template <bool VEC>
+__device__ __forceinline__ void wgt_stats_body(const sglkv_weights_params &p) {
+    extern __shared__ __attribute__((aligned(16))) uint16_t wgt_lds[];
+    const sglkv_attn_params &a = p.a;
+    const uint32_t lane = threadIdx.x, g = lane >> 4, r = lane & 15;
+    uint32_t bx = blockIdx.x;
+    const uint32_t hg = bx % a.head_groups;
+    bx /= a.head_groups;
+    attn_work w;
+    w.kvh = bx % a.kv_heads;
+    w.q = bx / a.kv_heads;
+    w.h0 = w.kvh * a.group + hg * SGLKV_ATTN_HEADS;
+    w.nh = a.group - hg * SGLKV_ATTN_HEADS < SGLKV_ATTN_HEADS ? a.group - hg * SGLKV_ATTN_HEADS : SGLKV_ATTN_HEADS;
+    uint64_t start, len;
+    const bool live =
+        wgt_query(p, w.q, lane == 0 && hg == 0 && w.kvh == 0 && blockIdx.y == 0, &start, &len);
+    const uint64_t t0 = static_cast<uint64_t>(blockIdx.y) * a.chunk_tokens;
+    float m = -INFINITY, l = 0.0f;
+    if (live && t0 < len) {
+        const uint64_t t1 = len < t0 + a.chunk_tokens ? len : t0 + a.chunk_tokens;
+        const uint32_t qstride = a.dk_pad + 8;
+        attn_stage_queries(a, w, lane, wgt_lds, qstride);
+        const uint64_t kbase = reinterpret_cast<uint64_t>(a.pool) + a.key_offset + w.kvh * a.key_head_stride;
+        m = -3.402823466e+38f;
+        for (uint64_t tb = t0; tb < t1; tb += 32) {
+            uint64_t row[2];
+            bool ok[2];
+#pragma unroll
+            for (uint32_t b = 0; b < 2; ++b)
+                ok[b] = wgt_row(a, kbase, start, tb + 16 * b + r, tb + 16 * b + r < t1, w.kvh == 0, &row[b]);
+            sglkv_f32x4 sc[2] = {sglkv_f32x4{0.f, 0.f, 0.f, 0.f}, sglkv_f32x4{0.f, 0.f, 0.f, 0.f}};
+            for (uint32_t kk = 0; kk < a.dk_pad; kk += 32) {
+                const sglkv_u16x8 qv = *reinterpret_cast<const sglkv_u16x8 *>(wgt_lds + r * qstride + kk + 8 * g);
+#pragma unroll
+                for (uint32_t b = 0; b < 2; ++b)
+                    sc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                        attn_as_bf16(attn_load8<VEC>(row[b], kk + 8 * g, a.dk, ok[b])), attn_as_bf16(qv), sc[b], 0, 0, 0);
+            }
+#pragma unroll
+            for (uint32_t b = 0; b < 2; ++b) {
+                const uint64_t valid = __ballot(ok[b]);
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) {
+                    const float x = (valid >> (4 * g + e)) & 1 ? sc[b][e] * a.scale_log2 : -INFINITY;
+                    const float m_new = fmaxf(m, x);
+                    l = l * exp2f(m - m_new) + exp2f(x - m_new);
+                    m = m_new;
+                }
+            }
+        }
+#pragma unroll
+        for (uint32_t s = 16; s < 64; s <<= 1) {
+            const float mo = __shfl_xor(m, s), lo = __shfl_xor(l, s), m_new = fmaxf(m, mo);
+            l = l * exp2f(m - m_new) + lo * exp2f(mo - m_new);
+            m = m_new;
+        }
+    }
+    if (g == 0 && r < w.nh) wgt_stats(p, w.q, w.h0 + r)[blockIdx.y] = make_float2(m, l);
+}
+
+// ---- Accumulation -----------------------------------------------------------
+//
+// One wave per (request, KV head, 64 tokens): for each of the request's
+// queries, 16 heads at a time, the scores again, and their weights added to the
+// lane's tokens; the 16 lanes of a token join at the end.
+template <bool VEC>
+__device__ __forceinline__ void wgt_accumulate_body(const sglkv_weights_params &p) {
+    const sglkv_attn_params &a = p.a;
+    const uint32_t lane = threadIdx.x, g = lane >> 4, r = lane & 15;
+    const uint32_t tile = blockIdx.x % p.tiles;
+    const uint32_t item = blockIdx.x / p.tiles, kvh = item % a.kv_heads, req = item / a.kv_heads;
+    const uint64_t start = a.request_slot_offsets[req], end = a.request_slot_offsets[req + 1];
+    const uint64_t tb = static_cast<uint64_t>(tile) * SGLKV_WEIGHTS_TILE;
+    if (start > end || end > a.sequence_slot_count || tb >= end - start) return;
+    // The request's queries.
+    auto first_of = [&](uint32_t key) {
+        uint64_t low = 0, high = a.query_count;
+        while (low < high) {
+            const uint64_t mid = low + (high - low) / 2;
+            if (a.query_request_indices[mid] < key)
+                low = mid + 1;
+            else
+                high = mid;
+        }
+        return low;
+    };
+    const uint64_t q0 = first_of(req), q1 = first_of(req + 1);
+    // The tokens that any of them attends.
+    auto length_of = [&](uint64_t q) {
+        const uint64_t n = a.query_sequence_lengths[q];
+        return n <= end - start && n <= p.max_length && a.query_request_indices[q] == req ? n : 0;
+    };
+    uint64_t longest = 0;
+    for (uint64_t q = q0 + lane; q < q1; q += 64) {
+        const uint64_t n = length_of(q);
+        longest = n > longest ? n : longest;
+    }
+#pragma unroll
+    for (uint32_t s = 1; s < 64; s <<= 1) {
+        const uint64_t n = __shfl_xor(longest, s);
+        longest = n > longest ? n : longest;
+    }
+    if (tb >= longest) return;
+    const uint64_t kbase = reinterpret_cast<uint64_t>(a.pool) + a.key_offset + kvh * a.key_head_stride;
+    // Lane (g, r) loads token 16 b + r's row and weighs tokens 16 b + 4 g .. + 3.
+    // (A token whose slot is no slot of the pool has been reported.)
+    uint64_t row[4];
+    uint32_t ok = 0;
+#pragma unroll
+    for (uint32_t b = 0; b < 4; ++b) {
+        const uint64_t tok = tb + 16 * b + r;
+        ok |= (wgt_row(a, kbase, start, tok, tok < longest, false, &row[b]) ? 1u : 0u) << b;
+    }
+    float sum[4][4] = {};
+    for (uint64_t q = q0; q < q1; ++q) {
+        const uint64_t len = length_of(q);
+        if (len <= tb) continue;
+        for (uint32_t h0 = 0; h0 < a.group; h0 += 16) {
+            const bool head = h0 + r < a.group;
+            const uint64_t hi = static_cast<uint64_t>(kvh) * a.group + (head ? h0 + r : 0);
+            // This lane's head: the softmax statistics of its splits joined.
+            const float2 *stats = wgt_stats(p, q, hi);
+            float m = -INFINITY, l = 0.0f;
+            for (uint32_t s = 0; s < a.splits; ++s) m = fmaxf(m, stats[s].x);
+            for (uint32_t s = 0; s < a.splits; ++s)
+                if (stats[s].x != -INFINITY) l += stats[s].y * exp2f(stats[s].x - m);
+            const bool weighs = head && m != -INFINITY;
+            const float inv = weighs ? 1.0f / l : 0.0f;
+            const uint32_t limit = !weighs ? 0 : len - tb < 64 ? static_cast<uint32_t>(len - tb) : 64;
+            const uint64_t qrow = reinterpret_cast<uint64_t>(a.queries + (q * a.query_heads + hi) * a.dk);
+            sglkv_f32x4 sc[4];
+#pragma unroll
+            for (uint32_t b = 0; b < 4; ++b) sc[b] = sglkv_f32x4{0.f, 0.f, 0.f, 0.f};
+            for (uint32_t kk = 0; kk < a.dk_pad; kk += 32) {
+                const sglkv_u16x8 qv = attn_load8<VEC>(qrow, kk + 8 * g, a.dk, head);
+#pragma unroll
+                for (uint32_t b = 0; b < 4; ++b)
+                    sc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                        attn_as_bf16(attn_load8<VEC>(row[b], kk + 8 * g, a.dk, (ok >> b) & 1)), attn_as_bf16(qv), sc[b], 0, 0,
+                        0);
+            }
+#pragma unroll
+            for (uint32_t b = 0; b < 4; ++b)
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) {
+                    const bool in = 16 * b + 4 * g + e < limit;
+                    const float x = in ? fmaf(sc[b][e], a.scale_log2, -m) : -INFINITY;
+                    sum[b][e] = fmaf(exp2f(x), in ? inv : 0.0f, sum[b][e]);
+                }
+        }
+    }
+#pragma unroll
+    for (uint32_t b = 0; b < 4; ++b)
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) {
+            float x = sum[b][e];
+#pragma unroll
+            for (uint32_t s = 1; s < 16; s <<= 1) x += __shfl_xor(x, s);
+            const uint64_t t = tb + 16 * b + 4 * g + e;
+            if (r == 0 && t < longest) p.weights[kvh * a.sequence_slot_count + start + t] += x;
+        }
+}
+
+// ---- The kept positions -----------------------------------------------------
+
+// A request's slots and length; false (length 0) where its metadata does not
+// hold, which sets the error word when `report`.
+__device__ __forceinline__ uint64_t evt_request(const sglkv_evict_params &p, uint64_t req, bool report, uint64_t *start) {
+    const uint64_t s = p.request_slot_offsets[req], e = p.request_slot_offsets[req + 1], n = p.request_lengths[req];
+    *start = s;
+    if (s <= e && e <= p.sequence_slot_count && n <= e - s && n <= p.max_length) return n;
+    if (report) atomicOr(p.flag, SGLKV_FLAG_ATTN_SEQUENCE);
+    return 0;
+}
+
+// Keys that order as the sums do: NaN above every number, and above it the
+// positions that are always kept.
+__device__ __forceinline__ uint32_t evt_key(float x) {
+    if (x != x) return ~0u - 1;
+    const uint32_t b = __float_as_uint(x + 0.0f);  // (-0 is 0)
+    return b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | (1u << 31));
+}
+
+__device__ __forceinline__ void evt_select_body(const sglkv_evict_params &p) {
+    __shared__ sel_pick_state state;
+    const uint32_t head = blockIdx.x % p.heads;
+    const uint64_t req = blockIdx.x / p.heads;
+    uint64_t start;
+    const uint64_t len = evt_request(p, req, head == 0 && threadIdx.x == 0, &start);
+    const float *weights = p.weights + head * p.sequence_slot_count + start;
+    sel_pick<uint32_t, SGLKV_EVICT_THREADS / 64>(
+        len, p.max_kept,
+        [&](uint64_t i) { return i < p.first_tokens || i + p.last_tokens >= len ? ~0u : evt_key(weights[i]); },
+        p.kept + (req * p.heads + head) * p.max_kept, state);
+}
+
+// ---- The copy ---------------------------------------------------------------
+//
+// A workgroup copies p.rows destination rows of a request for block_heads heads
+// of one tensor (grid y: head blocks, z: tensors). It resolves each (row,
+// head)'s kept position to the two addresses once, into LDS; then `lanes`
+// threads move a head chunk, W bytes each, U chunks in flight.
+template <typename V>
+__device__ __forceinline__ void evt_compact_body(const sglkv_evict_params &p) {
+    typedef __attribute__((address_space(1))) const V src_t;
+    typedef __attribute__((address_space(1))) V dst_t;
+    __shared__ uint64_t from[SGLKV_COMPACT_CHUNKS], to[SGLKV_COMPACT_CHUNKS];
+    constexpr uint32_t U = 8;
+    const uint32_t tid = threadIdx.x, tensor = blockIdx.z;
+    const uint32_t tile = blockIdx.x % p.row_tiles;
+    const uint64_t req = blockIdx.x / p.row_tiles;
+    const uint32_t h0 = blockIdx.y * p.block_heads, heads = p.heads - h0 < p.block_heads ? p.heads - h0 : p.block_heads;
+    uint64_t start;
+    const bool report = tile == 0 && h0 == 0 && tensor == 0 && tid == 0;
+    if (report && req == 0 && p.scale_dst)
+        for (uint32_t t = 0; t < p.tensors; ++t) p.scale_dst[t] = p.scale_src[t];
+    const uint64_t len = evt_request(p, req, report, &start);
+    const uint64_t d0 = p.to_offsets[req], d1 = p.to_offsets[req + 1];
+    const bool ranged = d0 <= d1 && d1 <= p.to_slot_count;
+    if (!ranged) {
+        if (report) atomicOr(p.flag, SGLKV_FLAG_ATTN_SEQUENCE);
+        return;
+    }
+    const uint64_t room = d1 - d0, r0 = static_cast<uint64_t>(tile) * p.rows;
+    // Positions of the destination that no list reaches: their sums begin at 0.
+    if (p.to_weights && tensor == 0)
+        for (uint64_t row = p.max_kept + r0; row < room; row += static_cast<uint64_t>(p.row_tiles) * p.rows)
+            for (uint32_t i = tid; i < p.rows * heads; i += SGLKV_COMPACT_THREADS) {
+                const uint32_t h = i / p.rows, j = i - h * p.rows;
+                if (row + j < room) p.to_weights[(h0 + h) * p.to_slot_count + d0 + row + j] = 0.0f;
+            }
+    const uint32_t rows = p.max_kept - r0 < p.rows ? static_cast<uint32_t>(p.max_kept - r0) : p.rows;
+    // One head's rows side by side: the lists and sums are read in runs.
+    for (uint32_t i = tid; i < rows * heads; i += SGLKV_COMPACT_THREADS) {
+        const uint32_t h = i / rows, j = i - h * rows;
+        const uint64_t row = r0 + j;
+        const uint32_t *list = p.kept + (req * p.heads + h0 + h) * p.max_kept;
+        const uint32_t kept = list[row];
+        uint64_t src = SGLKV_INVALID_OFFSET, dst = SGLKV_INVALID_OFFSET;
+        float weight = 0.0f;
+        if (kept != SGLKV_SELECT_NONE) {
+            if (kept >= len || row >= room) {
+                atomicOr(p.flag, SGLKV_FLAG_ATTN_SEQUENCE);
+            } else {
+                const uint64_t s = p.sequence_slots[start + kept], d = p.to_slots[d0 + row];
+                if (s >= p.src.slot_count || d >= p.dst.slot_count) {
+                    atomicOr(p.flag, SGLKV_FLAG_ATTN_SLOT);
+                } else {
+                    const uint32_t sp = static_cast<uint32_t>(s) / p.src.page_size, dp = static_cast<uint32_t>(d) / p.dst.page_size;
+                    src = p.src.plane[tensor] + sp * p.src.stride[tensor] +
+                          (static_cast<uint32_t>(s) - sp * p.src.page_size) * p.src.pos_mult[tensor] +
+                          (h0 + h) * p.src.head_stride[tensor];
+                    dst = p.dst.plane[tensor] + dp * p.dst.stride[tensor] +
+                          (static_cast<uint32_t>(d) - dp * p.dst.page_size) * p.dst.pos_mult[tensor] +
+                          (h0 + h) * p.dst.head_stride[tensor];
+                }
+                if (p.to_weights && tensor == 0) weight = p.weights[(h0 + h) * p.sequence_slot_count + start + kept];
+            }
+        }
+        from[j * heads + h] = src;
+        to[j * heads + h] = dst;
+        if (p.to_weights && tensor == 0 && row < room) p.to_weights[(h0 + h) * p.to_slot_count + d0 + row] = weight;
+    }
+    __syncthreads();
+    const uint32_t lanes = p.lanes[tensor], vectors = p.vectors[tensor], side = SGLKV_COMPACT_THREADS / lanes;
+    const uint32_t v0 = tid % lanes, chunks = rows * heads;
+    for (uint32_t c0 = tid / lanes; c0 < chunks; c0 += side * U)
+        for (uint32_t v = v0; v < vectors; v += lanes) {
+            V x[U];
+            uint64_t at[U];
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u) {
+                const uint32_t c = c0 + side * u;
+                const uint64_t s = c < chunks ? from[c] : SGLKV_INVALID_OFFSET;
+                at[u] = c < chunks ? to[c] : SGLKV_INVALID_OFFSET;
+                if (s != SGLKV_INVALID_OFFSET) x[u] = *reinterpret_cast<src_t *>(s + v * sizeof(V));
+            }
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u)
+                if (at[u] != SGLKV_INVALID_OFFSET) *reinterpret_cast<dst_t *>(at[u] + v * sizeof(V)) = x[u];
+        }
+}
+
+}  // namespace
+
+extern "C" __global__ __launch_bounds__(64) void sglkv_weight_stats_v16(sglkv_weights_params p) { wgt_stats_body<true>(p); }
+extern "C" __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void
+sglkv_weight_stats_v2(sglkv_weights_params p) {
+    wgt_stats_body<false>(p);
+}
+extern "C" __global__ __launch_bounds__(64) void sglkv_accumulate_weights_v16(sglkv_weights_params p) {
+    wgt_accumulate_body<true>(p);
+}
+extern "C" __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void
+sglkv_accumulate_weights_v2(sglkv_weights_params p) {
+    wgt_accumulate_body<false>(p);
+}
+
+extern "C" __global__ __launch_bounds__(SGLKV_EVICT_THREADS) void sglkv_select_tokens(sglkv_evict_params p) {
+    evt_select_body(p);
+}
+
+extern "C" __global__ __launch_bounds__(SGLKV_COMPACT_THREADS) void sglkv_compact_tokens_v16(sglkv_evict_params p) {
+    evt_compact_body<sglkv_v4u>(p);
+}
+extern "C" __global__ __launch_bounds__(SGLKV_COMPACT_THREADS) void sglkv_compact_tokens_v4(sglkv_evict_params p) {
+    evt_compact_body<uint32_t>(p);
+}
+extern "C" __global__ __launch_bounds__(SGLKV_COMPACT_THREADS) void sglkv_compact_tokens_v2(sglkv_evict_params p) {
+    evt_compact_body<uint16_t>(p);
+}
+extern "C" __global__ __launch_bounds__(SGLKV_COMPACT_THREADS) void sglkv_compact_tokens_v1(sglkv_evict_params p) {
+    evt_compact_body<uint8_t>(p);
+}

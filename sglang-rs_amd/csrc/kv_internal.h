@@ -116,6 +116,12 @@ int32_t check_device(const sgl_rocm_kv_ctx *ctx, const char *name, const sgl_kv_
 
 // A pool view by itself: its dimensions, regions and allocation.
 int32_t check_pool_view(const sgl_kv_pool_view *view);
+// The same for a view whose rows are moved head by head, and its kernel side
+// (slots unset).
+int32_t pool_heads_side(const sgl_kv_pool_view *view, sglkv_side *out);
+// One kernel launch on `s`; `what` names it in an error.
+int32_t launch_kernel(hipFunction_t f, uint64_t grid_x, uint64_t grid_y, uint64_t grid_z, unsigned threads, unsigned lds,
+                      hipStream_t s, void *params, const char *what);
 
 #define SGLKV_CHECK_HIP(call)                                              \
     do {                                                                   \
@@ -156,6 +162,10 @@ struct sgl_rocm_kv_ctx {
     hipFunction_t pick_pages;
     hipFunction_t selected_attention[2];  // 16-byte vectors, elements
     hipFunction_t selected_combine;
+    hipFunction_t weight_stats[2];        // 16-byte vectors, elements
+    hipFunction_t accumulate_weights[2];
+    hipFunction_t select_tokens;
+    hipFunction_t compact_tokens[4];      // pieces of 16, 4, 2 and 1 bytes
     uint32_t attention_occupancy[15];     // resident workgroups per CU of attention[i] ...
     uint32_t attention_occupancy_lds[15]; // ... at this LDS size (0 = not yet queried)
     int max_lds_per_block;                // device limit on a workgroup's LDS bytes

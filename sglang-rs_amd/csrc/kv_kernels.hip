@@ -793,3 +793,6 @@ extern "C" __global__ __launch_bounds__(SGLKV_BLOCK_THREADS) void sglkv_stream_w
 
 // Page selection and the attention over selected pages.
 #include "kv_select.hip"
+
+// Eviction from a cache by accumulated attention weight.
+#include "kv_evict.hip"

@@ -413,6 +413,52 @@ typedef struct sglkv_select_params {
     uint32_t heads;           /* select: KV heads * chunks of a query (scores), or KV heads */
 } sglkv_select_params;
 
+/* The softmax weights that each position of a sequence gets, summed over the
+ * queries: weights[kv head][position] += ..., positions numbered as
+ * sequence_slots. `a` as for paged attention; its partial holds a (maximum, sum)
+ * pair of 32-bit floats per (query, head, split), in log2 units. */
+#define SGLKV_WEIGHTS_TILE 64u /* tokens per wave of the accumulation */
+typedef struct sglkv_weights_params {
+    sglkv_attn_params a;
+    float *weights;
+    uint64_t max_length;      /* the longest query length that the launch covers */
+    uint32_t tiles;           /* SGLKV_WEIGHTS_TILE-token tiles of a sequence of max_length */
+    uint32_t reserved;
+} sglkv_weights_params;
+
+/* The positions of each (request, KV head) that are kept, and their rows' and
+ * sums' copy. */
+#define SGLKV_EVICT_THREADS 1024u       /* of a choosing workgroup */
+#define SGLKV_COMPACT_THREADS 256u
+#define SGLKV_COMPACT_CHUNKS 1024u      /* (row, head)s that a copying workgroup resolves: 16 bytes of LDS each */
+typedef struct sglkv_evict_params {
+    const uint64_t *request_lengths;
+    const uint64_t *request_slot_offsets;
+    const uint64_t *sequence_slots;
+    const float *weights;               /* [kv head][sequence_slot_count] */
+    uint32_t *kept;                     /* [request][kv head][max_kept] positions, ascending */
+    const uint64_t *to_offsets;         /* request_count + 1, into to_slots and to_weights */
+    const uint64_t *to_slots;
+    float *to_weights;                  /* [kv head][to_slot_count], or null */
+    uint32_t *flag;
+    const float *scale_src;             /* optional: the layer's quantisation scales, copied along */
+    float *scale_dst;
+    uint64_t request_count;
+    uint64_t sequence_slot_count;
+    uint64_t to_slot_count;
+    uint64_t max_length;
+    sglkv_side src, dst;                /* pool sides; their slots are unused */
+    uint32_t heads;
+    uint32_t max_kept;
+    uint32_t first_tokens, last_tokens;
+    uint32_t tensors;
+    uint32_t vectors[2];                /* access-sized pieces of tensor t's head chunk */
+    uint32_t lanes[2];                  /* threads to a chunk: a power of two, at most SGLKV_COMPACT_THREADS */
+    uint32_t rows;                      /* destination rows of a copying workgroup */
+    uint32_t row_tiles;                 /* workgroups of a request */
+    uint32_t block_heads;               /* heads of a copying workgroup */
+} sglkv_evict_params;
+
 /* Bytes of zeros the context keeps for reads that must contribute nothing
  * (>= the widest row piece a pipelined attention lane reads, 256 B). */
 #define SGLKV_ZERO_ROW_BYTES 1024u

@@ -353,14 +353,42 @@ int32_t validate_device(const sgl_rocm_kv_ctx *ctx, const char *name, const sgl_
 
 }  // namespace
 
-int32_t sglkv::check_pool_view(const sgl_kv_pool_view *view) {
-    int32_t rc = check_pool_shape(view);
-    if (rc) return rc;
-    // (The rules of a copy's pool side, for a copy of no rows.)
+namespace {
+
+// A pool side by the rules of a copy, for a copy of no rows.
+int32_t bare_side(const sgl_kv_pool_view *view, bool split, sglkv_side *out) {
     static const uint64_t none = 0;
     const sgl_kv_device_buffer slots = {const_cast<uint64_t *>(&none), sizeof none};
+    return pool_side(view, &slots, 0, shape_of(*view, split, view->heads), out);
+}
+
+}  // namespace
+
+int32_t sglkv::check_pool_view(const sgl_kv_pool_view *view) {
     sglkv_side side;
-    return pool_side(view, &slots, 0, shape_of(*view, view->head_layout == SGL_KV_HND, view->heads), &side);
+    const int32_t rc = check_pool_shape(view);
+    return rc ? rc : bare_side(view, view->head_layout == SGL_KV_HND, &side);
+}
+
+int32_t sglkv::pool_heads_side(const sgl_kv_pool_view *view, sglkv_side *out) {
+    int32_t rc = check_pool_shape(view);
+    if (rc) return rc;
+    for (uint32_t t = 0; t < view->tensor_count; ++t)
+        if (view_row_bytes(*view, t) % view->heads)
+            return fail(SGL_KV_INVALID_ARGUMENT, "heads", view->heads, view_row_bytes(*view, t), 0,
+                        "%u heads do not split a %llu-byte row evenly", view->heads,
+                        (unsigned long long)view_row_bytes(*view, t));
+    rc = bare_side(view, true, out);
+    out->slots = nullptr;
+    return rc;
+}
+
+int32_t sglkv::launch_kernel(hipFunction_t f, uint64_t grid_x, uint64_t grid_y, uint64_t grid_z, unsigned threads,
+                             unsigned lds, hipStream_t s, void *params, const char *what) {
+    void *args[] = {params};
+    const hipError_t err = hipModuleLaunchKernel(f, (unsigned)grid_x, (unsigned)grid_y, (unsigned)grid_z, threads, 1, 1, lds,
+                                                 s, args, nullptr);
+    return err == hipSuccess ? SGL_KV_OK : hip_fail(err, what);
 }
 
 int32_t sglkv::check_device(const sgl_rocm_kv_ctx *ctx, const char *name, const sgl_kv_device_buffer &b) {
@@ -552,7 +580,16 @@ extern "C" int32_t sgl_rocm_kv_init(int32_t device, const char *code_object_path
                      {"sglkv_pick_pages", &ctx->pick_pages},
                      {"sglkv_selected_attention_v16", &ctx->selected_attention[0]},
                      {"sglkv_selected_attention_v2", &ctx->selected_attention[1]},
-                     {"sglkv_selected_attention_combine", &ctx->selected_combine}};
+                     {"sglkv_selected_attention_combine", &ctx->selected_combine},
+                     {"sglkv_weight_stats_v16", &ctx->weight_stats[0]},
+                     {"sglkv_weight_stats_v2", &ctx->weight_stats[1]},
+                     {"sglkv_accumulate_weights_v16", &ctx->accumulate_weights[0]},
+                     {"sglkv_accumulate_weights_v2", &ctx->accumulate_weights[1]},
+                     {"sglkv_select_tokens", &ctx->select_tokens},
+                     {"sglkv_compact_tokens_v16", &ctx->compact_tokens[0]},
+                     {"sglkv_compact_tokens_v4", &ctx->compact_tokens[1]},
+                     {"sglkv_compact_tokens_v2", &ctx->compact_tokens[2]},
+                     {"sglkv_compact_tokens_v1", &ctx->compact_tokens[3]}};
     for (const auto &f : selection)
         if (err == hipSuccess) err = hipModuleGetFunction(f.function, ctx->module, f.name);
     if (err == hipSuccess) err = hipDeviceGetAttribute(&ctx->cu_count, hipDeviceAttributeMultiprocessorCount, device);

@@ -168,14 +168,6 @@ int32_t selection_params(sgl_rocm_kv_ctx *ctx, const sgl_kv_page_selection_plan 
 // not: 8, 16, 32 or 64 lanes to a row, or the element-wise one.
 int row_lanes(uint64_t dims, bool vector) { return !vector ? 4 : dims <= 64 ? 0 : dims <= 128 ? 1 : dims <= 256 ? 2 : 3; }
 
-int32_t launch(hipFunction_t f, uint64_t grid_x, uint64_t grid_y, unsigned threads, unsigned lds, hipStream_t s,
-               void *params, const char *what) {
-    void *args[] = {params};
-    const hipError_t err =
-        hipModuleLaunchKernel(f, (unsigned)grid_x, (unsigned)grid_y, 1, threads, 1, 1, lds, s, args, nullptr);
-    return err == hipSuccess ? SGL_KV_OK : hip_fail(err, what);
-}
-
 }  // namespace
 
 extern "C" int32_t sgl_kv_page_selection_plan_new(const sgl_kv_attention_plan *attention,
@@ -258,7 +250,7 @@ extern "C" int32_t sgl_rocm_kv_page_bounds(sgl_rocm_kv_ctx *ctx, const sgl_kv_po
                         ((base + p.key_offset) | p.page_stride | p.key_head_stride | p.key_token_stride) % 16 == 0;
     DeviceScope scope(ctx->device);
     if (scope.status() != hipSuccess) return hip_fail(scope.status(), "hipSetDevice");
-    rc = launch(ctx->page_bounds[row_lanes(dims, vector)], ceil_div(items, 4), 1, 256, 0, static_cast<hipStream_t>(stream),
+    rc = launch_kernel(ctx->page_bounds[row_lanes(dims, vector)], ceil_div(items, 4), 1, 1, 256, 0, static_cast<hipStream_t>(stream),
                 &p, "page bounds launch");
     return rc ? rc : ok();
 }
@@ -276,14 +268,14 @@ extern "C" int32_t sgl_rocm_kv_select_pages(sgl_rocm_kv_ctx *ctx, const sgl_kv_p
         const bool vector = p.a.dk % 8 == 0 && reinterpret_cast<uint64_t>(p.bounds) % 16 == 0;
         p.chunk_pages = (uint32_t)shape.chunk_pages;
         p.heads = p.a.kv_heads * (uint32_t)shape.chunks;
-        rc = launch(ctx->page_scores[row_lanes(p.a.dk, vector)], shape.items * shape.chunks, 1, SGLKV_SELECT_THREADS,
+        rc = launch_kernel(ctx->page_scores[row_lanes(p.a.dk, vector)], shape.items * shape.chunks, 1, 1, SGLKV_SELECT_THREADS,
                     2 * p.a.group * SGLKV_SELECT_QSTRIDE(p.a.dk), s, &p, "page scores launch");
         if (rc) return rc;
     }
     const uint64_t kept = shape.key_bytes == 0                                ? 0
                           : shape.sequence_pages < SGLKV_SELECT_LDS_PAGES     ? shape.sequence_pages
                                                                               : SGLKV_SELECT_LDS_PAGES;
-    rc = launch(ctx->pick_pages, shape.items, 1, SGLKV_SELECT_THREADS, (unsigned)(8 * kept), s, &p, "page pick launch");
+    rc = launch_kernel(ctx->pick_pages, shape.items, 1, 1, SGLKV_SELECT_THREADS, (unsigned)(8 * kept), s, &p, "page pick launch");
     return rc ? rc : ok();
 }
 
@@ -304,10 +296,10 @@ extern "C" int32_t sgl_rocm_kv_selected_attention(sgl_rocm_kv_ctx *ctx, const sg
                                 16 == 0;
     p.chunk_pages = (uint32_t)shape.split_pages;
     const unsigned lds = 2 * (SGLKV_ATTN_HEADS * (p.a.dk_pad + 8) + SGLKV_ATTN_DV * SGLKV_ATTN_VT_STRIDE);
-    rc = launch(ctx->selected_attention[vector ? 0 : 1], shape.items * p.a.head_groups * p.a.dv_blocks, p.a.splits, 64, lds,
+    rc = launch_kernel(ctx->selected_attention[vector ? 0 : 1], shape.items * p.a.head_groups * p.a.dv_blocks, p.a.splits, 1, 64, lds,
                 s, &p, "selected attention launch");
     if (!rc && p.a.splits > 1)
-        rc = launch(ctx->selected_combine, p.a.query_count * p.a.query_heads, 1, 64, 0, s, &p,
+        rc = launch_kernel(ctx->selected_combine, p.a.query_count * p.a.query_heads, 1, 1, 64, 0, s, &p,
                     "selected attention combine launch");
     return rc ? rc : ok();
 }

@@ -339,6 +339,35 @@ class _PageSelectionBuffers(ctypes.Structure):
                                                      for f in ((n, _DeviceBuffer), (n + "_offset", _u64))]
 
 
+class _WeightPlan(ctypes.Structure):
+    _fields_ = [("attention", _AttentionPlan)] + [
+        (n, _u64) for n in ("max_sequence_length", "weights_required_bytes", "workspace_required_bytes")]
+
+
+class _WeightBuffers(ctypes.Structure):
+    _fields_ = [("attention", _AttentionBuffers)] + [f for n in ("weights", "workspace")
+                                                     for f in ((n, _DeviceBuffer), (n + "_offset", _u64))]
+
+
+class _EvictionConfig(ctypes.Structure):
+    _fields_ = [(n, _u64) for n in ("request_count", "kv_head_count", "sequence_slot_count", "destination_slot_count",
+                                    "max_kept", "first_tokens", "last_tokens", "max_sequence_length")]
+
+
+class _EvictionPlan(ctypes.Structure):
+    _fields_ = [("config", _EvictionConfig)] + [
+        (n + "_required_bytes", _u64) for n in ("request_lengths", "request_slot_offsets", "sequence_slots", "weights",
+                                                "kept", "destination_slots", "destination_weights", "workspace")]
+
+
+_EVICTION_BUFFERS = ("request_lengths", "request_slot_offsets", "sequence_slots", "weights", "kept",
+                     "destination_slot_offsets", "destination_slots", "destination_weights", "workspace")
+
+
+class _EvictionBuffers(ctypes.Structure):
+    _fields_ = [f for n in _EVICTION_BUFFERS for f in ((n, _DeviceBuffer), (n + "_offset", _u64))]
+
+
 # SGL_KV_ATTN_BODY_*, by value
 ATTENTION_BODIES = ("vector", "element", "pipe128", "pipe", "wide576", "wide128", "latent", "staged128", "staged64",
                     "latent_exact", "staged256", "staged128k", "tile128", "tile64", "tile256")
@@ -549,6 +578,15 @@ _EXPORTS = {
                                                                    ctypes.POINTER(_AttentionPlan),
                                                                    ctypes.POINTER(_AttentionBuffers), _u64,
                                                                    ctypes.c_void_p]),
+    "sgl_kv_weight_plan_new": (ctypes.c_int32, [ctypes.POINTER(_AttentionPlan), _u64, ctypes.POINTER(_WeightPlan)]),
+    "sgl_rocm_kv_accumulate_weights": (ctypes.c_int32, [ctypes.c_void_p, ctypes.POINTER(_WeightPlan),
+                                                        ctypes.POINTER(_WeightBuffers), ctypes.c_void_p]),
+    "sgl_kv_eviction_plan_new": (ctypes.c_int32, [ctypes.POINTER(_EvictionConfig), ctypes.POINTER(_EvictionPlan)]),
+    "sgl_rocm_kv_select_tokens": (ctypes.c_int32, [ctypes.c_void_p, ctypes.POINTER(_EvictionPlan),
+                                                   ctypes.POINTER(_EvictionBuffers), ctypes.c_void_p]),
+    "sgl_rocm_kv_compact_tokens": (ctypes.c_int32, [ctypes.c_void_p, ctypes.POINTER(_EvictionPlan),
+                                                    ctypes.POINTER(_EvictionBuffers), ctypes.POINTER(PoolView),
+                                                    ctypes.POINTER(PoolView), ctypes.c_void_p]),
     "sgl_kv_page_selection_plan_new": (ctypes.c_int32, [ctypes.POINTER(_AttentionPlan),
                                                         ctypes.POINTER(_PageSelectionConfig),
                                                         ctypes.POINTER(_PageSelectionPlan)]),
@@ -1378,6 +1416,29 @@ class RocmKvPairCopyKernels:
         _call(lib().sgl_rocm_kv_selected_attention, self._h, ctypes.byref(plan._c), ctypes.byref(buffers._c),
               _stream(stream))
 
+    def accumulate_weights(self, plan: "WeightAccumulationPlan", buffers: "WeightAccumulationBuffers", *,
+                           stream=None):
+        """Adds the softmax weight that each position gets from the plan's
+        queries to `weights` (f32 [KV head][sequence_slot_count]).
+        Asynchronous."""
+        _call(lib().sgl_rocm_kv_accumulate_weights, self._h, ctypes.byref(plan._c), ctypes.byref(buffers._c),
+              _stream(stream))
+
+    def select_tokens(self, plan: "EvictionPlan", buffers: "EvictionBuffers", *, stream=None):
+        """The max_kept positions of each (request, KV head) with the largest
+        `weights`, into `kept` (u32 [request][KV head][max_kept], ascending,
+        UINT32_MAX behind them). Asynchronous."""
+        _call(lib().sgl_rocm_kv_select_tokens, self._h, ctypes.byref(plan._c), ctypes.byref(buffers._c),
+              _stream(stream))
+
+    def compact_tokens(self, plan: "EvictionPlan", buffers: "EvictionBuffers", source: PoolView,
+                       destination: PoolView, *, stream=None):
+        """Copies the `kept` positions' rows of one layer, head by head, from
+        `sequence_slots` of `source` to `destination_slots` of `destination`,
+        and their weights. Asynchronous."""
+        _call(lib().sgl_rocm_kv_compact_tokens, self._h, ctypes.byref(plan._c), ctypes.byref(buffers._c),
+              ctypes.byref(source), ctypes.byref(destination), _stream(stream))
+
     def check_errors(self, stream=None):
         _call(lib().sgl_rocm_kv_check_errors, self._h, _stream(stream))
 
@@ -1995,6 +2056,83 @@ class PageSelectionBuffers:
         self._given = buffers
         rest = _fill_buffers(self._c.attention, _ATTENTION_BUFFERS, buffers)
         rest = _fill_buffers(self._c, ("bounds", "selected", "workspace"), rest)
+        if rest:
+            raise TypeError(f"unknown buffers: {', '.join(sorted(rest))}")
+
+
+class WeightAccumulationPlan:
+    """What accumulate_weights needs to know: the attention plan of the queries
+    and the longest query length (0: as many as the plan's slots)."""
+
+    def __init__(self, c: _WeightPlan):
+        self._c = c
+
+    @classmethod
+    def new(cls, attention: PagedAttentionPlan, *, max_sequence_length: int = 0) -> "WeightAccumulationPlan":
+        out = _WeightPlan()
+        _call(lib().sgl_kv_weight_plan_new, ctypes.byref(attention._c), max_sequence_length, ctypes.byref(out))
+        return cls(out)
+
+    @property
+    def attention(self) -> PagedAttentionPlan:
+        return PagedAttentionPlan(self._c.attention)
+
+    def __getattr__(self, name):
+        c = self.__dict__["_c"]
+        if hasattr(c, name):
+            return getattr(c, name)
+        raise AttributeError(name)
+
+
+class WeightAccumulationBuffers:
+    """The buffers of accumulate_weights by name, each with an optional
+    <name>_offset: those of paged_attention (without its output), `weights` and
+    `workspace`. It keeps the given objects."""
+
+    def __init__(self, **buffers):
+        self._c = _WeightBuffers()
+        self._given = buffers
+        rest = _fill_buffers(self._c.attention, _ATTENTION_BUFFERS, buffers)
+        rest = _fill_buffers(self._c, ("weights", "workspace"), rest)
+        if rest:
+            raise TypeError(f"unknown buffers: {', '.join(sorted(rest))}")
+
+
+class EvictionPlan:
+    """What select_tokens and compact_tokens need to know: lists of `max_kept`
+    positions, of which a request's `first_tokens` and `last_tokens` are always
+    members, the sizes of the source's and the destination's slot lists, and the
+    longest request (0: as long as the slot list)."""
+
+    def __init__(self, c: _EvictionPlan):
+        self._c = c
+
+    @classmethod
+    def new(cls, *, request_count: int, kv_head_count: int, sequence_slot_count: int, max_kept: int,
+            destination_slot_count: int = 0, first_tokens: int = 0, last_tokens: int = 0,
+            max_sequence_length: int = 0) -> "EvictionPlan":
+        config, out = _EvictionConfig(request_count, kv_head_count, sequence_slot_count, destination_slot_count, max_kept,
+                                      first_tokens, last_tokens, max_sequence_length), _EvictionPlan()
+        _call(lib().sgl_kv_eviction_plan_new, ctypes.byref(config), ctypes.byref(out))
+        return cls(out)
+
+    def __getattr__(self, name):
+        c = self.__dict__["_c"]
+        for part in (c, c.config):
+            if hasattr(part, name) and name != "config":
+                return getattr(part, name)
+        raise AttributeError(name)
+
+
+class EvictionBuffers:
+    """The buffers of select_tokens and compact_tokens by name, each with an
+    optional <name>_offset (sgl_kv_eviction_buffers). It keeps the given
+    objects."""
+
+    def __init__(self, **buffers):
+        self._c = _EvictionBuffers()
+        self._given = buffers
+        rest = _fill_buffers(self._c, _EVICTION_BUFFERS, buffers)
         if rest:
             raise TypeError(f"unknown buffers: {', '.join(sorted(rest))}")
 
