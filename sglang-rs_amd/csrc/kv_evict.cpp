@@ -45,33 +45,88 @@ int32_t resolve(const sgl_rocm_kv_ctx *ctx, const Want (&all)[N]) {
     return SGL_KV_OK;
 }
 
-// The launch shape of accumulate_weights.
+// The launch shape of accumulate_weights. `rows`: the bodies for 16-byte rows of
+// 64, 128 or 256 dims can take it; whether the buffers let them is the call's to
+// see, so the workspace holds what either way needs.
 struct WeightShape {
-    uint64_t max_length, base, chunk, splits, tiles, waves;
+    uint64_t max_length;
+    struct Way {
+        uint64_t base, chunk, splits;  // statistics: workgroups of a split, its tokens
+        uint64_t tiles, groups;        // accumulation: token tiles of a sequence, workgroups
+        uint64_t bytes;                // workspace
+    } any, rows;
+    bool fits;                // `rows` is a way
+    int body;                 // of ctx->weight_rows[dims]: 0 many rows, 1 few, 2 few with their scores
+    uint64_t row_tiles, tile_queries, head_groups, waves;
+    uint64_t stats_bytes, score_stride;
 };
 
-// Waves of the statistics that fill the chip, each with 128 tokens or more.
-constexpr uint64_t kStatsWaves = 2048;
+constexpr uint64_t kMaxWorkgroups = UINT32_MAX / 64;  // of one wave: a dispatch counts its work-items in 32 bits
+
+// Splits of `tokens` that give `waves` waves where `base` are those of one
+// split, each of `least` tokens or more and a multiple of 64.
+void split_tokens(uint64_t tokens, uint64_t base, uint64_t waves, uint64_t least, WeightShape::Way *w) {
+    uint64_t chunk = ceil_div(tokens, base < waves ? waves / base : 1);
+    if (chunk < least) chunk = least;
+    if (chunk < ceil_div(tokens, 65535)) chunk = ceil_div(tokens, 65535);  // grid y
+    w->chunk = ceil_div(chunk, 64) * 64;
+    w->splits = ceil_div(tokens, w->chunk);
+}
 
 int32_t weight_shape(const sgl_kv_attention_plan_config &c, uint64_t max_sequence_length, WeightShape *out) {
     WeightShape &h = *out;
-    if (c.query_key_head_dim > SGLKV_ATTN_MAX_DK)
-        return too_large_dim("query_key_head_dim", c.query_key_head_dim, SGLKV_ATTN_MAX_DK);
+    memset(&h, 0, sizeof h);
+    const uint64_t dk = c.query_key_head_dim, group = c.query_head_count / c.kv_head_count;
+    if (dk > SGLKV_ATTN_MAX_DK) return too_large_dim("query_key_head_dim", dk, SGLKV_ATTN_MAX_DK);
     h.max_length =
         max_sequence_length && max_sequence_length < c.sequence_slot_count ? max_sequence_length : c.sequence_slot_count;
-    const uint64_t groups = ceil_div(c.query_head_count / c.kv_head_count, SGLKV_ATTN_HEADS);
-    if (mul_ovf(c.query_count, c.kv_head_count, &h.base) || mul_ovf(h.base, groups, &h.base)) return attention_overflow();
-    const uint64_t limit = UINT32_MAX / 64;  // a dispatch counts its work-items in 32 bits
-    if (h.base > limit) return too_large_dim("workgroups", h.base, limit);
-    uint64_t chunk = ceil_div(h.max_length, h.base < kStatsWaves ? kStatsWaves / h.base : 1);
-    if (chunk < 128) chunk = 128;
-    const uint64_t least = ceil_div(h.max_length, 65535);  // grid y
-    h.chunk = ceil_div(chunk < least ? least : chunk, 32) * 32;
-    h.splits = ceil_div(h.max_length, h.chunk);
-    h.tiles = ceil_div(h.max_length, SGLKV_WEIGHTS_TILE);
-    if (mul_ovf(h.tiles, c.kv_head_count, &h.waves) || mul_ovf(h.waves, c.request_count, &h.waves))
+    uint64_t pairs;
+    if (mul_ovf(c.query_count, c.query_head_count, &pairs)) return attention_overflow();
+
+    // Any rows: a wave to a (query, KV head, 16 heads), and to 64 tokens.
+    if (mul_ovf(c.query_count, c.kv_head_count, &h.any.base) ||
+        mul_ovf(h.any.base, ceil_div(group, SGLKV_ATTN_HEADS), &h.any.base))
         return attention_overflow();
-    if (h.waves > limit) return too_large_dim("workgroups", h.waves, limit);
+    if (h.any.base > kMaxWorkgroups) return too_large_dim("workgroups", h.any.base, kMaxWorkgroups);
+    split_tokens(h.max_length, h.any.base, 2048, 128, &h.any);
+    h.any.tiles = ceil_div(h.max_length, SGLKV_WEIGHTS_TILE);
+    if (mul_ovf(h.any.tiles, c.kv_head_count, &h.any.groups) || mul_ovf(h.any.groups, c.request_count, &h.any.groups))
+        return attention_overflow();
+    if (h.any.groups > kMaxWorkgroups) return too_large_dim("workgroups", h.any.groups, kMaxWorkgroups);
+    if (mul_ovf(pairs, h.any.splits, &h.any.bytes) || mul_ovf(h.any.bytes, 8, &h.any.bytes)) return attention_overflow();
+
+    // 16-byte rows of 64, 128 or 256 dims; rows and tokens are counted in 32 bits.
+    h.fits = (dk == 64 || dk == 128 || dk == 256) && pairs < (1ull << 31) && h.max_length <= (1ull << 31);
+    if (!h.fits) return SGL_KV_OK;
+    const uint64_t per = ceil_div(c.query_count, c.request_count);  // queries of a request
+    // Kept scores cost 8 bytes a (query head, token), written and read, K rows read
+    // a second time 2 dk bytes a token; 256 MiB of them at most.
+    h.score_stride = ceil_div(h.max_length, 64) * 64;
+    uint64_t score_bytes;
+    const bool keeps = 8 * group * per < 2 * dk && !mul_ovf(pairs, 4 * h.score_stride, &score_bytes) &&
+                       score_bytes <= (256ull << 20);
+    h.body = keeps ? 2 : per * group >= 32 ? 0 : 1;
+    const uint64_t tile_rows = h.body == 0 ? (dk == 256 ? 32 : 64) : 16;
+    h.head_groups = group > tile_rows ? ceil_div(group, tile_rows) : 1;
+    h.tile_queries = group > tile_rows ? 1 : tile_rows / group;
+    if (h.tile_queries > per) h.tile_queries = per;
+    h.row_tiles = ceil_div(c.query_count, h.tile_queries);
+    h.rows.base = h.row_tiles * h.head_groups * c.kv_head_count;
+    if (h.rows.base > kMaxWorkgroups) {
+        h.fits = false;
+        return SGL_KV_OK;
+    }
+    split_tokens(h.max_length, h.rows.base, h.body == 0 ? 2048 : 4096, h.body == 0 ? 256 : 64, &h.rows);
+    const uint64_t tile = keeps ? SGLKV_WEIGHTS_APPLY : dk == 256 ? SGLKV_WEIGHTS_TILE / 2 : SGLKV_WEIGHTS_TILE;
+    h.rows.tiles = ceil_div(h.max_length, tile);
+    h.rows.groups = h.rows.tiles * c.kv_head_count * c.request_count;  // (at most twice `any`'s)
+    h.waves = keeps ? SGLKV_WEIGHTS_APPLY / 64 : per * group >= 512 ? 8 : per * group >= 64 ? 4 : 1;
+    if (h.rows.groups > kMaxWorkgroups / h.waves || mul_ovf(pairs, 8 * h.rows.splits, &h.stats_bytes)) {
+        h.fits = false;
+        return SGL_KV_OK;
+    }
+    h.stats_bytes = ceil_div(h.stats_bytes, 256) * 256;
+    h.rows.bytes = h.stats_bytes + (keeps ? score_bytes : 0);
     return SGL_KV_OK;
 }
 
@@ -88,12 +143,10 @@ extern "C" int32_t sgl_kv_weight_plan_new(const sgl_kv_attention_plan *attention
     if (rc) return rc;
     const sgl_kv_attention_plan_config &c = p.attention.config;
     p.max_sequence_length = max_sequence_length;
-    uint64_t pairs;
     if (mul_ovf(c.kv_head_count, c.sequence_slot_count, &p.weights_required_bytes) ||
-        mul_ovf(p.weights_required_bytes, 4, &p.weights_required_bytes) ||
-        mul_ovf(c.query_count, c.query_head_count, &pairs) || mul_ovf(pairs, shape.splits, &pairs) ||
-        mul_ovf(pairs, 8, &p.workspace_required_bytes))
+        mul_ovf(p.weights_required_bytes, 4, &p.weights_required_bytes))
         return attention_overflow();
+    p.workspace_required_bytes = shape.fits && shape.rows.bytes > shape.any.bytes ? shape.rows.bytes : shape.any.bytes;
     *out = p;
     return ok();
 }
@@ -138,22 +191,37 @@ extern "C" int32_t sgl_rocm_kv_accumulate_weights(sgl_rocm_kv_ctx *ctx, const sg
     p.a.flag = ctx->attn_flag;
     attention_geometry(c, &p.a);
     p.a.zero_row = ctx->zero_row;
-    p.a.splits = (uint32_t)shape.splits;
-    p.a.chunk_tokens = shape.chunk;
     p.weights = reinterpret_cast<float *>(weights);
     p.max_length = shape.max_length;
-    p.tiles = (uint32_t)shape.tiles;
     const bool vector = p.a.dk % 8 == 0 && queries % 16 == 0 &&
                         ((pool + lay.key_in_page_offset) | lay.page_stride_bytes | p.a.key_head_stride |
                          p.a.key_token_stride) % 16 == 0;
+    const bool rows = vector && shape.fits;
+    const WeightShape::Way &way = rows ? shape.rows : shape.any;
+    p.a.splits = (uint32_t)way.splits;
+    p.a.chunk_tokens = way.chunk;
+    p.tiles = (uint32_t)way.tiles;
     DeviceScope scope(ctx->device);
     if (scope.status() != hipSuccess) return hip_fail(scope.status(), "hipSetDevice");
     hipStream_t s = static_cast<hipStream_t>(stream);
-    rc = launch_kernel(ctx->weight_stats[vector ? 0 : 1], shape.base, shape.splits, 1, 64,
-                       2 * SGLKV_ATTN_HEADS * (p.a.dk_pad + 8), s, &p, "weight statistics launch");
+    const char *const stats = "weight statistics launch", *const sums = "weight accumulation launch";
+    if (!rows) {
+        rc = launch_kernel(ctx->weight_stats[vector ? 0 : 1], way.base, way.splits, 1, 64,
+                           2 * SGLKV_ATTN_HEADS * (p.a.dk_pad + 8), s, &p, stats);
+        if (!rc) rc = launch_kernel(ctx->accumulate_weights[vector ? 0 : 1], way.groups, 1, 1, 64, 0, s, &p, sums);
+        return rc ? rc : ok();
+    }
+    p.row_tiles = (uint32_t)shape.row_tiles;
+    p.tile_queries = (uint32_t)shape.tile_queries;
+    p.tile_head_groups = (uint32_t)shape.head_groups;
+    p.score_stride = shape.score_stride;
+    const bool keeps = shape.body == 2;
+    if (keeps) p.scores = reinterpret_cast<float *>(workspace + shape.stats_bytes);
+    const auto &body = ctx->weight_rows[p.a.dk == 64 ? 0 : p.a.dk == 128 ? 1 : 2];
+    rc = launch_kernel(body[shape.body], way.base, way.splits, 1, 64, 0, s, &p, stats);
     if (!rc)
-        rc = launch_kernel(ctx->accumulate_weights[vector ? 0 : 1], shape.waves, 1, 1, 64, 0, s, &p,
-                           "weight accumulation launch");
+        rc = launch_kernel(keeps ? ctx->apply_scores : body[3], way.groups, 1, 1, 64 * (unsigned)shape.waves,
+                           keeps ? 0 : 4 * SGLKV_WEIGHTS_TILE * (unsigned)shape.waves, s, &p, sums);
     return rc ? rc : ok();
 }
 

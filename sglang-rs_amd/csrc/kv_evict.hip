@@ -215,6 +215,376 @@ __device__ __forceinline__ void wgt_accumulate_body(const sglkv_weights_params &
         }
 }
 
+// ---- Rows bodies: 16-byte rows of 64, 128 or 256 dims ------------------------
+//
+// The same two steps for the shapes that models have, with the operands in
+// registers. A row is a (query, query head) of one KV head; a tile of rows is
+// `tile_queries` consecutive queries (or a group of one query's heads where those
+// alone pass a tile), so a prompt's K rows are read once for NR * 16 rows.
+
+// K rows of 64 tokens from t0 as addresses, lane l token t0 + l; the zero row
+// past `end` and where a slot lies outside the pool (reported where `report`).
+__device__ __forceinline__ uint64_t wgt_rows_at(const sglkv_attn_params &p, uint64_t kbase, uint64_t start, uint32_t t0,
+                                                uint32_t end, bool report) {
+    const uint32_t t = t0 + (threadIdx.x & 63);
+    uint64_t row;
+    return wgt_row(p, kbase, start, t, t < end, report, &row) ? row : reinterpret_cast<uint64_t>(p.zero_row);
+}
+
+// The 16-byte pieces of token `16 b + r`'s row (addresses in lanes as above)
+// that lane (g, r) feeds to the matrix product: dims 32 c + 8 g.
+template <uint32_t DKC>
+__device__ __forceinline__ void wgt_load_rows(uint64_t rows, uint32_t b, uint32_t g, uint32_t r, sglkv_u16x8 (&k)[DKC]) {
+    const uint64_t at = __shfl(rows, 16 * b + r) + 16 * g;
+#pragma unroll
+    for (uint32_t c = 0; c < DKC; ++c) k[c] = sel_load(at + 64 * c);
+}
+
+// Statistics of NR * 16 rows over the tokens of split blockIdx.y; TB tiles of 16
+// tokens are loaded at a time. STORE: the scores go to the workspace, where the
+// second step takes them from (one query a request: K is read once).
+template <uint32_t DKC, uint32_t NR, uint32_t TB, bool STORE>
+__device__ __forceinline__ void wgt_rows_body(const sglkv_weights_params &p) {
+    const sglkv_attn_params &a = p.a;
+    const uint32_t lane = threadIdx.x, g = lane >> 4, r = lane & 15;
+    // The KV head varies fastest: with 8 of them each XCD reads one head's rows.
+    uint32_t bx = blockIdx.x;
+    const uint32_t kvh = bx % a.kv_heads;
+    bx /= a.kv_heads;
+    const uint32_t hg = bx % p.tile_head_groups;
+    // (A prompt's last queries attend the most: they start first.)
+    const uint32_t tile = p.row_tiles - 1 - bx / p.tile_head_groups;
+    const uint32_t qa = tile * p.tile_queries;
+    const uint32_t heads = p.tile_head_groups > 1 ? 16 * NR : a.group;  // rows of a query in this tile
+    sglkv_u16x8 qf[NR][DKC];
+    uint64_t start[NR];
+    uint32_t len[NR], req[NR], row[NR];
+    float m[NR], l[NR];
+#pragma unroll
+    for (uint32_t n = 0; n < NR; ++n) {
+        const uint32_t rho = 16 * n + r, qi = rho / heads, hi = hg * 16 * NR + rho - qi * heads;
+        const uint32_t q = qa + qi;
+        const bool own = qi < p.tile_queries && q < a.query_count && hi < a.group;
+        uint64_t n64 = 0;
+        start[n] = 0;
+        if (own) wgt_query(p, q, g == 0 && hi == 0 && kvh == 0 && blockIdx.y == 0, &start[n], &n64);
+        len[n] = static_cast<uint32_t>(n64);  // (the host bounds it)
+        req[n] = n64 ? a.query_request_indices[q] : ~0u;
+        row[n] = own ? q * a.query_heads + kvh * a.group + hi : ~0u;
+        m[n] = -3.402823466e+38f;
+        l[n] = 0.0f;
+        const uint64_t at = reinterpret_cast<uint64_t>(a.queries) + 2ull * (own ? row[n] : 0) * (32 * DKC) + 16 * g;
+#pragma unroll
+        for (uint32_t c = 0; c < DKC; ++c) qf[n][c] = sel_load(at + 64 * c);
+    }
+    const uint64_t kbase = reinterpret_cast<uint64_t>(a.pool) + a.key_offset + kvh * a.key_head_stride;
+    const uint32_t t0 = blockIdx.y * static_cast<uint32_t>(a.chunk_tokens);
+    // One request after another (nearly always there is one).
+    uint32_t seen = 0;  // bit n: row n's request has been taken
+    for (;;) {
+        uint32_t now = ~0u;
+#pragma unroll
+        for (uint32_t n = 0; n < NR; ++n)
+            if (!(seen >> n & 1) && req[n] < now) now = req[n];
+#pragma unroll
+        for (uint32_t s = 1; s < 64; s <<= 1) {
+            const uint32_t o = __shfl_xor(now, s);
+            now = o < now ? o : now;
+        }
+        if (now == ~0u) break;
+        uint32_t limit[NR], longest = 0, whole = ~0u;
+        uint64_t first = 0;
+#pragma unroll
+        for (uint32_t n = 0; n < NR; ++n) {
+            const bool in = req[n] == now;
+            limit[n] = in ? len[n] : 0;
+            if (in) {
+                seen |= 1u << n;
+                first = start[n];
+            }
+            longest = limit[n] > longest ? limit[n] : longest;
+            if (row[n] != ~0u && limit[n] < whole) whole = limit[n];  // (a row of no query may hold anything)
+        }
+#pragma unroll
+        for (uint32_t s = 1; s < 64; s <<= 1) {
+            const uint32_t x = __shfl_xor(longest, s), y = __shfl_xor(whole, s);
+            const uint64_t z = __shfl_xor(first, s);
+            longest = x > longest ? x : longest;
+            whole = y < whole ? y : whole;
+            first = z > first ? z : first;
+        }
+        longest = __builtin_amdgcn_readfirstlane(longest);
+        whole = __builtin_amdgcn_readfirstlane(whole);
+        const uint32_t most = t0 + static_cast<uint32_t>(a.chunk_tokens), t1 = longest < most ? longest : most;
+        if (t0 >= t1) continue;
+        uint64_t rows = wgt_rows_at(a, kbase, first, t0, t1, kvh == 0);
+        for (uint32_t t = t0; t < t1; t += 64) {
+            const uint64_t next = t + 64 < t1 ? wgt_rows_at(a, kbase, first, t + 64, t1, kvh == 0) : rows;
+#pragma unroll
+            for (uint32_t half = 0; half < 4; half += TB) {
+                if (t + 16 * half >= t1) break;
+                sglkv_u16x8 kf[TB][DKC];
+#pragma unroll
+                for (uint32_t b = 0; b < TB; ++b) wgt_load_rows<DKC>(rows, half + b, g, r, kf[b]);
+#pragma unroll
+                for (uint32_t b = 0; b < TB; ++b) {
+                    const uint32_t tt = t + 16 * (half + b) + 4 * g;  // this lane's tokens
+                    sglkv_f32x4 sc[NR];
+#pragma unroll
+                    for (uint32_t n = 0; n < NR; ++n) {
+                        sc[n] = sglkv_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (uint32_t c = 0; c < DKC; ++c)
+                            sc[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(attn_as_bf16(kf[b][c]), attn_as_bf16(qf[n][c]),
+                                                                            sc[n], 0, 0, 0);
+                    }
+                    bool moves = false;
+#pragma unroll
+                    for (uint32_t n = 0; n < NR; ++n) {
+#pragma unroll
+                        for (uint32_t e = 0; e < 4; ++e) sc[n][e] *= a.scale_log2;
+                        if (STORE) {
+                            if (tt < limit[n])
+                                *reinterpret_cast<sglkv_f32x4 *>(p.scores + row[n] * p.score_stride + tt) = sc[n];
+                        }
+                    }
+                    if (t + 16 * (half + b) + 16 > whole) {
+#pragma unroll
+                        for (uint32_t n = 0; n < NR; ++n)
+#pragma unroll
+                            for (uint32_t e = 0; e < 4; ++e)
+                                if (tt + e >= limit[n]) sc[n][e] = -INFINITY;
+                    }
+                    // The maximum moves only where a score passes it by more than 8 (log2
+                    // units): terms stay below 2^8 and most steps rescale nothing.
+                    float top[NR];
+#pragma unroll
+                    for (uint32_t n = 0; n < NR; ++n) {
+                        top[n] = fmaxf(fmaxf(sc[n][0], sc[n][1]), fmaxf(sc[n][2], sc[n][3]));
+                        moves |= top[n] > m[n] + 8.0f;
+                    }
+                    if (__ballot(moves)) {
+#pragma unroll
+                        for (uint32_t n = 0; n < NR; ++n) {
+                            const float up = fmaxf(m[n], top[n]);
+                            l[n] *= exp2f(m[n] - up);
+                            m[n] = up;
+                        }
+                    }
+#pragma unroll
+                    for (uint32_t n = 0; n < NR; ++n)
+#pragma unroll
+                        for (uint32_t e = 0; e < 4; ++e) l[n] += __builtin_amdgcn_exp2f(sc[n][e] - m[n]);
+                }
+            }
+            rows = next;
+        }
+    }
+#pragma unroll
+    for (uint32_t n = 0; n < NR; ++n) {
+        float mm = m[n], ll = l[n];
+#pragma unroll
+        for (uint32_t s = 16; s < 64; s <<= 1) {
+            const float mo = __shfl_xor(mm, s), lo = __shfl_xor(ll, s), up = fmaxf(mm, mo);
+            ll = ll * exp2f(mm - up) + lo * exp2f(mo - up);
+            mm = up;
+        }
+        if (g == 0 && row[n] != ~0u) {
+            const bool some = t0 < len[n];
+            reinterpret_cast<float2 *>(a.partial)[static_cast<uint64_t>(row[n]) * a.splits + blockIdx.y] =
+                make_float2(some ? mm : -INFINITY, some ? ll : 0.0f);
+        }
+    }
+}
+
+// The queries [*q0, *q1) of request `req`, whose indices never fall: 64 places
+// probed at once, so two or three loads in a row.
+__device__ __forceinline__ void wgt_queries_of(const sglkv_attn_params &p, uint32_t req, uint32_t *q0, uint32_t *q1) {
+    const uint32_t lane = threadIdx.x & 63;
+    uint32_t found[2];
+#pragma unroll
+    for (uint32_t k = 0; k < 2; ++k) {
+        uint32_t low = 0, high = static_cast<uint32_t>(p.query_count);  // the first index >= req + k lies in [low, high]
+        while (low < high) {
+            const uint32_t step = (high - low + 63) / 64, at = low + lane * step;
+            const uint32_t below = __popcll(__ballot(at < high && p.query_request_indices[at < high ? at : low] < req + k));
+            // (below == 0: at low itself)
+            if (below == 0) {
+                high = low;
+            } else {
+                const uint32_t from = low + (below - 1) * step + 1, to = low + below * step;
+                low = from;
+                high = to < high ? to : high;
+            }
+        }
+        found[k] = low;
+    }
+    *q0 = found[0];
+    *q1 = found[1] > found[0] ? found[1] : found[0];  // (indices that fall have been reported)
+}
+
+// A row's joined statistics: the reference m and 1 / l (0: it weighs nothing).
+__device__ __forceinline__ void wgt_joined(const sglkv_attn_params &a, uint64_t row, float *m, float *inv) {
+    const float2 *stats = reinterpret_cast<const float2 *>(a.partial) + row * a.splits;
+    float top = -INFINITY, l = 0.0f;
+    for (uint32_t s = 0; s < a.splits; ++s) top = fmaxf(top, stats[s].x);
+    for (uint32_t s = 0; s < a.splits; ++s)
+        if (stats[s].x != -INFINITY) l += stats[s].y * exp2f(stats[s].x - top);
+    *m = top == -INFINITY ? 0.0f : top;
+    *inv = top == -INFINITY ? 0.0f : 1.0f / l;
+}
+
+// Accumulation from K rows: a workgroup has TT tiles of 16 tokens of a (request,
+// KV head) in registers; its waves take the request's rows 16 at a time, and
+// their sums join in LDS, wave by wave in order.
+template <uint32_t DKC, uint32_t TT>
+__device__ __forceinline__ void wgt_accumulate_rows_body(const sglkv_weights_params &p) {
+    extern __shared__ __attribute__((aligned(16))) float wgt_sums[];
+    const sglkv_attn_params &a = p.a;
+    const uint32_t lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), waves = blockDim.x / 64;
+    uint32_t bx = blockIdx.x;
+    const uint32_t kvh = bx % a.kv_heads;
+    bx /= a.kv_heads;
+    const uint32_t tile = bx % p.tiles, req = bx / p.tiles, tb = tile * 16 * TT;
+    const uint64_t start = a.request_slot_offsets[req], end = a.request_slot_offsets[req + 1];
+    if (start > end || end > a.sequence_slot_count || tb >= end - start) return;
+    uint32_t q0, q1;
+    wgt_queries_of(a, req, &q0, &q1);
+    const uint64_t most = end - start < p.max_length ? end - start : p.max_length;
+    auto length_of = [&](uint32_t q) {
+        const uint64_t n = a.query_sequence_lengths[q];
+        return n <= most && a.query_request_indices[q] == req ? static_cast<uint32_t>(n) : 0;
+    };
+    // The tokens that any query attends, and the first query that attends this tile.
+    uint32_t longest = 0, q_from = q1;
+    for (uint32_t q = q0 + lane; q < q1; q += 64) {
+        const uint32_t n = length_of(q);
+        longest = n > longest ? n : longest;
+        if (n > tb && q < q_from) q_from = q;
+    }
+#pragma unroll
+    for (uint32_t s = 1; s < 64; s <<= 1) {
+        const uint32_t x = __shfl_xor(longest, s), y = __shfl_xor(q_from, s);
+        longest = x > longest ? x : longest;
+        q_from = y < q_from ? y : q_from;
+    }
+    longest = __builtin_amdgcn_readfirstlane(longest);
+    q_from = __builtin_amdgcn_readfirstlane(q_from);
+    if (tb >= longest) return;
+    const uint64_t kbase = reinterpret_cast<uint64_t>(a.pool) + a.key_offset + kvh * a.key_head_stride;
+    const uint64_t at = wgt_rows_at(a, kbase, start, tb, longest, false);
+    sglkv_u16x8 kf[TT][DKC];
+#pragma unroll
+    for (uint32_t b = 0; b < TT; ++b) wgt_load_rows<DKC>(at, b, g, r, kf[b]);
+    float sum[TT][4] = {};
+    // Rows rho = (query - q_from) * group + head; this wave's 16 w, 16 (w + waves), ...
+    const uint32_t count = (q1 - q_from) * a.group, step = 16 * waves, dq = step / a.group, dh = step - dq * a.group;
+    uint32_t rho = 16 * wave + r, q = q_from + rho / a.group, h = rho % a.group;
+    for (uint32_t first = 16 * wave; first < count; first += step) {
+        const bool own = rho < count;
+        const uint32_t n = own ? length_of(q) : 0;
+        const uint64_t row = own ? static_cast<uint64_t>(q) * a.query_heads + kvh * a.group + h : 0;
+        rho += step;
+        q += dq;
+        h += dh;
+        if (h >= a.group) {
+            h -= a.group;
+            ++q;
+        }
+        const uint32_t limit = n <= tb ? 0 : n - tb;
+        if (!__ballot(limit > 0)) continue;
+        const uint64_t from = reinterpret_cast<uint64_t>(a.queries) + row * (64 * DKC) + 16 * g;
+        sglkv_u16x8 qf[DKC];
+#pragma unroll
+        for (uint32_t c = 0; c < DKC; ++c) qf[c] = sel_load(from + 64 * c);
+        float m, inv;
+        wgt_joined(a, row, &m, &inv);
+        if (limit == 0) inv = 0.0f;
+        const bool whole = !__ballot(limit < 16 * TT);
+#pragma unroll
+        for (uint32_t b = 0; b < TT; ++b) {
+            sglkv_f32x4 sc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (uint32_t c = 0; c < DKC; ++c)
+                sc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(attn_as_bf16(kf[b][c]), attn_as_bf16(qf[c]), sc, 0, 0, 0);
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) sc[e] = fmaf(sc[e], a.scale_log2, -m);
+            if (!whole) {
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e)
+                    if (16 * b + 4 * g + e >= limit) sc[e] = -INFINITY;
+            }
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) sum[b][e] = fmaf(__builtin_amdgcn_exp2f(sc[e]), inv, sum[b][e]);
+        }
+    }
+#pragma unroll
+    for (uint32_t b = 0; b < TT; ++b)
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) {
+            float x = sum[b][e];
+            x += __uint_as_float(sel_join<1>(__float_as_uint(x)));
+            x += __uint_as_float(sel_join<2>(__float_as_uint(x)));
+            x += __uint_as_float(sel_join<4>(__float_as_uint(x)));
+            x += __uint_as_float(sel_join<8>(__float_as_uint(x)));
+            if (r == 0) wgt_sums[wave * 16 * TT + 16 * b + 4 * g + e] = x;
+        }
+    __syncthreads();
+    if (threadIdx.x < 16 * TT && tb + threadIdx.x < longest) {
+        float x = 0.0f;
+        for (uint32_t w = 0; w < waves; ++w) x += wgt_sums[w * 16 * TT + threadIdx.x];
+        p.weights[kvh * a.sequence_slot_count + start + tb + threadIdx.x] += x;
+    }
+}
+
+// Accumulation from kept scores: a thread to a token of a (request, KV head),
+// its (query, head)s in turn.
+__device__ __forceinline__ void wgt_apply_body(const sglkv_weights_params &p) {
+    __shared__ float2 joined[SGLKV_WEIGHTS_APPLY];
+    __shared__ uint32_t limits[SGLKV_WEIGHTS_APPLY];
+    const sglkv_attn_params &a = p.a;
+    const uint32_t tid = threadIdx.x;
+    uint32_t bx = blockIdx.x;
+    const uint32_t kvh = bx % a.kv_heads;
+    bx /= a.kv_heads;
+    const uint32_t tile = bx % p.tiles, req = bx / p.tiles, tb = tile * SGLKV_WEIGHTS_APPLY;
+    const uint64_t start = a.request_slot_offsets[req], end = a.request_slot_offsets[req + 1];
+    if (start > end || end > a.sequence_slot_count || tb >= end - start) return;
+    uint32_t q0, q1;
+    wgt_queries_of(a, req, &q0, &q1);
+    const uint64_t most = end - start < p.max_length ? end - start : p.max_length;
+    const uint32_t count = (q1 - q0) * a.group, t = tb + tid;
+    float sum = 0.0f;
+    bool any = false;
+    for (uint32_t base = 0; base < count; base += SGLKV_WEIGHTS_APPLY) {
+        const uint32_t here = count - base < SGLKV_WEIGHTS_APPLY ? count - base : SGLKV_WEIGHTS_APPLY;
+        __syncthreads();
+        if (tid < here) {
+            const uint32_t q = q0 + (base + tid) / a.group, h = (base + tid) % a.group;
+            const uint64_t n = a.query_sequence_lengths[q];
+            const bool own = n <= most && a.query_request_indices[q] == req;
+            limits[tid] = own ? static_cast<uint32_t>(n) : 0;
+            wgt_joined(a, static_cast<uint64_t>(q) * a.query_heads + kvh * a.group + h, &joined[tid].x, &joined[tid].y);
+        }
+        __syncthreads();
+        uint32_t q = q0 + base / a.group, h = base % a.group;
+#pragma unroll 4
+        for (uint32_t i = 0; i < here; ++i) {
+            const uint64_t row = static_cast<uint64_t>(q) * a.query_heads + kvh * a.group + h;
+            if (++h == a.group) {
+                h = 0;
+                ++q;
+            }
+            if (t < limits[i]) {
+                any = true;
+                sum = fmaf(__builtin_amdgcn_exp2f(p.scores[row * p.score_stride + t] - joined[i].x), joined[i].y, sum);
+            }
+        }
+    }
+    if (any) p.weights[kvh * a.sequence_slot_count + start + t] += sum;
+}
+
 // ---- The kept positions -----------------------------------------------------
 
 // A request's slots and length; false (length 0) where its metadata does not
@@ -348,6 +718,46 @@ extern "C" __global__ __launch_bounds__(64) void sglkv_accumulate_weights_v16(sg
 extern "C" __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void
 sglkv_accumulate_weights_v2(sglkv_weights_params p) {
     wgt_accumulate_body<false>(p);
+}
+
+extern "C" __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void sglkv_weight_rows64(sglkv_weights_params p) {
+    wgt_rows_body<2, 4, 2, false>(p);
+}
+extern "C" __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void sglkv_weight_few64(sglkv_weights_params p) {
+    wgt_rows_body<2, 1, 4, false>(p);
+}
+extern "C" __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void sglkv_weight_scores64(sglkv_weights_params p) {
+    wgt_rows_body<2, 1, 4, true>(p);
+}
+extern "C" __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void sglkv_accumulate_rows64(sglkv_weights_params p) {
+    wgt_accumulate_rows_body<2, 4>(p);
+}
+extern "C" __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void sglkv_weight_rows128(sglkv_weights_params p) {
+    wgt_rows_body<4, 4, 2, false>(p);
+}
+extern "C" __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void sglkv_weight_few128(sglkv_weights_params p) {
+    wgt_rows_body<4, 1, 4, false>(p);
+}
+extern "C" __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void sglkv_weight_scores128(sglkv_weights_params p) {
+    wgt_rows_body<4, 1, 4, true>(p);
+}
+extern "C" __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void sglkv_accumulate_rows128(sglkv_weights_params p) {
+    wgt_accumulate_rows_body<4, 4>(p);
+}
+extern "C" __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void sglkv_weight_rows256(sglkv_weights_params p) {
+    wgt_rows_body<8, 2, 1, false>(p);
+}
+extern "C" __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void sglkv_weight_few256(sglkv_weights_params p) {
+    wgt_rows_body<8, 1, 2, false>(p);
+}
+extern "C" __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void sglkv_weight_scores256(sglkv_weights_params p) {
+    wgt_rows_body<8, 1, 2, true>(p);
+}
+extern "C" __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void sglkv_accumulate_rows256(sglkv_weights_params p) {
+    wgt_accumulate_rows_body<8, 2>(p);
+}
+extern "C" __global__ __launch_bounds__(SGLKV_WEIGHTS_APPLY) void sglkv_apply_scores(sglkv_weights_params p) {
+    wgt_apply_body(p);
 }
 
 extern "C" __global__ __launch_bounds__(SGLKV_EVICT_THREADS) void sglkv_select_tokens(sglkv_evict_params p) {

@@ -417,13 +417,18 @@ typedef struct sglkv_select_params {
  * queries: weights[kv head][position] += ..., positions numbered as
  * sequence_slots. `a` as for paged attention; its partial holds a (maximum, sum)
  * pair of 32-bit floats per (query, head, split), in log2 units. */
-#define SGLKV_WEIGHTS_TILE 64u /* tokens per wave of the accumulation */
+#define SGLKV_WEIGHTS_TILE 64u    /* tokens of a tile of the accumulation (32 at dims 256) */
+#define SGLKV_WEIGHTS_APPLY 256u  /* tokens (and threads) of a workgroup that applies kept scores */
 typedef struct sglkv_weights_params {
     sglkv_attn_params a;
     float *weights;
+    float *scores;            /* [query][query head][score_stride] scores in log2 units, or null */
     uint64_t max_length;      /* the longest query length that the launch covers */
-    uint32_t tiles;           /* SGLKV_WEIGHTS_TILE-token tiles of a sequence of max_length */
-    uint32_t reserved;
+    uint64_t score_stride;    /* a multiple of 64 */
+    uint32_t tiles;           /* token tiles of a sequence of max_length */
+    uint32_t row_tiles;       /* rows bodies: tiles of queries */
+    uint32_t tile_queries;    /* queries of one */
+    uint32_t tile_head_groups;/* groups of a KV head's query heads, where one query's rows pass a tile */
 } sglkv_weights_params;
 
 /* The positions of each (request, KV head) that are kept, and their rows' and

@@ -585,6 +585,19 @@ extern "C" int32_t sgl_rocm_kv_init(int32_t device, const char *code_object_path
                      {"sglkv_weight_stats_v2", &ctx->weight_stats[1]},
                      {"sglkv_accumulate_weights_v16", &ctx->accumulate_weights[0]},
                      {"sglkv_accumulate_weights_v2", &ctx->accumulate_weights[1]},
+                     {"sglkv_weight_rows64", &ctx->weight_rows[0][0]},
+                     {"sglkv_weight_few64", &ctx->weight_rows[0][1]},
+                     {"sglkv_weight_scores64", &ctx->weight_rows[0][2]},
+                     {"sglkv_accumulate_rows64", &ctx->weight_rows[0][3]},
+                     {"sglkv_weight_rows128", &ctx->weight_rows[1][0]},
+                     {"sglkv_weight_few128", &ctx->weight_rows[1][1]},
+                     {"sglkv_weight_scores128", &ctx->weight_rows[1][2]},
+                     {"sglkv_accumulate_rows128", &ctx->weight_rows[1][3]},
+                     {"sglkv_weight_rows256", &ctx->weight_rows[2][0]},
+                     {"sglkv_weight_few256", &ctx->weight_rows[2][1]},
+                     {"sglkv_weight_scores256", &ctx->weight_rows[2][2]},
+                     {"sglkv_accumulate_rows256", &ctx->weight_rows[2][3]},
+                     {"sglkv_apply_scores", &ctx->apply_scores},
                      {"sglkv_select_tokens", &ctx->select_tokens},
                      {"sglkv_compact_tokens_v16", &ctx->compact_tokens[0]},
                      {"sglkv_compact_tokens_v4", &ctx->compact_tokens[1]},

@@ -91,6 +91,13 @@ def _check_weights(got, want, label=""):
     (16, 2, 2, 128, 128, False, 0, (600, 40), 17),
     (16, 1, 33, 64, 64, False, 0, (300,), 40),                     # 33 query heads: three groups of 16
     (64, 8, 64, 128, 128, False, 0, tuple(range(100, 2100, 100)), 1),
+    (16, 2, 4, 128, 128, False, 0, (3, 100, 0, 1, 64, 65, 2, 90), 20),   # tiles of queries of several requests
+    (16, 2, 14, 64, 64, False, 0, (3, 100, 0, 1, 64, 65, 2, 90, 30), 11),
+    (8, 1, 130, 64, 64, False, 0, (200, 31), 3),                         # a query's heads pass a tile
+    (8, 1, 70, 256, 256, True, 0, (200, 31), 2),
+    (16, 1, 1, 128, 128, False, 0, (5000,), 1),
+    (16, 1, 2, 256, 256, False, 0, (700, 300), 300),
+    (4, 8, 8, 64, 64, True, 0, (10, 20, 30, 4000), 2),
 ])
 def test_weights(k, page, heads, qheads, dk, dv, hnd, shift, lengths, per):
     rng = np.random.default_rng(page + dk)

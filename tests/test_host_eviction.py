@@ -85,3 +85,19 @@ def test_random_plans_never_overflow():
             assert p.kept_required_bytes == p.request_count * p.kv_head_count * p.max_kept * 4
         except kv.KvError as e:
             assert e.variant in ("DimensionTooLarge", "ShapeOverflow"), e
+
+
+def test_random_weight_plans_never_overflow():
+    rng = np.random.default_rng(2)
+
+    def size(most):
+        return int(2 ** rng.uniform(0, most))
+    for _ in range(3000):
+        heads = size(8)
+        try:
+            a = _attention(page=size(20), heads=heads, dk=int(rng.choice([64, 128, 256, size(11)])), query_count=size(33),
+                           query_head_count=heads * size(9), request_count=size(33), sequence_slot_count=size(60))
+            p = kv.WeightAccumulationPlan.new(a, max_sequence_length=size(60))
+            assert p.workspace_required_bytes >= a.query_count * a.query_head_count * 8
+        except kv.KvError as e:
+            assert e.variant in ("DimensionTooLarge", "ShapeOverflow"), e
