@@ -57,8 +57,8 @@ struct WeightShape {
     } any, rows;
     bool fits;                // `rows` is a way
     int body;                 // of ctx->weight_rows[dims]: 0 many rows, 1 few, 2 few with their scores
-    uint64_t row_tiles, tile_queries, head_groups, waves;
-    uint64_t stats_bytes, score_stride;
+    uint64_t row_tiles, tile_queries, head_groups, segments;
+    uint64_t stats_bytes, joined_bytes, score_stride;
 };
 
 constexpr uint64_t kMaxWorkgroups = UINT32_MAX / 64;  // of one wave: a dispatch counts its work-items in 32 bits
@@ -96,37 +96,54 @@ int32_t weight_shape(const sgl_kv_attention_plan_config &c, uint64_t max_sequenc
     if (mul_ovf(pairs, h.any.splits, &h.any.bytes) || mul_ovf(h.any.bytes, 8, &h.any.bytes)) return attention_overflow();
 
     // 16-byte rows of 64, 128 or 256 dims; rows and tokens are counted in 32 bits.
-    h.fits = (dk == 64 || dk == 128 || dk == 256) && pairs < (1ull << 31) && h.max_length <= (1ull << 31);
+    h.fits = (dk == 64 || dk == 128 || dk == 256) && pairs < (1ull << 27) && h.max_length <= (1ull << 31);
     if (!h.fits) return SGL_KV_OK;
     const uint64_t per = ceil_div(c.query_count, c.request_count);  // queries of a request
     // Kept scores cost 8 bytes a (query head, token), written and read, K rows read
     // a second time 2 dk bytes a token; 256 MiB of them at most.
     h.score_stride = ceil_div(h.max_length, 64) * 64;
-    uint64_t score_bytes;
+    uint64_t score_bytes = 0;
     const bool keeps = 8 * group * per < 2 * dk && !mul_ovf(pairs, 4 * h.score_stride, &score_bytes) &&
                        score_bytes <= (256ull << 20);
     h.body = keeps ? 2 : per * group >= 32 ? 0 : 1;
-    const uint64_t tile_rows = h.body == 0 ? (dk == 256 ? 32 : 64) : 16;
+    const uint64_t tile_rows = h.body == 0 ? (dk == 256 ? 128 : 256) : 16;
     h.head_groups = group > tile_rows ? ceil_div(group, tile_rows) : 1;
     h.tile_queries = group > tile_rows ? 1 : tile_rows / group;
     if (h.tile_queries > per) h.tile_queries = per;
     h.row_tiles = ceil_div(c.query_count, h.tile_queries);
     h.rows.base = h.row_tiles * h.head_groups * c.kv_head_count;
-    if (h.rows.base > kMaxWorkgroups) {
+    // (Workgroups of four waves are placed eight items at a time.)
+    auto placed = [&](uint64_t items) { return ceil_div(items, 8) * 8 * c.kv_head_count; };
+    if (h.body == 0) h.rows.base = placed(h.row_tiles * h.head_groups);
+    if (h.rows.base > kMaxWorkgroups / 4) {
         h.fits = false;
         return SGL_KV_OK;
     }
-    split_tokens(h.max_length, h.rows.base, h.body == 0 ? 2048 : 4096, h.body == 0 ? 256 : 64, &h.rows);
-    const uint64_t tile = keeps ? SGLKV_WEIGHTS_APPLY : dk == 256 ? SGLKV_WEIGHTS_TILE / 2 : SGLKV_WEIGHTS_TILE;
+    // (Ragged sequences: as many workgroups have tokens as equal ones of the mean would.)
+    const uint64_t mean = ceil_div(c.sequence_slot_count, c.request_count),
+                   live = ceil_div(h.rows.base * (mean < h.max_length ? mean : h.max_length), h.max_length);
+    split_tokens(h.max_length, live, h.body == 0 ? 2048 : 4096, h.body == 0 ? 256 : 64, &h.rows);
+    const uint64_t tile = keeps ? SGLKV_WEIGHTS_APPLY : dk == 256 ? 2 * SGLKV_WEIGHTS_TILE : 4 * SGLKV_WEIGHTS_TILE;
     h.rows.tiles = ceil_div(h.max_length, tile);
-    h.rows.groups = h.rows.tiles * c.kv_head_count * c.request_count;  // (at most twice `any`'s)
-    h.waves = keeps ? SGLKV_WEIGHTS_APPLY / 64 : per * group >= 512 ? 8 : per * group >= 64 ? 4 : 1;
-    if (h.rows.groups > kMaxWorkgroups / h.waves || mul_ovf(pairs, 8 * h.rows.splits, &h.stats_bytes)) {
+    // A prompt's first tokens are attended by all of its queries, its last by a
+    // few: parts of 512 rows or more even the workgroups out.
+    h.segments = keeps ? 1 : per * group / 512 < 16 ? per * group / 512 : 16;
+    if (h.segments < 1) h.segments = 1;
+    // (At most 16 times `any`'s.)
+    h.rows.groups = keeps ? h.rows.tiles * c.kv_head_count * c.request_count : placed(h.rows.tiles * c.request_count * h.segments);
+    if (h.rows.groups > kMaxWorkgroups / 4 || mul_ovf(pairs, 8 * h.rows.splits, &h.stats_bytes)) {
         h.fits = false;
         return SGL_KV_OK;
     }
     h.stats_bytes = ceil_div(h.stats_bytes, 256) * 256;
-    h.rows.bytes = h.stats_bytes + (keeps ? score_bytes : 0);
+    h.joined_bytes = keeps || h.rows.splits == 1 ? 0 : ceil_div(8 * pairs, 256) * 256;
+    uint64_t sums = 0;
+    if (h.segments > 1 && (mul_ovf(h.segments * 4, c.kv_head_count, &sums) || mul_ovf(sums, c.sequence_slot_count, &sums) ||
+                           sums >> 40)) {
+        h.fits = false;
+        return SGL_KV_OK;
+    }
+    h.rows.bytes = h.stats_bytes + (keeps ? score_bytes : h.joined_bytes + sums);
     return SGL_KV_OK;
 }
 
@@ -217,11 +234,22 @@ extern "C" int32_t sgl_rocm_kv_accumulate_weights(sgl_rocm_kv_ctx *ctx, const sg
     p.score_stride = shape.score_stride;
     const bool keeps = shape.body == 2;
     if (keeps) p.scores = reinterpret_cast<float *>(workspace + shape.stats_bytes);
+    p.joined = reinterpret_cast<float *>(way.splits > 1 ? workspace + shape.stats_bytes : workspace);
+    p.segments = (uint32_t)shape.segments;
+    if (shape.segments > 1) p.partial_sums = reinterpret_cast<float *>(workspace + shape.stats_bytes + shape.joined_bytes);
     const auto &body = ctx->weight_rows[p.a.dk == 64 ? 0 : p.a.dk == 128 ? 1 : 2];
-    rc = launch_kernel(body[shape.body], way.base, way.splits, 1, 64, 0, s, &p, stats);
-    if (!rc)
-        rc = launch_kernel(keeps ? ctx->apply_scores : body[3], way.groups, 1, 1, 64 * (unsigned)shape.waves,
-                           keeps ? 0 : 4 * SGLKV_WEIGHTS_TILE * (unsigned)shape.waves, s, &p, sums);
+    rc = launch_kernel(body[shape.body], way.base, way.splits, 1, shape.body == 0 ? 256 : 64, 0, s, &p, stats);
+    for (p.join_lanes = 1; p.join_lanes < way.splits && p.join_lanes < 16;) p.join_lanes *= 2;
+    if (!rc && !keeps && way.splits > 1)
+        rc = launch_kernel(ctx->join_statistics,
+                           ceil_div(c.query_count * c.query_head_count, SGLKV_WEIGHTS_THREADS / p.join_lanes), 1, 1,
+                           SGLKV_WEIGHTS_THREADS, 0, s, &p, "weight statistics join launch");
+    if (!rc && keeps) rc = launch_kernel(ctx->apply_scores, way.groups, 1, 1, SGLKV_WEIGHTS_THREADS, 0, s, &p, sums);
+    if (!rc && !keeps) rc = launch_kernel(body[3], way.groups, 1, 1, 256, 0, s, &p, sums);
+    if (!rc && shape.segments > 1)
+        rc = launch_kernel(ctx->add_segments,
+                           ceil_div(shape.max_length, SGLKV_WEIGHTS_THREADS) * c.kv_head_count * c.request_count, 1, 1,
+                           SGLKV_WEIGHTS_THREADS, 0, s, &p, "weight segments launch");
     return rc ? rc : ok();
 }
 

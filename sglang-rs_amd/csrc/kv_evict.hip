@@ -240,228 +240,422 @@ __device__ __forceinline__ void wgt_load_rows(uint64_t rows, uint32_t b, uint32_
     for (uint32_t c = 0; c < DKC; ++c) k[c] = sel_load(at + 64 * c);
 }
 
-// Statistics of NR * 16 rows over the tokens of split blockIdx.y; TB tiles of 16
-// tokens are loaded at a time. STORE: the scores go to the workspace, where the
-// second step takes them from (one query a request: K is read once).
-template <uint32_t DKC, uint32_t NR, uint32_t TB, bool STORE>
+// The NR * 16 rows of a wave (lane (g, r) has rows 16 n + r): queries, running
+// (maximum, sum) and metadata.
+template <uint32_t NR, uint32_t DKC>
+struct wgt_row_set {
+    sglkv_u16x8 q[NR][DKC];
+    float m[NR], l[NR];
+    uint32_t len[NR], req[NR], row[NR];  // row: query * query_heads + head, ~0 where there is none
+};
+
+// Rows `from` + 16 n + r of the tile of queries qa .., whose heads h0 .. h0 +
+// heads - 1 of a KV head are its rows. The loads of a kind go out at once (a lane
+// without a row takes the first query's).
+template <uint32_t DKC, uint32_t NR>
+__device__ __forceinline__ void wgt_load_row_set(const sglkv_weights_params &p, uint32_t qa, uint32_t h0, uint32_t heads,
+                                                 uint32_t from, uint32_t kvh, wgt_row_set<NR, DKC> &w) {
+    const sglkv_attn_params &a = p.a;
+    const uint32_t lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
+    uint64_t lengths[NR], starts[NR], ends[NR];
+    uint32_t previous[NR];
+    bool reports[NR];
+#pragma unroll
+    for (uint32_t n = 0; n < NR; ++n) {
+        const uint32_t rho = from + 16 * n + r, qi = rho / heads, hi = h0 + rho - qi * heads;
+        const uint32_t q = qa + qi;
+        const bool own = qi < p.tile_queries && q < a.query_count && hi < a.group;
+        const uint32_t query = own ? q : 0;
+        w.row[n] = own ? q * a.query_heads + kvh * a.group + hi : ~0u;
+        reports[n] = own && g == 0 && hi == 0 && kvh == 0 && blockIdx.y == 0;
+        lengths[n] = a.query_sequence_lengths[query];
+        w.req[n] = a.query_request_indices[query];
+        previous[n] = a.query_request_indices[query > 0 ? query - 1 : 0];
+        const uint64_t at = reinterpret_cast<uint64_t>(a.queries) + 2ull * (own ? w.row[n] : 0) * (32 * DKC) + 16 * g;
+#pragma unroll
+        for (uint32_t c = 0; c < DKC; ++c) w.q[n][c] = sel_load(at + 64 * c);
+    }
+#pragma unroll
+    for (uint32_t n = 0; n < NR; ++n) {
+        const uint32_t known = w.req[n] < a.request_count ? w.req[n] : 0;
+        starts[n] = a.request_slot_offsets[known];
+        ends[n] = a.request_slot_offsets[known + 1];
+    }
+#pragma unroll
+    for (uint32_t n = 0; n < NR; ++n) {
+        const bool known = w.req[n] < a.request_count;
+        const bool holds = known && starts[n] <= ends[n] && ends[n] <= a.sequence_slot_count &&
+                           lengths[n] <= ends[n] - starts[n] && lengths[n] <= p.max_length;
+        if (reports[n]) {
+            if (previous[n] > w.req[n] || (lengths[n] > 0 && !known))
+                atomicOr(a.flag, SGLKV_FLAG_ATTN_REQUEST);
+            else if (lengths[n] > 0 && !holds)
+                atomicOr(a.flag, SGLKV_FLAG_ATTN_SEQUENCE);
+        }
+        w.len[n] = w.row[n] != ~0u && holds ? static_cast<uint32_t>(lengths[n]) : 0;  // (the host bounds it)
+        if (w.len[n] == 0) w.req[n] = ~0u;
+        w.m[n] = -3.402823466e+38f;
+        w.l[n] = 0.0f;
+    }
+}
+
+// The lowest request of the wave's rows whose bit is not in `seen`; ~0: none.
+template <uint32_t NR>
+__device__ __forceinline__ uint32_t wgt_next_request(const uint32_t (&req)[NR], uint32_t seen) {
+    uint32_t now = ~0u;
+#pragma unroll
+    for (uint32_t n = 0; n < NR; ++n)
+        if (!(seen >> n & 1) && req[n] < now) now = req[n];
+#pragma unroll
+    for (uint32_t s = 1; s < 64; s <<= 1) {
+        const uint32_t o = __shfl_xor(now, s);
+        now = o < now ? o : now;
+    }
+    return now;
+}
+
+// Marks request `now`'s rows seen; their lengths (0 for the others), and the
+// longest and shortest in the wave.
+template <uint32_t NR, uint32_t DKC>
+__device__ __forceinline__ void wgt_take_request(const wgt_row_set<NR, DKC> &w, uint32_t now, uint32_t &seen,
+                                                 uint32_t (&limit)[NR], uint32_t *longest, uint32_t *whole) {
+    uint32_t most = 0, least = ~0u;
+#pragma unroll
+    for (uint32_t n = 0; n < NR; ++n) {
+        const bool in = w.req[n] == now;
+        limit[n] = in ? w.len[n] : 0;
+        if (in) seen |= 1u << n;
+        most = limit[n] > most ? limit[n] : most;
+        if (w.row[n] != ~0u && limit[n] < least) least = limit[n];  // (a row of no query may hold anything)
+    }
+#pragma unroll
+    for (uint32_t s = 1; s < 64; s <<= 1) {
+        const uint32_t x = __shfl_xor(most, s), y = __shfl_xor(least, s);
+        most = x > most ? x : most;
+        least = y < least ? y : least;
+    }
+    *longest = __builtin_amdgcn_readfirstlane(most);
+    *whole = __builtin_amdgcn_readfirstlane(least);
+}
+
+// 16 tokens from `t` (their K rows in kf) for all rows: scores, kept where STORE,
+// and the running maximum and sum. `whole`: the rows' shortest length.
+template <uint32_t DKC, uint32_t NR, bool STORE>
+__device__ __forceinline__ void wgt_weigh_tile(const sglkv_weights_params &p, const sglkv_u16x8 (&kf)[DKC],
+                                               wgt_row_set<NR, DKC> &w, const uint32_t (&limit)[NR], uint32_t t,
+                                               uint32_t whole, uint32_t g) {
+    const float scale = p.a.scale_log2;
+    const uint32_t tt = t + 4 * g;  // this lane's tokens
+    sglkv_f32x4 sc[NR];
+#pragma unroll
+    for (uint32_t n = 0; n < NR; ++n) sc[n] = sglkv_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (uint32_t c = 0; c < DKC; ++c)
+#pragma unroll
+        for (uint32_t n = 0; n < NR; ++n)
+            sc[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(attn_as_bf16(kf[c]), attn_as_bf16(w.q[n][c]), sc[n], 0, 0, 0);
+    if (STORE) {
+#pragma unroll
+        for (uint32_t n = 0; n < NR; ++n)
+            if (tt < limit[n])
+                *reinterpret_cast<sglkv_f32x4 *>(p.scores + w.row[n] * p.score_stride + tt) = sc[n] * scale;
+    }
+    if (t + 16 > whole) {
+#pragma unroll
+        for (uint32_t n = 0; n < NR; ++n)
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e)
+                if (tt + e >= limit[n]) sc[n][e] = -INFINITY;
+    }
+    // The reference moves only where a score passes it by more than 8 log2 units:
+    // terms stay below 2^8 and most steps rescale nothing.
+    float top[NR];
+    bool moves = false;
+#pragma unroll
+    for (uint32_t n = 0; n < NR; ++n) {
+        top[n] = fmaxf(fmaxf(sc[n][0], sc[n][1]), fmaxf(sc[n][2], sc[n][3])) * scale;
+        moves |= top[n] > w.m[n] + 8.0f;
+    }
+    if (__ballot(moves)) {
+#pragma unroll
+        for (uint32_t n = 0; n < NR; ++n) {
+            const float up = fmaxf(w.m[n], top[n]);
+            w.l[n] *= __builtin_amdgcn_exp2f(w.m[n] - up);
+            w.m[n] = up;
+        }
+    }
+#pragma unroll
+    for (uint32_t n = 0; n < NR; ++n)
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) w.l[n] += __builtin_amdgcn_exp2f(fmaf(sc[n][e], scale, -w.m[n]));
+}
+
+// The rows' statistics for the split whose tokens start at t0: the four lanes of
+// a row join. One split's leave joined (wgt_joined).
+template <uint32_t DKC, uint32_t NR>
+__device__ __forceinline__ void wgt_leave_stats(const sglkv_weights_params &p, const wgt_row_set<NR, DKC> &w, uint32_t t0,
+                                                uint32_t g) {
+    const sglkv_attn_params &a = p.a;
+#pragma unroll
+    for (uint32_t n = 0; n < NR; ++n) {
+        float m = w.m[n], l = w.l[n];
+#pragma unroll
+        for (uint32_t s = 16; s < 64; s <<= 1) {
+            const float mo = __shfl_xor(m, s), lo = __shfl_xor(l, s), up = fmaxf(m, mo);
+            l = l * exp2f(m - up) + lo * exp2f(mo - up);
+            m = up;
+        }
+        if (g == 0 && w.row[n] != ~0u) {
+            const bool some = t0 < w.len[n];
+            float2 pair = some ? make_float2(m, l) : make_float2(-INFINITY, 0.0f);
+            if (a.splits == 1) pair = some ? make_float2(m, 1.0f / l) : make_float2(INFINITY, 0.0f);
+            reinterpret_cast<float2 *>(a.partial)[static_cast<uint64_t>(w.row[n]) * a.splits + blockIdx.y] = pair;
+        }
+    }
+}
+
+// Statistics of 16 rows, a wave each, over the tokens of split blockIdx.y; TB
+// tiles of 16 tokens are weighed while the next TB are loading. STORE: the scores
+// go to the workspace, where the second step takes them from (K is read once).
+template <uint32_t DKC, uint32_t TB, bool STORE>
 __device__ __forceinline__ void wgt_rows_body(const sglkv_weights_params &p) {
     const sglkv_attn_params &a = p.a;
     const uint32_t lane = threadIdx.x, g = lane >> 4, r = lane & 15;
-    // The KV head varies fastest: with 8 of them each XCD reads one head's rows.
     uint32_t bx = blockIdx.x;
     const uint32_t kvh = bx % a.kv_heads;
     bx /= a.kv_heads;
     const uint32_t hg = bx % p.tile_head_groups;
-    // (A prompt's last queries attend the most: they start first.)
     const uint32_t tile = p.row_tiles - 1 - bx / p.tile_head_groups;
-    const uint32_t qa = tile * p.tile_queries;
-    const uint32_t heads = p.tile_head_groups > 1 ? 16 * NR : a.group;  // rows of a query in this tile
-    sglkv_u16x8 qf[NR][DKC];
-    uint64_t start[NR];
-    uint32_t len[NR], req[NR], row[NR];
-    float m[NR], l[NR];
-#pragma unroll
-    for (uint32_t n = 0; n < NR; ++n) {
-        const uint32_t rho = 16 * n + r, qi = rho / heads, hi = hg * 16 * NR + rho - qi * heads;
-        const uint32_t q = qa + qi;
-        const bool own = qi < p.tile_queries && q < a.query_count && hi < a.group;
-        uint64_t n64 = 0;
-        start[n] = 0;
-        if (own) wgt_query(p, q, g == 0 && hi == 0 && kvh == 0 && blockIdx.y == 0, &start[n], &n64);
-        len[n] = static_cast<uint32_t>(n64);  // (the host bounds it)
-        req[n] = n64 ? a.query_request_indices[q] : ~0u;
-        row[n] = own ? q * a.query_heads + kvh * a.group + hi : ~0u;
-        m[n] = -3.402823466e+38f;
-        l[n] = 0.0f;
-        const uint64_t at = reinterpret_cast<uint64_t>(a.queries) + 2ull * (own ? row[n] : 0) * (32 * DKC) + 16 * g;
-#pragma unroll
-        for (uint32_t c = 0; c < DKC; ++c) qf[n][c] = sel_load(at + 64 * c);
-    }
+    wgt_row_set<1, DKC> w;
+    wgt_load_row_set<DKC, 1>(p, tile * p.tile_queries, hg * 16, p.tile_head_groups > 1 ? 16 : a.group, 0, kvh, w);
     const uint64_t kbase = reinterpret_cast<uint64_t>(a.pool) + a.key_offset + kvh * a.key_head_stride;
     const uint32_t t0 = blockIdx.y * static_cast<uint32_t>(a.chunk_tokens);
-    // One request after another (nearly always there is one).
-    uint32_t seen = 0;  // bit n: row n's request has been taken
-    for (;;) {
-        uint32_t now = ~0u;
-#pragma unroll
-        for (uint32_t n = 0; n < NR; ++n)
-            if (!(seen >> n & 1) && req[n] < now) now = req[n];
-#pragma unroll
-        for (uint32_t s = 1; s < 64; s <<= 1) {
-            const uint32_t o = __shfl_xor(now, s);
-            now = o < now ? o : now;
-        }
+    uint32_t seen = 0;
+    for (;;) {  // one request after another (nearly always there is one)
+        const uint32_t now = wgt_next_request<1>(w.req, seen);
         if (now == ~0u) break;
-        uint32_t limit[NR], longest = 0, whole = ~0u;
-        uint64_t first = 0;
-#pragma unroll
-        for (uint32_t n = 0; n < NR; ++n) {
-            const bool in = req[n] == now;
-            limit[n] = in ? len[n] : 0;
-            if (in) {
-                seen |= 1u << n;
-                first = start[n];
-            }
-            longest = limit[n] > longest ? limit[n] : longest;
-            if (row[n] != ~0u && limit[n] < whole) whole = limit[n];  // (a row of no query may hold anything)
-        }
-#pragma unroll
-        for (uint32_t s = 1; s < 64; s <<= 1) {
-            const uint32_t x = __shfl_xor(longest, s), y = __shfl_xor(whole, s);
-            const uint64_t z = __shfl_xor(first, s);
-            longest = x > longest ? x : longest;
-            whole = y < whole ? y : whole;
-            first = z > first ? z : first;
-        }
-        longest = __builtin_amdgcn_readfirstlane(longest);
-        whole = __builtin_amdgcn_readfirstlane(whole);
+        uint32_t limit[1], longest, whole;
+        wgt_take_request<1>(w, now, seen, limit, &longest, &whole);
+        const uint64_t first = a.request_slot_offsets[__builtin_amdgcn_readfirstlane(now)];
         const uint32_t most = t0 + static_cast<uint32_t>(a.chunk_tokens), t1 = longest < most ? longest : most;
         if (t0 >= t1) continue;
         uint64_t rows = wgt_rows_at(a, kbase, first, t0, t1, kvh == 0);
+        sglkv_u16x8 kf[2][TB][DKC];
+#pragma unroll
+        for (uint32_t b = 0; b < TB; ++b) wgt_load_rows<DKC>(rows, b, g, r, kf[0][b]);
         for (uint32_t t = t0; t < t1; t += 64) {
-            const uint64_t next = t + 64 < t1 ? wgt_rows_at(a, kbase, first, t + 64, t1, kvh == 0) : rows;
+            const uint64_t next = t + 64 < t1 ? wgt_rows_at(a, kbase, first, t + 64, t1, kvh == 0)
+                                              : reinterpret_cast<uint64_t>(p.a.zero_row);
 #pragma unroll
-            for (uint32_t half = 0; half < 4; half += TB) {
-                if (t + 16 * half >= t1) break;
-                sglkv_u16x8 kf[TB][DKC];
-#pragma unroll
-                for (uint32_t b = 0; b < TB; ++b) wgt_load_rows<DKC>(rows, half + b, g, r, kf[b]);
+            for (uint32_t part = 0; part < 4 / TB; ++part) {
+                static_assert(TB == 1 || TB == 2, "the buffers come round with every 64 tokens");
 #pragma unroll
                 for (uint32_t b = 0; b < TB; ++b) {
-                    const uint32_t tt = t + 16 * (half + b) + 4 * g;  // this lane's tokens
-                    sglkv_f32x4 sc[NR];
-#pragma unroll
-                    for (uint32_t n = 0; n < NR; ++n) {
-                        sc[n] = sglkv_f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                        for (uint32_t c = 0; c < DKC; ++c)
-                            sc[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(attn_as_bf16(kf[b][c]), attn_as_bf16(qf[n][c]),
-                                                                            sc[n], 0, 0, 0);
-                    }
-                    bool moves = false;
-#pragma unroll
-                    for (uint32_t n = 0; n < NR; ++n) {
-#pragma unroll
-                        for (uint32_t e = 0; e < 4; ++e) sc[n][e] *= a.scale_log2;
-                        if (STORE) {
-                            if (tt < limit[n])
-                                *reinterpret_cast<sglkv_f32x4 *>(p.scores + row[n] * p.score_stride + tt) = sc[n];
-                        }
-                    }
-                    if (t + 16 * (half + b) + 16 > whole) {
-#pragma unroll
-                        for (uint32_t n = 0; n < NR; ++n)
-#pragma unroll
-                            for (uint32_t e = 0; e < 4; ++e)
-                                if (tt + e >= limit[n]) sc[n][e] = -INFINITY;
-                    }
-                    // The maximum moves only where a score passes it by more than 8 (log2
-                    // units): terms stay below 2^8 and most steps rescale nothing.
-                    float top[NR];
-#pragma unroll
-                    for (uint32_t n = 0; n < NR; ++n) {
-                        top[n] = fmaxf(fmaxf(sc[n][0], sc[n][1]), fmaxf(sc[n][2], sc[n][3]));
-                        moves |= top[n] > m[n] + 8.0f;
-                    }
-                    if (__ballot(moves)) {
-#pragma unroll
-                        for (uint32_t n = 0; n < NR; ++n) {
-                            const float up = fmaxf(m[n], top[n]);
-                            l[n] *= exp2f(m[n] - up);
-                            m[n] = up;
-                        }
-                    }
-#pragma unroll
-                    for (uint32_t n = 0; n < NR; ++n)
-#pragma unroll
-                        for (uint32_t e = 0; e < 4; ++e) l[n] += __builtin_amdgcn_exp2f(sc[n][e] - m[n]);
+                    const uint32_t ahead = part * TB + TB + b;
+                    wgt_load_rows<DKC>(ahead < 4 ? rows : next, ahead & 3, g, r, kf[1 - part % 2][b]);
                 }
+                __builtin_amdgcn_sched_barrier(0);
+                if (t + 16 * TB * part >= t1) continue;
+#pragma unroll
+                for (uint32_t b = 0; b < TB; ++b)
+                    wgt_weigh_tile<DKC, 1, STORE>(p, kf[part % 2][b], w, limit, t + 16 * (part * TB + b), whole, g);
             }
             rows = next;
         }
     }
-#pragma unroll
-    for (uint32_t n = 0; n < NR; ++n) {
-        float mm = m[n], ll = l[n];
-#pragma unroll
-        for (uint32_t s = 16; s < 64; s <<= 1) {
-            const float mo = __shfl_xor(mm, s), lo = __shfl_xor(ll, s), up = fmaxf(mm, mo);
-            ll = ll * exp2f(mm - up) + lo * exp2f(mo - up);
-            mm = up;
-        }
-        if (g == 0 && row[n] != ~0u) {
-            const bool some = t0 < len[n];
-            reinterpret_cast<float2 *>(a.partial)[static_cast<uint64_t>(row[n]) * a.splits + blockIdx.y] =
-                make_float2(some ? mm : -INFINITY, some ? ll : 0.0f);
-        }
-    }
+    wgt_leave_stats<DKC, 1>(p, w, t0, g);
 }
 
-// The queries [*q0, *q1) of request `req`, whose indices never fall: 64 places
-// probed at once, so two or three loads in a row.
+// The queries [*q0, *q1) of request `req`, whose indices never fall: 32 places
+// probed at once for either end, so three loads in a row up to 32,768 queries.
 __device__ __forceinline__ void wgt_queries_of(const sglkv_attn_params &p, uint32_t req, uint32_t *q0, uint32_t *q1) {
-    const uint32_t lane = threadIdx.x & 63;
-    uint32_t found[2];
-#pragma unroll
-    for (uint32_t k = 0; k < 2; ++k) {
-        uint32_t low = 0, high = static_cast<uint32_t>(p.query_count);  // the first index >= req + k lies in [low, high]
-        while (low < high) {
-            const uint32_t step = (high - low + 63) / 64, at = low + lane * step;
-            const uint32_t below = __popcll(__ballot(at < high && p.query_request_indices[at < high ? at : low] < req + k));
-            // (below == 0: at low itself)
-            if (below == 0) {
-                high = low;
-            } else {
-                const uint32_t from = low + (below - 1) * step + 1, to = low + below * step;
-                low = from;
-                high = to < high ? to : high;
-            }
+    const uint32_t lane = threadIdx.x & 63, side = lane >> 5, place = lane & 31;
+    uint32_t low = 0, high = static_cast<uint32_t>(p.query_count);  // the first index >= req + side lies in [low, high]
+    while (__ballot(low < high)) {
+        const uint32_t step = (high - low + 31) / 32, at = low + place * step;
+        const bool less = at < high && p.query_request_indices[at] < req + side;
+        const uint64_t all = __ballot(less);
+        const uint32_t below = __popc(static_cast<uint32_t>(side ? all >> 32 : all));
+        if (below == 0) {
+            high = low;  // (at low itself)
+        } else {
+            const uint32_t to = low + below * step;
+            low += (below - 1) * step + 1;
+            high = to < high ? to : high;
         }
-        found[k] = low;
     }
-    *q0 = found[0];
-    *q1 = found[1] > found[0] ? found[1] : found[0];  // (indices that fall have been reported)
+    *q0 = __builtin_amdgcn_readlane(low, 0);
+    const uint32_t end = __builtin_amdgcn_readlane(low, 32);
+    *q1 = end > *q0 ? end : *q0;  // (indices that fall have been reported)
 }
 
-// A row's joined statistics: the reference m and 1 / l (0: it weighs nothing).
-__device__ __forceinline__ void wgt_joined(const sglkv_attn_params &a, uint64_t row, float *m, float *inv) {
+// The splits' statistics of a row joined: the reference m and 1 / l, or (inf, 0)
+// where the row weighs nothing. `lanes` lanes to a row (a power of two up to 16),
+// this one lane v of them. (One split's statistics leave the first kernel like
+// this.)
+__device__ __forceinline__ float2 wgt_joined(const sglkv_attn_params &a, uint64_t row, uint32_t v, uint32_t lanes) {
     const float2 *stats = reinterpret_cast<const float2 *>(a.partial) + row * a.splits;
     float top = -INFINITY, l = 0.0f;
-    for (uint32_t s = 0; s < a.splits; ++s) top = fmaxf(top, stats[s].x);
-    for (uint32_t s = 0; s < a.splits; ++s)
-        if (stats[s].x != -INFINITY) l += stats[s].y * exp2f(stats[s].x - top);
-    *m = top == -INFINITY ? 0.0f : top;
-    *inv = top == -INFINITY ? 0.0f : 1.0f / l;
+    auto join = [&](float m, float x) {
+        const float up = fmaxf(top, m);
+        if (up != -INFINITY) l = l * __builtin_amdgcn_exp2f(top - up) + x * __builtin_amdgcn_exp2f(m - up);
+        top = up;
+    };
+    for (uint32_t s = v; s < a.splits; s += lanes) join(stats[s].x, stats[s].y);
+    for (uint32_t s = 1; s < lanes; s <<= 1) join(__shfl_xor(top, s), __shfl_xor(l, s));
+    return top == -INFINITY ? make_float2(INFINITY, 0.0f) : make_float2(top, 1.0f / l);
 }
 
-// Accumulation from K rows: a workgroup has TT tiles of 16 tokens of a (request,
-// KV head) in registers; its waves take the request's rows 16 at a time, and
-// their sums join in LDS, wave by wave in order.
-template <uint32_t DKC, uint32_t TT>
-__device__ __forceinline__ void wgt_accumulate_rows_body(const sglkv_weights_params &p) {
-    extern __shared__ __attribute__((aligned(16))) float wgt_sums[];
+// Each row's statistics joined into p.joined, p.join_lanes lanes to a row.
+__device__ __forceinline__ void wgt_join_body(const sglkv_weights_params &p) {
+    const uint32_t lanes = p.join_lanes, v = threadIdx.x % lanes;
+    const uint64_t row = (static_cast<uint64_t>(blockIdx.x) * SGLKV_WEIGHTS_THREADS + threadIdx.x) / lanes;
+    if (row >= p.a.query_count * p.a.query_heads) return;
+    const float2 x = wgt_joined(p.a, row, v, lanes);
+    if (v == 0) reinterpret_cast<float2 *>(p.joined)[row] = x;
+}
+
+// One workgroup's place among items * kv_heads of them. XCDs take workgroups in
+// turn: eight items go side by side, each with all its KV heads on one XCD, whose
+// L2 then holds whole token rows and query rows instead of one head's slice of
+// many (with a head to an XCD these slices, a power of two apart, meet in a few
+// of its channels).
+__device__ __forceinline__ void wgt_place(uint32_t kv_heads, uint32_t *item, uint32_t *kvh) {
+    const uint32_t b = blockIdx.x, inner = b / 8, eight = inner / kv_heads;
+    *kvh = inner - eight * kv_heads;
+    // (Which of the eight goes to which XCD turns from eight to eight, so that work
+    // that grows with a power of two in the items does not pile up on one.)
+    *item = 8 * eight + ((b + 5 * eight + eight / 8) & 7);
+}
+
+// Row pitch in LDS: 16 rows' pieces land in all banks once.
+template <uint32_t DKC>
+constexpr uint32_t kWgtPitch = 64 * DKC + 16;
+
+// Statistics of many rows: four waves of NR * 16 rows each share the K rows of 64
+// tokens through LDS, two stages deep, so K is read once for 64 NR rows.
+template <uint32_t DKC, uint32_t NR>
+__device__ __forceinline__ void wgt_tile_stats_body(const sglkv_weights_params &p) {
+    constexpr uint32_t PIECES = 4 * DKC, SIDE = 256 / PIECES, LOADS = 64 / SIDE, PITCH = kWgtPitch<DKC>;
+    __shared__ __attribute__((aligned(16))) uint8_t stages[2][64 * PITCH];
+    __shared__ uint32_t shared_words[4];
     const sglkv_attn_params &a = p.a;
-    const uint32_t lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), waves = blockDim.x / 64;
-    uint32_t bx = blockIdx.x;
-    const uint32_t kvh = bx % a.kv_heads;
-    bx /= a.kv_heads;
-    const uint32_t tile = bx % p.tiles, req = bx / p.tiles, tb = tile * 16 * TT;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, g = lane >> 4, r = lane & 15;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    uint32_t item, kvh;
+    wgt_place(a.kv_heads, &item, &kvh);
+    if (item >= p.row_tiles * p.tile_head_groups) return;
+    const uint32_t hg = item % p.tile_head_groups;
+    // (A prompt's last queries attend the most: they start first.)
+    const uint32_t tile = p.row_tiles - 1 - item / p.tile_head_groups;
+    const uint32_t heads = p.tile_head_groups > 1 ? 64 * NR : a.group;  // rows of a query in this tile
+    wgt_row_set<NR, DKC> w;
+    wgt_load_row_set<DKC, NR>(p, tile * p.tile_queries, hg * 64 * NR, heads, wave * 16 * NR, kvh, w);
+    const uint64_t kbase = reinterpret_cast<uint64_t>(a.pool) + a.key_offset + kvh * a.key_head_stride;
+    const uint32_t t0 = blockIdx.y * static_cast<uint32_t>(a.chunk_tokens);
+    const uint32_t piece = 16 * (tid % PIECES), own = tid / PIECES;  // of a row; the first token it loads
+    uint32_t seen = 0;
+    for (;;) {  // one request after another (nearly always there is one)
+        uint32_t now = wgt_next_request<NR>(w.req, seen);
+        if (lane == 0) shared_words[wave] = now;
+        __syncthreads();
+        for (uint32_t i = 0; i < 4; ++i) now = shared_words[i] < now ? shared_words[i] : now;
+        __syncthreads();
+        if (now == ~0u) break;
+        uint32_t limit[NR], longest, whole;
+        wgt_take_request<NR>(w, now, seen, limit, &longest, &whole);
+        const uint64_t first = a.request_slot_offsets[__builtin_amdgcn_readfirstlane(now)];
+        if (lane == 0) shared_words[wave] = longest;
+        __syncthreads();
+        uint32_t t1 = 0;
+        for (uint32_t i = 0; i < 4; ++i) t1 = shared_words[i] > t1 ? shared_words[i] : t1;
+        __syncthreads();
+        t1 = __builtin_amdgcn_readfirstlane(t1);
+        const uint32_t most = t0 + static_cast<uint32_t>(a.chunk_tokens);
+        t1 = t1 < most ? t1 : most;
+        if (t0 >= t1) continue;
+        sglkv_u16x8 ahead[LOADS];
+        auto load = [&](uint64_t rows) {
+#pragma unroll
+            for (uint32_t i = 0; i < LOADS; ++i) ahead[i] = sel_load(__shfl(rows, own + SIDE * i) + piece);
+        };
+        auto put = [&](uint32_t stage) {
+#pragma unroll
+            for (uint32_t i = 0; i < LOADS; ++i)
+                *reinterpret_cast<sglkv_u16x8 *>(stages[stage] + (own + SIDE * i) * PITCH + piece) = ahead[i];
+        };
+        const bool report = kvh == 0 && wave == 0;
+        load(wgt_rows_at(a, kbase, first, t0, t1, report));
+        uint64_t rows = wgt_rows_at(a, kbase, first, t0 + 64, t1, report);
+        put(0);
+        __syncthreads();
+        uint32_t stage = 0;
+        for (uint32_t t = t0; t < t1; t += 64, stage ^= 1) {
+            const bool more = t + 64 < t1;
+            if (more) {
+                load(rows);
+                rows = wgt_rows_at(a, kbase, first, t + 128, t1, report);
+            }
+            if (t < longest) {
+                const uint32_t tiles = longest - t < 64 ? (longest - t + 15) / 16 : 4;
+                for (uint32_t b = 0; b < tiles; ++b) {
+                    const uint8_t *at = stages[stage] + (16 * b + r) * PITCH + 16 * g;
+                    sglkv_u16x8 kf[DKC];
+#pragma unroll
+                    for (uint32_t c = 0; c < DKC; ++c) kf[c] = *reinterpret_cast<const sglkv_u16x8 *>(at + 64 * c);
+                    wgt_weigh_tile<DKC, NR, false>(p, kf, w, limit, t + 16 * b, whole, g);
+                }
+            }
+            if (more) {
+                put(stage ^ 1);
+                __syncthreads();
+            }
+        }
+        __syncthreads();  // (the next request's first stage)
+    }
+    wgt_leave_stats<DKC, NR>(p, w, t0, g);
+}
+
+// Accumulation of many rows: a wave has TT tiles of 16 tokens of a (request, KV
+// head) in registers, a workgroup four waves' side by side; the request's rows
+// (or a segment's) pass through LDS, 32 at a time and two stages deep.
+template <uint32_t DKC, uint32_t TT>
+__device__ __forceinline__ void wgt_tile_accumulate_body(const sglkv_weights_params &p) {
+    constexpr uint32_t ROWS = 32, PIECES = 4 * DKC, SIDE = 256 / PIECES, LOADS = ROWS / SIDE, PITCH = kWgtPitch<DKC>;
+    struct info {
+        float m, inv;
+        uint64_t length;
+    };
+    __shared__ __attribute__((aligned(16))) uint8_t stages[2][ROWS * PITCH];
+    __shared__ info infos[2][ROWS];
+    __shared__ uint32_t extents[2][4];
+    const sglkv_attn_params &a = p.a;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, g = lane >> 4, r = lane & 15;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    uint32_t item, kvh;
+    wgt_place(a.kv_heads, &item, &kvh);
+    const uint32_t requests = static_cast<uint32_t>(a.request_count);
+    const uint32_t segment = item % p.segments, tile = item / p.segments / requests;
+    const uint32_t req = item / p.segments - tile * requests, tg = tile * 64 * TT, tb = tg + wave * 16 * TT;
+    if (tile >= p.tiles) return;
     const uint64_t start = a.request_slot_offsets[req], end = a.request_slot_offsets[req + 1];
-    if (start > end || end > a.sequence_slot_count || tb >= end - start) return;
+    if (start > end || end > a.sequence_slot_count || tg >= end - start) return;
     uint32_t q0, q1;
     wgt_queries_of(a, req, &q0, &q1);
+    // (A segment of the request's queries: its sums go to the workspace.)
+    const uint32_t share = (q1 - q0 + p.segments - 1) / p.segments;
+    q0 = q1 - q0 > segment * share ? q0 + segment * share : q1;
+    q1 = q1 - q0 > share ? q0 + share : q1;
+    // (A length that does not hold has been reported: its row weighs nothing.)
     const uint64_t most = end - start < p.max_length ? end - start : p.max_length;
-    auto length_of = [&](uint32_t q) {
-        const uint64_t n = a.query_sequence_lengths[q];
-        return n <= most && a.query_request_indices[q] == req ? static_cast<uint32_t>(n) : 0;
-    };
-    // The tokens that any query attends, and the first query that attends this tile.
+    // The tokens that any of these queries attends, and the first that attends
+    // this tile: every wave looks at its share of the lengths.
     uint32_t longest = 0, q_from = q1;
-    for (uint32_t q = q0 + lane; q < q1; q += 64) {
-        const uint32_t n = length_of(q);
+    for (uint32_t q = q0 + tid; q < q1; q += 256) {
+        const uint64_t n64 = a.query_sequence_lengths[q];
+        const uint32_t n = n64 <= most ? static_cast<uint32_t>(n64) : 0;
         longest = n > longest ? n : longest;
-        if (n > tb && q < q_from) q_from = q;
+        if (n > tg && q < q_from) q_from = q;
     }
 #pragma unroll
     for (uint32_t s = 1; s < 64; s <<= 1) {
@@ -469,56 +663,121 @@ __device__ __forceinline__ void wgt_accumulate_rows_body(const sglkv_weights_par
         longest = x > longest ? x : longest;
         q_from = y < q_from ? y : q_from;
     }
+    if (lane == 0) {
+        extents[0][wave] = longest;
+        extents[1][wave] = q_from;
+    }
+    __syncthreads();
+    for (uint32_t i = 0; i < 4; ++i) {
+        longest = extents[0][i] > longest ? extents[0][i] : longest;
+        q_from = extents[1][i] < q_from ? extents[1][i] : q_from;
+    }
     longest = __builtin_amdgcn_readfirstlane(longest);
     q_from = __builtin_amdgcn_readfirstlane(q_from);
-    if (tb >= longest) return;
-    const uint64_t kbase = reinterpret_cast<uint64_t>(a.pool) + a.key_offset + kvh * a.key_head_stride;
-    const uint64_t at = wgt_rows_at(a, kbase, start, tb, longest, false);
-    sglkv_u16x8 kf[TT][DKC];
-#pragma unroll
-    for (uint32_t b = 0; b < TT; ++b) wgt_load_rows<DKC>(at, b, g, r, kf[b]);
     float sum[TT][4] = {};
-    // Rows rho = (query - q_from) * group + head; this wave's 16 w, 16 (w + waves), ...
-    const uint32_t count = (q1 - q_from) * a.group, step = 16 * waves, dq = step / a.group, dh = step - dq * a.group;
-    uint32_t rho = 16 * wave + r, q = q_from + rho / a.group, h = rho % a.group;
-    for (uint32_t first = 16 * wave; first < count; first += step) {
-        const bool own = rho < count;
-        const uint32_t n = own ? length_of(q) : 0;
-        const uint64_t row = own ? static_cast<uint64_t>(q) * a.query_heads + kvh * a.group + h : 0;
-        rho += step;
-        q += dq;
-        h += dh;
-        if (h >= a.group) {
-            h -= a.group;
-            ++q;
+    if (tg < longest) {
+        const uint64_t kbase = reinterpret_cast<uint64_t>(a.pool) + a.key_offset + kvh * a.key_head_stride;
+        const uint64_t at = wgt_rows_at(a, kbase, start, tb, longest, false);
+        sglkv_u16x8 kf[TT][DKC];
+#pragma unroll
+        for (uint32_t b = 0; b < TT; ++b) wgt_load_rows<DKC>(at, b, g, r, kf[b]);
+        // Rows rho = (query - q_from) * group + head. A thread's pieces of a stage are
+        // rows own + SIDE i; a row past the last is the first, weighed 0.
+        const uint32_t count = (q1 - q_from) * a.group, dq = ROWS / a.group, dh = ROWS - dq * a.group;
+        const uint32_t piece = 16 * (tid % PIECES), own = tid / PIECES;
+        const uint64_t qbase = reinterpret_cast<uint64_t>(a.queries) + piece;
+        const uint32_t head0 = kvh * a.group;
+        uint32_t rq[LOADS + 1], rh[LOADS + 1];  // the last: row tid's, for its statistics
+#pragma unroll
+        for (uint32_t i = 0; i <= LOADS; ++i) {
+            const uint32_t rho = i < LOADS ? own + SIDE * i : tid & (ROWS - 1);
+            rq[i] = rho / a.group;
+            rh[i] = rho - rq[i] * a.group;
         }
-        const uint32_t limit = n <= tb ? 0 : n - tb;
-        if (!__ballot(limit > 0)) continue;
-        const uint64_t from = reinterpret_cast<uint64_t>(a.queries) + row * (64 * DKC) + 16 * g;
-        sglkv_u16x8 qf[DKC];
+        sglkv_u16x8 ahead[LOADS];
+        info next;
+        auto load = [&] {
+            const uint32_t last = q1 - q_from;
 #pragma unroll
-        for (uint32_t c = 0; c < DKC; ++c) qf[c] = sel_load(from + 64 * c);
-        float m, inv;
-        wgt_joined(a, row, &m, &inv);
-        if (limit == 0) inv = 0.0f;
-        const bool whole = !__ballot(limit < 16 * TT);
-#pragma unroll
-        for (uint32_t b = 0; b < TT; ++b) {
-            sglkv_f32x4 sc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (uint32_t c = 0; c < DKC; ++c)
-                sc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(attn_as_bf16(kf[b][c]), attn_as_bf16(qf[c]), sc, 0, 0, 0);
-#pragma unroll
-            for (uint32_t e = 0; e < 4; ++e) sc[e] = fmaf(sc[e], a.scale_log2, -m);
-            if (!whole) {
-#pragma unroll
-                for (uint32_t e = 0; e < 4; ++e)
-                    if (16 * b + 4 * g + e >= limit) sc[e] = -INFINITY;
+            for (uint32_t i = 0; i <= LOADS; ++i) {
+                const bool in = rq[i] < last;
+                const uint64_t q = q_from + (in ? rq[i] : 0), row = q * a.query_heads + head0 + (in ? rh[i] : 0);
+                if (i < LOADS) {
+                    ahead[i] = sel_load(qbase + row * (64 * DKC));
+                } else if (tid < ROWS) {
+                    const float2 x = reinterpret_cast<const float2 *>(p.joined)[row];
+                    const uint64_t n = a.query_sequence_lengths[q];
+                    next = info{x.x, x.y, in && n <= most ? n : 0};
+                }
+                rq[i] += dq;
+                rh[i] += dh;
+                if (rh[i] >= a.group) {
+                    rh[i] -= a.group;
+                    ++rq[i];
+                }
             }
+        };
+        auto put = [&](uint32_t stage) {
 #pragma unroll
-            for (uint32_t e = 0; e < 4; ++e) sum[b][e] = fmaf(__builtin_amdgcn_exp2f(sc[e]), inv, sum[b][e]);
+            for (uint32_t i = 0; i < LOADS; ++i)
+                *reinterpret_cast<sglkv_u16x8 *>(stages[stage] + (own + SIDE * i) * PITCH + piece) = ahead[i];
+            if (tid < ROWS) infos[stage][tid] = next;
+        };
+        load();
+        put(0);
+        __syncthreads();
+        uint32_t stage = 0;
+        for (uint32_t done = 0; done < count; done += ROWS, stage ^= 1) {
+            const bool more = done + ROWS < count;
+            if (more) load();
+#pragma unroll
+            for (uint32_t n = 0; n < ROWS / 16; ++n) {
+                const info x = infos[stage][16 * n + r];
+                const uint64_t past = x.length > tb ? x.length - tb : 0;
+                const uint32_t limit = past < 16 * TT ? static_cast<uint32_t>(past) : 16 * TT;
+                if (!__ballot(limit > 0)) continue;
+                const bool whole = !__ballot(limit < 16 * TT);
+                const float inv = limit > 0 ? x.inv : 0.0f;
+                const uint8_t *from = stages[stage] + (16 * n + r) * PITCH + 16 * g;
+                sglkv_u16x8 qf[DKC];
+#pragma unroll
+                for (uint32_t c = 0; c < DKC; ++c) qf[c] = *reinterpret_cast<const sglkv_u16x8 *>(from + 64 * c);
+                sglkv_f32x4 sc[TT];
+#pragma unroll
+                for (uint32_t b = 0; b < TT; ++b) sc[b] = sglkv_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (uint32_t c = 0; c < DKC; ++c)
+#pragma unroll
+                    for (uint32_t b = 0; b < TT; ++b)
+                        sc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(attn_as_bf16(kf[b][c]), attn_as_bf16(qf[c]), sc[b], 0,
+                                                                        0, 0);
+                if (whole) {
+#pragma unroll
+                    for (uint32_t b = 0; b < TT; ++b)
+#pragma unroll
+                        for (uint32_t e = 0; e < 4; ++e)
+                            sum[b][e] =
+                                fmaf(__builtin_amdgcn_exp2f(fmaf(sc[b][e], a.scale_log2, -x.m)), inv, sum[b][e]);
+                } else {
+#pragma unroll
+                    for (uint32_t b = 0; b < TT; ++b)
+#pragma unroll
+                        for (uint32_t e = 0; e < 4; ++e) {
+                            const float y =
+                                16 * b + 4 * g + e < limit ? fmaf(sc[b][e], a.scale_log2, -x.m) : -INFINITY;
+                            sum[b][e] = fmaf(__builtin_amdgcn_exp2f(y), inv, sum[b][e]);
+                        }
+                }
+            }
+            if (more) {
+                put(stage ^ 1);
+                __syncthreads();
+            }
         }
+    } else if (p.segments == 1) {
+        return;
     }
+    // The 16 lanes of a token join; a segment writes all of its tokens.
 #pragma unroll
     for (uint32_t b = 0; b < TT; ++b)
 #pragma unroll
@@ -528,21 +787,42 @@ __device__ __forceinline__ void wgt_accumulate_rows_body(const sglkv_weights_par
             x += __uint_as_float(sel_join<2>(__float_as_uint(x)));
             x += __uint_as_float(sel_join<4>(__float_as_uint(x)));
             x += __uint_as_float(sel_join<8>(__float_as_uint(x)));
-            if (r == 0) wgt_sums[wave * 16 * TT + 16 * b + 4 * g + e] = x;
+            const uint32_t t = tb + 16 * b + 4 * g + e;
+            if (r != 0) continue;
+            const uint64_t to = kvh * a.sequence_slot_count + start + t;
+            if (p.segments > 1) {
+                if (t < end - start) p.partial_sums[segment * a.kv_heads * a.sequence_slot_count + to] = x;
+            } else if (t < longest) {
+                p.weights[to] += x;
+            }
         }
-    __syncthreads();
-    if (threadIdx.x < 16 * TT && tb + threadIdx.x < longest) {
-        float x = 0.0f;
-        for (uint32_t w = 0; w < waves; ++w) x += wgt_sums[w * 16 * TT + threadIdx.x];
-        p.weights[kvh * a.sequence_slot_count + start + tb + threadIdx.x] += x;
-    }
 }
 
-// Accumulation from kept scores: a thread to a token of a (request, KV head),
-// its (query, head)s in turn.
+// The segments' sums, in order, added to the weights: a thread to a position of
+// a request.
+__device__ __forceinline__ void wgt_segments_body(const sglkv_weights_params &p) {
+    const sglkv_attn_params &a = p.a;
+    uint32_t bx = blockIdx.x;
+    const uint32_t kvh = bx % a.kv_heads;
+    bx /= a.kv_heads;
+    const uint32_t blocks = (p.max_length + SGLKV_WEIGHTS_THREADS - 1) / SGLKV_WEIGHTS_THREADS;
+    const uint32_t req = bx / blocks;
+    const uint64_t t = static_cast<uint64_t>(bx - req * blocks) * SGLKV_WEIGHTS_THREADS + threadIdx.x;
+    const uint64_t start = a.request_slot_offsets[req], end = a.request_slot_offsets[req + 1];
+    if (start > end || end > a.sequence_slot_count || t >= end - start || t >= p.max_length) return;
+    const uint64_t at = kvh * a.sequence_slot_count + start + t;
+    float x = 0.0f;
+    for (uint32_t s = 0; s < p.segments; ++s) x += p.partial_sums[s * a.kv_heads * a.sequence_slot_count + at];
+    if (x != 0.0f) p.weights[at] += x;  // (NaN is added; nothing leaves a position as it is)
+}
+
+// Accumulation from kept scores: a workgroup has SGLKV_WEIGHTS_APPLY tokens of a
+// (request, KV head), a thread every SGLKV_WEIGHTS_THREADS-th of them, its
+// (query, head)s in turn.
 __device__ __forceinline__ void wgt_apply_body(const sglkv_weights_params &p) {
-    __shared__ float2 joined[SGLKV_WEIGHTS_APPLY];
-    __shared__ uint32_t limits[SGLKV_WEIGHTS_APPLY];
+    constexpr uint32_t THREADS = SGLKV_WEIGHTS_THREADS, EACH = SGLKV_WEIGHTS_APPLY / THREADS, ROWS = THREADS / 16;
+    __shared__ float2 joined[ROWS];
+    __shared__ uint32_t limits[ROWS];
     const sglkv_attn_params &a = p.a;
     const uint32_t tid = threadIdx.x;
     uint32_t bx = blockIdx.x;
@@ -554,35 +834,48 @@ __device__ __forceinline__ void wgt_apply_body(const sglkv_weights_params &p) {
     uint32_t q0, q1;
     wgt_queries_of(a, req, &q0, &q1);
     const uint64_t most = end - start < p.max_length ? end - start : p.max_length;
-    const uint32_t count = (q1 - q0) * a.group, t = tb + tid;
-    float sum = 0.0f;
-    bool any = false;
-    for (uint32_t base = 0; base < count; base += SGLKV_WEIGHTS_APPLY) {
-        const uint32_t here = count - base < SGLKV_WEIGHTS_APPLY ? count - base : SGLKV_WEIGHTS_APPLY;
+    const uint32_t count = (q1 - q0) * a.group;
+    float sum[EACH] = {};
+    uint32_t longest = 0;
+    for (uint32_t base = 0; base < count; base += ROWS) {
+        const uint32_t here = count - base < ROWS ? count - base : ROWS;
         __syncthreads();
-        if (tid < here) {
-            const uint32_t q = q0 + (base + tid) / a.group, h = (base + tid) % a.group;
-            const uint64_t n = a.query_sequence_lengths[q];
-            const bool own = n <= most && a.query_request_indices[q] == req;
-            limits[tid] = own ? static_cast<uint32_t>(n) : 0;
-            wgt_joined(a, static_cast<uint64_t>(q) * a.query_heads + kvh * a.group + h, &joined[tid].x, &joined[tid].y);
+        // 16 lanes to a row: its splits' statistics joined.
+        const uint32_t i = tid / 16, v = tid % 16;
+        if (i < here) {
+            const uint32_t q = q0 + (base + i) / a.group, h = (base + i) % a.group;
+            const uint64_t row = static_cast<uint64_t>(q) * a.query_heads + kvh * a.group + h;
+            const float2 x = a.splits == 1 ? reinterpret_cast<const float2 *>(a.partial)[row] : wgt_joined(a, row, v, 16);
+            if (v == 0) {
+                const uint64_t n = a.query_sequence_lengths[q];
+                limits[i] = n <= most && a.query_request_indices[q] == req ? static_cast<uint32_t>(n) : 0;
+                joined[i] = x;
+            }
         }
         __syncthreads();
         uint32_t q = q0 + base / a.group, h = base % a.group;
 #pragma unroll 4
-        for (uint32_t i = 0; i < here; ++i) {
-            const uint64_t row = static_cast<uint64_t>(q) * a.query_heads + kvh * a.group + h;
+        for (uint32_t j = 0; j < here; ++j) {
+            const float *scores = p.scores + (static_cast<uint64_t>(q) * a.query_heads + kvh * a.group + h) * p.score_stride;
             if (++h == a.group) {
                 h = 0;
                 ++q;
             }
-            if (t < limits[i]) {
-                any = true;
-                sum = fmaf(__builtin_amdgcn_exp2f(p.scores[row * p.score_stride + t] - joined[i].x), joined[i].y, sum);
+            const uint32_t limit = limits[j];
+            const float2 stats = joined[j];
+            longest = limit > longest ? limit : longest;
+#pragma unroll
+            for (uint32_t e = 0; e < EACH; ++e) {
+                const uint32_t t = tb + THREADS * e + tid;
+                if (t < limit) sum[e] = fmaf(__builtin_amdgcn_exp2f(scores[t] - stats.x), stats.y, sum[e]);
             }
         }
     }
-    if (any) p.weights[kvh * a.sequence_slot_count + start + t] += sum;
+#pragma unroll
+    for (uint32_t e = 0; e < EACH; ++e) {
+        const uint32_t t = tb + THREADS * e + tid;
+        if (t < longest) p.weights[kvh * a.sequence_slot_count + start + t] += sum[e];
+    }
 }
 
 // ---- The kept positions -----------------------------------------------------
@@ -720,43 +1013,49 @@ sglkv_accumulate_weights_v2(sglkv_weights_params p) {
     wgt_accumulate_body<false>(p);
 }
 
-extern "C" __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void sglkv_weight_rows64(sglkv_weights_params p) {
-    wgt_rows_body<2, 4, 2, false>(p);
+extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void sglkv_weight_rows64(sglkv_weights_params p) {
+    wgt_tile_stats_body<2, 4>(p);
 }
 extern "C" __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void sglkv_weight_few64(sglkv_weights_params p) {
-    wgt_rows_body<2, 1, 4, false>(p);
+    wgt_rows_body<2, 2, false>(p);
 }
 extern "C" __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void sglkv_weight_scores64(sglkv_weights_params p) {
-    wgt_rows_body<2, 1, 4, true>(p);
+    wgt_rows_body<2, 2, true>(p);
 }
-extern "C" __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void sglkv_accumulate_rows64(sglkv_weights_params p) {
-    wgt_accumulate_rows_body<2, 4>(p);
+extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void sglkv_accumulate_rows64(sglkv_weights_params p) {
+    wgt_tile_accumulate_body<2, 4>(p);
 }
-extern "C" __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void sglkv_weight_rows128(sglkv_weights_params p) {
-    wgt_rows_body<4, 4, 2, false>(p);
+extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void sglkv_weight_rows128(sglkv_weights_params p) {
+    wgt_tile_stats_body<4, 4>(p);
 }
 extern "C" __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void sglkv_weight_few128(sglkv_weights_params p) {
-    wgt_rows_body<4, 1, 4, false>(p);
+    wgt_rows_body<4, 2, false>(p);
 }
 extern "C" __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void sglkv_weight_scores128(sglkv_weights_params p) {
-    wgt_rows_body<4, 1, 4, true>(p);
+    wgt_rows_body<4, 2, true>(p);
 }
-extern "C" __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void sglkv_accumulate_rows128(sglkv_weights_params p) {
-    wgt_accumulate_rows_body<4, 4>(p);
+extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void sglkv_accumulate_rows128(sglkv_weights_params p) {
+    wgt_tile_accumulate_body<4, 4>(p);
 }
-extern "C" __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void sglkv_weight_rows256(sglkv_weights_params p) {
-    wgt_rows_body<8, 2, 1, false>(p);
+extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void sglkv_weight_rows256(sglkv_weights_params p) {
+    wgt_tile_stats_body<8, 2>(p);
 }
 extern "C" __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void sglkv_weight_few256(sglkv_weights_params p) {
-    wgt_rows_body<8, 1, 2, false>(p);
+    wgt_rows_body<8, 1, false>(p);
 }
 extern "C" __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void sglkv_weight_scores256(sglkv_weights_params p) {
-    wgt_rows_body<8, 1, 2, true>(p);
+    wgt_rows_body<8, 1, true>(p);
 }
-extern "C" __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void sglkv_accumulate_rows256(sglkv_weights_params p) {
-    wgt_accumulate_rows_body<8, 2>(p);
+extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void sglkv_accumulate_rows256(sglkv_weights_params p) {
+    wgt_tile_accumulate_body<8, 2>(p);
 }
-extern "C" __global__ __launch_bounds__(SGLKV_WEIGHTS_APPLY) void sglkv_apply_scores(sglkv_weights_params p) {
+extern "C" __global__ __launch_bounds__(SGLKV_WEIGHTS_THREADS) void sglkv_add_segments(sglkv_weights_params p) {
+    wgt_segments_body(p);
+}
+extern "C" __global__ __launch_bounds__(SGLKV_WEIGHTS_THREADS) void sglkv_join_statistics(sglkv_weights_params p) {
+    wgt_join_body(p);
+}
+extern "C" __global__ __launch_bounds__(SGLKV_WEIGHTS_THREADS) void sglkv_apply_scores(sglkv_weights_params p) {
     wgt_apply_body(p);
 }
 

@@ -166,7 +166,7 @@ struct sgl_rocm_kv_ctx {
     hipFunction_t accumulate_weights[2];
     // dims 64, 128, 256: statistics of many rows, of few, of few with their scores; the accumulation
     hipFunction_t weight_rows[3][4];
-    hipFunction_t apply_scores;
+    hipFunction_t join_statistics, add_segments, apply_scores;
     hipFunction_t select_tokens;
     hipFunction_t compact_tokens[4];      // pieces of 16, 4, 2 and 1 bytes
     uint32_t attention_occupancy[15];     // resident workgroups per CU of attention[i] ...

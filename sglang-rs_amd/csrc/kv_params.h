@@ -417,17 +417,22 @@ typedef struct sglkv_select_params {
  * queries: weights[kv head][position] += ..., positions numbered as
  * sequence_slots. `a` as for paged attention; its partial holds a (maximum, sum)
  * pair of 32-bit floats per (query, head, split), in log2 units. */
-#define SGLKV_WEIGHTS_TILE 64u    /* tokens of a tile of the accumulation (32 at dims 256) */
-#define SGLKV_WEIGHTS_APPLY 256u  /* tokens (and threads) of a workgroup that applies kept scores */
+#define SGLKV_WEIGHTS_TILE 64u    /* tokens of a wave of the accumulation (32 at dims 256) */
+#define SGLKV_WEIGHTS_THREADS 256u
+#define SGLKV_WEIGHTS_APPLY 1024u /* tokens of a workgroup that applies kept scores */
 typedef struct sglkv_weights_params {
     sglkv_attn_params a;
     float *weights;
+    float *joined;            /* a pair per (query, head): its splits' statistics joined, m and 1 / sum */
     float *scores;            /* [query][query head][score_stride] scores in log2 units, or null */
     uint64_t max_length;      /* the longest query length that the launch covers */
     uint64_t score_stride;    /* a multiple of 64 */
     uint32_t tiles;           /* token tiles of a sequence of max_length */
     uint32_t row_tiles;       /* rows bodies: tiles of queries */
     uint32_t tile_queries;    /* queries of one */
+    uint32_t segments;        /* accumulation: parts of a request's queries, a workgroup to each */
+    uint32_t join_lanes;      /* threads to a row's splits: a power of two up to 16 */
+    float *partial_sums;      /* [segment][kv head][sequence_slot_count], or null */
     uint32_t tile_head_groups;/* groups of a KV head's query heads, where one query's rows pass a tile */
 } sglkv_weights_params;
 

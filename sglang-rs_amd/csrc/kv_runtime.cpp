@@ -597,6 +597,8 @@ extern "C" int32_t sgl_rocm_kv_init(int32_t device, const char *code_object_path
                      {"sglkv_weight_few256", &ctx->weight_rows[2][1]},
                      {"sglkv_weight_scores256", &ctx->weight_rows[2][2]},
                      {"sglkv_accumulate_rows256", &ctx->weight_rows[2][3]},
+                     {"sglkv_join_statistics", &ctx->join_statistics},
+                     {"sglkv_add_segments", &ctx->add_segments},
                      {"sglkv_apply_scores", &ctx->apply_scores},
                      {"sglkv_select_tokens", &ctx->select_tokens},
                      {"sglkv_compact_tokens_v16", &ctx->compact_tokens[0]},
