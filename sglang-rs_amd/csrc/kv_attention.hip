@@ -2028,6 +2028,39 @@ __device__ __forceinline__ void attn_stg_softmax_pv(const sglkv_attn_params &p, 
     }
 }
 
+// One staged block: q.k from the stage's K rows, then attn_stg_softmax_pv over its
+// first nv tokens.
+template <uint32_t D>
+__device__ __forceinline__ void attn_stg_block(const sglkv_attn_params &p, uint32_t g, uint32_t r,
+                                               const sglkv_u16x8 (&qf)[attn_stg<D>::KC], const uint8_t *kst, uint32_t nv,
+                                               attn_state_n<attn_stg<D>::NJ> &st) {
+    typedef attn_stg<D> S;
+    // The K reads of a group of q.k steps first, then the two score
+    // tiles' MFMA chains interleaved (groups of 4 steps at dims 256, to
+    // bound the registers the reads hold).
+    constexpr uint32_t KG = S::KC > 4 ? 4 : S::KC;
+    sglkv_f32x4 sc[2] = {sglkv_f32x4{0.f, 0.f, 0.f, 0.f}, sglkv_f32x4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+    for (uint32_t c0 = 0; c0 < S::KC; c0 += KG) {
+        sglkv_u16x8 kf[2][KG];
+#pragma unroll
+        for (uint32_t b = 0; b < 2; ++b) {
+            const uint32_t t = 8 * (r >> 2) + 4 * b + (r & 3);
+#pragma unroll
+            for (uint32_t c = 0; c < KG; ++c)
+                kf[b][c] = *reinterpret_cast<const sglkv_u16x8 *>(kst + S::ROW * t +
+                                                                  16 * S::kpos(t, 4 * (c0 + c) + g));
+        }
+#pragma unroll
+        for (uint32_t c = 0; c < KG; ++c)
+#pragma unroll
+            for (uint32_t b = 0; b < 2; ++b)
+                sc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(attn_as_bf16(kf[b][c]), attn_as_bf16(qf[c0 + c]),
+                                                                sc[b], 0, 0, 0);
+    }
+    attn_stg_softmax_pv<D>(p, g, r, sc, nv, kst + S::V, st);
+}
+
 template <uint32_t D, bool LIVE>
 __device__ __forceinline__ void attn_staged_body(const sglkv_attn_params &p) {
     typedef attn_stg<D> S;
@@ -2082,31 +2115,8 @@ __device__ __forceinline__ void attn_staged_body(const sglkv_attn_params &p) {
         attn_stg_slots<D>(blk(k + 2), lane, sl);
         asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * S::LOADS) : "memory");
         const uint8_t *kst = stage(k);
-        // The K reads of a group of q.k steps first, then the two score
-        // tiles' MFMA chains interleaved (groups of 4 steps at dims 256, to
-        // bound the registers the reads hold).
-        constexpr uint32_t KG = S::KC > 4 ? 4 : S::KC;
-        sglkv_f32x4 sc[2] = {sglkv_f32x4{0.f, 0.f, 0.f, 0.f}, sglkv_f32x4{0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-        for (uint32_t c0 = 0; c0 < S::KC; c0 += KG) {
-            sglkv_u16x8 kf[2][KG];
-#pragma unroll
-            for (uint32_t b = 0; b < 2; ++b) {
-                const uint32_t t = 8 * (r >> 2) + 4 * b + (r & 3);
-#pragma unroll
-                for (uint32_t c = 0; c < KG; ++c)
-                    kf[b][c] = *reinterpret_cast<const sglkv_u16x8 *>(kst + S::ROW * t +
-                                                                      16 * S::kpos(t, 4 * (c0 + c) + g));
-            }
-#pragma unroll
-            for (uint32_t c = 0; c < KG; ++c)
-#pragma unroll
-                for (uint32_t b = 0; b < 2; ++b)
-                    sc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(attn_as_bf16(kf[b][c]), attn_as_bf16(qf[c0 + c]),
-                                                                    sc[b], 0, 0, 0);
-        }
         const uint64_t left = w.t1 - w.t0 - static_cast<uint64_t>(kLatB) * k;
-        attn_stg_softmax_pv<D>(p, g, r, sc, left < kLatB ? static_cast<uint32_t>(left) : kLatB, kst + S::V, st);
+        attn_stg_block<D>(p, g, r, qf, kst, left < kLatB ? static_cast<uint32_t>(left) : kLatB, st);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the zero-row loads issued past the chunk
     attn_finish(p, w, g, r, st);

@@ -161,6 +161,7 @@ struct sgl_rocm_kv_ctx {
     hipFunction_t page_scores[5];
     hipFunction_t pick_pages;
     hipFunction_t selected_attention[2];  // 16-byte vectors, elements
+    hipFunction_t selected_staged[3];     // dims 64, 128, 256, rows staged in LDS
     hipFunction_t selected_combine;
     hipFunction_t weight_stats[2];        // 16-byte vectors, elements
     hipFunction_t accumulate_weights[2];

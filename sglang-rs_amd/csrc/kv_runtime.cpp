@@ -580,6 +580,9 @@ extern "C" int32_t sgl_rocm_kv_init(int32_t device, const char *code_object_path
                      {"sglkv_pick_pages", &ctx->pick_pages},
                      {"sglkv_selected_attention_v16", &ctx->selected_attention[0]},
                      {"sglkv_selected_attention_v2", &ctx->selected_attention[1]},
+                     {"sglkv_selected_attention_staged64", &ctx->selected_staged[0]},
+                     {"sglkv_selected_attention_staged128", &ctx->selected_staged[1]},
+                     {"sglkv_selected_attention_staged256", &ctx->selected_staged[2]},
                      {"sglkv_selected_attention_combine", &ctx->selected_combine},
                      {"sglkv_weight_stats_v16", &ctx->weight_stats[0]},
                      {"sglkv_weight_stats_v2", &ctx->weight_stats[1]},

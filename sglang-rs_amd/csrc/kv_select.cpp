@@ -40,8 +40,20 @@ struct SelectionShape {
 // Workgroups of scores that fill the chip several times over, 64 pages or more
 // each.
 constexpr uint64_t kScoreWorkgroups = 2048;
-// Waves of the attention that fill the chip, each with 64 tokens or more.
-constexpr uint64_t kAttendWaves = 1024;
+// Waves of the attention that stay resident at once, each with 64 tokens or
+// more: what the staged body's LDS leaves room for on 256 CUs (its registers, at
+// dims 64), or the generic one's LDS.
+uint64_t attend_waves(const sgl_kv_attention_plan_config &c) {
+    return 256 * (c.value_head_dim > 128 ? 2 : c.value_head_dim > 64 ? 5 : 8);
+}
+
+// The staged body's shapes (its alignments are the call's to see).
+bool staged_shape(const sgl_kv_attention_plan_config &c) {
+    const uint64_t d = c.query_key_head_dim, page = c.layout.page_size;
+    return d == c.value_head_dim && (d == 64 || d == 128 || d == 256) && page >= 8 && (page & (page - 1)) == 0 &&
+           c.query_head_count / c.kv_head_count <= SGLKV_ATTN_HEADS && c.slot_count < (1ull << 32) &&
+           c.layout.page_stride_bytes <= UINT32_MAX;
+}
 
 int32_t selection_shape(const sgl_kv_attention_plan_config &c, const sgl_kv_page_selection_config &s,
                         SelectionShape *out) {
@@ -75,7 +87,8 @@ int32_t selection_shape(const sgl_kv_attention_plan_config &c, const sgl_kv_page
     const uint64_t head_groups = ceil_div(group, SGLKV_ATTN_HEADS), dv_blocks = ceil_div(c.value_head_dim, SGLKV_ATTN_DV);
     uint64_t base;
     if (mul_ovf(h.items, head_groups, &base) || mul_ovf(base, dv_blocks, &base)) return attention_overflow();
-    h.split_pages = ceil_div(list, base < kAttendWaves ? kAttendWaves / base : 1);
+    const uint64_t waves = attend_waves(c), shared = staged_shape(c) ? h.items : base;
+    h.split_pages = ceil_div(list, shared < waves ? waves / shared : 1);
     const uint64_t least = ceil_div(64, page);
     if (h.split_pages < least) h.split_pages = least;
     if (h.split_pages > SGLKV_SELECT_CHUNK_PAGES) h.split_pages = SGLKV_SELECT_CHUNK_PAGES;
@@ -295,9 +308,19 @@ extern "C" int32_t sgl_rocm_kv_selected_attention(sgl_rocm_kv_ctx *ctx, const sg
                          p.a.key_head_stride | p.a.key_token_stride | p.a.value_head_stride | p.a.value_token_stride) %
                                 16 == 0;
     p.chunk_pages = (uint32_t)shape.split_pages;
-    const unsigned lds = 2 * (SGLKV_ATTN_HEADS * (p.a.dk_pad + 8) + SGLKV_ATTN_DV * SGLKV_ATTN_VT_STRIDE);
-    rc = launch_kernel(ctx->selected_attention[vector ? 0 : 1], shape.items * p.a.head_groups * p.a.dv_blocks, p.a.splits, 1, 64, lds,
-                s, &p, "selected attention launch");
+    const bool staged = vector && staged_shape(plan->attention.config) && reinterpret_cast<uint64_t>(p.a.queries) % 16 == 0 &&
+                        p.a.key_token_stride == p.a.value_token_stride && p.a.key_token_stride < (1u << 24);
+    if (staged) {
+        p.a.dv_blocks = 1;
+        p.a.page_stride32 = (uint32_t)p.a.page_stride;
+        p.a.key_token_stride32 = p.a.value_token_stride32 = (uint32_t)p.a.key_token_stride;
+        rc = launch_kernel(ctx->selected_staged[p.a.dk == 64 ? 0 : p.a.dk == 128 ? 1 : 2], shape.items, p.a.splits, 1, 64,
+                           256 * p.a.dk, s, &p, "selected attention launch");
+    } else {
+        const unsigned lds = 2 * (SGLKV_ATTN_HEADS * (p.a.dk_pad + 8) + SGLKV_ATTN_DV * SGLKV_ATTN_VT_STRIDE);
+        rc = launch_kernel(ctx->selected_attention[vector ? 0 : 1], shape.items * p.a.head_groups * p.a.dv_blocks, p.a.splits,
+                           1, 64, lds, s, &p, "selected attention launch");
+    }
     if (!rc && p.a.splits > 1)
         rc = launch_kernel(ctx->selected_combine, p.a.query_count * p.a.query_heads, 1, 1, 64, 0, s, &p,
                     "selected attention combine launch");

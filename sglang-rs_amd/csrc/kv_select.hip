@@ -565,6 +565,137 @@ __device__ __forceinline__ void sel_attend_body(const sglkv_select_params &p) {
     attn_finish(a, w, g, r, st);
 }
 
+// Head dims 64, 128 or 256 of keys and values alike, 16-byte rows, pages of 8
+// tokens or more (a power of two), at most 16 query heads a KV head: the staged
+// layout of paged attention (attn_stg: rows straight from the pool into LDS, two
+// stages of 32 tokens, one wave a workgroup), which its loads' addresses are
+// cheaper for. Lane l keeps the pool page of entry l, so a load's page and first
+// token are one scalar base, and what a lane adds to it (its token of the load and
+// its swizzled piece) is the same for every block: kept at dims 64 and 128, and
+// at dims 256, whose accumulators leave no registers for it, made again from the
+// lane's part and the load's, which do not share bits (attn_stg's swizzles are
+// exclusive ors). LDS holds the two stages and nothing else, which leaves room
+// for five workgroups a CU at dims 128.
+// Four loads: lane l's 16 bytes from base[i] + off[i] to LDS at at + 1024 i +
+// 16 l (non-temporal). (The leading s_nop covers the vector write of a base just
+// before.)
+__device__ __forceinline__ void sel_load4(const uint64_t (&base)[4], const uint32_t *off, uint32_t at) {
+    uint32_t save;
+    asm volatile(
+        "s_nop 4\n\ts_mov_b32 %0, m0\n\t"
+        "s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %6 nt\n\t"
+        "s_add_u32 m0, %1, 1024\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %7 nt\n\t"
+        "s_add_u32 m0, %1, 2048\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %4, %8 nt\n\t"
+        "s_add_u32 m0, %1, 0xc00\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %5, %9 nt\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(save)
+        : "s"(at), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base[0]), "s"(base[1]), "s"(base[2]),
+          "s"(base[3])
+        : "scc");
+}
+
+template <uint32_t D>
+__device__ __forceinline__ void sel_staged_body(const sglkv_select_params &p) {
+    typedef attn_stg<D> S;
+    extern __shared__ __attribute__((aligned(16))) uint8_t sel_stg_lds[];
+    const sglkv_attn_params &a = p.a;
+    const uint32_t lane = threadIdx.x, g = lane >> 4, r = lane & 15;
+    sel_work s;
+    const uint64_t mine = sel_decode(p, lane, &s);
+    if (s.tokens == 0) {
+        sel_empty(p, s, lane, D);
+        return;
+    }
+    const attn_work &w = s.w;
+    const uint32_t page_lo = static_cast<uint32_t>(mine);  // (the host keeps pages below 2^32)
+    sglkv_u16x8 qf[S::KC];
+#pragma unroll
+    for (uint32_t c = 0; c < S::KC; ++c) {
+        qf[c] = sglkv_u16x8{0, 0, 0, 0, 0, 0, 0, 0};
+        if (r < w.nh)
+            qf[c] = *reinterpret_cast<const sglkv_u16x8 *>(a.queries + (w.q * a.query_heads + w.h0 + r) * D + 32 * c + 8 * g);
+    }
+    const uint64_t pool = reinterpret_cast<uint64_t>(a.pool);
+    const uint64_t kbase = pool + a.key_offset + w.kvh * a.key_head_stride;
+    const uint64_t vbase = pool + a.value_offset + w.kvh * a.value_head_stride;
+    const uint32_t mask = (1u << a.page_shift) - 1, stride = a.key_token_stride32;
+    const uint32_t c = lane / S::PIECES, pc = lane % S::PIECES;
+    // Load j takes tokens TPL j + c of a block: its base is the page of token TPL j
+    // and that token's place in it, the lane's part token c and piece pc.
+    const uint32_t lane_row = __umul24(c, stride), lane_k = S::kpos(c, pc), lane_v = S::vpos(c, pc);
+    auto koff_of = [&](uint32_t j) { return lane_row + 16 * (lane_k ^ S::kpos(S::TPL * j, 0)); };
+    auto voff_of = [&](uint32_t j) { return lane_row + 16 * (lane_v ^ S::vpos(S::TPL * j, 0)); };
+    constexpr uint32_t KEPT = D == 256 ? 1 : S::LOADS;
+    uint32_t koff[KEPT], voff[KEPT];
+    if constexpr (D != 256)
+#pragma unroll
+        for (uint32_t j = 0; j < S::LOADS; ++j) {
+            koff[j] = koff_of(j);
+            voff[j] = voff_of(j);
+        }
+    const uint32_t nb = (s.tokens + kLatB - 1) / kLatB, full = s.tokens / kLatB;
+    auto stage_at = [&](uint32_t b) { return attn_lat_lds_at(sel_stg_lds) + (b & 1) * S::STAGE; };
+    auto token_base = [&](uint32_t token) {
+        const uint32_t page = __builtin_amdgcn_readlane(page_lo, token >> a.page_shift);
+        return static_cast<uint64_t>(page) * a.page_stride32 + static_cast<uint64_t>(token & mask) * stride;
+    };
+    auto issue = [&](uint32_t b) {
+        const uint32_t t0 = kLatB * b, at = stage_at(b);
+        const uint64_t zero = reinterpret_cast<uint64_t>(a.zero_row) + 16 * pc;
+#pragma unroll
+        for (uint32_t h = 0; h < S::LOADS / 4; ++h) {
+            uint32_t ko[4], vo[4];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                ko[i] = D == 256 ? koff_of(4 * h + i) : koff[D == 256 ? 0 : 4 * h + i];
+                vo[i] = D == 256 ? voff_of(4 * h + i) : voff[D == 256 ? 0 : 4 * h + i];
+            }
+            if (b < full) {
+                uint64_t kb[4], vb[4];
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    const uint64_t off = token_base(t0 + S::TPL * (4 * h + i));
+                    kb[i] = kbase + off;
+                    vb[i] = vbase + off;
+                }
+                sel_load4(kb, ko, at + 4096 * h);
+                sel_load4(vb, vo, at + S::V + 4096 * h);
+            } else {  // the last block: tokens past the end read the zero row
+                uint64_t x[8];
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    const uint32_t t = t0 + S::TPL * (4 * h + i);
+                    const uint64_t off = token_base(t < s.tokens ? t : t0);
+                    attn_sel64x2(t + c < s.tokens, kbase + off + ko[i], vbase + off + vo[i], zero, x[i], x[4 + i]);
+                }
+                attn_lat_load4v<1024>(x, at + 4096 * h);
+                attn_lat_load4v<1024>(x + 4, at + S::V + 4096 * h);
+            }
+        }
+    };
+    // The queries (which the compiler counts) are there before the loop, whose
+    // waits count the rows alone.
+    __builtin_amdgcn_s_waitcnt(0x0F70);
+    issue(0);
+    attn_state_n<S::NJ> st;
+    attn_state_init(st);
+    for (uint32_t k = 0; k < nb; ++k) {
+        // Block k-1's reads are done before block k+1's rows take its stage; then
+        // block k's rows, older than block k+1's, have landed.
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (k + 1 < nb) {
+            issue(k + 1);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * S::LOADS) : "memory");
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        const uint8_t *kst = sel_stg_lds + (k & 1) * S::STAGE;
+        const uint32_t left = s.tokens - kLatB * k;
+        attn_stg_block<D>(a, g, r, qf, kst, left < kLatB ? left : kLatB, st);
+    }
+    attn_finish(a, w, g, r, st);
+}
+
 }  // namespace
 
 extern "C" __global__ __launch_bounds__(256) void sglkv_page_bounds_8(sglkv_bounds_params p) { bounds_body<8>(p); }
@@ -602,34 +733,76 @@ sglkv_selected_attention_v2(sglkv_select_params p) {
     sel_attend_body<false>(p);
 }
 
-// Merges the split records of a (query, head), one wave each: lane l takes
-// dims 4l .. 4l+3 (+256 ...). Empty splits' records are not read; a (query,
-// head) of nothing else is zeros.
+// (Two waves a SIMD: the accumulators stay in vector registers.)
+extern "C" __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void
+sglkv_selected_attention_staged64(sglkv_select_params p) {
+    sel_staged_body<64>(p);
+}
+extern "C" __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void
+sglkv_selected_attention_staged128(sglkv_select_params p) {
+    sel_staged_body<128>(p);
+}
+extern "C" __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void
+sglkv_selected_attention_staged256(sglkv_select_params p) {
+    sel_staged_body<256>(p);
+}
+
+// Merges the split records of a (query, head), one wave each. Lane s weighs split
+// s once (64 at a time); then sets of ceil(dv / 4) lanes, 4 dims a lane, add every
+// so many splits' rows, eight in flight, and join. An empty split weighs nothing
+// (its row holds anything); a (query, head) of nothing else is zeros.
 extern "C" __global__ __launch_bounds__(64) void sglkv_selected_attention_combine(sglkv_select_params p) {
     const sglkv_attn_params &a = p.a;
     const uint64_t item = blockIdx.x;
-    const uint32_t lane = threadIdx.x;
+    const uint32_t lane = threadIdx.x, opad = SGLKV_ATTN_OPAD(a.dv);
     const float2 *ml = reinterpret_cast<const float2 *>(attn_rec_ml(a, item * a.splits));
-    float m = -INFINITY;
-    for (uint32_t s = lane; s < a.splits; s += 64) m = fmaxf(m, ml[s].x);
+    const float *rows = attn_rec_o(a, item * a.splits);
+    const uint32_t wide = (a.dv + 3) / 4, lanes = wide <= 16 ? 16 : wide <= 32 ? 32 : 64, sets = 64 / lanes;
+    const uint32_t set = lane / lanes, v = lane % lanes;
+    for (uint32_t d0 = 0; d0 < a.dv; d0 += 4 * lanes) {
+        const uint32_t d = d0 + 4 * v < opad ? d0 + 4 * v : 0;
+        float m = -INFINITY, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (uint32_t s0 = 0; s0 < a.splits; s0 += 64) {
+            const uint32_t here = a.splits - s0 < 64 ? a.splits - s0 : 64;
+            const float2 mine = lane < here ? ml[s0 + lane] : make_float2(-INFINITY, 0.0f);
+            float top = fmaxf(m, mine.x);
 #pragma unroll
-    for (uint32_t x = 1; x < 64; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
-    for (uint32_t d = 4 * lane; d < a.dv; d += 256) {
-        float l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (uint32_t s = 0; s < a.splits; ++s) {
-            const float2 r = ml[s];
-            if (r.x == -INFINITY) continue;
-            const float w = exp2f(r.x - m);
-            const float4 v = *reinterpret_cast<const float4 *>(attn_rec_o(a, item * a.splits + s) + d);
-            l += w * r.y;
-            o[0] += w * v.x;
-            o[1] += w * v.y;
-            o[2] += w * v.z;
-            o[3] += w * v.w;
+            for (uint32_t x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
+            if (top == -INFINITY) continue;
+            const float w = __builtin_amdgcn_exp2f(mine.x - top), back = __builtin_amdgcn_exp2f(m - top);
+            float sum = mine.x == -INFINITY ? 0.0f : w * mine.y;
+#pragma unroll
+            for (uint32_t x = 1; x < 64; x <<= 1) sum += __shfl_xor(sum, x);
+            l = l * back + sum;
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) o[e] *= back;
+            m = top;
+            for (uint32_t s = set; s < here; s += 8 * sets) {
+                float4 x[8];
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i) {
+                    const uint32_t at = s + i * sets < here ? s + i * sets : s;
+                    x[i] = *reinterpret_cast<const float4 *>(rows + static_cast<uint64_t>(s0 + at) * opad + d);
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i) {
+                    const float ws = s + i * sets < here ? __shfl(w, s + i * sets) : 0.0f;
+                    if (ws != 0.0f) {
+                        o[0] = fmaf(ws, x[i].x, o[0]);
+                        o[1] = fmaf(ws, x[i].y, o[1]);
+                        o[2] = fmaf(ws, x[i].z, o[2]);
+                        o[3] = fmaf(ws, x[i].w, o[3]);
+                    }
+                }
+            }
         }
-        const float linv = m == -INFINITY ? 0.0f : 1.0f / l;
+        for (uint32_t x = lanes; x < 64; x <<= 1)
 #pragma unroll
-        for (uint32_t e = 0; e < 4; ++e)
-            if (d + e < a.dv) a.output[item * a.dv + d + e] = attn_to_bf16(o[e] * linv);
+            for (uint32_t e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], x);
+        const float linv = m == -INFINITY ? 0.0f : 1.0f / l;
+        if (set == 0)
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e)
+                if (d0 + 4 * v + e < a.dv) a.output[item * a.dv + d0 + 4 * v + e] = attn_to_bf16(o[e] * linv);
     }
 }
