@@ -159,6 +159,7 @@ struct sgl_rocm_kv_ctx {
     // 8, 16, 32, 64 lanes to a row of 16-byte vectors; any row
     hipFunction_t page_bounds[5];
     hipFunction_t page_scores[5];
+    hipFunction_t page_scores_fast[3][3];  // dims 64, 128, 256; 4, 8, 16 query heads a turn (8 at dims 256)
     hipFunction_t pick_pages;
     hipFunction_t selected_attention[2];  // 16-byte vectors, elements
     hipFunction_t selected_staged[3];     // dims 64, 128, 256, rows staged in LDS

@@ -577,6 +577,15 @@ extern "C" int32_t sgl_rocm_kv_init(int32_t device, const char *code_object_path
                      {"sglkv_page_scores_32", &ctx->page_scores[2]},
                      {"sglkv_page_scores_64", &ctx->page_scores[3]},
                      {"sglkv_page_scores_element", &ctx->page_scores[4]},
+                     {"sglkv_page_scores64_4", &ctx->page_scores_fast[0][0]},
+                     {"sglkv_page_scores64_8", &ctx->page_scores_fast[0][1]},
+                     {"sglkv_page_scores64_16", &ctx->page_scores_fast[0][2]},
+                     {"sglkv_page_scores128_4", &ctx->page_scores_fast[1][0]},
+                     {"sglkv_page_scores128_8", &ctx->page_scores_fast[1][1]},
+                     {"sglkv_page_scores128_16", &ctx->page_scores_fast[1][2]},
+                     {"sglkv_page_scores256_4", &ctx->page_scores_fast[2][0]},
+                     {"sglkv_page_scores256_8", &ctx->page_scores_fast[2][1]},
+                     {"sglkv_page_scores256_8", &ctx->page_scores_fast[2][2]},
                      {"sglkv_pick_pages", &ctx->pick_pages},
                      {"sglkv_selected_attention_v16", &ctx->selected_attention[0]},
                      {"sglkv_selected_attention_v2", &ctx->selected_attention[1]},

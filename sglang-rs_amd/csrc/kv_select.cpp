@@ -281,8 +281,19 @@ extern "C" int32_t sgl_rocm_kv_select_pages(sgl_rocm_kv_ctx *ctx, const sgl_kv_p
         const bool vector = p.a.dk % 8 == 0 && reinterpret_cast<uint64_t>(p.bounds) % 16 == 0;
         p.chunk_pages = (uint32_t)shape.chunk_pages;
         p.heads = p.a.kv_heads * (uint32_t)shape.chunks;
-        rc = launch_kernel(ctx->page_scores[row_lanes(p.a.dk, vector)], shape.items * shape.chunks, 1, 1, SGLKV_SELECT_THREADS,
-                    2 * p.a.group * SGLKV_SELECT_QSTRIDE(p.a.dk), s, &p, "page scores launch");
+        const int dims = p.a.dk == 64 ? 0 : p.a.dk == 128 ? 1 : p.a.dk == 256 ? 2 : -1;
+        if (vector && dims >= 0 && reinterpret_cast<uint64_t>(p.a.queries) % 16 == 0 &&
+            shape.chunk_pages <= SGLKV_SELECT_LDS_PAGES) {
+            // 4, 8 or 16 query heads a turn; past that several, whose maxima wait in LDS.
+            const int heads = p.a.group <= 4 ? 0 : p.a.group <= 8 || dims == 2 ? 1 : 2;
+            rc = launch_kernel(ctx->page_scores_fast[dims][heads], shape.items * shape.chunks, 1, 1, SGLKV_SELECT_THREADS,
+                               p.a.group > (4u << heads) ? (unsigned)(8 * shape.chunk_pages) : 0, s, &p,
+                               "page scores launch");
+        } else {
+            rc = launch_kernel(ctx->page_scores[row_lanes(p.a.dk, vector)], shape.items * shape.chunks, 1, 1,
+                               SGLKV_SELECT_THREADS, 2 * p.a.group * SGLKV_SELECT_QSTRIDE(p.a.dk), s, &p,
+                               "page scores launch");
+        }
         if (rc) return rc;
     }
     const uint64_t kept = shape.key_bytes == 0                                ? 0

@@ -405,6 +405,163 @@ __device__ __forceinline__ void sel_scores_body(const sglkv_select_params &p) {
                           [&](uint64_t j, uint64_t key) { keys[j] = key; });
 }
 
+// The same for keys of 64, 128 or 256 dims on 16-byte rows, as a matrix product in
+// 64 bits. A page's row is its 2 D bounds, low then high; a query head's, min(q, 0)
+// then max(q, 0). v_mfma_f64_4x4x4 multiplies four 4 x 4 blocks: lane l holds, of
+// page l % 4 and of query head l % 4, element l / 4 of 16, and gets block (l / 4)
+// % 4's share of page l / 16's product with head l % 4. So a lane's 16 bytes of a
+// row, for 16 lanes to a row, are eight steps, no lane holds more of a query than
+// its 16th, and only four shares are left to add across lanes. (With a row's dims
+// spread over lanes and 64-bit vector multiply-adds the query took 128 registers,
+// one or two waves fitted a SIMD, and the sums across 16 lanes took as long as the
+// products: 64 ragged sequences of up to 2,048 pages, 8 KV heads of 4 query heads,
+// dims 128, 136 us.) 4 NG query heads a turn; more take several turns over the
+// chunk, whose maxima wait in LDS.
+__device__ __forceinline__ double sel_ror(double x, bool by8) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = static_cast<uint32_t>(b), hi = static_cast<uint32_t>(b >> 32);
+    const uint32_t rl = by8 ? __builtin_amdgcn_update_dpp(lo, lo, 0x128, 0xF, 0xF, true)
+                            : __builtin_amdgcn_update_dpp(lo, lo, 0x124, 0xF, 0xF, true);
+    const uint32_t rh = by8 ? __builtin_amdgcn_update_dpp(hi, hi, 0x128, 0xF, 0xF, true)
+                            : __builtin_amdgcn_update_dpp(hi, hi, 0x124, 0xF, 0xF, true);
+    return __builtin_bit_cast(double, (static_cast<uint64_t>(rh) << 32) | rl);
+}
+
+// The larger of two scores, NaN above every number.
+__device__ __forceinline__ double sel_larger(double a, double b) { return a != a || b <= a ? a : b; }
+
+template <uint32_t D, uint32_t NG>
+__device__ __forceinline__ void sel_scores_fast_body(const sglkv_select_params &p) {
+    constexpr uint32_t NV = D / 64, U = 256 / D, TURN = 16 * U;  // vectors of a lane; 4-page steps of a wave; pages of a workgroup
+    extern __shared__ __attribute__((aligned(16))) double sel_best[];  // the chunk's maxima, if there are several turns
+    const uint32_t chunks = p.heads / p.a.kv_heads;
+    const uint32_t chunk = blockIdx.x % chunks, item = blockIdx.x / chunks, head = item % p.a.kv_heads;
+    const uint64_t q = item / p.a.kv_heads;
+    uint64_t start, len;
+    sel_sequence(p.a, p.max_length, q, false, &start, &len);
+    const uint32_t page_size = static_cast<uint32_t>(p.a.page_size);
+    const uint32_t count = static_cast<uint32_t>((len + page_size - 1) / page_size);
+    const uint32_t first = chunk * p.chunk_pages;
+    if (first >= count || count <= p.max_pages) return;  // (nothing to choose from)
+    const uint32_t last = first + p.chunk_pages < count ? first + p.chunk_pages : count;
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64, slot4 = lane >> 2, in4 = lane & 3;
+    const uint64_t bounds = reinterpret_cast<uint64_t>(p.bounds) + head * (4ull * D) + 16 * slot4;
+    const uint64_t page_bytes = p.a.kv_heads * (4ull * D);
+    uint64_t *keys = p.keys + (q * p.a.kv_heads + head) * p.sequence_pages;
+    // This wave's pages of a turn of the workgroup: j0 + 4 u + l % 4, their slots first,
+    // then (a turn later) the rows that they name; past the last page, the last
+    // one's. A slot that is no page's first is reported; its row is page 0's and its
+    // key 0.
+    auto slots_of = [&](uint32_t j0, uint64_t (&slot)[U]) {
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) {
+            const uint32_t j = j0 + 4 * u + in4;
+            slot[u] = p.a.sequence_slots[start + static_cast<uint64_t>(j < last ? j : last - 1) * page_size];
+        }
+    };
+    auto rows_of = [&](uint32_t j0, const uint64_t (&slot)[U], sglkv_u16x8 (&row)[U][NV]) {
+        uint32_t bad = 0;
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) {
+            const uint32_t j = j0 + 4 * u + in4 < last ? j0 + 4 * u + in4 : last - 1;
+            const uint64_t left = len - static_cast<uint64_t>(j) * page_size, tokens = left < page_size ? left : page_size;
+            uint64_t page, in_page;
+            attn_split_slot(p.a, slot[u], &page, &in_page);
+            const bool ok = slot[u] < p.a.slot_count && tokens <= p.a.slot_count - slot[u] && in_page == 0;
+            if (!ok) bad |= 1u << u;
+            const uint64_t at = bounds + (ok ? page : 0) * page_bytes;
+#pragma unroll
+            for (uint32_t n = 0; n < NV; ++n) row[u][n] = sel_load(at + 256 * n);
+        }
+        if (bad) atomicOr(p.a.flag, SGLKV_FLAG_ATTN_SLOT);
+        return bad;
+    };
+    const uint32_t turns = (p.a.group + 4 * NG - 1) / (4 * NG);
+    for (uint32_t turn = 0; turn < turns; ++turn) {
+        const uint32_t begin = first + 4 * U * wave;
+        uint64_t slot[U];
+        sglkv_u16x8 row[U][NV];
+        if (begin < last) slots_of(begin, slot);
+        // Element 8 (slot4 + 16 n) + e of query head g0 + 4 m + l % 4's row of parts.
+        double qv[NG][NV][8];
+#pragma unroll
+        for (uint32_t m = 0; m < NG; ++m) {
+            const uint32_t g = turn * 4 * NG + 4 * m + in4;
+            const uint64_t from = reinterpret_cast<uint64_t>(p.a.queries) +
+                                  2 * (q * p.a.query_heads + head * p.a.group + (g < p.a.group ? g : 0)) * D;
+#pragma unroll
+            for (uint32_t n = 0; n < NV; ++n) {
+                const uint32_t at = 8 * (slot4 + 16 * n);
+                const sglkv_u16x8 x = sel_load(from + 2 * (at & (D - 1)));
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e) {
+                    const float f = sel_f32(x[e]);  // (a NaN stays with the low bounds)
+                    qv[m][n][e] = at < D ? (f > 0.0f ? 0.0f : f) : (f > 0.0f ? f : 0.0f);
+                }
+            }
+        }
+        uint32_t bad = 0, bad_next = 0;
+        if (begin < last) bad = rows_of(begin, slot, row);
+        if (begin + TURN < last) slots_of(begin + TURN, slot);
+        for (uint32_t j0 = begin; j0 < last; j0 += TURN) {
+            sglkv_u16x8 next[U][NV];
+            const bool more = j0 + TURN < last;
+            if (more) {
+                bad_next = rows_of(j0 + TURN, slot, next);
+                if (j0 + 2 * TURN < last) slots_of(j0 + 2 * TURN, slot);
+            }
+            double sum[U][NG] = {};
+#pragma unroll
+            for (uint32_t n = 0; n < NV; ++n)
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e)
+#pragma unroll
+                    for (uint32_t u = 0; u < U; ++u) {
+                        const double x = sel_f32(row[u][n][e]);
+#pragma unroll
+                        for (uint32_t m = 0; m < NG; ++m)
+                            sum[u][m] = __builtin_amdgcn_mfma_f64_4x4x4f64(x, qv[m][n][e], sum[u][m], 0, 0, 0);
+                    }
+            // Page l / 16 of step u; lane 16 i + u of them writes page j0 + 4 u + i.
+            double mine = 0.0;
+            uint32_t mine_bad = 0;
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u) {
+                double best = -INFINITY;
+#pragma unroll
+                for (uint32_t m = 0; m < NG; ++m) {
+                    double x = sum[u][m];
+                    x += sel_ror(x, true);
+                    x += sel_ror(x, false);
+                    if (turn * 4 * NG + 4 * m + in4 < p.a.group) best = sel_larger(best, x);
+                }
+                best = sel_larger(best, sel_join<1>(best));
+                best = sel_larger(best, sel_join<2>(best));
+                const uint64_t bads = __ballot(bad >> u & 1);
+                if ((lane & 15) == u) {
+                    mine = best;
+                    mine_bad = bads >> (lane >> 4) & 1;
+                }
+            }
+            const uint32_t j = j0 + 4 * (lane & 15) + (lane >> 4);
+            if ((lane & 15) < U && j < last) {
+                if (turn > 0) mine = sel_larger(sel_best[j - first], mine);
+                if (turn + 1 < turns)
+                    sel_best[j - first] = mine;
+                else
+                    keys[j] = j < p.first_pages || j + p.last_pages >= count ? kSelForced : mine_bad ? 0 : sel_key(mine);
+            }
+            if (more) {
+                bad = bad_next;
+#pragma unroll
+                for (uint32_t u = 0; u < U; ++u)
+#pragma unroll
+                    for (uint32_t n = 0; n < NV; ++n) row[u][n] = next[u][n];
+            }
+        }
+    }
+}
+
 // The pages of a (query, KV head) from the workspace's keys.
 __device__ __forceinline__ void sel_pick_body(const sglkv_select_params &p) {
     extern __shared__ __attribute__((aligned(16))) uint8_t sel_lds[];
@@ -720,6 +877,31 @@ extern "C" __global__ __launch_bounds__(SGLKV_SELECT_THREADS) void sglkv_page_sc
 }
 extern "C" __global__ __launch_bounds__(SGLKV_SELECT_THREADS) void sglkv_page_scores_element(sglkv_select_params p) {
     sel_scores_body<64, 2, false>(p);
+}
+// Keys of 64, 128 or 256 dims; 4, 8 or 16 query heads a turn.
+extern "C" __global__ __launch_bounds__(SGLKV_SELECT_THREADS) void sglkv_page_scores64_4(sglkv_select_params p) {
+    sel_scores_fast_body<64, 1>(p);
+}
+extern "C" __global__ __launch_bounds__(SGLKV_SELECT_THREADS) void sglkv_page_scores64_8(sglkv_select_params p) {
+    sel_scores_fast_body<64, 2>(p);
+}
+extern "C" __global__ __launch_bounds__(SGLKV_SELECT_THREADS) void sglkv_page_scores64_16(sglkv_select_params p) {
+    sel_scores_fast_body<64, 4>(p);
+}
+extern "C" __global__ __launch_bounds__(SGLKV_SELECT_THREADS) void sglkv_page_scores128_4(sglkv_select_params p) {
+    sel_scores_fast_body<128, 1>(p);
+}
+extern "C" __global__ __launch_bounds__(SGLKV_SELECT_THREADS) void sglkv_page_scores128_8(sglkv_select_params p) {
+    sel_scores_fast_body<128, 2>(p);
+}
+extern "C" __global__ __launch_bounds__(SGLKV_SELECT_THREADS) void sglkv_page_scores128_16(sglkv_select_params p) {
+    sel_scores_fast_body<128, 4>(p);
+}
+extern "C" __global__ __launch_bounds__(SGLKV_SELECT_THREADS) void sglkv_page_scores256_4(sglkv_select_params p) {
+    sel_scores_fast_body<256, 1>(p);
+}
+extern "C" __global__ __launch_bounds__(SGLKV_SELECT_THREADS) void sglkv_page_scores256_8(sglkv_select_params p) {
+    sel_scores_fast_body<256, 2>(p);
 }
 extern "C" __global__ __launch_bounds__(SGLKV_SELECT_THREADS) void sglkv_pick_pages(sglkv_select_params p) {
     sel_pick_body(p);
