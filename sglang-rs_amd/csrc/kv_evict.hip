@@ -515,19 +515,6 @@ __device__ __forceinline__ void wgt_join_body(const sglkv_weights_params &p) {
     if (v == 0) reinterpret_cast<float2 *>(p.joined)[row] = x;
 }
 
-// One workgroup's place among items * kv_heads of them. XCDs take workgroups in
-// turn: eight items go side by side, each with all its KV heads on one XCD, whose
-// L2 then holds whole token rows and query rows instead of one head's slice of
-// many (with a head to an XCD these slices, a power of two apart, meet in a few
-// of its channels).
-__device__ __forceinline__ void wgt_place(uint32_t kv_heads, uint32_t *item, uint32_t *kvh) {
-    const uint32_t b = blockIdx.x, inner = b / 8, eight = inner / kv_heads;
-    *kvh = inner - eight * kv_heads;
-    // (Which of the eight goes to which XCD turns from eight to eight, so that work
-    // that grows with a power of two in the items does not pile up on one.)
-    *item = 8 * eight + ((b + 5 * eight + eight / 8) & 7);
-}
-
 // Row pitch in LDS: 16 rows' pieces land in all banks once.
 template <uint32_t DKC>
 constexpr uint32_t kWgtPitch = 64 * DKC + 16;
@@ -543,7 +530,7 @@ __device__ __forceinline__ void wgt_tile_stats_body(const sglkv_weights_params &
     const uint32_t tid = threadIdx.x, lane = tid & 63, g = lane >> 4, r = lane & 15;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid / 64);
     uint32_t item, kvh;
-    wgt_place(a.kv_heads, &item, &kvh);
+    sel_place(a.kv_heads, &item, &kvh);  // (whole token and query rows in an XCD's L2)
     if (item >= p.row_tiles * p.tile_head_groups) return;
     const uint32_t hg = item % p.tile_head_groups;
     // (A prompt's last queries attend the most: they start first.)
@@ -633,7 +620,7 @@ __device__ __forceinline__ void wgt_tile_accumulate_body(const sglkv_weights_par
     const uint32_t tid = threadIdx.x, lane = tid & 63, g = lane >> 4, r = lane & 15;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid / 64);
     uint32_t item, kvh;
-    wgt_place(a.kv_heads, &item, &kvh);
+    sel_place(a.kv_heads, &item, &kvh);  // (whole token and query rows in an XCD's L2)
     const uint32_t requests = static_cast<uint32_t>(a.request_count);
     const uint32_t segment = item % p.segments, tile = item / p.segments / requests;
     const uint32_t req = item / p.segments - tile * requests, tg = tile * 64 * TT, tb = tg + wave * 16 * TT;

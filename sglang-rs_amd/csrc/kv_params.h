@@ -410,7 +410,9 @@ typedef struct sglkv_select_params {
     uint32_t first_pages, last_pages;
     uint32_t sequence_pages;  /* pages of a sequence of max_length tokens */
     uint32_t chunk_pages;     /* attention: pages per split; scores: pages per workgroup */
-    uint32_t heads;           /* select: KV heads * chunks of a query (scores), or KV heads */
+    uint32_t heads;           /* scores: KV heads * chunks of a query */
+    uint32_t block_heads;     /* scores: KV heads of a workgroup (1, 2 or 4) */
+    uint32_t reserved;
 } sglkv_select_params;
 
 /* The softmax weights that each position of a sequence gets, summed over the

@@ -37,9 +37,14 @@ struct SelectionShape {
     uint64_t record_bytes;
 };
 
-// Workgroups of scores that fill the chip several times over, 64 pages or more
-// each.
-constexpr uint64_t kScoreWorkgroups = 2048;
+// Chunks of pages that the scores are cut into, 16 pages or more each: a wave to
+// each where the KV heads come in fours. A wave waits some 4 us for its length, slots
+// and first rows, which short shares do not hide; long ones leave CUs idle at the end
+// of ragged batches. Rows of 64 dims are half as long and want half the chunks: 24
+// sequences of up to 40,000 tokens on 5 heads took 32, 26 and 34 us with 1,536, 2,048
+// and 4,096 of them; 64 of up to 32,768 on 8 heads of 128 dims 107, 77 and 95 us with
+// 2,048, 4,096 and 8,192.
+uint64_t score_chunks(uint64_t dk) { return dk <= 64 ? 2048 : 4096; }
 // Waves of the attention that stay resident at once, each with 64 tokens or
 // more: what the staged body's LDS leaves room for on 256 CUs (its registers, at
 // dims 64), or the generic one's LDS.
@@ -79,8 +84,8 @@ int32_t selection_shape(const sgl_kv_attention_plan_config &c, const sgl_kv_page
     uint64_t pages;
     if (mul_ovf(h.items, h.sequence_pages, &pages) || mul_ovf(pages, 8, &h.key_bytes)) return attention_overflow();
     if (h.sequence_pages <= s.max_pages) h.key_bytes = 0;
-    const uint64_t share = ceil_div(pages, kScoreWorkgroups);
-    h.chunk_pages = ceil_div(share < h.sequence_pages ? share : h.sequence_pages, 64) * 64;
+    const uint64_t share = ceil_div(pages, score_chunks(c.query_key_head_dim));
+    h.chunk_pages = ceil_div(share < h.sequence_pages ? share : h.sequence_pages, 16) * 16;
     h.chunks = ceil_div(h.sequence_pages, h.chunk_pages);
     // Attention.
     const uint64_t list = s.max_pages < h.sequence_pages ? s.max_pages : h.sequence_pages;
@@ -283,11 +288,13 @@ extern "C" int32_t sgl_rocm_kv_select_pages(sgl_rocm_kv_ctx *ctx, const sgl_kv_p
         p.heads = p.a.kv_heads * (uint32_t)shape.chunks;
         const int dims = p.a.dk == 64 ? 0 : p.a.dk == 128 ? 1 : p.a.dk == 256 ? 2 : -1;
         if (vector && dims >= 0 && reinterpret_cast<uint64_t>(p.a.queries) % 16 == 0 &&
-            shape.chunk_pages <= SGLKV_SELECT_LDS_PAGES) {
+            shape.chunk_pages <= SGLKV_SELECT_LDS_PAGES / 4) {
             // 4, 8 or 16 query heads a turn; past that several, whose maxima wait in LDS.
             const int heads = p.a.group <= 4 ? 0 : p.a.group <= 8 || dims == 2 ? 1 : 2;
-            rc = launch_kernel(ctx->page_scores_fast[dims][heads], shape.items * shape.chunks, 1, 1, SGLKV_SELECT_THREADS,
-                               p.a.group > (4u << heads) ? (unsigned)(8 * shape.chunk_pages) : 0, s, &p,
+            p.block_heads = p.a.kv_heads % 4 == 0 ? 4 : p.a.kv_heads % 2 == 0 ? 2 : 1;
+            const uint64_t groups = ceil_div(p.a.query_count * shape.chunks, 8) * 8 * (p.a.kv_heads / p.block_heads);
+            rc = launch_kernel(ctx->page_scores_fast[dims][heads], groups, 1, 1, SGLKV_SELECT_THREADS,
+                               p.a.group > (4u << heads) ? (unsigned)(8 * shape.chunk_pages * p.block_heads) : 0, s, &p,
                                "page scores launch");
         } else {
             rc = launch_kernel(ctx->page_scores[row_lanes(p.a.dk, vector)], shape.items * shape.chunks, 1, 1,

@@ -51,6 +51,17 @@ __device__ __forceinline__ double sel_sum(double x) {
     return x;
 }
 
+// This workgroup's place among items * inner_count of them. XCDs take workgroups in
+// turn: eight items go side by side, each with all its inner_count parts on one
+// XCD, whose L2 then shares what the parts read in common. Which of the eight
+// goes to which XCD turns from eight to eight, so that work that grows with the
+// item within a power of two of them does not pile up on one.
+__device__ __forceinline__ void sel_place(uint32_t inner_count, uint32_t *item, uint32_t *inner) {
+    const uint32_t b = blockIdx.x, k = b / 8, eight = k / inner_count;
+    *inner = k - eight * inner_count;
+    *item = 8 * eight + ((b + 5 * eight + eight / 8) & 7);
+}
+
 // ---- Page key bounds ------------------------------------------------------
 //
 // One wave per (page, KV head). NaN carries into both bounds (minimum and
@@ -416,7 +427,10 @@ __device__ __forceinline__ void sel_scores_body(const sglkv_select_params &p) {
 // one or two waves fitted a SIMD, and the sums across 16 lanes took as long as the
 // products: 64 ragged sequences of up to 2,048 pages, 8 KV heads of 4 query heads,
 // dims 128, 136 us.) 4 NG query heads a turn; more take several turns over the
-// chunk, whose maxima wait in LDS.
+// chunk, whose maxima wait in LDS. Bound by the bounds' bytes: those sequences take
+// 77 us for 293 MB, 3.8 TB/s, where a plain streaming read of them takes 45 (loads
+// that keep the rows in the caches, 83; slots found row by row, 113). Sixteen pages
+// a wave's step at 64 and 128 dims, 8 at 256 for the registers; 8 at 128 took 97 us.
 __device__ __forceinline__ double sel_ror(double x, bool by8) {
     const uint64_t b = __builtin_bit_cast(uint64_t, x);
     const uint32_t lo = static_cast<uint32_t>(b), hi = static_cast<uint32_t>(b >> 32);
@@ -432,11 +446,21 @@ __device__ __forceinline__ double sel_larger(double a, double b) { return a != a
 
 template <uint32_t D, uint32_t NG>
 __device__ __forceinline__ void sel_scores_fast_body(const sglkv_select_params &p) {
-    constexpr uint32_t NV = D / 64, U = 256 / D, TURN = 16 * U;  // vectors of a lane; 4-page steps of a wave; pages of a workgroup
+    constexpr uint32_t NV = D / 64, U = D == 256 ? 2 : 4;  // vectors of a lane; steps of four pages that a wave takes at once
     extern __shared__ __attribute__((aligned(16))) double sel_best[];  // the chunk's maxima, if there are several turns
     const uint32_t chunks = p.heads / p.a.kv_heads;
-    const uint32_t chunk = blockIdx.x % chunks, item = blockIdx.x / chunks, head = item % p.a.kv_heads;
-    const uint64_t q = item / p.a.kv_heads;
+    // A workgroup's waves take block_heads KV heads (1, 2 or 4) of the same pages, whose
+    // bounds lie side by side, and the workgroups of the other heads run on the same
+    // XCD: a page's slot, a line of its own in a long slot list, is then fetched once.
+    uint32_t item, block;
+    sel_place(p.a.kv_heads / p.block_heads, &item, &block);
+    const uint32_t chunk = item % chunks;
+    const uint64_t q = item / chunks;
+    if (q >= p.a.query_count) return;
+    const uint32_t lane = threadIdx.x & 63, slot4 = lane >> 2, in4 = lane & 3;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const uint32_t head = block * p.block_heads + wave % p.block_heads;
+    const uint32_t part = wave / p.block_heads, parts = 4 / p.block_heads;  // of the pages
     uint64_t start, len;
     sel_sequence(p.a, p.max_length, q, false, &start, &len);
     const uint32_t page_size = static_cast<uint32_t>(p.a.page_size);
@@ -444,44 +468,47 @@ __device__ __forceinline__ void sel_scores_fast_body(const sglkv_select_params &
     const uint32_t first = chunk * p.chunk_pages;
     if (first >= count || count <= p.max_pages) return;  // (nothing to choose from)
     const uint32_t last = first + p.chunk_pages < count ? first + p.chunk_pages : count;
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64, slot4 = lane >> 2, in4 = lane & 3;
-    const uint64_t bounds = reinterpret_cast<uint64_t>(p.bounds) + head * (4ull * D) + 16 * slot4;
+    double *best_of = sel_best + (wave % p.block_heads) * p.chunk_pages;
+    const uint64_t bounds = reinterpret_cast<uint64_t>(p.bounds) + head * (4ull * D);
     const uint64_t page_bytes = p.a.kv_heads * (4ull * D);
     uint64_t *keys = p.keys + (q * p.a.kv_heads + head) * p.sequence_pages;
-    // This wave's pages of a turn of the workgroup: j0 + 4 u + l % 4, their slots first,
-    // then (a turn later) the rows that they name; past the last page, the last
-    // one's. A slot that is no page's first is reported; its row is page 0's and its
-    // key 0.
-    auto slots_of = [&](uint32_t j0, uint64_t (&slot)[U]) {
-#pragma unroll
-        for (uint32_t u = 0; u < U; ++u) {
-            const uint32_t j = j0 + 4 * u + in4;
-            slot[u] = p.a.sequence_slots[start + static_cast<uint64_t>(j < last ? j : last - 1) * page_size];
-        }
+    // The wave's pages, in turns of 4 U: number w is page first + 4 U part + w / (4 U) *
+    // 4 U parts + w % (4 U). Lane l finds the bounds row of number base + l: 64 pages'
+    // slots are one load. A slot that is no page's first is reported; its row is page
+    // 0's and its key 0.
+    constexpr uint32_t STEP = 4 * U;
+    const uint32_t TURN = STEP * parts, begin = first + STEP * part;
+    auto page_of = [&](uint32_t w) { return begin + w / STEP * TURN + w % STEP; };
+    auto slot_of = [&](uint32_t base) {
+        const uint32_t j = page_of(base + lane);
+        return p.a.sequence_slots[start + static_cast<uint64_t>(j < last ? j : last - 1) * page_size];
     };
-    auto rows_of = [&](uint32_t j0, const uint64_t (&slot)[U], sglkv_u16x8 (&row)[U][NV]) {
-        uint32_t bad = 0;
+    auto row_of = [&](uint32_t base, uint64_t slot, uint64_t *bad) {
+        const uint32_t j = page_of(base + lane) < last ? page_of(base + lane) : last - 1;
+        const uint64_t left = len - static_cast<uint64_t>(j) * page_size, tokens = left < page_size ? left : page_size;
+        uint64_t page, in_page;
+        attn_split_slot(p.a, slot, &page, &in_page);
+        const bool ok = slot < p.a.slot_count && tokens <= p.a.slot_count - slot && in_page == 0;
+        *bad = __ballot(!ok);
+        if (!ok) atomicOr(p.a.flag, SGLKV_FLAG_ATTN_SLOT);
+        return bounds + (ok ? page : 0) * page_bytes;
+    };
+    auto load = [&](uint64_t rows, uint32_t w, sglkv_u16x8 (&row)[U][NV]) {
 #pragma unroll
         for (uint32_t u = 0; u < U; ++u) {
-            const uint32_t j = j0 + 4 * u + in4 < last ? j0 + 4 * u + in4 : last - 1;
-            const uint64_t left = len - static_cast<uint64_t>(j) * page_size, tokens = left < page_size ? left : page_size;
-            uint64_t page, in_page;
-            attn_split_slot(p.a, slot[u], &page, &in_page);
-            const bool ok = slot[u] < p.a.slot_count && tokens <= p.a.slot_count - slot[u] && in_page == 0;
-            if (!ok) bad |= 1u << u;
-            const uint64_t at = bounds + (ok ? page : 0) * page_bytes;
+            const uint64_t at = __shfl(rows, w + 4 * u + in4) + 16 * slot4;
 #pragma unroll
-            for (uint32_t n = 0; n < NV; ++n) row[u][n] = sel_load(at + 256 * n);
+            for (uint32_t n = 0; n < NV; ++n) row[u][n] = __builtin_nontemporal_load(reinterpret_cast<sel_vec_t *>(at + 256 * n));
         }
-        if (bad) atomicOr(p.a.flag, SGLKV_FLAG_ATTN_SLOT);
-        return bad;
     };
     const uint32_t turns = (p.a.group + 4 * NG - 1) / (4 * NG);
     for (uint32_t turn = 0; turn < turns; ++turn) {
-        const uint32_t begin = first + 4 * U * wave;
-        uint64_t slot[U];
+        if (begin >= last) break;
+        uint64_t bad, bad_next = 0;
+        uint64_t rows = row_of(0, slot_of(0), &bad), rows_next = 0;
+        uint64_t slot = slot_of(64);
         sglkv_u16x8 row[U][NV];
-        if (begin < last) slots_of(begin, slot);
+        load(rows, 0, row);
         // Element 8 (slot4 + 16 n) + e of query head g0 + 4 m + l % 4's row of parts.
         double qv[NG][NV][8];
 #pragma unroll
@@ -500,16 +527,18 @@ __device__ __forceinline__ void sel_scores_fast_body(const sglkv_select_params &
                 }
             }
         }
-        uint32_t bad = 0, bad_next = 0;
-        if (begin < last) bad = rows_of(begin, slot, row);
-        if (begin + TURN < last) slots_of(begin + TURN, slot);
-        for (uint32_t j0 = begin; j0 < last; j0 += TURN) {
+        uint32_t w = 0;  // of the 64
+        for (uint32_t base = 0, j0 = begin; j0 < last; j0 += TURN) {
+            // The next turn's rows load while this one's are multiplied.
             sglkv_u16x8 next[U][NV];
-            const bool more = j0 + TURN < last;
-            if (more) {
-                bad_next = rows_of(j0 + TURN, slot, next);
-                if (j0 + 2 * TURN < last) slots_of(j0 + 2 * TURN, slot);
+            if (w + STEP < 64) {
+                load(rows, w + STEP, next);
+            } else {
+                rows_next = row_of(base + 64, slot, &bad_next);
+                slot = slot_of(base + 128);
+                load(rows_next, 0, next);
             }
+            __builtin_amdgcn_sched_barrier(0);
             double sum[U][NG] = {};
 #pragma unroll
             for (uint32_t n = 0; n < NV; ++n)
@@ -537,27 +566,30 @@ __device__ __forceinline__ void sel_scores_fast_body(const sglkv_select_params &
                 }
                 best = sel_larger(best, sel_join<1>(best));
                 best = sel_larger(best, sel_join<2>(best));
-                const uint64_t bads = __ballot(bad >> u & 1);
                 if ((lane & 15) == u) {
                     mine = best;
-                    mine_bad = bads >> (lane >> 4) & 1;
+                    mine_bad = bad >> (w + 4 * u + (lane >> 4)) & 1;
                 }
             }
             const uint32_t j = j0 + 4 * (lane & 15) + (lane >> 4);
             if ((lane & 15) < U && j < last) {
-                if (turn > 0) mine = sel_larger(sel_best[j - first], mine);
+                if (turn > 0) mine = sel_larger(best_of[j - first], mine);
                 if (turn + 1 < turns)
-                    sel_best[j - first] = mine;
+                    best_of[j - first] = mine;
                 else
                     keys[j] = j < p.first_pages || j + p.last_pages >= count ? kSelForced : mine_bad ? 0 : sel_key(mine);
             }
-            if (more) {
+            w += STEP;
+            if (w == 64) {
+                w = 0;
+                base += 64;
+                rows = rows_next;
                 bad = bad_next;
-#pragma unroll
-                for (uint32_t u = 0; u < U; ++u)
-#pragma unroll
-                    for (uint32_t n = 0; n < NV; ++n) row[u][n] = next[u][n];
             }
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u)
+#pragma unroll
+                for (uint32_t n = 0; n < NV; ++n) row[u][n] = next[u][n];
         }
     }
 }
