@@ -403,9 +403,9 @@ extern "C" int32_t sgl_rocm_kv_compact_tokens(sgl_rocm_kv_ctx *ctx, const sgl_kv
         p.lanes[t] = 1;
         while (p.lanes[t] < pieces && p.lanes[t] < SGLKV_COMPACT_THREADS) p.lanes[t] *= 2;
     }
-    // Workgroups of up to 16 heads and 64 destination rows.
+    // Workgroups of up to 16 heads and 16 destination rows.
     p.block_heads = p.heads < 16 ? p.heads : 16;
-    p.rows = 64;
+    p.rows = 16;
     const uint64_t tiles = ceil_div(p.max_kept, p.rows), blocks = ceil_div(p.heads, p.block_heads);
     uint64_t grid;
     if (mul_ovf(tiles, p.request_count, &grid)) return attention_overflow();

@@ -106,7 +106,7 @@ __device__ __forceinline__ void bounds_body(const sglkv_bounds_params &p) {
 #pragma unroll
             for (uint32_t u = 0; u < U; ++u) {
                 const uint32_t t = t0 + GROUPS * u < tokens ? t0 + GROUPS * u : tokens - 1;
-                r[u] = sel_load(rows + static_cast<uint64_t>(t) * p.key_token_stride + 2 * d);
+                r[u] = __builtin_nontemporal_load(reinterpret_cast<sel_vec_t *>(rows + static_cast<uint64_t>(t) * p.key_token_stride + 2 * d));
             }
 #pragma unroll
             for (uint32_t u = 0; u < U; ++u)
