@@ -238,7 +238,8 @@ extern "C" int32_t sgl_rocm_kv_accumulate_weights(sgl_rocm_kv_ctx *ctx, const sg
     p.segments = (uint32_t)shape.segments;
     if (shape.segments > 1) p.partial_sums = reinterpret_cast<float *>(workspace + shape.stats_bytes + shape.joined_bytes);
     const auto &body = ctx->weight_rows[p.a.dk == 64 ? 0 : p.a.dk == 128 ? 1 : 2];
-    rc = launch_kernel(body[shape.body], way.base, way.splits, 1, shape.body == 0 ? 256 : 64, 0, s, &p, stats);
+    rc = launch_kernel(body[shape.body], way.base, way.splits, 1, shape.body == 0 ? 256 : 64,
+                       keeps ? SGLKV_WEIGHTS_LDS_BYTES(p.a.dk) : 0, s, &p, stats);
     for (p.join_lanes = 1; p.join_lanes < way.splits && p.join_lanes < 16;) p.join_lanes *= 2;
     if (!rc && !keeps && way.splits > 1)
         rc = launch_kernel(ctx->join_statistics,

@@ -338,9 +338,9 @@ __device__ __forceinline__ void wgt_take_request(const wgt_row_set<NR, DKC> &w, 
     *whole = __builtin_amdgcn_readfirstlane(least);
 }
 
-// 16 tokens from `t` (their K rows in kf) for all rows: scores, kept where STORE,
-// and the running maximum and sum. `whole`: the rows' shortest length.
-template <uint32_t DKC, uint32_t NR, bool STORE>
+// 16 tokens from `t` (their K rows in kf) for all rows: scores and the running
+// maximum and sum. `whole`: the rows' shortest length.
+template <uint32_t DKC, uint32_t NR>
 __device__ __forceinline__ void wgt_weigh_tile(const sglkv_weights_params &p, const sglkv_u16x8 (&kf)[DKC],
                                                wgt_row_set<NR, DKC> &w, const uint32_t (&limit)[NR], uint32_t t,
                                                uint32_t whole, uint32_t g) {
@@ -354,12 +354,6 @@ __device__ __forceinline__ void wgt_weigh_tile(const sglkv_weights_params &p, co
 #pragma unroll
         for (uint32_t n = 0; n < NR; ++n)
             sc[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(attn_as_bf16(kf[c]), attn_as_bf16(w.q[n][c]), sc[n], 0, 0, 0);
-    if (STORE) {
-#pragma unroll
-        for (uint32_t n = 0; n < NR; ++n)
-            if (tt < limit[n])
-                *reinterpret_cast<sglkv_f32x4 *>(p.scores + w.row[n] * p.score_stride + tt) = sc[n] * scale;
-    }
     if (t + 16 > whole) {
 #pragma unroll
         for (uint32_t n = 0; n < NR; ++n)
@@ -415,9 +409,8 @@ __device__ __forceinline__ void wgt_leave_stats(const sglkv_weights_params &p, c
 }
 
 // Statistics of 16 rows, a wave each, over the tokens of split blockIdx.y; TB
-// tiles of 16 tokens are weighed while the next TB are loading. STORE: the scores
-// go to the workspace, where the second step takes them from (K is read once).
-template <uint32_t DKC, uint32_t TB, bool STORE>
+// tiles of 16 tokens are weighed while the next TB are loading.
+template <uint32_t DKC, uint32_t TB>
 __device__ __forceinline__ void wgt_rows_body(const sglkv_weights_params &p) {
     const sglkv_attn_params &a = p.a;
     const uint32_t lane = threadIdx.x, g = lane >> 4, r = lane & 15;
@@ -458,12 +451,130 @@ __device__ __forceinline__ void wgt_rows_body(const sglkv_weights_params &p) {
                 if (t + 16 * TB * part >= t1) continue;
 #pragma unroll
                 for (uint32_t b = 0; b < TB; ++b)
-                    wgt_weigh_tile<DKC, 1, STORE>(p, kf[part % 2][b], w, limit, t + 16 * (part * TB + b), whole, g);
+                    wgt_weigh_tile<DKC, 1>(p, kf[part % 2][b], w, limit, t + 16 * (part * TB + b), whole, g);
             }
             rows = next;
         }
     }
     wgt_leave_stats<DKC, 1>(p, w, t0, g);
+}
+
+// The same where the scores are kept in the workspace for the second step, so that K
+// is read once: a decode step, which the bytes of K bound. K goes from the pool into
+// LDS in blocks of 32 tokens, one in flight while another is weighed, laid out as in
+// paged attention's staged body (attn_stg): a lane gets the scores of eight tokens in a
+// row, and the four lanes of a row write 128 bytes. 64 sequences of up to 4,096 tokens,
+// 8 KV heads of 4 query heads, dims 128 (266 MB of K, 17 MB of scores): 66 us, 4.3
+// TB/s, and 13 for the second step; with K straight to registers, 64 bytes of 16 rows
+// at a time, 76 and 17. The writes in between bound it: without them K alone goes at
+// 5.9 TB/s (128 sequences of 4,096: 183 us of 232). Three or four stages, scores in
+// blocks of 32 tokens, and stores past the caches take as long or longer.
+template <uint32_t D>
+__device__ __forceinline__ void wgt_scores_body(const sglkv_weights_params &p) {
+    typedef attn_stg<D> S;
+    constexpr uint32_t SECTION = SGLKV_WEIGHTS_SECTION;
+    extern __shared__ __attribute__((aligned(16))) uint8_t wgt_stages[];
+    uint64_t *const table = reinterpret_cast<uint64_t *>(wgt_stages + 2 * S::V);
+    const sglkv_attn_params &a = p.a;
+    const float scale = a.scale_log2;
+    const uint32_t lane = threadIdx.x, g = lane >> 4, r = lane & 15;
+    uint32_t bx = blockIdx.x;
+    const uint32_t kvh = bx % a.kv_heads;
+    bx /= a.kv_heads;
+    const uint32_t hg = bx % p.tile_head_groups;
+    const uint32_t tile = p.row_tiles - 1 - bx / p.tile_head_groups;
+    wgt_row_set<1, S::KC> w;
+    wgt_load_row_set<S::KC, 1>(p, tile * p.tile_queries, hg * 16, p.tile_head_groups > 1 ? 16 : a.group, 0, kvh, w);
+    const uint64_t kbase = reinterpret_cast<uint64_t>(a.pool) + a.key_offset + kvh * a.key_head_stride;
+    const uint32_t t0 = blockIdx.y * static_cast<uint32_t>(a.chunk_tokens);
+    const uint32_t c = lane / S::PIECES, pc = lane % S::PIECES;
+    auto issue = [&](uint32_t b) {
+        const uint64_t *rows = table + kLatB * b + S::LOADS * c;  // tokens c, TPL + c, ..
+        const uint32_t at = attn_lat_lds_at(wgt_stages) + (b & 1) * S::V;
+#pragma unroll
+        for (uint32_t h = 0; h < S::LOADS / 4; ++h) {
+            uint64_t x[4];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) x[i] = rows[4 * h + i] + 16 * S::kpos(S::TPL * (4 * h + i) + c, pc);
+            attn_lat_load4v<1024>(x, at + 4096 * h);
+        }
+    };
+    float *const scores = p.scores + static_cast<uint64_t>(w.row[0] == ~0u ? 0 : w.row[0]) * p.score_stride;
+    uint32_t seen = 0;
+    for (;;) {  // one request after another (nearly always there is one)
+        const uint32_t now = wgt_next_request<1>(w.req, seen);
+        if (now == ~0u) break;
+        uint32_t limit[1], longest, whole;
+        wgt_take_request<1>(w, now, seen, limit, &longest, &whole);
+        const uint64_t first = a.request_slot_offsets[__builtin_amdgcn_readfirstlane(now)];
+        const uint32_t most = t0 + static_cast<uint32_t>(a.chunk_tokens), t1 = longest < most ? longest : most;
+        for (uint32_t s0 = t0; s0 < t1; s0 += SECTION) {
+            uint64_t found[SECTION / 64];
+#pragma unroll
+            for (uint32_t i = 0; i < SECTION / 64; ++i)
+                found[i] = wgt_rows_at(a, kbase, first, s0 + 64 * i, t1, kvh == 0);
+            // (The last section's reads of the table are done: a wave's LDS accesses keep their order.)
+#pragma unroll
+            for (uint32_t i = 0; i < SECTION / 64; ++i) {
+                const uint32_t at = 64 * i + lane;
+                table[(at & ~31u) + S::entry(at & 31)] = found[i];
+            }
+            const uint32_t nb = ((t1 - s0 < SECTION ? t1 - s0 : SECTION) + kLatB - 1) / kLatB;
+            // The last section's stages have been read, and nothing but the rows' loads and
+            // the scores' stores counts from here on.
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            issue(0);
+            for (uint32_t k = 0; k < nb; ++k) {
+                // Block k - 1's reads are done before block k + 1 takes its stage; then block
+                // k has landed once no more is outstanding than block k + 1 (the stores
+                // between make the wait longer, which costs nothing: counting them in took
+                // as long).
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                if (k + 1 < nb) {
+                    issue(k + 1);
+                    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(S::LOADS) : "memory");
+                } else {
+                    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                }
+                const uint8_t *kst = wgt_stages + (k & 1) * S::V;
+                const uint32_t t = s0 + kLatB * k, tt = t + 8 * g;  // this lane's eight tokens
+                sglkv_f32x4 sc[2] = {sglkv_f32x4{0.f, 0.f, 0.f, 0.f}, sglkv_f32x4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+                for (uint32_t q = 0; q < S::KC; ++q)
+#pragma unroll
+                    for (uint32_t b = 0; b < 2; ++b) {
+                        const uint32_t j = 8 * (r >> 2) + 4 * b + (r & 3);
+                        const sglkv_u16x8 kf = *reinterpret_cast<const sglkv_u16x8 *>(kst + S::ROW * j + 16 * S::kpos(j, 4 * q + g));
+                        sc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(attn_as_bf16(kf), attn_as_bf16(w.q[0][q]), sc[b], 0, 0, 0);
+                    }
+                float x[8];
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e) x[e] = sc[e / 4][e % 4] * scale;
+                if (tt < limit[0]) {
+                    sglkv_f32x4 *to = reinterpret_cast<sglkv_f32x4 *>(scores + tt);
+                    to[0] = sglkv_f32x4{x[0], x[1], x[2], x[3]};
+                    to[1] = sglkv_f32x4{x[4], x[5], x[6], x[7]};
+                }
+                if (t + kLatB > whole) {
+#pragma unroll
+                    for (uint32_t e = 0; e < 8; ++e)
+                        if (tt + e >= limit[0]) x[e] = -INFINITY;
+                }
+                // (As wgt_weigh_tile: the reference moves where a score passes it by 8.)
+                float top = x[0];
+#pragma unroll
+                for (uint32_t e = 1; e < 8; ++e) top = fmaxf(top, x[e]);
+                if (__ballot(top > w.m[0] + 8.0f)) {
+                    const float up = fmaxf(w.m[0], top);
+                    w.l[0] *= __builtin_amdgcn_exp2f(w.m[0] - up);
+                    w.m[0] = up;
+                }
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e) w.l[0] += __builtin_amdgcn_exp2f(x[e] - w.m[0]);
+            }
+        }
+    }
+    wgt_leave_stats<S::KC, 1>(p, w, t0, g);
 }
 
 // The queries [*q0, *q1) of request `req`, whose indices never fall: 32 places
@@ -590,7 +701,7 @@ __device__ __forceinline__ void wgt_tile_stats_body(const sglkv_weights_params &
                     sglkv_u16x8 kf[DKC];
 #pragma unroll
                     for (uint32_t c = 0; c < DKC; ++c) kf[c] = *reinterpret_cast<const sglkv_u16x8 *>(at + 64 * c);
-                    wgt_weigh_tile<DKC, NR, false>(p, kf, w, limit, t + 16 * b, whole, g);
+                    wgt_weigh_tile<DKC, NR>(p, kf, w, limit, t + 16 * b, whole, g);
                 }
             }
             if (more) {
@@ -1008,10 +1119,10 @@ extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(
     wgt_tile_stats_body<2, 4>(p);
 }
 extern "C" __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void sglkv_weight_few64(sglkv_weights_params p) {
-    wgt_rows_body<2, 2, false>(p);
+    wgt_rows_body<2, 2>(p);
 }
 extern "C" __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void sglkv_weight_scores64(sglkv_weights_params p) {
-    wgt_rows_body<2, 2, true>(p);
+    wgt_scores_body<64>(p);
 }
 extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void sglkv_accumulate_rows64(sglkv_weights_params p) {
     wgt_tile_accumulate_body<2, 4>(p);
@@ -1020,10 +1131,10 @@ extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(
     wgt_tile_stats_body<4, 4>(p);
 }
 extern "C" __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void sglkv_weight_few128(sglkv_weights_params p) {
-    wgt_rows_body<4, 2, false>(p);
+    wgt_rows_body<4, 2>(p);
 }
 extern "C" __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void sglkv_weight_scores128(sglkv_weights_params p) {
-    wgt_rows_body<4, 2, true>(p);
+    wgt_scores_body<128>(p);
 }
 extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void sglkv_accumulate_rows128(sglkv_weights_params p) {
     wgt_tile_accumulate_body<4, 4>(p);
@@ -1032,10 +1143,10 @@ extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(
     wgt_tile_stats_body<8, 2>(p);
 }
 extern "C" __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void sglkv_weight_few256(sglkv_weights_params p) {
-    wgt_rows_body<8, 1, false>(p);
+    wgt_rows_body<8, 1>(p);
 }
 extern "C" __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void sglkv_weight_scores256(sglkv_weights_params p) {
-    wgt_rows_body<8, 1, true>(p);
+    wgt_scores_body<256>(p);
 }
 extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void sglkv_accumulate_rows256(sglkv_weights_params p) {
     wgt_tile_accumulate_body<8, 2>(p);

@@ -421,6 +421,9 @@ typedef struct sglkv_select_params {
  * pair of 32-bit floats per (query, head, split), in log2 units. */
 #define SGLKV_WEIGHTS_TILE 64u    /* tokens of a wave of the accumulation (32 at dims 256) */
 #define SGLKV_WEIGHTS_THREADS 256u
+/* Scores kept (wgt_scores_body): blocks of 32 tokens' keys in LDS, a table of rows. */
+#define SGLKV_WEIGHTS_SECTION 256u
+#define SGLKV_WEIGHTS_LDS_BYTES(d) (2u * 64u * (d) + 8u * SGLKV_WEIGHTS_SECTION)
 #define SGLKV_WEIGHTS_APPLY 1024u /* tokens of a workgroup that applies kept scores */
 typedef struct sglkv_weights_params {
     sglkv_attn_params a;
