@@ -1003,7 +1003,7 @@ __device__ __forceinline__ void evt_select_body(const sglkv_evict_params &p) {
     uint64_t start;
     const uint64_t len = evt_request(p, req, head == 0 && threadIdx.x == 0, &start);
     const float *weights = p.weights + head * p.sequence_slot_count + start;
-    sel_pick<uint32_t, SGLKV_EVICT_THREADS / 64>(
+    sel_pick<uint32_t, SGLKV_EVICT_THREADS / 64, 16>(
         len, p.max_kept,
         [&](uint64_t i) { return i < p.first_tokens || i + p.last_tokens >= len ? ~0u : evt_key(weights[i]); },
         p.kept + (req * p.heads + head) * p.max_kept, state);

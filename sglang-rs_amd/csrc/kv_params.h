@@ -397,7 +397,7 @@ typedef struct sglkv_bounds_params {
  * page_size, whose tokens are the page's first ones in order. */
 #define SGLKV_SELECT_NONE 0xFFFFFFFFu   /* past the end of a page list */
 #define SGLKV_SELECT_THREADS 256u
-#define SGLKV_SELECT_LDS_PAGES 8192u    /* keys a picking workgroup keeps in LDS (8 bytes each) */
+#define SGLKV_SELECT_LDS_PAGES 2048u    /* most pages of a chunk whose maxima wait in LDS (8 bytes each) */
 #define SGLKV_SELECT_CHUNK_PAGES 64u    /* most pages of a split of the attention: one lane's each */
 #define SGLKV_SELECT_QSTRIDE(dk) (((dk) + 7u) & ~7u) /* dims of a query head in a scoring workgroup's LDS */
 typedef struct sglkv_select_params {

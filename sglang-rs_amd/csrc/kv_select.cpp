@@ -288,7 +288,7 @@ extern "C" int32_t sgl_rocm_kv_select_pages(sgl_rocm_kv_ctx *ctx, const sgl_kv_p
         p.heads = p.a.kv_heads * (uint32_t)shape.chunks;
         const int dims = p.a.dk == 64 ? 0 : p.a.dk == 128 ? 1 : p.a.dk == 256 ? 2 : -1;
         if (vector && dims >= 0 && reinterpret_cast<uint64_t>(p.a.queries) % 16 == 0 &&
-            shape.chunk_pages <= SGLKV_SELECT_LDS_PAGES / 4) {
+            shape.chunk_pages <= SGLKV_SELECT_LDS_PAGES) {
             // 4, 8 or 16 query heads a turn; past that several, whose maxima wait in LDS.
             const int heads = p.a.group <= 4 ? 0 : p.a.group <= 8 || dims == 2 ? 1 : 2;
             p.block_heads = p.a.kv_heads % 4 == 0 ? 4 : p.a.kv_heads % 2 == 0 ? 2 : 1;
@@ -303,10 +303,7 @@ extern "C" int32_t sgl_rocm_kv_select_pages(sgl_rocm_kv_ctx *ctx, const sgl_kv_p
         }
         if (rc) return rc;
     }
-    const uint64_t kept = shape.key_bytes == 0                                ? 0
-                          : shape.sequence_pages < SGLKV_SELECT_LDS_PAGES     ? shape.sequence_pages
-                                                                              : SGLKV_SELECT_LDS_PAGES;
-    rc = launch_kernel(ctx->pick_pages, shape.items, 1, 1, SGLKV_SELECT_THREADS, (unsigned)(8 * kept), s, &p, "page pick launch");
+    rc = launch_kernel(ctx->pick_pages, shape.items, 1, 1, SGLKV_SELECT_THREADS, 0, s, &p, "page pick launch");
     return rc ? rc : ok();
 }
 

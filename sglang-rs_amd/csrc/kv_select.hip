@@ -265,75 +265,117 @@ __device__ __forceinline__ void sel_stage_queries(const sglkv_attn_params &p, ui
     }
 }
 
+constexpr uint32_t kSelBuckets = 1024;
+
 struct sel_pick_state {
-    uint32_t histogram[256];
-    uint64_t ors[16], ands[16];
-    uint32_t above[16], equal[16];
-    uint64_t prefix;
-    uint32_t shift, need, done;
+    uint32_t histogram[kSelBuckets];
+    uint64_t low[16], high[16], lo, hi;
+    uint32_t special[16], above[16], equal[16];
+    uint32_t need, done;
 };
 
 // Writes the indices of the `keep` largest of keys load(0..n), ties to the
 // lowest index, ascending, to out[0..keep), SGLKV_SELECT_NONE behind them.
-// A workgroup of WAVES waves. Radix selection from the first bit in which the
-// keys differ, 8 bits a round, until a bucket is taken whole: about two rounds
-// on scores, at most one per 8 bits. Counting uses LDS atomics, whose order
-// does not show.
-template <typename Key, uint32_t WAVES, class Load>
+// A workgroup of WAVES waves, each with a run of indices, whose keys stay in
+// registers where a thread has EACH or fewer: one round trip to memory, where five
+// passes over the keys each waited for their own (32 requests of up to 10,000 floats
+// on 8 heads: 22 us of 32). Each round counts the keys of [lo, hi] in 1,024 equal steps and
+// goes on in the step where the count from above reaches `keep`, until a step is
+// taken whole: two rounds on most scores. Forced entries and NaN, the two
+// largest keys, are counted apart: they would stretch the steps over the whole
+// type. Counting uses LDS atomics, whose order does not show.
+template <typename Key, uint32_t WAVES, uint32_t EACH, class Load>
 __device__ __forceinline__ void sel_pick(uint64_t n, uint64_t keep, Load load, uint32_t *out, sel_pick_state &s) {
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid / 64;
-    constexpr uint32_t THREADS = 64 * WAVES;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    constexpr uint32_t THREADS = 64 * WAVES, U = EACH < 8 ? EACH : 8;
+    constexpr Key kSpecial = static_cast<Key>(~static_cast<Key>(0)) - 1;
     if (n <= keep) {
         for (uint64_t i = tid; i < keep; i += THREADS) out[i] = i < n ? static_cast<uint32_t>(i) : SGLKV_SELECT_NONE;
         return;
     }
-    Key ors = 0, ands = static_cast<Key>(~static_cast<Key>(0));
-    for (uint64_t i = tid; i < n; i += THREADS) {
-        const Key k = load(i);
-        ors |= k;
-        ands &= k;
-    }
+    const uint64_t run = (n + THREADS - 1) / THREADS * 64, i0 = wave * run, i1 = i0 + run < n ? i0 + run : n;
+    const bool fits = n <= static_cast<uint64_t>(THREADS) * EACH;
+    Key held[EACH];
+    if (fits)
+#pragma unroll
+        for (uint32_t j = 0; j < EACH; ++j) {
+            const uint64_t i = i0 + 64 * j + lane;
+            held[j] = i < i1 ? load(i) : 0;
+        }
+    // f(index, key) for the wave's run, 64 at a time (the last ones may pass i1).
+    auto each = [&](auto f) {
+        if (fits) {
+#pragma unroll
+            for (uint32_t j = 0; j < EACH; ++j)
+                if (i0 + 64 * j < i1) f(i0 + 64 * j + lane, held[j]);
+        } else {
+            for (uint64_t base = i0; base < i1; base += 64 * U) {
+                Key x[U];
+#pragma unroll
+                for (uint32_t u = 0; u < U; ++u) {
+                    const uint64_t i = base + 64 * u + lane;
+                    x[u] = load(i < i1 ? i : i1 - 1);
+                }
+#pragma unroll
+                for (uint32_t u = 0; u < U; ++u)
+                    if (base + 64 * u < i1) f(base + 64 * u + lane, x[u]);
+            }
+        }
+    };
+    Key low = static_cast<Key>(~static_cast<Key>(0)), high = 0;
+    uint32_t special = 0;
+    each([&](uint64_t i, Key k) {
+        const bool in = i < i1, ordinary = in && k < kSpecial;
+        special += __popcll(__ballot(in && !ordinary));
+        low = ordinary && k < low ? k : low;
+        high = ordinary && k > high ? k : high;
+    });
 #pragma unroll
     for (uint32_t m = 1; m < 64; m <<= 1) {
-        ors |= __shfl_xor(ors, m);
-        ands &= __shfl_xor(ands, m);
+        const Key l = __shfl_xor(low, m), h = __shfl_xor(high, m);
+        low = l < low ? l : low;
+        high = h > high ? h : high;
     }
     if (lane == 0) {
-        s.ors[wave] = ors;
-        s.ands[wave] = ands;
+        s.low[wave] = low;
+        s.high[wave] = high;
+        s.special[wave] = special;
     }
     __syncthreads();
     if (tid == 0) {
-        Key o = 0, a = static_cast<Key>(~static_cast<Key>(0));
-        for (uint32_t w = 0; w < WAVES; ++w) {
-            o |= static_cast<Key>(s.ors[w]);
-            a &= static_cast<Key>(s.ands[w]);
+        uint64_t lo = s.low[0], hi = s.high[0];
+        uint32_t count = s.special[0];
+        for (uint32_t w = 1; w < WAVES; ++w) {
+            lo = s.low[w] < lo ? s.low[w] : lo;
+            hi = s.high[w] > hi ? s.high[w] : hi;
+            count += s.special[w];
         }
-        const uint64_t differ = static_cast<uint64_t>(static_cast<Key>(o ^ a));
-        const uint32_t bits = differ ? 64 - __builtin_clzll(differ) : 0;  // the bits below which keys differ
-        s.shift = bits;
-        s.prefix = bits < 64 ? static_cast<uint64_t>(o) >> bits : 0;
-        s.need = static_cast<uint32_t>(keep);
-        s.done = bits == 0;
+        const bool enough = count >= keep;
+        s.lo = enough ? static_cast<uint64_t>(kSpecial) : lo;
+        s.hi = enough ? static_cast<uint64_t>(kSpecial) + 1 : hi;
+        s.need = static_cast<uint32_t>(enough ? keep : keep - count);
+        s.done = s.lo == s.hi;
     }
     __syncthreads();
-    // Keys are `prefix` above bit `shift`; `need` of those that are, are taken.
+    // `need` of the keys in [lo, hi] are taken, and all above.
     while (!s.done) {
-        const uint32_t shift = s.shift, next = shift > 8 ? shift - 8 : 0;
-        const uint64_t prefix = s.prefix;
-        for (uint32_t b = tid; b < 256; b += THREADS) s.histogram[b] = 0;
+        const uint64_t lo = s.lo, hi = s.hi;
+        const uint32_t bits = 64 - __builtin_clzll(hi - lo), shift = bits > 10 ? bits - 10 : 0;
+        for (uint32_t b = tid; b < kSelBuckets; b += THREADS) s.histogram[b] = 0;
         __syncthreads();
-        for (uint64_t i = tid; i < n; i += THREADS) {
-            const uint64_t k = static_cast<uint64_t>(load(i));
-            const uint64_t top = shift < 64 ? k >> shift : 0;
-            if (top == prefix) atomicAdd(&s.histogram[(k >> next) & ((1u << (shift - next)) - 1)], 1u);
-        }
+        each([&](uint64_t i, Key k) {
+            if (i < i1 && k >= lo && k <= hi) atomicAdd(&s.histogram[(k - lo) >> shift], 1u);
+        });
         __syncthreads();
         if (wave == 0) {
-            // Lane l holds buckets 4 (63 - l) .. + 3: sums from the top down.
-            const uint32_t b0 = 4 * (63 - lane);
-            const uint32_t c[4] = {s.histogram[b0 + 3], s.histogram[b0 + 2], s.histogram[b0 + 1], s.histogram[b0]};
-            const uint32_t sum = c[0] + c[1] + c[2] + c[3];
+            // Lane l holds buckets B (63 - l) .. + B - 1: sums from the top down.
+            constexpr uint32_t B = kSelBuckets / 64;
+            const uint32_t b0 = B * (63 - lane);
+            uint32_t c[B], sum = 0;
+#pragma unroll
+            for (uint32_t b = 0; b < B; ++b) c[b] = s.histogram[b0 + B - 1 - b];
+#pragma unroll
+            for (uint32_t b = 0; b < B; ++b) sum += c[b];
             uint32_t upto = sum;
 #pragma unroll
             for (uint32_t m = 1; m < 64; m <<= 1) {
@@ -343,30 +385,31 @@ __device__ __forceinline__ void sel_pick(uint64_t n, uint64_t keep, Load load, u
             const uint32_t need = s.need;
             uint32_t before = upto - sum;
             if (before < need && upto >= need) {  // (one lane: the counts reach `need`)
-                uint32_t j = 0;
-                while (j < 3 && before + c[j] < need) before += c[j++];
+                uint32_t down = 0, here = c[0];
+#pragma unroll
+                for (uint32_t b = 1; b < B; ++b)
+                    if (down + 1 == b && before + here < need) {
+                        before += here;
+                        here = c[b];
+                        down = b;
+                    }
+                const uint64_t from = lo + (static_cast<uint64_t>(b0 + B - 1 - down) << shift), width = (1ull << shift) - 1;
                 s.need = need - before;
-                s.prefix = (shift < 64 ? prefix << (shift - next) : 0) | (b0 + 3 - j);
-                s.shift = next;
-                s.done = c[j] == need - before || next == 0;
+                s.lo = from;
+                s.hi = hi - from < width ? hi : from + width;
+                s.done = here == need - before || shift == 0;
             }
         }
         __syncthreads();
     }
-    const uint32_t shift = s.shift, need = s.need;
-    const uint64_t prefix = s.prefix;
-    auto top = [&](uint64_t i) {
-        const uint64_t k = static_cast<uint64_t>(load(i));
-        return shift < 64 ? k >> shift : 0;
-    };
-    // Each wave a run of indices: count, then write in order.
-    const uint64_t run = (n + WAVES - 1) / WAVES, i0 = wave * run, i1 = i0 + run < n ? i0 + run : n;
+    const uint64_t lo = s.lo, hi = s.hi;
+    const uint32_t need = s.need;
+    // Count, then write in order.
     uint32_t above = 0, equal = 0;
-    for (uint64_t i = i0; i < i1; i += 64) {
-        const uint64_t t = i + lane < i1 ? top(i + lane) : 0;
-        above += __popcll(__ballot(i + lane < i1 && t > prefix));
-        equal += __popcll(__ballot(i + lane < i1 && t == prefix));
-    }
+    each([&](uint64_t i, Key k) {
+        above += __popcll(__ballot(i < i1 && k > hi));
+        equal += __popcll(__ballot(i < i1 && k >= lo && k <= hi));
+    });
     if (lane == 0) {
         s.above[wave] = above;
         s.equal[wave] = equal;
@@ -378,21 +421,20 @@ __device__ __forceinline__ void sel_pick(uint64_t n, uint64_t keep, Load load, u
         ties += s.equal[w];
     }
     at += ties < need ? ties : need;
-    for (uint64_t i = i0; i < i1; i += 64) {
-        const bool in = i + lane < i1;
-        const uint64_t t = in ? top(i + lane) : 0;
-        const uint64_t eq = __ballot(in && t == prefix);
+    each([&](uint64_t i, Key k) {
+        const bool in = i < i1, tie = in && k >= lo && k <= hi;
+        const uint64_t eq = __ballot(tie);
         const uint32_t rank = ties + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(eq >> 32),
                                                                __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(eq), 0));
-        const bool take = in && (t > prefix || (t == prefix && rank < need));
+        const bool take = in && (k > hi || (tie && rank < need));
         const uint64_t taken = __ballot(take);
         if (take)
             out[at + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(taken >> 32),
                                                __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(taken), 0))] =
-                static_cast<uint32_t>(i + lane);
+                static_cast<uint32_t>(i);
         at += __popcll(taken);
         ties += __popcll(eq);
-    }
+    });
 }
 
 // Scores of a chunk of a (query, KV head)'s pages into the workspace.
@@ -596,24 +638,15 @@ __device__ __forceinline__ void sel_scores_fast_body(const sglkv_select_params &
 
 // The pages of a (query, KV head) from the workspace's keys.
 __device__ __forceinline__ void sel_pick_body(const sglkv_select_params &p) {
-    extern __shared__ __attribute__((aligned(16))) uint8_t sel_lds[];
     __shared__ sel_pick_state state;
-    uint64_t *kept = reinterpret_cast<uint64_t *>(sel_lds);
     const uint32_t head = blockIdx.x % p.a.kv_heads;
     const uint64_t q = blockIdx.x / p.a.kv_heads;
     uint64_t start, len;
     sel_sequence(p.a, p.max_length, q, head == 0 && threadIdx.x == 0, &start, &len);
     const uint64_t count = (len + p.a.page_size - 1) / p.a.page_size;
     const uint64_t *keys = p.keys + (q * p.a.kv_heads + head) * p.sequence_pages;
-    uint32_t *out = p.selected + (q * p.a.kv_heads + head) * p.max_pages;
-    if (count <= SGLKV_SELECT_LDS_PAGES) {
-        if (count > p.max_pages)
-            for (uint64_t i = threadIdx.x; i < count; i += SGLKV_SELECT_THREADS) kept[i] = keys[i];
-        __syncthreads();
-        sel_pick<uint64_t, SGLKV_SELECT_THREADS / 64>(count, p.max_pages, [&](uint64_t i) { return kept[i]; }, out, state);
-    } else {
-        sel_pick<uint64_t, SGLKV_SELECT_THREADS / 64>(count, p.max_pages, [&](uint64_t i) { return keys[i]; }, out, state);
-    }
+    sel_pick<uint64_t, SGLKV_SELECT_THREADS / 64, 8>(count, p.max_pages, [&](uint64_t i) { return keys[i]; },
+                                                     p.selected + (q * p.a.kv_heads + head) * p.max_pages, state);
 }
 
 // ---- Attention over the selected pages --------------------------------------
