@@ -1121,9 +1121,10 @@ typedef struct sgl_kv_weight_buffers {
  * statistics and sums are held in 32 bits; positions that no query attends stay
  * as they are. The result does not depend on the order in which workgroups run.
  * The queries come request by request: query_request_indices never fall
- * (otherwise REQUEST is reported and the sums are unspecified). A query of
- * length 0 (padding) adds nothing, nor does one whose metadata does not hold
- * (reported as paged attention does). */
+ * (otherwise REQUEST is reported and the sums are unspecified), those of padding
+ * among them: a query of length 0 adds nothing and may have any index that keeps
+ * the order, UINT32_MAX behind a batch. Nor does a query add anything whose
+ * metadata does not hold (reported as paged attention does). */
 int32_t sgl_rocm_kv_accumulate_weights(sgl_rocm_kv_ctx *ctx, const sgl_kv_weight_plan *plan,
                                        const sgl_kv_weight_buffers *buffers, void *stream);
 
@@ -1198,7 +1199,8 @@ int32_t sgl_rocm_kv_select_tokens(sgl_rocm_kv_ctx *ctx, const sgl_kv_eviction_pl
  * also for a position past the length); a slot past its pool is reported
  * (SLOT); such rows are skipped. No destination slot may be a source slot of
  * the call: a row could be overwritten before it is read. Passing one buffer as
- * both slot lists of the same layer is refused (InvalidArgument "in place"). */
+ * both slot lists of the same layer, or as both sums, is refused
+ * (InvalidArgument "in place"). */
 int32_t sgl_rocm_kv_compact_tokens(sgl_rocm_kv_ctx *ctx, const sgl_kv_eviction_plan *plan,
                                    const sgl_kv_eviction_buffers *buffers, const sgl_kv_pool_view *source,
                                    const sgl_kv_pool_view *destination, void *stream);

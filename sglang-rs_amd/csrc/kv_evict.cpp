@@ -378,6 +378,8 @@ extern "C" int32_t sgl_rocm_kv_compact_tokens(sgl_rocm_kv_ctx *ctx, const sgl_kv
     if ((rc = check_device(ctx, "source", from)) || (rc = check_device(ctx, "destination", to))) return rc;
     if (p.sequence_slots == p.to_slots && p.src.plane[0] == p.dst.plane[0])
         return fail(SGL_KV_INVALID_ARGUMENT, "in place", 0, 0, 0, "rows cannot be compacted onto their own slots");
+    if (p.to_weights && p.to_weights == p.weights)
+        return fail(SGL_KV_INVALID_ARGUMENT, "in place", 0, 0, 0, "sums cannot be compacted onto their own columns");
     if (source->scale && destination->scale) {
         const sgl_kv_device_buffer scales[2] = {{source->scale, 4ull * source->tensor_count},
                                                 {destination->scale, 4ull * source->tensor_count}};
@@ -404,9 +406,8 @@ extern "C" int32_t sgl_rocm_kv_compact_tokens(sgl_rocm_kv_ctx *ctx, const sgl_kv
         p.lanes[t] = 1;
         while (p.lanes[t] < pieces && p.lanes[t] < SGLKV_COMPACT_THREADS) p.lanes[t] *= 2;
     }
-    // Workgroups of up to 16 heads and 16 destination rows.
-    p.block_heads = p.heads < 16 ? p.heads : 16;
-    p.rows = 16;
+    p.block_heads = p.heads < SGLKV_COMPACT_HEADS ? p.heads : SGLKV_COMPACT_HEADS;
+    p.rows = SGLKV_COMPACT_ROWS;
     const uint64_t tiles = ceil_div(p.max_kept, p.rows), blocks = ceil_div(p.heads, p.block_heads);
     uint64_t grid;
     if (mul_ovf(tiles, p.request_count, &grid)) return attention_overflow();

@@ -445,7 +445,9 @@ typedef struct sglkv_weights_params {
  * sums' copy. */
 #define SGLKV_EVICT_THREADS 1024u       /* of a choosing workgroup */
 #define SGLKV_COMPACT_THREADS 256u
-#define SGLKV_COMPACT_CHUNKS 1024u      /* (row, head)s that a copying workgroup resolves: 16 bytes of LDS each */
+#define SGLKV_COMPACT_ROWS 16u          /* destination rows of a copying workgroup ... */
+#define SGLKV_COMPACT_HEADS 16u         /* ... and at most this many heads: 16 bytes of LDS for each (row, head) */
+#define SGLKV_COMPACT_CHUNKS (SGLKV_COMPACT_ROWS * SGLKV_COMPACT_HEADS)
 typedef struct sglkv_evict_params {
     const uint64_t *request_lengths;
     const uint64_t *request_slot_offsets;

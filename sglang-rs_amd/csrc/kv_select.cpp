@@ -106,8 +106,13 @@ int32_t selection_shape(const sgl_kv_attention_plan_config &c, const sgl_kv_page
                          mul_ovf(h.record_bytes, 4ull * (SGLKV_ATTN_OPAD(c.value_head_dim) + 2), &h.record_bytes)))
         return attention_overflow();
     // A dispatch counts its work-items in 32 bits.
-    if (h.items > UINT32_MAX / SGLKV_SELECT_THREADS / h.chunks)
-        return too_large_dim("workgroups", h.items, UINT32_MAX / SGLKV_SELECT_THREADS / h.chunks);
+    // (The scores' workgroups are placed eight (query, chunk)s at a time.)
+    uint64_t placed;
+    if (mul_ovf(c.query_count, h.chunks, &placed) || placed > UINT64_MAX - 7 ||
+        mul_ovf(ceil_div(placed, 8) * 8, c.kv_head_count, &placed))
+        return attention_overflow();
+    if (placed > UINT32_MAX / SGLKV_SELECT_THREADS)
+        return too_large_dim("workgroups", placed, UINT32_MAX / SGLKV_SELECT_THREADS);
     if (base > UINT32_MAX / 64) return too_large_dim("workgroups", base, UINT32_MAX / 64);
     if (heads > UINT32_MAX / 64) return too_large_dim("workgroups", heads, UINT32_MAX / 64);
     return SGL_KV_OK;

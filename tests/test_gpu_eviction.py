@@ -113,6 +113,66 @@ def test_weights(k, page, heads, qheads, dk, dv, hnd, shift, lengths, per):
     assert (got[want == start] == start[want == start]).all()  # untouched positions
 
 
+@pytest.mark.parametrize("dk", [64, 128, 256])
+def test_weights_of_a_long_slot_list(k, dk):
+    """A plan for 4.4 million positions, whose scores are not kept: the few rows' way."""
+    rng = np.random.default_rng(dk)
+    pool = Pool(rng, page=16, heads=1, dk=dk, pages=60)
+    batch = Batch(rng, pool, (500, 60, 300), 20, 1, spare=1_500_000)
+    assert 4 * 60 * len(batch.slots) > 256 << 20
+    start = rng.random((1, len(batch.slots))).astype(np.float32)
+    _say(f"weights of a long slot list, dims {dk}")
+    got = _run_weights(k, batch, start)
+    k.check_errors()
+    want = _weights(batch, start)
+    _check_weights(got, want)
+    assert (got[want == start] == start[want == start]).all()
+
+
+@pytest.mark.parametrize("dk,qheads,per", [(128, 8, 1), (128, 8, 40), (64, 40, 2), (40, 6, 2)])
+def test_weights_of_a_padded_batch(k, dk, qheads, per):
+    """Queries of length 0 between the requests' and behind them (index UINT32_MAX) add nothing."""
+    rng = np.random.default_rng(dk + per)
+    pool = Pool(rng, page=16, heads=2, dk=dk, pages=80)
+    batch = Batch(rng, pool, (500, 60, 0, 300), qheads, per)
+    start = rng.random((2, len(batch.slots))).astype(np.float32)
+    want = _weights(batch, start)
+    batch.requests = np.concatenate([batch.requests, np.full(9, NONE, np.uint32)])
+    batch.ends = np.concatenate([batch.ends, np.zeros(9, np.uint64)])
+    padding = np.full((9, *batch.queries.shape[1:]), 0x7FC0, np.uint16)  # NaN
+    batch.queries = np.concatenate([batch.queries, padding])
+    batch.upload()
+    _say(f"weights of a padded batch, dims {dk}")
+    got = _run_weights(k, batch, start)
+    k.check_errors()
+    _check_weights(got, want)
+
+
+def test_weights_refusals(k):
+    rng = np.random.default_rng(12)
+    pool = Pool(rng, page=8, heads=2, dk=64, pages=4)
+    batch = Batch(rng, pool, (20,), 4)
+    plan = kv.WeightAccumulationPlan.new(batch.plan())
+    sums, workspace = _filled(plan.weights_required_bytes), _filled(plan.workspace_required_bytes)
+    sound = dict(batch.device, pool=pool.buffer, weights=sums, workspace=workspace)
+
+    def refused(variant, name, **more):
+        with pytest.raises(kv.KvError) as e:
+            k.accumulate_weights(plan, kv.WeightAccumulationBuffers(**{**sound, **more}))
+        assert (e.value.variant, e.value.name) == (variant, name)
+
+    host = np.zeros(1 << 16, np.uint8)
+    for name in sound:
+        refused("DeviceMismatch", name, **{name: kv.device_buffer(host.ctypes.data, host.nbytes)})
+        refused("AllocationOutOfBounds", name, **{name + "_offset": 1 << 20})
+    for name in ("queries", "query_request_indices", "query_sequence_lengths", "request_slot_offsets", "sequence_slots",
+                 "weights", "workspace"):
+        big = _filled(1 << 16)
+        refused("InvalidArgument", "alignment", **{name: big, name + "_offset": 1})
+    assert (sums.download() == 0xA5).all()
+    k.check_errors()
+
+
 def test_weights_of_one_call_add_up_and_repeat(k):
     """Two calls add twice; the same call gives the same bits; a row's weights sum to 1."""
     rng = np.random.default_rng(2)
@@ -474,5 +534,6 @@ def test_compact_refusals(k):
                    dict(heads=2, chunk=64, value_chunk=32)):
         _, kept_alive, wrong, _ = _side(rng, page=8, pages=2, **change)
         refused("InvalidArgument", "views", destination=wrong, destination_slots=other)
+    refused("InvalidArgument", "in place", destination_slots=other, weights=other, destination_weights=other)
     host = np.zeros(64, np.uint8)
     refused("DeviceMismatch", "kept", destination_slots=other, kept=kv.device_buffer(host.ctypes.data, 64))

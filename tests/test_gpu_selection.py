@@ -418,3 +418,65 @@ def test_select_then_attend_matches_the_definition(k):
     want, absolute = ref.attend(batch, lists)
     _check(_run_attend(k, batch, lists), want, absolute)
     k.check_errors()
+
+
+def test_padded_batches_select_and_attend_nothing(k):
+    """Queries of length 0 behind the batch, of any request index, get no pages and zeros."""
+    rng = np.random.default_rng(17)
+    pool = Pool(rng, page=16, heads=2, dk=64, pages=90)
+    batch = Batch(rng, pool, (700, 90, 400), 8)
+    bounds = _bounds(rng, pool)
+    want = ref.select(batch, bounds, 6)
+    want_output, absolute = ref.attend(batch, want)
+    batch.requests = np.concatenate([batch.requests, np.array([0, 2, NONE, 7], np.uint32)])
+    batch.ends = np.concatenate([batch.ends, np.zeros(4, np.uint64)])
+    batch.queries = np.concatenate([batch.queries, np.full((4, 8, 64), 0x7FC0, np.uint16)])
+    batch.upload()
+    lists = _run_select(k, batch, bounds, 6)
+    assert np.array_equal(lists[:3], want) and (lists[3:] == NONE).all()
+    output = _run_attend(k, batch, lists)
+    _check(output[:3], want_output, absolute)
+    assert (output[3:] == 0).all()
+    k.check_errors()
+
+
+def test_refusals(k):
+    rng = np.random.default_rng(18)
+    pool = Pool(rng, page=8, heads=2, dk=64, pages=40)
+    batch = Batch(rng, pool, (250,), 4)
+    plan = kv.PageSelectionPlan.new(batch.plan(), max_pages=20)
+    bounds = _filled(plan.bounds_required_bytes)
+    selected, output = _filled(plan.selected_required_bytes), _filled(plan.attention.output_required_bytes)
+    sound = dict(batch.device, pool=pool.buffer, bounds=bounds, selected=selected, output=output,
+                 workspace=_workspace(plan))
+    shared = ("queries", "query_request_indices", "query_sequence_lengths", "request_slot_offsets", "sequence_slots",
+              "selected", "workspace")
+    host = np.zeros(1 << 16, np.uint8)
+    for call, own in ((k.select_pages, ("bounds",)), (k.selected_attention, ("pool", "output"))):
+        def refused(variant, name, **more):
+            with pytest.raises(kv.KvError) as e:
+                call(plan, kv.PageSelectionBuffers(**{**sound, **more}))
+            assert (e.value.variant, e.value.name) == (variant, name)
+        for name in shared + own:
+            refused("DeviceMismatch", name, **{name: kv.device_buffer(host.ctypes.data, host.nbytes)})
+            refused("AllocationOutOfBounds", name, **{name + "_offset": 1 << 30})
+            if name != "pool":
+                big = _filled(1 << 18)
+                with pytest.raises(kv.KvError) as e:
+                    call(plan, kv.PageSelectionBuffers(**{**sound, name: big, name + "_offset": 1}))
+                assert e.value.variant == "InvalidArgument"
+    assert (selected.download() == 0xA5).all() and (output.download() == 0xA5).all()
+    # page_bounds
+    lists = dict(pages=_filled(64), counts=_filled(64), bounds=bounds)
+
+    def refused_bounds(variant, name, **more):
+        with pytest.raises(kv.KvError) as e:
+            k.page_bounds(pool.view(), **{**lists, "page_count": 4, **more})
+        assert (e.value.variant, e.value.name) == (variant, name)
+    for name in lists:
+        refused_bounds("DeviceMismatch", name, **{name: kv.device_buffer(host.ctypes.data, host.nbytes)})
+    refused_bounds("AllocationOutOfBounds", "pages", page_count=17)
+    refused_bounds("AllocationOutOfBounds", "bounds", bounds=_filled(64))
+    k.page_bounds(pool.view(), **lists, page_count=0)
+    assert (bounds.download() == 0xA5).all()
+    k.check_errors()
