@@ -412,7 +412,7 @@ typedef struct sglkv_select_params {
     uint32_t chunk_pages;     /* attention: pages per split; scores: pages per workgroup */
     uint32_t heads;           /* scores: KV heads * chunks of a query */
     uint32_t block_heads;     /* scores: KV heads of a workgroup (1, 2 or 4) */
-    uint32_t reserved;
+    uint32_t near_queries;    /* scores: consecutive queries whose workgroups share an XCD */
 } sglkv_select_params;
 
 /* The softmax weights that each position of a sequence gets, summed over the

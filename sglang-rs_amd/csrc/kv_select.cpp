@@ -31,7 +31,7 @@ int32_t misaligned(const char *name) {
 // The launch shapes of a plan's two calls.
 struct SelectionShape {
     uint64_t max_length, sequence_pages, items;  // items: (query, KV head)s
-    uint64_t chunk_pages, chunks;                // of the scores
+    uint64_t chunk_pages, chunks, near_queries;  // of the scores
     uint64_t key_bytes;
     uint64_t split_pages, splits;                // of the attention
     uint64_t record_bytes;
@@ -40,10 +40,10 @@ struct SelectionShape {
 // Chunks of pages that the scores are cut into, 16 pages or more each: a wave to
 // each where the KV heads come in fours. A wave waits some 4 us for its length, slots
 // and first rows, which short shares do not hide; long ones leave CUs idle at the end
-// of ragged batches. Rows of 64 dims are half as long and want half the chunks: 24
-// sequences of up to 40,000 tokens on 5 heads took 32, 26 and 34 us with 1,536, 2,048
-// and 4,096 of them; 64 of up to 32,768 on 8 heads of 128 dims 107, 77 and 95 us with
-// 2,048, 4,096 and 8,192.
+// of ragged batches. Rows of 64 dims are half as long and want half the chunks: 120
+// drafted queries of 24 sequences of up to 20,000 tokens on 2 heads took 24.7, 26.7
+// and 27.6 us with 2,048, 4,096 and 8,192 of them; 64 of up to 32,768 on 8 heads of
+// 128 dims 107, 77 and 95 us with 2,048, 4,096 and 8,192.
 uint64_t score_chunks(uint64_t dk) { return dk <= 64 ? 2048 : 4096; }
 // Waves of the attention that stay resident at once, each with 64 tokens or
 // more: what the staged body's LDS leaves room for on 256 CUs (its registers, at
@@ -106,10 +106,11 @@ int32_t selection_shape(const sgl_kv_attention_plan_config &c, const sgl_kv_page
                          mul_ovf(h.record_bytes, 4ull * (SGLKV_ATTN_OPAD(c.value_head_dim) + 2), &h.record_bytes)))
         return attention_overflow();
     // A dispatch counts its work-items in 32 bits.
-    // (The scores' workgroups are placed eight (query, chunk)s at a time.)
+    // (The scores' workgroups are placed eight (near queries, chunk)s at a time.)
+    h.near_queries = ceil_div(c.query_count, c.request_count);
     uint64_t placed;
-    if (mul_ovf(c.query_count, h.chunks, &placed) || placed > UINT64_MAX - 7 ||
-        mul_ovf(ceil_div(placed, 8) * 8, c.kv_head_count, &placed))
+    if (mul_ovf(ceil_div(c.query_count, h.near_queries), h.chunks, &placed) || placed > UINT64_MAX - 7 ||
+        mul_ovf(ceil_div(placed, 8) * 8, h.near_queries, &placed) || mul_ovf(placed, c.kv_head_count, &placed))
         return attention_overflow();
     if (placed > UINT32_MAX / SGLKV_SELECT_THREADS)
         return too_large_dim("workgroups", placed, UINT32_MAX / SGLKV_SELECT_THREADS);
@@ -297,7 +298,9 @@ extern "C" int32_t sgl_rocm_kv_select_pages(sgl_rocm_kv_ctx *ctx, const sgl_kv_p
             // 4, 8 or 16 query heads a turn; past that several, whose maxima wait in LDS.
             const int heads = p.a.group <= 4 ? 0 : p.a.group <= 8 || dims == 2 ? 1 : 2;
             p.block_heads = p.a.kv_heads % 4 == 0 ? 4 : p.a.kv_heads % 2 == 0 ? 2 : 1;
-            const uint64_t groups = ceil_div(p.a.query_count * shape.chunks, 8) * 8 * (p.a.kv_heads / p.block_heads);
+            p.near_queries = (uint32_t)shape.near_queries;
+            const uint64_t groups = ceil_div(ceil_div(p.a.query_count, shape.near_queries) * shape.chunks, 8) * 8 *
+                                    shape.near_queries * (p.a.kv_heads / p.block_heads);
             rc = launch_kernel(ctx->page_scores_fast[dims][heads], groups, 1, 1, SGLKV_SELECT_THREADS,
                                p.a.group > (4u << heads) ? (unsigned)(8 * shape.chunk_pages * p.block_heads) : 0, s, &p,
                                "page scores launch");

@@ -494,10 +494,13 @@ __device__ __forceinline__ void sel_scores_fast_body(const sglkv_select_params &
     // A workgroup's waves take block_heads KV heads (1, 2 or 4) of the same pages, whose
     // bounds lie side by side, and the workgroups of the other heads run on the same
     // XCD: a page's slot, a line of its own in a long slot list, is then fetched once.
-    uint32_t item, block;
-    sel_place(p.a.kv_heads / p.block_heads, &item, &block);
-    const uint32_t chunk = item % chunks;
-    const uint64_t q = item / chunks;
+    // So do those of near_queries queries in a row, as many as a request has on
+    // average: drafted tokens read the same bounds (24.7 us for five queries each of
+    // 24 sequences of up to 1,250 pages on 2 heads of 64 dims; 26.2 without).
+    uint32_t item, inner;
+    sel_place(p.a.kv_heads / p.block_heads * p.near_queries, &item, &inner);
+    const uint32_t chunk = item % chunks, block = inner / p.near_queries;
+    const uint64_t q = static_cast<uint64_t>(item / chunks) * p.near_queries + inner % p.near_queries;
     if (q >= p.a.query_count) return;
     const uint32_t lane = threadIdx.x & 63, slot4 = lane >> 2, in4 = lane & 3;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
