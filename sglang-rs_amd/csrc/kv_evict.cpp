@@ -126,9 +126,17 @@ int32_t weight_shape(const sgl_kv_attention_plan_config &c, uint64_t max_sequenc
     const uint64_t tile = keeps ? SGLKV_WEIGHTS_APPLY : dk == 256 ? 2 * SGLKV_WEIGHTS_TILE : 4 * SGLKV_WEIGHTS_TILE;
     h.rows.tiles = ceil_div(h.max_length, tile);
     // A prompt's first tokens are attended by all of its queries, its last by a
-    // few: parts of 512 rows or more even the workgroups out.
-    h.segments = keeps ? 1 : per * group / 512 < 16 ? per * group / 512 : 16;
-    if (h.segments < 1) h.segments = 1;
+    // few: parts of 512 rows or more even the workgroups out. Short prompts leave CUs
+    // idle while a few workgroups go through all rows, 32 in 0.8 us: their parts may be
+    // as small as 64 rows where 384 or more are saved the joining launch's 6 us.
+    const uint64_t rows = per * group, alone = h.rows.tiles * c.kv_head_count * c.request_count;
+    h.segments = rows / 512;
+    if (rows >= 384 && alone * h.segments < 1024) {
+        const uint64_t fill = ceil_div(1024, alone);
+        h.segments = fill < rows / 64 ? fill : rows / 64;
+    }
+    if (keeps || h.segments < 1) h.segments = 1;
+    if (h.segments > 16) h.segments = 16;
     // (At most 16 times `any`'s.)
     h.rows.groups = keeps ? h.rows.tiles * c.kv_head_count * c.request_count : placed(h.rows.tiles * c.request_count * h.segments);
     if (h.rows.groups > kMaxWorkgroups / 4 || mul_ovf(pairs, 8 * h.rows.splits, &h.stats_bytes)) {
