@@ -43,7 +43,7 @@ struct SelectionShape {
 // of ragged batches. Rows of 64 dims are half as long and want half the chunks: 120
 // drafted queries of 24 sequences of up to 20,000 tokens on 2 heads took 24.7, 26.7
 // and 27.6 us with 2,048, 4,096 and 8,192 of them; 64 of up to 32,768 on 8 heads of
-// 128 dims 107, 77 and 95 us with 2,048, 4,096 and 8,192.
+// 128 dims 107 and 77 us with 2,048 and 4,096.
 uint64_t score_chunks(uint64_t dk) { return dk <= 64 ? 2048 : 4096; }
 // Waves of the attention that stay resident at once, each with 64 tokens or
 // more: what the staged body's LDS leaves room for on 256 CUs (its registers, at
