@@ -106,9 +106,12 @@ int32_t selection_shape(const sgl_kv_attention_plan_config &c, const sgl_kv_page
                          mul_ovf(h.record_bytes, 4ull * (SGLKV_ATTN_OPAD(c.value_head_dim) + 2), &h.record_bytes)))
         return attention_overflow();
     // A dispatch counts its work-items in 32 bits.
-    // (The scores' workgroups are placed eight (near queries, chunk)s at a time.)
+    // (The scores' workgroups are placed eight (near queries, chunk)s at a time: 64 or
+    // more of them, or all queries of one prompt would share one XCD.)
     h.near_queries = ceil_div(c.query_count, c.request_count);
     uint64_t placed;
+    if (mul_ovf(c.query_count, h.chunks, &placed)) return attention_overflow();
+    if (h.near_queries > placed / 64) h.near_queries = placed < 64 ? 1 : placed / 64;
     if (mul_ovf(ceil_div(c.query_count, h.near_queries), h.chunks, &placed) || placed > UINT64_MAX - 7 ||
         mul_ovf(ceil_div(placed, 8) * 8, h.near_queries, &placed) || mul_ovf(placed, c.kv_head_count, &placed))
         return attention_overflow();

@@ -137,6 +137,8 @@ def _run_select(k, batch, bounds, keep, first=0, last=0, longest=0, stream=None)
 @pytest.mark.parametrize("page,heads,qheads,dk,dv,lengths,per,keep,first,last", [
     (64, 8, 32, 128, 128, (5000,), 1, 8, 1, 1),
     (16, 2, 14, 64, 64, (700, 1, 33, 2000), 5, 9, 1, 2),
+    (16, 2, 14, 64, 64, (700,), 333, 9, 1, 2),              # a prompt's queries
+    (16, 4, 8, 128, 128, (1700, 300), 150, 12, 0, 1),
     (16, 8, 8, 128, 128, (1600, 900), 1, 33, 0, 0),
     (16, 1, 16, 256, 256, (3000, 16, 17), 3, 12, 2, 1),
     (1, 2, 4, 64, 64, (300, 0, 2), 1, 20, 4, 16),
