@@ -123,8 +123,8 @@ int32_t weight_shape(const sgl_kv_attention_plan_config &c, uint64_t max_sequenc
     // Many rows: four workgroups a CU. A split reads all queries again and starts for 5
     // us: four prompts of up to 2,048 tokens, 8 KV heads of 4, dims 128, took 80, 86 and
     // 107 us with 1,024, 2,048 and 4,096; one of 2,048 tokens 40 and 50 with the first two.
-    const uint64_t mean = ceil_div(c.sequence_slot_count, c.request_count),
-                   live = ceil_div(h.rows.base * (mean < h.max_length ? mean : h.max_length), h.max_length);
+    const uint64_t mean = ceil_div(c.sequence_slot_count, c.request_count), base = h.row_tiles * h.head_groups * c.kv_head_count,
+                   live = ceil_div(base * (mean < h.max_length ? mean : h.max_length), h.max_length);
     split_tokens(h.max_length, live, h.body == 0 ? 1024 : 4096, h.body == 0 ? 256 : 64, &h.rows);
     const uint64_t tile = keeps ? SGLKV_WEIGHTS_APPLY : dk == 256 ? 2 * SGLKV_WEIGHTS_TILE : 4 * SGLKV_WEIGHTS_TILE;
     h.rows.tiles = ceil_div(h.max_length, tile);

@@ -59,7 +59,7 @@ __device__ __forceinline__ double sel_sum(double x) {
 __device__ __forceinline__ void sel_place(uint32_t inner_count, uint32_t *item, uint32_t *inner) {
     const uint32_t b = blockIdx.x, k = b / 8, eight = k / inner_count;
     *inner = k - eight * inner_count;
-    *item = 8 * eight + ((b + 5 * eight + eight / 8) & 7);
+    *item = 8 * eight + ((b + blockIdx.y + 5 * eight + eight / 8) & 7);
 }
 
 // ---- Page key bounds ------------------------------------------------------
