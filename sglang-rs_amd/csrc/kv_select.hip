@@ -1036,16 +1036,18 @@ extern "C" __global__ __launch_bounds__(64) void sglkv_selected_attention_combin
 #pragma unroll
             for (uint32_t e = 0; e < 4; ++e) o[e] *= back;
             m = top;
-            for (uint32_t s = set; s < here; s += 8 * sets) {
+            // (All lanes make every round: a weight's lane may belong to a set whose own splits
+            // are done. 8 sets divides 64, so `at` is a lane, and those past `here` hold 0.)
+            for (uint32_t base = 0; base < here; base += 8 * sets) {
                 float4 x[8];
 #pragma unroll
                 for (uint32_t i = 0; i < 8; ++i) {
-                    const uint32_t at = s + i * sets < here ? s + i * sets : s;
-                    x[i] = *reinterpret_cast<const float4 *>(rows + static_cast<uint64_t>(s0 + at) * opad + d);
+                    const uint32_t at = base + set + i * sets;
+                    x[i] = *reinterpret_cast<const float4 *>(rows + static_cast<uint64_t>(s0 + (at < here ? at : here - 1)) * opad + d);
                 }
 #pragma unroll
                 for (uint32_t i = 0; i < 8; ++i) {
-                    const float ws = s + i * sets < here ? __shfl(w, s + i * sets) : 0.0f;
+                    const float ws = __shfl(w, base + set + i * sets);
                     if (ws != 0.0f) {
                         o[0] = fmaf(ws, x[i].x, o[0]);
                         o[1] = fmaf(ws, x[i].y, o[1]);

@@ -302,6 +302,35 @@ def test_attend(k, page, heads, qheads, dk, dv, hnd, shift, lengths, per, keep):
     k.check_errors()
 
 
+@pytest.mark.parametrize("heads,qheads,dk,dv,pages", [
+    *[(2, 8, 64, 64, n) for n in (17, 21, 34, 51, 63, 81, 98)],
+    *[(2, 8, 128, 128, n) for n in (33, 47, 63, 97, 127, 131)],
+    (2, 8, 40, 40, 29), (2, 8, 40, 40, 50),                 # the generic body, four sets of lanes in the merge
+    (2, 8, 97, 97, 35), (2, 8, 97, 97, 63),                 # and two
+    (1, 4, 64, 20, 17), (1, 4, 64, 24, 97), (2, 8, 256, 256, 35), (1, 16, 576, 512, 33)])
+def test_attend_in_any_number_of_splits(k, heads, qheads, dk, dv, pages):
+    """A page to a split and none of them empty: every split's record counts, whichever of the merge's rounds and
+    sets of lanes it falls to; and lists of all pages give paged attention's output."""
+    rng = np.random.default_rng(dk + pages)
+    pool = Pool(rng, page=64, heads=heads, dk=dk, dv=dv, pages=pages + 1)
+    batch = Batch(rng, pool, (64 * pages - 9,), qheads)
+    lists = np.ascontiguousarray(np.broadcast_to(np.arange(pages, dtype=np.uint32), (1, heads, pages)))
+    # Lists of every page need no scores: the workspace is the records, an output row in fp32 (its dims in 32s) and
+    # two floats for each (query head, split).
+    plan = kv.PageSelectionPlan.new(batch.plan(), max_pages=pages)
+    assert plan.workspace_required_bytes == qheads * pages * 4 * (-(-dv // 32) * 32 + 2)
+    _say(f"attend {dk}/{dv} in {pages} splits")
+    want, absolute = ref.attend(batch, lists)
+    got = _run_attend(k, batch, lists)
+    _check(got, want, absolute, f"{dk}/{dv} in {pages} splits")
+    out = _filled(qheads * dv * 2)
+    k.paged_attention(batch.plan(), **batch.device, pool=pool.buffer, output=out)
+    paged = f64(out.download().view(np.uint16).reshape(1, qheads, dv))
+    # (Both within the bound of the 64-bit form: twice it.)
+    _check(got, paged, 2 * absolute + 16 * np.abs(paged))
+    k.check_errors()
+
+
 def test_attend_lists_of_any_kind(k):
     """Lists from elsewhere: empty ones, one page, no newest page, short ones in long buffers."""
     rng = np.random.default_rng(11)
