@@ -287,7 +287,8 @@ struct sel_pick_state {
 // passes over the keys each waited for their own (32 requests of up to 10,000 floats
 // on 8 heads: 22 us of 32). Each round counts the keys of [lo, hi] in 1,024 equal steps and
 // goes on in the step where the count from above reaches `keep`, until a step is
-// taken whole: two rounds on most scores. Forced entries and NaN, the two
+// taken whole or holds one key alone (lo == hi, of which the lowest indices are
+// taken): two rounds on most scores. Forced entries and NaN, the two
 // largest keys, are counted apart: they would stretch the steps over the whole
 // type. Counting uses LDS atomics, whose order does not show.
 template <typename Key, uint32_t WAVES, uint32_t EACH, class Load>
@@ -403,7 +404,7 @@ __device__ __forceinline__ void sel_pick(uint64_t n, uint64_t keep, Load load, u
                 s.need = need - before;
                 s.lo = from;
                 s.hi = hi - from < width ? hi : from + width;
-                s.done = here == need - before || shift == 0;
+                s.done = here == need - before || shift == 0 || s.lo == s.hi;
             }
         }
         __syncthreads();

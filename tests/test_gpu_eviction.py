@@ -339,6 +339,21 @@ def test_kept_ties_signs_nan_and_infinities(k):
     k.check_errors()
 
 
+@pytest.mark.parametrize("values", [(0, 1), (0, 1, 2, 3), (0, 4), (1, 3), (-4, 0), (-2, -1, 2, 8), (np.inf, 0)])
+def test_kept_ties_of_round_values(k, values):
+    """Sums a power of two apart, whose largest alone are more than the list takes: a counting step that holds
+    just the largest key. The longest request has more positions than a workgroup keeps in registers."""
+    rng = np.random.default_rng(9)
+    lengths = (40000, 900, 3000)
+    offsets = _offsets(lengths)
+    weights = rng.choice(np.asarray(values, np.float32), (2, int(offsets[-1])))
+    _say(f"kept among sums of {values}")
+    for keep in (1, 40, 200):
+        got = _run_kept(k, weights, lengths, offsets, keep)
+        assert np.array_equal(got, _kept(weights, lengths, offsets, keep, 0, 0))
+    k.check_errors()
+
+
 def test_kept_reports_bad_requests(k):
     rng = np.random.default_rng(8)
     lengths = (100, 50, 70)

@@ -189,6 +189,25 @@ def test_select_ties_go_to_the_lower_page(k):
     k.check_errors()
 
 
+@pytest.mark.parametrize("values", [(0, 1), (0, 1, 2, 3), (0, 4), (1, 3), (-4, 0), (-2, -1, 2, 8)])
+@pytest.mark.parametrize("dk,lengths", [(64, (3200, 500)), (40, (3200, 500)), (64, (40000, 3200))])
+def test_select_ties_of_round_scores(k, values, dk, lengths):
+    """Scores a power of two apart, whose largest alone are more than the list takes: a counting step that holds
+    just the largest key. The last lengths have more pages than a workgroup keeps in registers."""
+    rng = np.random.default_rng(dk)
+    pool = Pool(rng, page=8, heads=2, dk=dk, pages=sum(-(-n // 8) for n in lengths) + 2, layers=1, layer=0)
+    batch = Batch(rng, pool, lengths, 4)
+    batch.queries[:] = 0
+    batch.queries[:, :, 0] = 0x3F80  # 1.0: a page's score is its bound
+    batch.upload()
+    bounds = np.zeros((pool.pages, 2, 2, dk), np.uint16)
+    bounds[:, :, :, 0] = bf16(rng.choice(np.asarray(values, np.float32), (pool.pages, 2, 1)))
+    _say(f"select among scores of {values}, dims {dk}, {lengths} tokens")
+    for keep in (1, 7, 50):
+        assert np.array_equal(_run_select(k, batch, bounds, keep), ref.select(batch, bounds, keep))
+    k.check_errors()
+
+
 def test_select_infinities_and_nan(k):
     """An infinite or NaN bound makes its page's score infinite or NaN; NaN ranks above every number,
     also where only some query heads see it."""
