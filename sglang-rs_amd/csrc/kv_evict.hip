@@ -841,7 +841,6 @@ __device__ __forceinline__ void wgt_tile_accumulate_body(const sglkv_weights_par
                 const uint32_t limit = past < 16 * TT ? static_cast<uint32_t>(past) : 16 * TT;
                 if (!__ballot(limit > 0)) continue;
                 const bool whole = !__ballot(limit < 16 * TT);
-                const float inv = limit > 0 ? x.inv : 0.0f;
                 const uint8_t *from = stages[stage] + (16 * n + r) * PITCH + 16 * g;
                 sglkv_u16x8 qf[DKC];
 #pragma unroll
@@ -861,15 +860,16 @@ __device__ __forceinline__ void wgt_tile_accumulate_body(const sglkv_weights_par
 #pragma unroll
                         for (uint32_t e = 0; e < 4; ++e)
                             sum[b][e] =
-                                fmaf(__builtin_amdgcn_exp2f(fmaf(sc[b][e], a.scale_log2, -x.m)), inv, sum[b][e]);
+                                fmaf(__builtin_amdgcn_exp2f(fmaf(sc[b][e], a.scale_log2, -x.m)), x.inv, sum[b][e]);
                 } else {
 #pragma unroll
                     for (uint32_t b = 0; b < TT; ++b)
 #pragma unroll
                         for (uint32_t e = 0; e < 4; ++e) {
-                            const float y =
-                                16 * b + 4 * g + e < limit ? fmaf(sc[b][e], a.scale_log2, -x.m) : -INFINITY;
-                            sum[b][e] = fmaf(__builtin_amdgcn_exp2f(y), inv, sum[b][e]);
+                            // (Factor and exponent both: 1 / l is NaN or infinite where the scores are.)
+                            const bool in = 16 * b + 4 * g + e < limit;
+                            const float y = in ? fmaf(sc[b][e], a.scale_log2, -x.m) : -INFINITY;
+                            sum[b][e] = fmaf(__builtin_amdgcn_exp2f(y), in ? x.inv : 0.0f, sum[b][e]);
                         }
                 }
             }

@@ -237,6 +237,43 @@ def test_weights_nan_keys_reach_only_their_request(k):
     k.check_errors()
 
 
+@pytest.mark.parametrize("kind", ["query", "key", "infinity"])
+@pytest.mark.parametrize("dk,heads,qheads,per", [
+    (64, 2, 8, 40), (128, 2, 8, 40), (256, 2, 8, 40),     # many rows, a request's queries in one part
+    (64, 2, 8, 200), (128, 2, 8, 200), (256, 2, 8, 200),  # in several
+    (64, 2, 8, 5), (128, 2, 8, 2), (40, 2, 6, 30)])       # few rows; kept scores; any dims
+def test_weights_nan_ends_where_its_queries_end(k, kind, dk, heads, qheads, per):
+    """A NaN query, a NaN key and a query whose scores are all -inf make NaN of what their queries attend, and of
+    nothing behind it: neither what longer queries attend further on nor what none does."""
+    rng = np.random.default_rng(dk + per)
+    pool = Pool(rng, page=16, heads=heads, dk=dk, pages=60)
+    batch = Batch(rng, pool, (500, 300), qheads, per, spare=70)
+    batch.ends[batch.requests == 0] -= 39  # (from 461 down: inside a wave's tokens)
+    odd = int(np.flatnonzero(batch.requests == 0)[len(np.flatnonzero(batch.requests == 0)) // 2])
+    if kind == "query":
+        batch.queries[odd, 1, 3] = 0x7FC0
+    elif kind == "key":
+        pool.rows(0).put(batch.slots[int(batch.ends[odd]) - 1], 0, np.full(dk, 0x7FC0))
+    else:  # a positive key everywhere, times -inf
+        for slot in batch.slots[:500]:
+            pool.rows(0).put(slot, 0, np.where(np.arange(dk) == 3, 0x3F80, pool.rows(0).get([slot], 0)[0]))
+        batch.queries[odd, 1, 3] = 0xFF80
+    batch.upload()
+    pool.upload()
+    start = rng.random((heads, len(batch.slots))).astype(np.float32)
+    _say(f"weights with a {kind} of NaN, dims {dk}, {per} queries a request")
+    with np.errstate(invalid="ignore"):
+        want = _weights(batch, start)
+    got = _run_weights(k, batch, start, longest=500)
+    k.check_errors()
+    assert np.isnan(want[0, int(batch.ends[odd]) - 1]) and not np.isnan(want[0, 461:]).any()
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    fine = ~np.isnan(want)
+    _check_weights(got[fine], want[fine], f"{kind}, dims {dk}")
+    same = want == start
+    assert same[:, 461:500].all() and (got[same] == start[same]).all()
+
+
 def test_weights_report_bad_metadata(k):
     rng = np.random.default_rng(6)
     pool = Pool(rng, page=16, heads=2, dk=64, pages=60, layers=1, layer=0)
