@@ -1148,7 +1148,7 @@ typedef struct sgl_kv_eviction_plan {
     uint64_t kept_required_bytes;                   /* u32 [request][KV head][max_kept] */
     uint64_t destination_slots_required_bytes;
     uint64_t destination_weights_required_bytes;
-    uint64_t workspace_required_bytes;              /* select_tokens; 0: none is needed */
+    uint64_t workspace_required_bytes;              /* reserved: 0, neither call needs one */
 } sgl_kv_eviction_plan;
 
 /* Errors: ZeroDimension (request_count, kv_head_count, sequence_slot_count,
@@ -1163,8 +1163,9 @@ int32_t sgl_kv_eviction_plan_new(const sgl_kv_eviction_config *config, sgl_kv_ev
  * destination_slot_offsets u64 (request_count + 1) into destination_slots (u64)
  * and the columns of destination_weights (f32 [KV
  * head][destination_slot_count]). select_tokens reads request_lengths,
- * request_slot_offsets and weights and writes kept; compact_tokens reads all but
- * the workspace, and weights and destination_weights may both be null. */
+ * request_slot_offsets and weights and writes kept; compact_tokens reads them all,
+ * and weights and destination_weights may both be null. workspace is reserved:
+ * neither call looks at it, and it may be null. */
 typedef struct sgl_kv_eviction_buffers {
     sgl_kv_device_buffer request_lengths;          uint64_t request_lengths_offset;
     sgl_kv_device_buffer request_slot_offsets;     uint64_t request_slot_offsets_offset;

@@ -2126,8 +2126,8 @@ class EvictionPlan:
 
 class EvictionBuffers:
     """The buffers of select_tokens and compact_tokens by name, each with an
-    optional <name>_offset (sgl_kv_eviction_buffers). It keeps the given
-    objects."""
+    optional <name>_offset (sgl_kv_eviction_buffers; `workspace` is reserved, and
+    neither call looks at it). It keeps the given objects."""
 
     def __init__(self, **buffers):
         self._c = _EvictionBuffers()

@@ -391,6 +391,34 @@ def test_kept_ties_of_round_values(k, values):
     k.check_errors()
 
 
+def test_kept_and_compact_do_not_look_at_the_reserved_workspace(k):
+    """Neither a missing one nor one that is no device memory changes a result."""
+    rng = np.random.default_rng(10)
+    lengths, offsets = (300, 20), _offsets((300, 20))
+    weights = rng.random((2, 320)).astype(np.float32)
+    plan = kv.EvictionPlan.new(request_count=2, kv_head_count=2, sequence_slot_count=320, max_kept=30,
+                               destination_slot_count=50)
+    raw, held, view, at = _side(rng, page=16, heads=2, chunk=64, pages=20)
+    want = _kept(weights, lengths, offsets, 30, 0, 0)
+    host = np.zeros(64, np.uint8)
+    for more in ({}, dict(workspace=kv.device_buffer(host.ctypes.data, 64), workspace_offset=1 << 40)):
+        to_raw, to_held, to_view, to_at = _side(rng, page=16, heads=2, chunk=64, pages=4)
+        given = dict(request_lengths=np.asarray(lengths, np.uint64), request_slot_offsets=offsets, weights=weights,
+                     sequence_slots=np.arange(320, dtype=np.uint64), destination_slots=np.arange(50, dtype=np.uint64),
+                     destination_slot_offsets=np.array([0, 30, 50], np.uint64))
+        given = {n: hip.DeviceBuffer.from_array(a) for n, a in given.items()}
+        kept, moved = _filled(plan.kept_required_bytes), _filled(plan.destination_weights_required_bytes)
+        buffers = kv.EvictionBuffers(**given, kept=kept, destination_weights=moved, **more)
+        k.select_tokens(plan, buffers)
+        k.compact_tokens(plan, buffers, view, to_view)
+        hip.synchronize()
+        k.check_errors()
+        assert np.array_equal(kept.download().view(np.uint32).reshape(want.shape), want)
+        for h in (0, 1):
+            for i, t in enumerate(want[0, h]):
+                assert np.array_equal(to_held.download()[to_at(1, i, h)], raw[at(1, t, h)])
+
+
 def test_kept_reports_bad_requests(k):
     rng = np.random.default_rng(8)
     lengths = (100, 50, 70)

@@ -40,6 +40,11 @@ def test_eviction_plan_sizes():
     assert p.destination_weights_required_bytes == 2 * 120 * 4
 
 
+def test_the_eviction_plans_workspace_is_reserved():
+    for change in ({}, dict(sequence_slot_count=2 ** 31), dict(request_count=2 ** 20, max_kept=2 ** 20)):
+        assert _plan(**change).workspace_required_bytes == 0
+
+
 @pytest.mark.parametrize("change,variant,name", [
     *[({n: 0}, "ZeroDimension", n) for n in ("request_count", "kv_head_count", "sequence_slot_count", "max_kept")],
     (dict(first_tokens=30, last_tokens=11), "InvalidArgument", "first_tokens"),
