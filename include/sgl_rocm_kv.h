@@ -1023,7 +1023,8 @@ typedef struct sgl_kv_page_selection_config {
     uint64_t max_pages;           /* entries of a (query, KV head)'s list */
     uint64_t first_pages;         /* pages at the sequence's start that are always listed ... */
     uint64_t last_pages;          /* ... and at its end (together at most max_pages) */
-    uint64_t max_sequence_length; /* longest query length; 0: sequence_slot_count */
+    uint64_t max_sequence_length; /* longest query length; 0: sequence_slot_count, as if one sequence
+                                     had all slots: a larger workspace and slower scores */
 } sgl_kv_page_selection_config;
 
 typedef struct sgl_kv_page_selection_plan {
@@ -1063,7 +1064,9 @@ typedef struct sgl_kv_page_selection_buffers {
  *     sum_d max(q_id, 0) high_d + min(q_id, 0) low_d
  * (an upper bound of q_i . k over the page, scale aside), summed in 64 bits;
  * equal scores go to the lower page, a NaN score ranks above every number, and
- * the first_pages and last_pages rank above all. Ascending, followed by
+ * the first_pages and last_pages rank above all. (An infinite bound times the 0
+ * of the other sign's part is NaN: its page ranks with those, even where the
+ * infinity is on the side that the query does not look at.) Ascending, followed by
  * UINT32_MAX; a sequence of at most max_pages pages has them all. A query of
  * length 0 (padding) has none, and so has one whose metadata does not hold
  * (reported as paged attention does). */
@@ -1074,7 +1077,8 @@ int32_t sgl_rocm_kv_select_pages(sgl_rocm_kv_ctx *ctx, const sgl_kv_page_selecti
  * pages that lie before the query's length; with lists of all pages the result
  * is paged attention's. The lists may come from anywhere: they ascend, without
  * repeats, UINT32_MAX behind the last; a list that does not, or that names a
- * page past the sequence, is reported (SEQUENCE) and its output unspecified. A
+ * page past the sequence, is reported (SEQUENCE) and its output unspecified
+ * (entries behind as many as the longest sequence has pages may go unread). A
  * (query, KV head) of no pages gives zeros. Softmax statistics and sums are held
  * in 32 bits, the weights enter the products as hi + lo bf16 pairs, and the
  * output is rounded to bf16. */
@@ -1094,7 +1098,8 @@ int32_t sgl_rocm_kv_selected_attention(sgl_rocm_kv_ctx *ctx, const sgl_kv_page_s
 
 typedef struct sgl_kv_weight_plan {
     sgl_kv_attention_plan attention;
-    uint64_t max_sequence_length;      /* longest query length; 0: sequence_slot_count */
+    uint64_t max_sequence_length;      /* longest query length; 0: sequence_slot_count, as if one
+                                          sequence had all slots: larger and slower */
     uint64_t weights_required_bytes;   /* f32 [KV head][sequence_slot_count] */
     uint64_t workspace_required_bytes;
 } sgl_kv_weight_plan;

@@ -632,7 +632,7 @@ constexpr uint32_t kWgtPitch = 64 * DKC + 16;
 
 // Statistics of many rows: four waves of NR * 16 rows each share the K rows of 64
 // tokens through LDS, two stages deep, so K is read once for 64 NR rows. Four prompts
-// of up to 2,048 tokens, 8 KV heads of 4 query heads, dims 128 (33 GFLOP): 80 us, 415
+// of up to 2,048 tokens, 8 KV heads of 4 query heads, dims 128 (33 GFLOP): 77 us, 430
 // TFLOP/s; 16 of 2,048 tokens 660, four of 8,192 840. With few workgroups the wait for
 // the next stage's rows bounds it: half the rows a wave, four waves a SIMD or a fifth
 // fewer vector instructions leave it where it is.
@@ -721,7 +721,7 @@ __device__ __forceinline__ void wgt_tile_stats_body(const sglkv_weights_params &
 // Accumulation of many rows: a wave has TT tiles of 16 tokens of a (request, KV
 // head) in registers, a workgroup four waves' side by side; the request's rows
 // (or a segment's) pass through LDS, 32 at a time and two stages deep. The prompts
-// above: 103 us, 320 TFLOP/s; 16 of 2,048 tokens 520, four of 8,192 730. Bound as the
+// above: 100 us, 330 TFLOP/s; 16 of 2,048 tokens 520, four of 8,192 730. Bound as the
 // statistics are; half the tokens a wave took as long.
 template <uint32_t DKC, uint32_t TT>
 __device__ __forceinline__ void wgt_tile_accumulate_body(const sglkv_weights_params &p) {

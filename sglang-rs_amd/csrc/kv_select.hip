@@ -476,9 +476,11 @@ __device__ __forceinline__ void sel_scores_body(const sglkv_select_params &p) {
 // one or two waves fitted a SIMD, and the sums across 16 lanes took as long as the
 // products: 64 ragged sequences of up to 2,048 pages, 8 KV heads of 4 query heads,
 // dims 128, 136 us.) 4 NG query heads a turn; more take several turns over the
-// chunk, whose maxima wait in LDS. Bound by the bounds' bytes: those sequences take
-// 77 us for 293 MB, 3.8 TB/s, where a plain streaming read of them takes 45 (loads
-// that keep the rows in the caches, 83; slots found row by row, 113). Sixteen pages
+// chunk, whose maxima wait in LDS. Those sequences take 77 to 81 us for 293 MB, 3.7
+// TB/s, where a plain streaming read of them takes 45 (loads that keep the rows in the
+// caches, 83; slots found row by row, 113): bound by issue before bytes. Waves wait
+// for their turn to issue in 0.42 of their cycles and for anything else in 0.36: each
+// element is converted to 64 bits, and the products are small. Sixteen pages
 // a wave's step at 64 and 128 dims, 8 at 256 for the registers; 8 at 128 took 97 us.
 __device__ __forceinline__ double sel_ror(double x, bool by8) {
     const uint64_t b = __builtin_bit_cast(uint64_t, x);
