@@ -100,6 +100,7 @@ typedef enum sgl_kv_status {
     SGL_KV_DEVICE_PAGE_INDEX_OUT_OF_RANGE = 50, /* a page-table entry is negative, past the table or past the pool */
     SGL_KV_DEVICE_SPAN_OUT_OF_RANGE = 51,       /* a row is not covered by its span list */
     SGL_KV_DEVICE_REQUEST_OUT_OF_RANGE = 52,    /* a page request outside its source or target region */
+    SGL_KV_DEVICE_OUT_OF_PAGES = 53,            /* a fork wants more pages than are free */
 
     /* 60.. mirror MooncakeRequestBuildError (crates/sglang-srt/src/transfer.rs:2092-2112) */
     SGL_KV_REQ_ZERO_PAGE_SIZE = 60,
@@ -1210,6 +1211,229 @@ int32_t sgl_rocm_kv_select_tokens(sgl_rocm_kv_ctx *ctx, const sgl_kv_eviction_pl
 int32_t sgl_rocm_kv_compact_tokens(sgl_rocm_kv_ctx *ctx, const sgl_kv_eviction_plan *plan,
                                    const sgl_kv_eviction_buffers *buffers, const sgl_kv_pool_view *source,
                                    const sgl_kv_pool_view *destination, void *stream);
+
+/* ---- Decoding along several continuations: drafted trees and beams ----
+ * No counterpart in the reference, whose requests have one continuation each.
+ *
+ * A verification step scores a tree of drafted tokens at once: the caller writes
+ * every draft's K and V rows into the slots behind its request's tokens,
+ * tree_attention attends each draft to the request's tokens and its own
+ * ancestors, and once a path is accepted keep_drafts moves its rows together,
+ * so that the sequence goes on at its new length with the slots it has.
+ *
+ * A beam step takes the best continuations of all beams (select_beams), whose
+ * parents fork_sequences turns into the next step's page tables: beams of one
+ * parent share its full pages, the last page is copied for all but the first of
+ * them, and pages that no beam holds any more are freed.
+ * sgl_rocm_kv_resolve_spans makes slots of the tables.
+ *
+ * All are asynchronous: nothing waits, nothing is allocated, and errors found on
+ * the device surface at sgl_rocm_kv_check_errors. They can be captured into a
+ * graph. A workspace is scratch for one call: calls that may run at the same time
+ * (on two streams, in two graphs) need one each. */
+
+#define SGL_KV_TREE_MASK_WORDS_MAX 16ull
+typedef struct sgl_kv_tree_attention_config {
+    uint64_t mask_words;          /* 64-bit words of a query's mask, at most SGL_KV_TREE_MASK_WORDS_MAX */
+    uint64_t max_sequence_length; /* most tokens that a query reaches to, drafts among them; 0: sequence_slot_count,
+                                     as if one sequence had all slots: a larger workspace */
+} sgl_kv_tree_attention_config;
+
+typedef struct sgl_kv_tree_attention_plan {
+    sgl_kv_attention_plan attention;
+    sgl_kv_tree_attention_config config;
+    uint64_t masks_required_bytes;     /* u64 [query][mask_words] */
+    uint64_t workspace_required_bytes; /* 0: none is needed */
+} sgl_kv_tree_attention_plan;
+
+/* Errors: attention_plan_new's; ZeroDimension ("mask_words"); DimensionTooLarge:
+ * "mask_words", "max_sequence_length" past 2^31, "query_key_head_dim" past 1,024,
+ * "workgroups" past one dispatch. The plan's flags are ignored: weights enter the
+ * products as hi + lo bf16 pairs. */
+int32_t sgl_kv_tree_attention_plan_new(const sgl_kv_attention_plan *attention,
+                                       const sgl_kv_tree_attention_config *config,
+                                       sgl_kv_tree_attention_plan *out);
+
+/* `attention` as for sgl_rocm_kv_paged_attention, where query_sequence_lengths[q]
+ * counts the tokens that q attends whole (the request's tokens before its
+ * drafts); masks: bit j of q's mask (bit j % 64 of word j / 64) is the token j
+ * places behind these. The workspace's address is a multiple of 16. */
+typedef struct sgl_kv_tree_attention_buffers {
+    sgl_kv_attention_buffers attention;
+    sgl_kv_device_buffer masks;     uint64_t masks_offset;
+    sgl_kv_device_buffer workspace; uint64_t workspace_offset;
+} sgl_kv_tree_attention_buffers;
+
+/* Softmax attention of every query head over the first query_sequence_lengths[q]
+ * tokens of q's request and those behind them whose bit is set in its mask. A
+ * query that attends nothing (length 0, no bit set; padding) gives zeros, and may
+ * have any request index that keeps the order. The queries come request by
+ * request: query_request_indices never fall (otherwise REQUEST is reported and
+ * the outputs are unspecified). A query whose index is no request's (REQUEST), or
+ * which reaches past its request's slots or past max_sequence_length (SEQUENCE),
+ * gives zeros; a token whose slot is outside the pool is reported (SLOT) and left
+ * out. Keys and values of tokens that a query does not attend never reach its
+ * output, whatever they hold. Softmax statistics and sums are held in 32 bits;
+ * the output is rounded to bf16. */
+int32_t sgl_rocm_kv_tree_attention(sgl_rocm_kv_ctx *ctx, const sgl_kv_tree_attention_plan *plan,
+                                   const sgl_kv_tree_attention_buffers *buffers, void *stream);
+
+typedef struct sgl_kv_draft_config {
+    uint64_t request_count;
+    uint64_t sequence_slot_count;
+    uint64_t max_kept;            /* entries of a request's list */
+} sgl_kv_draft_config;
+
+typedef struct sgl_kv_draft_plan {
+    sgl_kv_draft_config config;
+    uint64_t request_lengths_required_bytes;
+    uint64_t request_slot_offsets_required_bytes;
+    uint64_t sequence_slots_required_bytes;
+    uint64_t kept_required_bytes;
+} sgl_kv_draft_plan;
+
+/* Errors: ZeroDimension (request_count, sequence_slot_count, max_kept);
+ * DimensionTooLarge: "max_kept" past 2^31. */
+int32_t sgl_kv_draft_plan_new(const sgl_kv_draft_config *config, sgl_kv_draft_plan *out);
+
+/* request_lengths u64: each request's tokens before its drafts;
+ * request_slot_offsets and sequence_slots as for paged attention; kept u32
+ * [request][max_kept]: the accepted drafts' places behind these tokens,
+ * ascending, UINT32_MAX behind the last. */
+typedef struct sgl_kv_draft_buffers {
+    sgl_kv_device_buffer request_lengths;      uint64_t request_lengths_offset;
+    sgl_kv_device_buffer request_slot_offsets; uint64_t request_slot_offsets_offset;
+    sgl_kv_device_buffer sequence_slots;       uint64_t sequence_slots_offset;
+    sgl_kv_device_buffer kept;                 uint64_t kept_offset;
+} sgl_kv_draft_buffers;
+
+/* For every request and i in turn, the row of position length + i <- the row of
+ * position length + kept[i], of every tensor and of `layer_count` layers: `pool`
+ * describes the first, and each further one's tensors lie layer_stride bytes
+ * behind the one before (as sgl_rocm_kv_transfer_layers). Elements of any type;
+ * all other rows stay as they are. A request whose list does not ascend or
+ * reaches past its slots (SEQUENCE), or which has a row that moves from or to a
+ * slot outside the pool (SLOT), is reported and left as it is. The positions that
+ * a call moves have slots of their own: no two of them, of one request or two,
+ * share one. */
+int32_t sgl_rocm_kv_keep_drafts(sgl_rocm_kv_ctx *ctx, const sgl_kv_draft_plan *plan,
+                                const sgl_kv_draft_buffers *buffers, const sgl_kv_pool_view *pool,
+                                uint32_t layer_count, uint64_t layer_stride, void *stream);
+
+#define SGL_KV_BEAM_MAX_KEPT 128ull
+typedef struct sgl_kv_beam_config {
+    uint64_t request_count;
+    uint64_t beam_count;   /* beams of each request: row r beam_count + b of the logits is beam b of request r */
+    uint64_t vocab_size;
+    uint64_t row_stride;   /* elements between rows of the logits; 0: vocab_size */
+    uint64_t max_kept;     /* continuations of each request, at most SGL_KV_BEAM_MAX_KEPT */
+    int32_t dtype;         /* of the logits: SGL_KV_DTYPE_BFLOAT16 or SGL_KV_DTYPE_FLOAT32 */
+    uint32_t reserved;
+} sgl_kv_beam_config;
+
+typedef struct sgl_kv_beam_plan {
+    sgl_kv_beam_config config;
+    uint64_t logits_required_bytes;
+    uint64_t scores_required_bytes;       /* f32 [request][beam] */
+    uint64_t best_scores_required_bytes;  /* f32 [request][max_kept] */
+    uint64_t best_parents_required_bytes; /* u32 [request][max_kept] */
+    uint64_t best_tokens_required_bytes;  /* u32 [request][max_kept] */
+    uint64_t workspace_required_bytes;
+} sgl_kv_beam_plan;
+
+/* Errors: ZeroDimension (request_count, beam_count, vocab_size, max_kept);
+ * InvalidArgument ("dtype"; "row_stride" where it is below vocab_size);
+ * DimensionTooLarge: "max_kept", "beam_count" past 1,024, "vocab_size" past
+ * 524,288, "workgroups" past one dispatch. */
+int32_t sgl_kv_beam_plan_new(const sgl_kv_beam_config *config, sgl_kv_beam_plan *out);
+
+typedef struct sgl_kv_beam_buffers {
+    sgl_kv_device_buffer logits;       uint64_t logits_offset;
+    sgl_kv_device_buffer scores;       uint64_t scores_offset;
+    sgl_kv_device_buffer best_scores;  uint64_t best_scores_offset;
+    sgl_kv_device_buffer best_parents; uint64_t best_parents_offset;
+    sgl_kv_device_buffer best_tokens;  uint64_t best_tokens_offset;
+    sgl_kv_device_buffer workspace;    uint64_t workspace_offset;
+} sgl_kv_beam_buffers;
+
+/* The max_kept continuations (beam b, token v) of each request with the largest
+ *   scores[b] + logits[b][v] - log sum_u exp(logits[b][u]),
+ * best first: the score (rounded to f32), the sequence request * beam_count + b
+ * that goes on (a parent, as fork_sequences takes it) and the token. Continuations
+ * of one beam are ordered by their logits, those of two by this score in 64 bits
+ * (of a sum of exponentials held in 32 bits a workgroup and 64 across them); equal
+ * ones go to the lower beam, then the lower token. A continuation whose score is
+ * not finite is none: a beam whose score is -inf or NaN takes no part, nor does a
+ * token of logit -inf, nor a beam with a logit of NaN or +inf. Fewer than max_kept
+ * are followed by -inf, UINT32_MAX and UINT32_MAX. */
+int32_t sgl_rocm_kv_select_beams(sgl_rocm_kv_ctx *ctx, const sgl_kv_beam_plan *plan,
+                                 const sgl_kv_beam_buffers *buffers, void *stream);
+
+typedef struct sgl_kv_fork_config {
+    uint64_t sequence_count; /* the sequences that go on: entries of parents */
+    uint64_t parent_count;   /* the sequences that there were */
+    uint64_t table_pages;    /* entries of a sequence's page table */
+    uint64_t page_size;
+    uint64_t page_count;     /* pages of the pool */
+    uint64_t append_tokens;  /* tokens that each sequence has to have pages for behind its own */
+} sgl_kv_fork_config;
+
+typedef struct sgl_kv_fork_plan {
+    sgl_kv_fork_config config;
+    uint64_t parents_required_bytes;         /* u32 [sequence] */
+    uint64_t lengths_required_bytes;         /* u64 [parent] */
+    uint64_t page_tables_required_bytes;     /* i32 [parent][table_pages] */
+    uint64_t forked_lengths_required_bytes;  /* u64 [sequence] */
+    uint64_t forked_tables_required_bytes;   /* i32 [sequence][table_pages] */
+    uint64_t page_references_required_bytes; /* u32 [page] */
+    uint64_t free_pages_required_bytes;      /* i32 [page] */
+    uint64_t free_count_required_bytes;      /* one u64 */
+    uint64_t workspace_required_bytes;
+} sgl_kv_fork_plan;
+
+/* Errors: ZeroDimension (all but append_tokens); DimensionTooLarge: "page_count"
+ * past 2^31 - 1, "page_size" past 2^32 - 1, "append_tokens" past 2^32 - 1,
+ * "sequence_count" or "parent_count" past 2^24, "table_pages" past 2^31,
+ * "workgroups" past one dispatch. */
+int32_t sgl_kv_fork_plan_new(const sgl_kv_fork_config *config, sgl_kv_fork_plan *out);
+
+/* A sequence of n tokens has ceil(n / page_size) pages, the first entries of its
+ * table's row; entries behind them are -1 in the forked tables and not looked at
+ * in the old ones. page_references counts the rows that hold a page (a caller
+ * that holds pages itself, as a prefix cache does, adds its own). free_pages is a
+ * stack of free_count pages that nothing holds. */
+typedef struct sgl_kv_fork_buffers {
+    sgl_kv_device_buffer parents;         uint64_t parents_offset;
+    sgl_kv_device_buffer lengths;         uint64_t lengths_offset;
+    sgl_kv_device_buffer page_tables;     uint64_t page_tables_offset;
+    sgl_kv_device_buffer forked_lengths;  uint64_t forked_lengths_offset;
+    sgl_kv_device_buffer forked_tables;   uint64_t forked_tables_offset;
+    sgl_kv_device_buffer page_references; uint64_t page_references_offset;
+    sgl_kv_device_buffer free_pages;      uint64_t free_pages_offset;
+    sgl_kv_device_buffer free_count;      uint64_t free_count_offset;
+    sgl_kv_device_buffer workspace;       uint64_t workspace_offset;
+} sgl_kv_fork_buffers;
+
+/* Every old sequence ends, and sequence s goes on from sequence parents[s], whose
+ * tokens it has: forked_lengths[s] = lengths[parents[s]], or 0 and a row of -1
+ * where parents[s] is UINT32_MAX. Its full pages are its parent's. A last page
+ * that is not full is taken over by the lowest s of that parent; the others get a
+ * page of their own with its rows so far (every tensor of `layer_count` layers,
+ * `pool` and layer_stride as for keep_drafts). Pages for append_tokens more tokens
+ * follow. The k-th new page of the call (by sequence, then by place in the row) is
+ * free_pages[free_count - 1 - k]. page_references follow the tables; pages whose
+ * count falls to 0 are appended to free_pages in ascending order, behind what is
+ * left of it.
+ * The call does nothing but report where a parent is no sequence (REQUEST), a
+ * length, with append_tokens, passes table_pages pages or free_count the pool
+ * (SEQUENCE), a free page that it would take is outside the pool (PAGE) or more
+ * are wanted than there are (OUT_OF_PAGES: SGL_KV_DEVICE_OUT_OF_PAGES). A table
+ * entry outside the pool is reported (PAGE) and passed on as -1; nothing is
+ * counted for it, and nothing copied. forked_lengths and forked_tables overlap no
+ * other buffer (InvalidArgument "in place"). */
+int32_t sgl_rocm_kv_fork_sequences(sgl_rocm_kv_ctx *ctx, const sgl_kv_fork_plan *plan,
+                                   const sgl_kv_fork_buffers *buffers, const sgl_kv_pool_view *pool,
+                                   uint32_t layer_count, uint64_t layer_stride, void *stream);
 
 /* ---- Bootstrap wire format: the decode side's page table and layout ----
  * The multipart frames a decode worker sends a prefill worker's bootstrap

@@ -1,0 +1,71 @@
+// kv_call.h -- what the entry points of several files check alike: named buffers
+// of a call, and a pool of several layers.
+#ifndef SGLKV_CALL_H
+#define SGLKV_CALL_H
+
+#include "kv_attention_route.h"
+#include "kv_internal.h"
+
+namespace sglkv {
+
+inline uint64_t divide_up(uint64_t a, uint64_t b) { return a / b + (a % b != 0); }
+
+inline int32_t null_arguments(const char *name) {
+    return fail(SGL_KV_INVALID_ARGUMENT, name, 0, 0, 0, "null argument");
+}
+
+// A named buffer of a call and what it has to hold.
+struct CallBuffer {
+    const char *name;
+    const sgl_kv_device_buffer *buffer;
+    uint64_t offset, need;
+    uint64_t *address;
+    uint64_t align;
+    bool used;
+};
+
+// Devices first, then ranges, then alignments: the order of the other calls.
+template <size_t N>
+int32_t resolve_buffers(const sgl_rocm_kv_ctx *ctx, const CallBuffer (&all)[N]) {
+    int32_t rc;
+    for (const CallBuffer &x : all)
+        if (x.used && (rc = check_device(ctx, x.name, *x.buffer))) return rc;
+    for (const CallBuffer &x : all)
+        if (x.used && (rc = attention_ptr(x.name, *x.buffer, x.offset, x.need, x.address))) return rc;
+    for (const CallBuffer &x : all)
+        if (x.used && *x.address % x.align)
+            return fail(SGL_KV_INVALID_ARGUMENT, "alignment", 0, 0, 0, "%s must be aligned to %llu bytes", x.name,
+                        (unsigned long long)x.align);
+    return SGL_KV_OK;
+}
+
+// The kernel side of `layer_count` layers of a pool, of which `pool` describes
+// the first; `chunks` are a row's parts that lie apart: the heads of head-major
+// pages, else one.
+inline int32_t pool_layers(const sgl_rocm_kv_ctx *ctx, const sgl_kv_pool_view *pool, uint32_t layer_count,
+                           uint64_t layer_stride, sglkv_side *side, uint32_t *chunks) {
+    if (!pool) return null_arguments("pool");
+    if (!layer_count)
+        return fail(SGL_KV_ZERO_DIMENSION, "layer_count", 0, 0, 0, "KV copy dimension layer_count must be non-zero");
+    if (layer_count > 65535) return too_large_dim("layer_count", layer_count, 65535);
+    // The first layer and the last: those between lie between.
+    sgl_kv_pool_view last = *pool;
+    last.scale = nullptr;
+    if (pool->head_layout == SGL_KV_NHD) last.heads = 1;
+    int32_t rc = pool_heads_side(&last, side);
+    for (uint32_t t = 0; t < 2; ++t) {
+        uint64_t far;
+        if (mul_ovf(layer_count - 1, layer_stride, &far) || add_ovf(last.tensor_offset[t], far, &last.tensor_offset[t]))
+            return fail(SGL_KV_SHAPE_OVERFLOW, nullptr, 0, 0, 0, "KV copy layers overflowed");
+    }
+    if (rc || (rc = check_pool_view(&last))) return rc;
+    const sgl_kv_device_buffer whole = {pool->base, pool->byte_len};
+    if ((rc = check_device(ctx, "pool", whole))) return rc;
+    side->layer_stride = layer_stride;
+    *chunks = last.heads;
+    return SGL_KV_OK;
+}
+
+}  // namespace sglkv
+
+#endif

@@ -171,6 +171,12 @@ struct sgl_rocm_kv_ctx {
     hipFunction_t join_statistics, add_segments, apply_scores;
     hipFunction_t select_tokens;
     hipFunction_t compact_tokens[4];      // pieces of 16, 4, 2 and 1 bytes
+    hipFunction_t tree_attention[2];      // 16-byte vectors, elements
+    hipFunction_t tree_combine;
+    hipFunction_t keep_drafts[3];         // pieces of 16, 4 and 1 bytes
+    hipFunction_t fork_plan, fork_tables, fork_copy, fork_free;
+    hipFunction_t beam_rows[2];           // bf16, f32
+    hipFunction_t beam_join;
     uint32_t attention_occupancy[15];     // resident workgroups per CU of attention[i] ...
     uint32_t attention_occupancy_lds[15]; // ... at this LDS size (0 = not yet queried)
     int max_lds_per_block;                // device limit on a workgroup's LDS bytes

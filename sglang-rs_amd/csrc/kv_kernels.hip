@@ -796,3 +796,6 @@ extern "C" __global__ __launch_bounds__(SGLKV_BLOCK_THREADS) void sglkv_stream_w
 
 // Eviction from a cache by accumulated attention weight.
 #include "kv_evict.hip"
+#include "kv_tree.hip"
+#include "kv_branch.hip"
+#include "kv_beam.hip"

@@ -109,6 +109,7 @@ extern "C" const char *sgl_kv_status_name(int32_t code) {
     case SGL_KV_DEVICE_PAGE_INDEX_OUT_OF_RANGE: return "DevicePageIndexOutOfRange";
     case SGL_KV_DEVICE_SPAN_OUT_OF_RANGE: return "DeviceSpanOutOfRange";
     case SGL_KV_DEVICE_REQUEST_OUT_OF_RANGE: return "DeviceRequestOutOfRange";
+    case SGL_KV_DEVICE_OUT_OF_PAGES: return "DeviceOutOfPages";
     case SGL_KV_REQ_ZERO_PAGE_SIZE: return "ZeroPageSize";
     case SGL_KV_REQ_ZERO_REMOTE_ITEM_SIZE: return "ZeroRemoteKvItemSize";
     case SGL_KV_REQ_MISSING_REMOTE_POINTERS: return "MissingRemoteKvPointers";

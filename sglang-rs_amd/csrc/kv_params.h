@@ -59,6 +59,7 @@
 #define SGLKV_FLAG_ATTN_REQUEST 16u  /* query_request_indices entry >= request_count */
 #define SGLKV_FLAG_ATTN_SEQUENCE 32u /* request range or query length invalid */
 #define SGLKV_FLAG_ATTN_SLOT 64u     /* a sequence slot >= slot_count */
+#define SGLKV_FLAG_OUT_OF_PAGES 128u /* a fork wants more pages than are free */
 
 /* A resolved row offset that must not be touched. */
 #define SGLKV_INVALID_OFFSET 0xFFFFFFFFFFFFFFFFull
@@ -475,6 +476,100 @@ typedef struct sglkv_evict_params {
     uint32_t row_tiles;                 /* workgroups of a request */
     uint32_t block_heads;               /* heads of a copying workgroup */
 } sglkv_evict_params;
+
+/* Attention of drafted tokens: query q attends the first
+ * query_sequence_lengths[q] tokens of its request and those behind them whose
+ * bit its mask has. `a` as for paged attention. */
+typedef struct sglkv_tree_params {
+    sglkv_attn_params a;
+    const uint64_t *masks;    /* [query][mask_words] */
+    uint64_t max_length;      /* the farthest that a query of the launch reaches */
+    uint32_t mask_words;
+    uint32_t reserved;
+} sglkv_tree_params;
+
+/* Accepted drafts' rows, moved together in place. Thread t of a workgroup owns
+ * piece t, t + 256, ... of every row of a (request, layer): rows go in the order
+ * of the list, so a piece is read before anything is written to its place. */
+#define SGLKV_KEEP_THREADS 256u
+#define SGLKV_KEEP_ROWS 256u  /* list entries whose places are in LDS at a time */
+typedef struct sglkv_keep_params {
+    const uint64_t *request_lengths;
+    const uint64_t *request_slot_offsets;
+    const uint64_t *sequence_slots;
+    const uint32_t *kept;     /* [request][max_kept] */
+    uint32_t *flag;
+    uint64_t request_count;
+    uint64_t sequence_slot_count;
+    sglkv_side pool;          /* layer_stride: between layers */
+    uint32_t max_kept;
+    uint32_t tensors;
+    uint32_t heads;           /* chunks of a row: the heads of head-major pages, else 1 */
+    uint32_t layers;
+    uint32_t chunk_pieces[2]; /* access-sized pieces of tensor t's chunk */
+    uint32_t pieces;          /* of a row, all tensors and chunks */
+    uint32_t groups;          /* workgroups of a (request, layer) */
+} sglkv_keep_params;
+
+/* Beam selection. A workgroup reads SGLKV_BEAM_THREADS * SGLKV_BEAM_OWN logits of
+ * a row (a split), and leaves their maximum, the sum of their exponentials and
+ * the `kept` largest in order; one workgroup a request joins them. */
+#define SGLKV_BEAM_THREADS 256u
+#define SGLKV_BEAM_JOIN_THREADS 256u
+#define SGLKV_BEAM_OWN 32u    /* logits of a thread */
+#define SGLKV_BEAM_CHUNK (SGLKV_BEAM_THREADS * SGLKV_BEAM_OWN)
+#define SGLKV_BEAM_MAX_SPLITS 64u  /* a lane each */
+#define SGLKV_BEAM_MAX_BEAMS 1024u
+typedef struct sglkv_beam_params {
+    const void *logits;
+    const float *scores;      /* [row] */
+    float *best_scores;       /* [request][kept] */
+    uint32_t *best_parents;
+    uint32_t *best_tokens;
+    float *partial;           /* [row][split] maximum and sum */
+    uint64_t *candidates;     /* [row][split][kept]: ordered logit and inverted token, descending; 0: none */
+    uint64_t *lists;          /* [row][kept]: a row's, joined */
+    uint64_t row_stride;
+    uint32_t requests, beams;
+    uint32_t vocab;
+    uint32_t kept;
+    uint32_t splits;
+    uint32_t reserved;
+} sglkv_beam_params;
+
+/* Forks. The workspace: word 0 is the plan's verdict (1: carried out), word 1 the
+ * pages taken; then each parent's lowest child and number of children, each
+ * sequence's first new page's number, and a bit for each page that is freed. */
+#define SGLKV_FORK_THREADS 256u
+#define SGLKV_FORK_PLAN_THREADS 1024u
+#define SGLKV_FORK_HEAD_WORDS 32u
+#define SGLKV_FORK_NONE 0xFFFFFFFFu
+typedef struct sglkv_fork_params {
+    const uint32_t *parents;
+    const uint64_t *lengths;
+    const int32_t *tables;
+    uint64_t *forked_lengths;
+    int32_t *forked_tables;
+    uint32_t *references;
+    int32_t *free_pages;
+    uint64_t *free_count;
+    uint32_t *head;           /* SGLKV_FORK_HEAD_WORDS */
+    uint32_t *first;          /* [parent] */
+    uint32_t *children;       /* [parent] */
+    uint32_t *before;         /* [sequence] */
+    uint32_t *freed;          /* [ceil(page_count / 32)] */
+    uint32_t *flag;
+    sglkv_side pool;
+    uint64_t table_pages;
+    uint32_t sequences, old_sequences;
+    uint32_t page_count;
+    uint32_t append;
+    uint32_t tensors;
+    uint32_t heads;           /* chunks of a token's row: the heads of head-major pages, else 1 */
+    uint32_t layers;
+    uint32_t chunk[2];        /* bytes of tensor t's chunk */
+    uint32_t wide;            /* pages and regions are 16-byte aligned alike: 16-byte accesses */
+} sglkv_fork_params;
 
 /* Bytes of zeros the context keeps for reads that must contribute nothing
  * (>= the widest row piece a pipelined attention lane reads, 256 B). */

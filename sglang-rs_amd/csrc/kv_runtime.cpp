@@ -616,7 +616,20 @@ extern "C" int32_t sgl_rocm_kv_init(int32_t device, const char *code_object_path
                      {"sglkv_compact_tokens_v16", &ctx->compact_tokens[0]},
                      {"sglkv_compact_tokens_v4", &ctx->compact_tokens[1]},
                      {"sglkv_compact_tokens_v2", &ctx->compact_tokens[2]},
-                     {"sglkv_compact_tokens_v1", &ctx->compact_tokens[3]}};
+                     {"sglkv_compact_tokens_v1", &ctx->compact_tokens[3]},
+                     {"sglkv_tree_attention_v16", &ctx->tree_attention[0]},
+                     {"sglkv_tree_attention_v2", &ctx->tree_attention[1]},
+                     {"sglkv_tree_attention_combine", &ctx->tree_combine},
+                     {"sglkv_keep_drafts_v16", &ctx->keep_drafts[0]},
+                     {"sglkv_keep_drafts_v4", &ctx->keep_drafts[1]},
+                     {"sglkv_keep_drafts_v1", &ctx->keep_drafts[2]},
+                     {"sglkv_fork_plan", &ctx->fork_plan},
+                     {"sglkv_fork_tables", &ctx->fork_tables},
+                     {"sglkv_fork_copy", &ctx->fork_copy},
+                     {"sglkv_fork_free", &ctx->fork_free},
+                     {"sglkv_beam_rows_bf16", &ctx->beam_rows[0]},
+                     {"sglkv_beam_rows_f32", &ctx->beam_rows[1]},
+                     {"sglkv_beam_join", &ctx->beam_join}};
     for (const auto &f : selection)
         if (err == hipSuccess) err = hipModuleGetFunction(f.function, ctx->module, f.name);
     if (err == hipSuccess) err = hipDeviceGetAttribute(&ctx->cu_count, hipDeviceAttributeMultiprocessorCount, device);
@@ -1168,6 +1181,8 @@ int32_t sglkv::flag_status(uint32_t flag) {
     if (flag & SGLKV_FLAG_REQUEST)
         return fail(SGL_KV_DEVICE_REQUEST_OUT_OF_RANGE, nullptr, 0, flag, 0,
                     "KV page request lies outside its source or target region");
+    if (flag & SGLKV_FLAG_OUT_OF_PAGES)
+        return fail(SGL_KV_DEVICE_OUT_OF_PAGES, nullptr, 0, flag, 0, "a fork wants more pages than are free");
     return attention_flag_status(flag);
 }
 

@@ -75,6 +75,7 @@ FORWARD_PREFILL, FORWARD_DECODE = 0, 1
 DEVICE_PAGE_INDEX_OUT_OF_RANGE = 50
 DEVICE_SPAN_OUT_OF_RANGE = 51
 DEVICE_REQUEST_OUT_OF_RANGE = 52
+DEVICE_OUT_OF_PAGES = 53
 STORAGE_SIZE_MISMATCH = 110
 STORAGE_SLOT_MAP_CAPACITY_MISMATCH = 111
 STORAGE_PAGE_BUFFER_SIZE_MISMATCH = 112
@@ -368,6 +369,68 @@ class _EvictionBuffers(ctypes.Structure):
     _fields_ = [f for n in _EVICTION_BUFFERS for f in ((n, _DeviceBuffer), (n + "_offset", _u64))]
 
 
+class _TreeAttentionConfig(ctypes.Structure):
+    _fields_ = [(n, _u64) for n in ("mask_words", "max_sequence_length")]
+
+
+class _TreeAttentionPlan(ctypes.Structure):
+    _fields_ = [("attention", _AttentionPlan), ("config", _TreeAttentionConfig)] + [
+        (n, _u64) for n in ("masks_required_bytes", "workspace_required_bytes")]
+
+
+class _TreeAttentionBuffers(ctypes.Structure):
+    _fields_ = [("attention", _AttentionBuffers)] + [f for n in ("masks", "workspace")
+                                                     for f in ((n, _DeviceBuffer), (n + "_offset", _u64))]
+
+
+class _DraftConfig(ctypes.Structure):
+    _fields_ = [(n, _u64) for n in ("request_count", "sequence_slot_count", "max_kept")]
+
+
+_DRAFT_BUFFERS = ("request_lengths", "request_slot_offsets", "sequence_slots", "kept")
+
+
+class _DraftPlan(ctypes.Structure):
+    _fields_ = [("config", _DraftConfig)] + [(n + "_required_bytes", _u64) for n in _DRAFT_BUFFERS]
+
+
+class _DraftBuffers(ctypes.Structure):
+    _fields_ = [f for n in _DRAFT_BUFFERS for f in ((n, _DeviceBuffer), (n + "_offset", _u64))]
+
+
+class _BeamConfig(ctypes.Structure):
+    _fields_ = [(n, _u64) for n in ("request_count", "beam_count", "vocab_size", "row_stride", "max_kept")] + [
+        ("dtype", ctypes.c_int32), ("reserved", ctypes.c_uint32)]
+
+
+_BEAM_BUFFERS = ("logits", "scores", "best_scores", "best_parents", "best_tokens", "workspace")
+
+
+class _BeamPlan(ctypes.Structure):
+    _fields_ = [("config", _BeamConfig)] + [(n + "_required_bytes", _u64) for n in _BEAM_BUFFERS]
+
+
+class _BeamBuffers(ctypes.Structure):
+    _fields_ = [f for n in _BEAM_BUFFERS for f in ((n, _DeviceBuffer), (n + "_offset", _u64))]
+
+
+class _ForkConfig(ctypes.Structure):
+    _fields_ = [(n, _u64) for n in ("sequence_count", "parent_count", "table_pages", "page_size", "page_count",
+                                    "append_tokens")]
+
+
+_FORK_BUFFERS = ("parents", "lengths", "page_tables", "forked_lengths", "forked_tables", "page_references", "free_pages",
+                 "free_count", "workspace")
+
+
+class _ForkPlan(ctypes.Structure):
+    _fields_ = [("config", _ForkConfig)] + [(n + "_required_bytes", _u64) for n in _FORK_BUFFERS]
+
+
+class _ForkBuffers(ctypes.Structure):
+    _fields_ = [f for n in _FORK_BUFFERS for f in ((n, _DeviceBuffer), (n + "_offset", _u64))]
+
+
 # SGL_KV_ATTN_BODY_*, by value
 ATTENTION_BODIES = ("vector", "element", "pipe128", "pipe", "wide576", "wide128", "latent", "staged128", "staged64",
                     "latent_exact", "staged256", "staged128k", "tile128", "tile64", "tile256")
@@ -590,6 +653,22 @@ _EXPORTS = {
     "sgl_kv_page_selection_plan_new": (ctypes.c_int32, [ctypes.POINTER(_AttentionPlan),
                                                         ctypes.POINTER(_PageSelectionConfig),
                                                         ctypes.POINTER(_PageSelectionPlan)]),
+    "sgl_kv_tree_attention_plan_new": (ctypes.c_int32, [ctypes.POINTER(_AttentionPlan),
+                                                        ctypes.POINTER(_TreeAttentionConfig),
+                                                        ctypes.POINTER(_TreeAttentionPlan)]),
+    "sgl_rocm_kv_tree_attention": (ctypes.c_int32, [ctypes.c_void_p, ctypes.POINTER(_TreeAttentionPlan),
+                                                    ctypes.POINTER(_TreeAttentionBuffers), ctypes.c_void_p]),
+    "sgl_kv_draft_plan_new": (ctypes.c_int32, [ctypes.POINTER(_DraftConfig), ctypes.POINTER(_DraftPlan)]),
+    "sgl_rocm_kv_keep_drafts": (ctypes.c_int32, [ctypes.c_void_p, ctypes.POINTER(_DraftPlan),
+                                                 ctypes.POINTER(_DraftBuffers), ctypes.POINTER(PoolView),
+                                                 ctypes.c_uint32, _u64, ctypes.c_void_p]),
+    "sgl_kv_beam_plan_new": (ctypes.c_int32, [ctypes.POINTER(_BeamConfig), ctypes.POINTER(_BeamPlan)]),
+    "sgl_rocm_kv_select_beams": (ctypes.c_int32, [ctypes.c_void_p, ctypes.POINTER(_BeamPlan),
+                                                  ctypes.POINTER(_BeamBuffers), ctypes.c_void_p]),
+    "sgl_kv_fork_plan_new": (ctypes.c_int32, [ctypes.POINTER(_ForkConfig), ctypes.POINTER(_ForkPlan)]),
+    "sgl_rocm_kv_fork_sequences": (ctypes.c_int32, [ctypes.c_void_p, ctypes.POINTER(_ForkPlan),
+                                                    ctypes.POINTER(_ForkBuffers), ctypes.POINTER(PoolView),
+                                                    ctypes.c_uint32, _u64, ctypes.c_void_p]),
     "sgl_rocm_kv_page_bounds": (ctypes.c_int32, [ctypes.c_void_p, ctypes.POINTER(PoolView),
                                                  ctypes.POINTER(_DeviceBuffer), ctypes.POINTER(_DeviceBuffer), _u64,
                                                  ctypes.POINTER(_DeviceBuffer), ctypes.c_void_p]),
@@ -1439,6 +1518,39 @@ class RocmKvPairCopyKernels:
         _call(lib().sgl_rocm_kv_compact_tokens, self._h, ctypes.byref(plan._c), ctypes.byref(buffers._c),
               ctypes.byref(source), ctypes.byref(destination), _stream(stream))
 
+    def tree_attention(self, plan: "TreeAttentionPlan", buffers: "TreeAttentionBuffers", *, stream=None):
+        """Attention of drafted tokens: each query over its first
+        `query_sequence_lengths` tokens and those behind them whose bit its mask
+        has, into `output`. Asynchronous."""
+        _call(lib().sgl_rocm_kv_tree_attention, self._h, ctypes.byref(plan._c), ctypes.byref(buffers._c),
+              _stream(stream))
+
+    def keep_drafts(self, plan: "DraftPlan", buffers: "DraftBuffers", pool: PoolView, *, layer_count: int = 1,
+                    layer_stride_bytes: int = 0, stream=None):
+        """Moves the `kept` drafts' rows together behind their request's tokens,
+        in place, in `layer_count` layers of which `pool` describes the first.
+        Asynchronous."""
+        _call(lib().sgl_rocm_kv_keep_drafts, self._h, ctypes.byref(plan._c), ctypes.byref(buffers._c),
+              ctypes.byref(pool), layer_count, layer_stride_bytes, _stream(stream))
+
+    def select_beams(self, plan: "BeamPlan", buffers: "BeamBuffers", *, stream=None):
+        """The max_kept best continuations of each request over its beams and
+        the vocabulary, best first: `best_scores` (f32), `best_parents` (u32
+        sequence numbers) and `best_tokens` (u32), UINT32_MAX where there are
+        fewer. Asynchronous."""
+        _call(lib().sgl_rocm_kv_select_beams, self._h, ctypes.byref(plan._c), ctypes.byref(buffers._c),
+              _stream(stream))
+
+    def fork_sequences(self, plan: "ForkPlan", buffers: "ForkBuffers", pool: PoolView, *, layer_count: int = 1,
+                       layer_stride_bytes: int = 0, stream=None):
+        """The page tables of sequences that go on from `parents` (UINT32_MAX:
+        none): full pages shared, last pages copied (in `layer_count` layers of
+        which `pool` describes the first) for all children of a parent but the
+        lowest, pages for append_tokens more, and the pages that nothing holds
+        any more back on the free list. Asynchronous."""
+        _call(lib().sgl_rocm_kv_fork_sequences, self._h, ctypes.byref(plan._c), ctypes.byref(buffers._c),
+              ctypes.byref(pool), layer_count, layer_stride_bytes, _stream(stream))
+
     def check_errors(self, stream=None):
         _call(lib().sgl_rocm_kv_check_errors, self._h, _stream(stream))
 
@@ -2135,6 +2247,142 @@ class EvictionBuffers:
         rest = _fill_buffers(self._c, _EVICTION_BUFFERS, buffers)
         if rest:
             raise TypeError(f"unknown buffers: {', '.join(sorted(rest))}")
+
+
+def _plan_attribute(c, name):
+    for part in (c, c.config):
+        if hasattr(part, name) and name not in ("attention", "config", "reserved"):
+            return getattr(part, name)
+    raise AttributeError(name)
+
+
+def _named_buffers(struct, names, given: dict):
+    c = struct()
+    rest = _fill_buffers(c, names, given)
+    if rest:
+        raise TypeError(f"unknown buffers: {', '.join(sorted(rest))}")
+    return c
+
+
+class TreeAttentionPlan:
+    """What tree_attention needs to know: the attention plan of the drafted
+    tokens, the 64-bit words of a query's mask, and the farthest that a query
+    reaches (0: as far as the plan's slots)."""
+
+    def __init__(self, c: _TreeAttentionPlan):
+        self._c = c
+
+    @classmethod
+    def new(cls, attention: PagedAttentionPlan, *, mask_words: int, max_sequence_length: int = 0) -> "TreeAttentionPlan":
+        config, out = _TreeAttentionConfig(mask_words, max_sequence_length), _TreeAttentionPlan()
+        _call(lib().sgl_kv_tree_attention_plan_new, ctypes.byref(attention._c), ctypes.byref(config), ctypes.byref(out))
+        return cls(out)
+
+    @property
+    def attention(self) -> PagedAttentionPlan:
+        return PagedAttentionPlan(self._c.attention)
+
+    def __getattr__(self, name):
+        return _plan_attribute(self.__dict__["_c"], name)
+
+
+class TreeAttentionBuffers:
+    """The buffers of tree_attention by name, each with an optional
+    <name>_offset: those of paged_attention, `masks` and `workspace`. It keeps
+    the given objects."""
+
+    def __init__(self, **buffers):
+        self._c = _TreeAttentionBuffers()
+        self._given = buffers
+        rest = _fill_buffers(self._c.attention, _ATTENTION_BUFFERS, buffers)
+        rest = _fill_buffers(self._c, ("masks", "workspace"), rest)
+        if rest:
+            raise TypeError(f"unknown buffers: {', '.join(sorted(rest))}")
+
+
+class DraftPlan:
+    """What keep_drafts needs to know: requests, slots and entries of a
+    request's list."""
+
+    def __init__(self, c: _DraftPlan):
+        self._c = c
+
+    @classmethod
+    def new(cls, *, request_count: int, sequence_slot_count: int, max_kept: int) -> "DraftPlan":
+        config, out = _DraftConfig(request_count, sequence_slot_count, max_kept), _DraftPlan()
+        _call(lib().sgl_kv_draft_plan_new, ctypes.byref(config), ctypes.byref(out))
+        return cls(out)
+
+    def __getattr__(self, name):
+        return _plan_attribute(self.__dict__["_c"], name)
+
+
+class DraftBuffers:
+    """The buffers of keep_drafts by name, each with an optional <name>_offset
+    (sgl_kv_draft_buffers). It keeps the given objects."""
+
+    def __init__(self, **buffers):
+        self._c = _named_buffers(_DraftBuffers, _DRAFT_BUFFERS, buffers)
+        self._given = buffers
+
+
+class BeamPlan:
+    """What select_beams needs to know: requests, beams of each, the
+    vocabulary, the continuations kept, and the logits' type ("bf16" or "f32")
+    and row stride in elements (0: rows side by side)."""
+
+    def __init__(self, c: _BeamPlan):
+        self._c = c
+
+    @classmethod
+    def new(cls, *, request_count: int, beam_count: int, vocab_size: int, max_kept: int, dtype: str = "bf16",
+            row_stride: int = 0) -> "BeamPlan":
+        config = _BeamConfig(request_count, beam_count, vocab_size, row_stride, max_kept,
+                             DTYPES["float32" if dtype == "f32" else dtype], 0)
+        out = _BeamPlan()
+        _call(lib().sgl_kv_beam_plan_new, ctypes.byref(config), ctypes.byref(out))
+        return cls(out)
+
+    def __getattr__(self, name):
+        return _plan_attribute(self.__dict__["_c"], name)
+
+
+class BeamBuffers:
+    """The buffers of select_beams by name, each with an optional
+    <name>_offset (sgl_kv_beam_buffers). It keeps the given objects."""
+
+    def __init__(self, **buffers):
+        self._c = _named_buffers(_BeamBuffers, _BEAM_BUFFERS, buffers)
+        self._given = buffers
+
+
+class ForkPlan:
+    """What fork_sequences needs to know: sequences before and after, entries
+    of a page table's row, the pool's pages and their size, and the tokens that
+    each sequence has to have pages for behind its own."""
+
+    def __init__(self, c: _ForkPlan):
+        self._c = c
+
+    @classmethod
+    def new(cls, *, sequence_count: int, parent_count: int, table_pages: int, page_size: int, page_count: int,
+            append_tokens: int = 0) -> "ForkPlan":
+        config = _ForkConfig(sequence_count, parent_count, table_pages, page_size, page_count, append_tokens)
+        out = _ForkPlan()
+        _call(lib().sgl_kv_fork_plan_new, ctypes.byref(config), ctypes.byref(out))
+        return cls(out)
+
+    def __getattr__(self, name):
+        return _plan_attribute(self.__dict__["_c"], name)
+
+
+class ForkBuffers:
+    """The buffers of fork_sequences by name, each with an optional
+    <name>_offset (sgl_kv_fork_buffers). It keeps the given objects."""
+
+    def __init__(self, **buffers):
+        self._c = _named_buffers(_ForkBuffers, _FORK_BUFFERS, buffers)
+        self._given = buffers
 
 
 def _attention_buffers(buffers: dict) -> _AttentionBuffers:
