@@ -112,7 +112,9 @@ __device__ __forceinline__ uint64_t beam_order(double x) {
 // has at most 64); then the first wave joins the beams, lane l beams l, l + 64, ....
 // Both join lists that descend: their heads are compared, the largest is taken.
 __device__ __forceinline__ void beam_join_body(const sglkv_beam_params &p) {
-    __shared__ double offset[SGLKV_BEAM_MAX_BEAMS];  // score - log sum exp, NaN: the beam takes no part
+    // A token's score is offset + (logit - top); an offset of NaN: the beam takes no part.
+    __shared__ double offset[SGLKV_BEAM_MAX_BEAMS];
+    __shared__ float tops[SGLKV_BEAM_MAX_BEAMS];
     __shared__ uint32_t place[SGLKV_BEAM_MAX_BEAMS];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t request = blockIdx.x, kept = p.kept;
@@ -127,9 +129,9 @@ __device__ __forceinline__ void beam_join_body(const sglkv_beam_params &p) {
         double sum = lane < p.splits && own.y > 0.0f ? static_cast<double>(own.y) * exp(static_cast<double>(own.x) - m) : 0.0;
 #pragma unroll
         for (uint32_t d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
-        const double off = static_cast<double>(p.scores[row]) - (static_cast<double>(m) + log(sum));
         if (lane == 0) {
-            offset[b] = odd || !(off - off == 0.0) ? NAN : off;  // (infinite or NaN: no difference of 0)
+            offset[b] = odd || m == -INFINITY ? NAN : static_cast<double>(p.scores[row]) - log(sum);
+            tops[b] = m;
             place[b] = 0;
         }
         uint64_t *list = p.lists + row * kept;
@@ -149,12 +151,13 @@ __device__ __forceinline__ void beam_join_body(const sglkv_beam_params &p) {
     // The lane's best beam: its score as an ordered key (0: none) and its list's head.
     uint64_t best, head;
     uint32_t beam;
+    auto score = [&](uint32_t b, uint64_t key) { return offset[b] + (static_cast<double>(beam_logit(key)) - tops[b]); };
     auto look = [&]() {
         best = 0;
         for (uint32_t b = lane; b < p.beams; b += 64) {
             const uint64_t key = place[b] < kept ? p.lists[(rows + b) * kept + place[b]] : 0;
-            const double total = offset[b] + static_cast<double>(beam_logit(key));
-            const uint64_t o = key != 0 && total - total == 0.0 ? beam_order(total) : 0;
+            const double total = score(b, key);
+            const uint64_t o = key != 0 && total - total == 0.0 ? beam_order(total) : 0;  // (infinite or NaN: no difference of 0)
             if (o > best) {
                 best = o;
                 beam = b;
@@ -180,7 +183,7 @@ __device__ __forceinline__ void beam_join_body(const sglkv_beam_params &p) {
                 p.best_parents[out] = p.best_tokens[out] = 0xFFFFFFFFu;
             }
         } else if (best == top && beam == lowest) {
-            p.best_scores[out] = static_cast<float>(offset[beam] + static_cast<double>(beam_logit(head)));
+            p.best_scores[out] = static_cast<float>(score(beam, head));
             p.best_parents[out] = static_cast<uint32_t>(rows) + beam;
             p.best_tokens[out] = beam_token(head);
             ++place[beam];
