@@ -1271,10 +1271,10 @@ typedef struct sgl_kv_tree_attention_buffers {
  * request: query_request_indices never fall (otherwise REQUEST is reported and
  * the outputs are unspecified). A query whose index is no request's (REQUEST), or
  * which reaches past its request's slots or past max_sequence_length (SEQUENCE),
- * gives zeros; a token whose slot is outside the pool is reported (SLOT) and left
- * out. Keys and values of tokens that a query does not attend never reach its
- * output, whatever they hold. Softmax statistics and sums are held in 32 bits;
- * the output is rounded to bf16. */
+ * gives zeros; a token whose slot is outside the pool is reported (SLOT), and the
+ * outputs of the queries that attend it are unspecified. Keys and values of tokens
+ * that a query does not attend never reach its output, whatever they hold. Softmax
+ * statistics and sums are held in 32 bits; the output is rounded to bf16. */
 int32_t sgl_rocm_kv_tree_attention(sgl_rocm_kv_ctx *ctx, const sgl_kv_tree_attention_plan *plan,
                                    const sgl_kv_tree_attention_buffers *buffers, void *stream);
 

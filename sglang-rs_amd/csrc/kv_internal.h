@@ -172,6 +172,7 @@ struct sgl_rocm_kv_ctx {
     hipFunction_t select_tokens;
     hipFunction_t compact_tokens[4];      // pieces of 16, 4, 2 and 1 bytes
     hipFunction_t tree_attention[2];      // 16-byte vectors, elements
+    hipFunction_t tree_tile[3][3];        // dims 64, 128, 256; 1, 2, 4 row waves (2 at dims 256)
     hipFunction_t tree_combine;
     hipFunction_t keep_drafts[3];         // pieces of 16, 4 and 1 bytes
     hipFunction_t fork_plan, fork_tables, fork_copy, fork_free;

@@ -485,8 +485,20 @@ typedef struct sglkv_tree_params {
     const uint64_t *masks;    /* [query][mask_words] */
     uint64_t max_length;      /* the farthest that a query of the launch reaches */
     uint32_t mask_words;
+    uint32_t tile_queries;    /* tiles: queries of one */
+    uint32_t tile_slots;      /* tiles: workgroups of a (split, request, KV head) */
     uint32_t reserved;
 } sglkv_tree_params;
+#define SGLKV_TREE_MAX_WORDS 16u
+/* Tiles: head dims d, `rows` row waves (32 rows each) of the workgroup's four.
+ * Tokens of a block; LDS: two stages of K and V rows for each token group, the
+ * raw slots of two blocks a wave (2 KiB), the drafts that the tile attends, a
+ * word for each wave, and each wave's rows (4 KiB). */
+#define SGLKV_TREE_SHARE(d) ((d) > 128u ? 2u : 1u)
+#define SGLKV_TREE_BLOCK(d, rows) ((rows) == 4u ? 64u : 32u)
+#define SGLKV_TREE_LDS_BYTES(d, rows)                                                              \
+    (2u * (4u / ((rows) * SGLKV_TREE_SHARE(d))) * 4u * (d) * SGLKV_TREE_BLOCK(d, rows) + 2048u +   \
+     8u * (SGLKV_TREE_MAX_WORDS + 2u) + 64u + 4096u)
 
 /* Accepted drafts' rows, moved together in place. Thread t of a workgroup owns
  * piece t, t + 256, ... of every row of a (request, layer): rows go in the order

@@ -619,6 +619,15 @@ extern "C" int32_t sgl_rocm_kv_init(int32_t device, const char *code_object_path
                      {"sglkv_compact_tokens_v1", &ctx->compact_tokens[3]},
                      {"sglkv_tree_attention_v16", &ctx->tree_attention[0]},
                      {"sglkv_tree_attention_v2", &ctx->tree_attention[1]},
+                     {"sglkv_tree_tile64_1", &ctx->tree_tile[0][0]},
+                     {"sglkv_tree_tile64_2", &ctx->tree_tile[0][1]},
+                     {"sglkv_tree_tile64_4", &ctx->tree_tile[0][2]},
+                     {"sglkv_tree_tile128_1", &ctx->tree_tile[1][0]},
+                     {"sglkv_tree_tile128_2", &ctx->tree_tile[1][1]},
+                     {"sglkv_tree_tile128_4", &ctx->tree_tile[1][2]},
+                     {"sglkv_tree_tile256_1", &ctx->tree_tile[2][0]},
+                     {"sglkv_tree_tile256_2", &ctx->tree_tile[2][1]},
+                     {"sglkv_tree_tile256_2", &ctx->tree_tile[2][2]},
                      {"sglkv_tree_attention_combine", &ctx->tree_combine},
                      {"sglkv_keep_drafts_v16", &ctx->keep_drafts[0]},
                      {"sglkv_keep_drafts_v4", &ctx->keep_drafts[1]},

@@ -13,11 +13,80 @@ namespace {
 
 constexpr uint64_t kMaxTokens = 1ull << 31;
 
-// The launch of the generic body: a wave to each (query, KV head, 16 query heads,
-// block of value dims) and split.
-struct TreeShape {
-    uint64_t max_length, base, chunk, splits, record_bytes, combine_grid;
+// A body's launch: `base` workgroups to a split for the generic one (a wave to
+// each (query, KV head, 16 query heads, block of value dims)), a number of all for
+// the tiles.
+struct TreeWay {
+    uint64_t base, chunk, splits, record_bytes, combine_grid;
 };
+
+struct TreeShape {
+    uint64_t max_length;
+    TreeWay any;
+    // Tiles: head dims 64, 128 or 256 on rows that the buffers' alignment, which is the call's to see, lets 16-byte
+    // accesses read.
+    bool tiles;
+    uint32_t row_waves, tile_queries, tile_slots;
+    TreeWay tile;
+};
+
+// Splits of `chunk` tokens, their records and their merge.
+int32_t split_records(const sgl_kv_attention_plan_config &c, uint64_t max_length, TreeWay *w) {
+    uint64_t heads;
+    if (mul_ovf(c.query_count, c.query_head_count, &heads)) return attention_overflow();
+    w->splits = divide_up(max_length, w->chunk);
+    w->record_bytes = w->combine_grid = 0;
+    if (w->splits > 1) {
+        if (mul_ovf(heads, w->splits, &w->record_bytes) ||
+            mul_ovf(w->record_bytes, 4ull * (SGLKV_ATTN_OPAD(c.value_head_dim) + 2), &w->record_bytes))
+            return attention_overflow();
+        const uint32_t dv = (uint32_t)c.value_head_dim;
+        w->combine_grid = divide_up(heads, SGLKV_ATTN_COMBINE_SETS(dv) / SGLKV_ATTN_COMBINE_PER(dv, (uint32_t)w->splits));
+    }
+    // A dispatch counts its work-items in 32 bits.
+    const uint64_t limit = UINT32_MAX / SGLKV_ATTN_COMBINE_THREADS;
+    if (w->combine_grid > limit) return too_large_dim("workgroups", w->combine_grid, limit);
+    return SGL_KV_OK;
+}
+
+int32_t tile_shape(const sgl_kv_attention_plan_config &c, const sgl_kv_tree_attention_config &t, TreeShape *out) {
+    TreeShape &h = *out;
+    const uint64_t group = c.query_head_count / c.kv_head_count, d = c.query_key_head_dim, page = c.layout.page_size;
+    const uint32_t most = d > 128 ? 2 : 4;
+    h.tiles = d == c.value_head_dim && (d == 64 || d == 128 || d == 256) && (page & (page - 1)) == 0 && page <= 1u << 24 &&
+              group <= 32 * most && c.slot_count < 1ull << 32 && c.layout.page_stride_bytes <= UINT32_MAX &&
+              c.layout.key_row_bytes < 1u << 24 && c.query_count < 1ull << 31;
+    if (!h.tiles) return SGL_KV_OK;
+    // Row waves for the rows that a request has on average: fewer leave more token groups.
+    const uint64_t mean = divide_up(c.query_count, c.request_count), rows = mean * group;
+    h.row_waves = rows <= 32 ? 1 : rows <= 64 || most == 2 ? 2 : 4;
+    while (group > 32 * h.row_waves) h.row_waves *= 2;
+    h.tile_queries = 32 * h.row_waves / (uint32_t)group;
+    // Workgroups for trees of up to twice the average; larger ones go on by their number.
+    const uint64_t drafts = 64 * t.mask_words < 2 * mean ? 64 * t.mask_words : 2 * mean;
+    h.tile_slots = (uint32_t)divide_up(drafts < c.query_count ? drafts : c.query_count, h.tile_queries);
+    // As many workgroups as stay resident at once, each with two blocks of each of its token groups or more. The
+    // sequences have sequence_slot_count tokens together; each ends inside a split.
+    const uint64_t groups = 4 / (h.row_waves * SGLKV_TREE_SHARE(d));
+    const uint64_t resident = 256 * (d == 64 ? (h.row_waves == 2 ? 3 : 2) : h.row_waves == 1 ? 1 : 2);
+    const uint64_t tiles = divide_up(mean, h.tile_queries), alike = c.kv_head_count * tiles;
+    const uint64_t total = c.sequence_slot_count, half = divide_up(c.request_count, 2);
+    const uint64_t live = resident / alike > c.request_count ? resident / alike - half : half;
+    const uint64_t least = 2 * groups * SGLKV_TREE_BLOCK(d, h.row_waves);
+    TreeWay &w = h.tile;
+    w.chunk = divide_up(total, live);
+    if (w.chunk > h.max_length) w.chunk = h.max_length;
+    if (w.chunk < least) w.chunk = least;
+    w.chunk = divide_up(w.chunk, least) * least;
+    int32_t rc = split_records(c, h.max_length, &w);
+    if (rc) return rc;
+    uint64_t items;
+    if (mul_ovf(c.request_count + 1, c.kv_head_count, &items) || mul_ovf(items, w.splits, &items) || items > UINT64_MAX - 7 ||
+        mul_ovf(divide_up(items, 8) * 8, h.tile_slots, &w.base))
+        return attention_overflow();
+    h.tiles = w.base <= UINT32_MAX / 256;
+    return SGL_KV_OK;
+}
 
 int32_t tree_shape(const sgl_kv_attention_plan_config &c, const sgl_kv_tree_attention_config &t, TreeShape *out) {
     TreeShape &h = *out;
@@ -33,30 +102,19 @@ int32_t tree_shape(const sgl_kv_attention_plan_config &c, const sgl_kv_tree_atte
                   {"value_head_dim", c.value_head_dim, UINT32_MAX / 4}};
     for (const auto &l : limits)
         if (l.value > l.maximum) return too_large_dim(l.name, l.value, l.maximum);
-    uint64_t heads;
-    if (mul_ovf(c.query_count, c.kv_head_count, &h.base) || mul_ovf(h.base, divide_up(group, SGLKV_ATTN_HEADS), &h.base) ||
-        mul_ovf(h.base, divide_up(c.value_head_dim, SGLKV_ATTN_DV), &h.base) ||
-        mul_ovf(c.query_count, c.query_head_count, &heads))
+    TreeWay &w = h.any;
+    if (mul_ovf(c.query_count, c.kv_head_count, &w.base) || mul_ovf(w.base, divide_up(group, SGLKV_ATTN_HEADS), &w.base) ||
+        mul_ovf(w.base, divide_up(c.value_head_dim, SGLKV_ATTN_DV), &w.base))
         return attention_overflow();
     // About 2,048 waves, each with 128 tokens or more.
-    const uint64_t wanted = h.base < 2048 ? 2048 / h.base : 1;
-    h.chunk = divide_up(h.max_length, wanted);
-    if (h.chunk < 128) h.chunk = 128;
-    h.chunk = divide_up(h.chunk, SGLKV_ATTN_TOKENS) * SGLKV_ATTN_TOKENS;
-    h.splits = divide_up(h.max_length, h.chunk);
-    h.record_bytes = h.combine_grid = 0;
-    if (h.splits > 1) {
-        if (mul_ovf(heads, h.splits, &h.record_bytes) ||
-            mul_ovf(h.record_bytes, 4ull * (SGLKV_ATTN_OPAD(c.value_head_dim) + 2), &h.record_bytes))
-            return attention_overflow();
-        const uint32_t dv = (uint32_t)c.value_head_dim;
-        h.combine_grid = divide_up(heads, SGLKV_ATTN_COMBINE_SETS(dv) / SGLKV_ATTN_COMBINE_PER(dv, (uint32_t)h.splits));
-    }
-    // A dispatch counts its work-items in 32 bits.
-    const uint64_t limit = UINT32_MAX / SGLKV_ATTN_COMBINE_THREADS;
-    if (h.base > limit) return too_large_dim("workgroups", h.base, limit);
-    if (h.combine_grid > limit) return too_large_dim("workgroups", h.combine_grid, limit);
-    return SGL_KV_OK;
+    const uint64_t wanted = w.base < 2048 ? 2048 / w.base : 1;
+    w.chunk = divide_up(h.max_length, wanted);
+    if (w.chunk < 128) w.chunk = 128;
+    w.chunk = divide_up(w.chunk, SGLKV_ATTN_TOKENS) * SGLKV_ATTN_TOKENS;
+    const uint64_t limit = UINT32_MAX / 64;  // a dispatch counts its work-items in 32 bits
+    if (w.base > limit) return too_large_dim("workgroups", w.base, limit);
+    int32_t rc = split_records(c, h.max_length, &w);
+    return rc ? rc : tile_shape(c, t, out);
 }
 
 }  // namespace
@@ -75,7 +133,8 @@ extern "C" int32_t sgl_kv_tree_attention_plan_new(const sgl_kv_attention_plan *a
     TreeShape shape;
     if ((rc = tree_shape(p.attention.config, *config, &shape))) return rc;
     if (mul_ovf(p.attention.config.query_count, 8 * config->mask_words, &p.masks_required_bytes)) return attention_overflow();
-    p.workspace_required_bytes = shape.record_bytes;
+    p.workspace_required_bytes = shape.any.record_bytes;
+    if (shape.tiles && shape.tile.record_bytes > shape.any.record_bytes) p.workspace_required_bytes = shape.tile.record_bytes;
     *out = p;
     return ok();
 }
@@ -105,7 +164,8 @@ extern "C" int32_t sgl_rocm_kv_tree_attention(sgl_rocm_kv_ctx *ctx, const sgl_kv
         {"pool", &ab.pool, ab.pool_offset, a.pool_required_bytes, &pool, 2, true},
         {"output", &ab.output, ab.output_offset, a.output_required_bytes, &output, 2, true},
         {"masks", &b->masks, b->masks_offset, fresh.masks_required_bytes, &masks, 8, true},
-        {"workspace", &b->workspace, b->workspace_offset, shape.record_bytes, &workspace, 16, shape.record_bytes > 0}};
+        {"workspace", &b->workspace, b->workspace_offset, fresh.workspace_required_bytes, &workspace, 16,
+         fresh.workspace_required_bytes > 0}};
     if ((rc = resolve_buffers(ctx, all))) return rc;
     if ((lay.key_in_page_offset | lay.value_in_page_offset | lay.page_stride_bytes) & 1)
         return fail(SGL_KV_INVALID_ARGUMENT, "alignment", 0, 0, 0, "pool rows must be aligned to their element size");
@@ -122,8 +182,6 @@ extern "C" int32_t sgl_rocm_kv_tree_attention(sgl_rocm_kv_ctx *ctx, const sgl_kv
     p.a.flag = ctx->attn_flag;
     attention_geometry(c, &p.a);
     p.a.zero_row = ctx->zero_row;
-    p.a.chunk_tokens = shape.chunk;
-    p.a.splits = (uint32_t)shape.splits;
     p.masks = reinterpret_cast<const uint64_t *>(masks);
     p.mask_words = (uint32_t)fresh.config.mask_words;
     p.max_length = shape.max_length;
@@ -131,13 +189,27 @@ extern "C" int32_t sgl_rocm_kv_tree_attention(sgl_rocm_kv_ctx *ctx, const sgl_kv
                         ((pool + lay.key_in_page_offset) | (pool + lay.value_in_page_offset) | lay.page_stride_bytes |
                          p.a.key_head_stride | p.a.key_token_stride | p.a.value_head_stride | p.a.value_token_stride) %
                                 16 == 0;
+    const bool tiles = vector && shape.tiles && queries % 16 == 0 && output % 8 == 0;
+    const TreeWay &way = tiles ? shape.tile : shape.any;
+    p.a.chunk_tokens = way.chunk;
+    p.a.splits = (uint32_t)way.splits;
     DeviceScope scope(ctx->device);
     if (scope.status() != hipSuccess) return hip_fail(scope.status(), "hipSetDevice");
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const unsigned lds = 2 * (SGLKV_ATTN_HEADS * (p.a.dk_pad + 8) + SGLKV_ATTN_DV * SGLKV_ATTN_VT_STRIDE);
-    rc = launch_kernel(ctx->tree_attention[vector ? 0 : 1], shape.base, shape.splits, 1, 64, lds, s, &p, "tree attention launch");
-    if (!rc && shape.splits > 1)
-        rc = launch_kernel(ctx->tree_combine, shape.combine_grid, 1, 1, SGLKV_ATTN_COMBINE_THREADS, 0, s, &p,
+    if (tiles) {
+        p.a.page_stride32 = (uint32_t)p.a.page_stride;
+        p.a.key_token_stride32 = p.a.value_token_stride32 = (uint32_t)p.a.key_token_stride;
+        p.tile_queries = shape.tile_queries;
+        p.tile_slots = shape.tile_slots;
+        const int dims = p.a.dk == 64 ? 0 : p.a.dk == 128 ? 1 : 2, rows = shape.row_waves == 1 ? 0 : shape.row_waves == 2 ? 1 : 2;
+        rc = launch_kernel(ctx->tree_tile[dims][rows], way.base, 1, 1, 256, SGLKV_TREE_LDS_BYTES(p.a.dk, shape.row_waves), s, &p,
+                           "tree attention launch");
+    } else {
+        const unsigned lds = 2 * (SGLKV_ATTN_HEADS * (p.a.dk_pad + 8) + SGLKV_ATTN_DV * SGLKV_ATTN_VT_STRIDE);
+        rc = launch_kernel(ctx->tree_attention[vector ? 0 : 1], way.base, way.splits, 1, 64, lds, s, &p, "tree attention launch");
+    }
+    if (!rc && way.splits > 1)
+        rc = launch_kernel(ctx->tree_combine, way.combine_grid, 1, 1, SGLKV_ATTN_COMBINE_THREADS, 0, s, &p,
                            "tree attention combine launch");
     return rc ? rc : ok();
 }

@@ -136,6 +136,608 @@ __device__ __forceinline__ void tree_body(const sglkv_tree_params &p) {
     attn_finish(a, w, g, r, st);
 }
 
+// ---- Tiles: head dims 64, 128 or 256 on 16-byte rows --------------------------
+//
+// A workgroup of four waves owns a tile: up to 32 RW (query, head) rows of one
+// request and KV head. RW (times SHARE) waves make a token group, which computes
+// 32 RW rows over blocks of B tokens; the 4 / (RW SHARE) groups of a workgroup take
+// the blocks in turn and join their outputs through LDS at the end, so that small
+// trees, which are bound by the rows' bytes, keep every wave busy.
+
+template <uint32_t D, uint32_t RW>
+struct tree_tl {
+    typedef attn_tl<D> A;                                 // the swizzles of a row's pieces
+    static constexpr uint32_t ROW = 2 * D;                // bytes of one token's head slice
+    static constexpr uint32_t PIECES = D / 8;             // 16-byte pieces per row
+    static constexpr uint32_t TPL = 1024 / ROW;           // tokens per load
+    static constexpr uint32_t SHARE = D > 128 ? 2 : 1;    // waves that share 32 rows, each with D / SHARE outputs
+    static constexpr uint32_t GW = RW * SHARE;            // waves of a token group
+    static constexpr uint32_t TW = 4 / GW;                // token groups
+    static constexpr uint32_t B = SGLKV_TREE_BLOCK(D, RW);
+    static constexpr uint32_t N = B / GW;                 // tokens of a block that a wave loads
+    static constexpr uint32_t LPW = N / TPL;              // its K loads (and V loads)
+    static constexpr uint32_t V = B * ROW;                // V rows' offset in a stage
+    static constexpr uint32_t STAGE = 2 * V;
+    static constexpr uint32_t KC = D / 16;                // q.k steps
+    static constexpr uint32_t NT = D / SHARE / 32;        // 32-dim output tiles of a wave
+    static constexpr uint32_t TB = B / 32;                // 32-token score tiles
+    static constexpr uint32_t AHEAD = 4;                  // products that the K reads run ahead
+    static constexpr uint32_t OWN = 16 * NT / TW;         // outputs of a lane after the groups are joined
+    static constexpr uint32_t RING = 2 * TW * STAGE;      // 256 bytes of raw slots for each wave and stage
+    static constexpr uint32_t UNION = RING + 2048;        // which drafts the tile attends at all
+    static constexpr uint32_t WORDS = UNION + 8 * (SGLKV_TREE_MAX_WORDS + 2);  // a word for each wave
+    static constexpr uint32_t TABLE = WORDS + 64;         // each wave's rows (tree_row)
+    static constexpr uint32_t VBUF = D > 128 && TW == 1 ? 1 : 2;  // steps whose values there are registers for
+    static_assert(TABLE + 4096 == SGLKV_TREE_LDS_BYTES(D, RW), "the host sizes the same LDS");
+    static_assert(N <= 32 && LPW * TPL == N && TW * GW == 4 && OWN * TW == 16 * NT && OWN % 4 == 0, "whole loads and shares");
+    static_assert(4 * 16 * NT * 256 <= RING, "the outputs are joined in the stages");
+};
+
+// One wave's slots of a block: the low words of tokens [0, N) and then the high
+// ones (lane l: token l % N, word l / N % 2), without registers: into the ring,
+// 256 bytes at `at`.
+__device__ __forceinline__ void tree_load_slots(uint64_t address, uint32_t at) {
+    uint32_t save;
+    asm volatile(
+        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %2, off\n\ts_mov_b32 m0, %0"
+        : "=&s"(save)
+        : "s"(at), "v"(address)
+        : "memory");
+}
+template <uint32_t COUNT>
+__device__ __forceinline__ void tree_wait() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(COUNT) : "memory");
+}
+template <uint32_t LPW>
+__device__ __forceinline__ void tree_load_rows(const uint64_t *a, uint32_t at) {
+    if constexpr (LPW == 8) {
+        attn_tile_load4(a, at);
+        attn_tile_load4(a + 4, at + 4096);
+    } else if constexpr (LPW == 4) {
+        attn_tile_load4(a, at);
+    } else {
+        static_assert(LPW == 2, "two, four or eight loads");
+        attn_tile_load2(a, at);
+    }
+}
+
+// The kernel's parameters, read again by whoever asks (as attn_tile_params).
+__device__ __forceinline__ const sglkv_tree_params &tree_params() {
+    typedef const __attribute__((address_space(4))) sglkv_tree_params kernarg;
+    kernarg *k = (kernarg *)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(k));
+    return *(const sglkv_tree_params *)k;
+}
+
+// What a pass over the tile's tokens needs: [t0, t1) of the request, all tokens
+// below `common` attended by every row, those below `whole` by some row whole.
+struct tree_pass {
+    uint64_t start;
+    uint32_t t0, t1, last;  // last: the request's last slot
+    uint32_t common, whole;
+};
+
+// A row of the tile, kept in LDS: the loop has no registers for what it needs at
+// its last blocks alone. Its mask's first two words, what it attends whole, how far
+// it reaches (0: no row, or one that attends nothing), its query and that's number
+// in the tile.
+struct tree_row {
+    uint64_t low, high;
+    uint32_t context, reach, query, number;
+};
+static_assert(sizeof(tree_row) == 32, "32 rows a wave in a KiB");
+__device__ __forceinline__ uint64_t tree_word(const tree_row &r, uint32_t i) {
+    uint64_t w = i == 0 ? r.low : i == 1 ? r.high : 0;
+    if (i >= 2) {
+        const sglkv_tree_params &p = tree_params();
+        if (i < p.mask_words) w = p.masks[static_cast<uint64_t>(r.query) * p.mask_words + i];
+    }
+    return w;
+}
+// The 64 bits of the row's mask from bit `at` on.
+__device__ __forceinline__ uint64_t tree_bits(const tree_row &r, uint32_t at) {
+    const uint32_t i = at >> 6, s = at & 63;
+    const uint64_t a = tree_word(r, i);
+    return s == 0 ? a : a >> s | tree_word(r, i + 1) << (64 - s);
+}
+
+template <uint32_t D, uint32_t RW>
+struct tree_state {
+    float m_run, l_part;               // row l % 32 (both half-waves hold the same m; l is this half's share)
+    sglkv_f32x16 o[tree_tl<D, RW>::NT];  // o[n][i]: dim 32n + 8(i/4) + 4(l/32) + i%4 of the wave's dims of the row
+};
+
+// A wave's share of a block's rows into its group's stage, from the slots in its
+// ring. A token that no row attends, or whose slot is outside the pool, reads the
+// zero row.
+template <uint32_t D, uint32_t RW>
+__device__ __forceinline__ void tree_issue(const sglkv_attn_params &p, const tree_pass &pass, uint64_t kbase, uint64_t vbase,
+                                           const uint32_t *ring, const uint64_t *seen, uint32_t tb, uint32_t gw, uint32_t lane,
+                                           uint32_t stage_at) {
+    typedef tree_tl<D, RW> T;
+    if (T::VBUF == 1) asm volatile("" : "+v"(lane));  // (what it computes from the lane is not held across the block)
+    const uint32_t c = lane / T::PIECES, pos = lane % T::PIECES;
+    const uint64_t zero = reinterpret_cast<uint64_t>(p.zero_row) + 16 * pos;
+    const uint32_t mask = (1u << p.page_shift) - 1, slots = static_cast<uint32_t>(p.slot_count);  // (host: below 2^32)
+    const bool inside = tb + T::B <= pass.t1 && tb + T::B <= pass.whole;
+    uint64_t ka[T::LPW], va[T::LPW];
+#pragma unroll
+    for (uint32_t j = 0; j < T::LPW; ++j) {
+        const uint32_t i = T::TPL * j + c, t = T::N * gw + i, tok = tb + t;
+        const uint32_t low = ring[i], high = ring[T::N + i];
+        bool ok = true;
+        if (!inside) {
+            const uint32_t place = tok - pass.whole;
+            ok = tok < pass.t1 && (tok < pass.whole || (place < 64 * SGLKV_TREE_MAX_WORDS && (seen[place >> 6] >> (place & 63)) & 1));
+        }
+        if (ok && (high != 0 || low >= slots)) {
+            atomicOr(p.flag, SGLKV_FLAG_ATTN_SLOT);
+            ok = false;
+        }
+        const uint32_t s = ok ? low : 0u;
+        // K and V share the token's offset (the host's rule, as for paged attention's tiles).
+        const uint64_t off = static_cast<uint64_t>(s >> p.page_shift) * p.page_stride32 + __umul24(s & mask, p.key_token_stride32);
+        attn_sel64x2(ok, kbase + off + 16 * (pos ^ T::A::kswz(t)), vbase + off + 16 * (pos ^ T::A::vswz(t)), zero, ka[j], va[j]);
+    }
+    const uint32_t at = stage_at + 1024 * T::LPW * gw;
+    tree_load_rows<T::LPW>(ka, at);
+    tree_load_rows<T::LPW>(va, at + T::V);
+}
+
+// One block from its stage: scores, softmax, o += p.v, as paged attention's tiles
+// compute it (attn_tile_block). masked: `bits` says which of the block's tokens
+// the lane's row attends.
+template <uint32_t D, uint32_t RW>
+__device__ __forceinline__ void tree_block(const sglkv_attn_params &p, const uint8_t *st_lds,
+                                           const sglkv_u16x8 (&qf)[tree_tl<D, RW>::KC], uint64_t bits, bool masked, uint32_t lane,
+                                           uint32_t part, tree_state<D, RW> &st) {
+    typedef tree_tl<D, RW> T;
+    const uint32_t t = lane & 31, h = lane >> 5;
+    sglkv_f32x16 s[T::TB];
+#pragma unroll
+    for (uint32_t b = 0; b < T::TB; ++b) s[b] = sglkv_f32x16{};
+    auto kread = [&](uint32_t i) {
+        return *reinterpret_cast<const sglkv_u16x8 *>(st_lds + T::ROW * (32 * (i % T::TB) + t) +
+                                                      16 * ((2 * (i / T::TB) + h) ^ T::A::kswz(t)));
+    };
+    __builtin_amdgcn_s_setprio(1);
+    sglkv_u16x8 kf[T::AHEAD];
+#pragma unroll
+    for (uint32_t i = 0; i < T::AHEAD; ++i) kf[i] = kread(i);
+#pragma unroll
+    for (uint32_t i = 0; i < T::KC * T::TB; ++i) {
+        __builtin_amdgcn_sched_barrier(0);
+        const sglkv_u16x8 a = kf[i % T::AHEAD];
+        s[i % T::TB] = attn_mfma32(a, qf[i / T::TB], s[i % T::TB]);
+        if (i + T::AHEAD < T::KC * T::TB) kf[i % T::AHEAD] = kread(i + T::AHEAD);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(0);
+    if (masked) {
+        // Bitwise selects: a bit's sign extension keeps the score or makes it -inf.
+        const uint64_t own = bits >> (4 * h);
+#pragma unroll
+        for (uint32_t b = 0; b < T::TB; ++b) {
+            const uint32_t half = static_cast<uint32_t>(b ? own >> 32 : own);
+#pragma unroll
+            for (uint32_t i = 0; i < 16; ++i) {
+                const uint32_t keep = static_cast<uint32_t>(__builtin_amdgcn_sbfe(static_cast<int32_t>(half), 8 * (i >> 2) + (i & 3), 1));
+                s[b][i] = __uint_as_float((__float_as_uint(s[b][i]) & keep) | (0xFF800000u & ~keep));
+            }
+        }
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (uint32_t b = 0; b < T::TB; ++b)
+#pragma unroll
+        for (uint32_t i = 0; i < 16; i += 2) mx = attn_max3(mx, s[b][i], s[b][i + 1]);
+    mx = fmaxf(mx, attn_xor32(mx)) * p.scale_log2;
+    if (__builtin_amdgcn_readfirstlane(__ballot(mx > st.m_run + 8.0f) != 0 ? 1u : 0u)) {
+        const float m_new = fmaxf(st.m_run, mx);
+        const float alpha = exp2f(st.m_run - m_new);
+        st.l_part *= alpha;
+        st.m_run = m_new;
+#pragma unroll
+        for (uint32_t n = 0; n < T::NT; ++n)
+#pragma unroll
+            for (uint32_t i = 0; i < 16; ++i) st.o[n][i] *= alpha;
+    }
+    // V^T operand of 32-dim tile n, 16-token step `step`: tokens 16 step +
+    // 4h + L/4 and + 8 (the same vswz), dims 32n + 16c + 4(L%4).
+    const uint32_t L = lane & 15, c = (lane >> 4) & 1, t0 = 4 * h + (L >> 2);
+    auto vread = [&](uint32_t n, uint32_t step) {
+        const uint32_t pc = (4 * (T::NT * part + n) + 2 * c + ((L & 3) >> 1)) ^ T::A::vswz(t0);
+        const uint8_t *at = st_lds + T::V + T::ROW * (16 * step + t0) + 16 * pc + 8 * (L & 1);
+        const attn_i16x4 lo = attn_lat_vtr(at), hi = attn_lat_vtr(at + 8 * T::ROW);
+        return sglkv_u16x8{(uint16_t)lo[0], (uint16_t)lo[1], (uint16_t)lo[2], (uint16_t)lo[3],
+                           (uint16_t)hi[0], (uint16_t)hi[1], (uint16_t)hi[2], (uint16_t)hi[3]};
+    };
+    float psum = 0.0f;
+    auto weights = [&](uint32_t step, sglkv_u16x8 &phi, sglkv_u16x8 &plo) {
+        attn_u32x4 hi, lo;
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            const uint32_t e = 8 * (step & 1) + 2 * i;
+            const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[step >> 1][e], p.scale_log2, -st.m_run));
+            const float b = __builtin_amdgcn_exp2f(__builtin_fmaf(s[step >> 1][e + 1], p.scale_log2, -st.m_run));
+            psum += a;
+            psum += b;
+            hi[i] = attn_pack_bf16(a, b);
+            lo[i] = attn_pack_bf16(a - __uint_as_float(hi[i] << 16), b - __uint_as_float(hi[i] & 0xFFFF0000u));
+        }
+        phi = __builtin_bit_cast(sglkv_u16x8, hi);
+        plo = __builtin_bit_cast(sglkv_u16x8, lo);
+    };
+    sglkv_u16x8 phi[2], plo[2], v[T::VBUF][T::NT];
+    if (T::VBUF == 2) {
+#pragma unroll
+        for (uint32_t n = 0; n < T::NT; ++n) v[0][n] = vread(n, 0);
+    }
+    weights(0, phi[0], plo[0]);
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (uint32_t step = 0; step < 2 * T::TB; ++step) {
+        const uint32_t x = step & 1;
+        __builtin_amdgcn_sched_barrier(0);
+        if (T::VBUF == 1 || step + 1 < 2 * T::TB) {
+#pragma unroll
+            for (uint32_t n = 0; n < T::NT; ++n) v[(x + 1) % T::VBUF][n] = vread(n, T::VBUF == 2 ? step + 1 : step);
+        }
+#pragma unroll
+        for (uint32_t n = 0; n < T::NT; ++n) st.o[n] = attn_mfma32(v[x % T::VBUF][n], phi[x], st.o[n]);
+#pragma unroll
+        for (uint32_t n = 0; n < T::NT; ++n) st.o[n] = attn_mfma32(v[x % T::VBUF][n], plo[x], st.o[n]);
+        if (step + 1 < 2 * T::TB) {
+            weights(step + 1, phi[x ^ 1], plo[x ^ 1]);
+#pragma unroll
+            for (uint32_t n = 0; n < 2 * T::NT; ++n) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                      // a product
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);                      // an LDS read
+                __builtin_amdgcn_sched_group_barrier(0x402, T::NT == 4 ? 8 : 16, 0);  // vector and exp instructions
+            }
+        }
+    }
+    __builtin_amdgcn_s_setprio(0);
+    st.l_part += psum;
+}
+
+// Tokens [t0, t1) of the tile's request for the wave's 32 rows: `reach` bounds
+// them, `least` is the fewest tokens that one of them attends whole.
+template <uint32_t D, uint32_t RW>
+__device__ __forceinline__ void tree_run(const sglkv_tree_params &p, const tree_pass &pass, uint64_t kbase, uint64_t vbase,
+                                         uint32_t w, uint32_t lane, uint8_t *lds, uint32_t lds_at, uint32_t least,
+                                         uint32_t reach,
+                                         const sglkv_u16x8 (&qf)[tree_tl<D, RW>::KC], tree_state<D, RW> &st) {
+    typedef tree_tl<D, RW> T;
+    const sglkv_attn_params &a = p.a;
+    const uint32_t tw = w / T::GW, gw = w % T::GW;
+    const uint64_t *seen = reinterpret_cast<const uint64_t *>(lds + T::UNION);
+    const uint64_t slot_base = reinterpret_cast<uint64_t>(a.sequence_slots + pass.start) + 4 * (lane / T::N % 2);
+    const uint32_t stage_at = lds_at + 2 * T::STAGE * tw, ring_at = lds_at + T::RING + 512 * w;
+    const uint8_t *stage = lds + 2 * T::STAGE * tw;
+    const uint32_t *ring = reinterpret_cast<const uint32_t *>(lds + T::RING + 512 * w);
+    const uint32_t all = (pass.t1 - pass.t0 + T::B - 1) / T::B;
+    // Blocks of each group (a group short of one loads zeros), and those that this wave's rows attend.
+    const uint32_t nb = (all + T::TW - 1) / T::TW;
+    const uint32_t first = pass.t0 + tw * T::B;
+    const uint32_t end = reach < pass.t1 ? reach : pass.t1;
+    const uint32_t mine = end <= first ? 0 : (end - first + T::B * T::TW - 1) / (T::B * T::TW);
+    auto block = [&](uint32_t k) { return first + k * T::B * T::TW; };
+    auto slots = [&](uint32_t k) {
+        const uint32_t tok = block(k) + T::N * gw + lane % T::N;
+        tree_load_slots(slot_base + 8ull * (tok < pass.last ? tok : pass.last), ring_at + 256 * (k & 1));
+    };
+    auto rows = [&](uint32_t k) {
+        tree_issue<D, RW>(a, pass, kbase, vbase, ring + 64 * (k & 1), seen, block(k), gw, lane, stage_at + T::STAGE * (k & 1));
+    };
+    st.m_run = -3.402823466e+38f;
+    st.l_part = 0.0f;
+#pragma unroll
+    for (uint32_t n = 0; n < T::NT; ++n) st.o[n] = sglkv_f32x16{};
+    // Everything that the compiler loaded has arrived: it puts no wait into the loop, where rows are in flight.
+    __builtin_amdgcn_s_waitcnt(0x0F70);
+    slots(0);
+    tree_wait<0>();
+    slots(1);
+    rows(0);
+    // Block k's rows have landed; block k + 1's are on their way.
+    auto next = [&](uint32_t k) {
+        if constexpr (T::GW == 1) {
+            // The wave's own stages: the slots of k + 1 are older than the rows of k.
+            tree_wait<2 * T::LPW>();
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // block k - 1's stage is read
+            slots(k + 2);
+            rows(k + 1);
+            tree_wait<2 * T::LPW + 1>();
+        } else {
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            slots(k + 2);
+            rows(k + 1);
+        }
+    };
+    for (uint32_t k = 0; k < mine; ++k) {
+        next(k);
+        const uint32_t tb = block(k);
+        const bool masked = tb + T::B > least;
+        uint64_t bits = 0;
+        if (masked) {
+            const tree_row &row = reinterpret_cast<const tree_row *>(lds + T::TABLE)[32 * w + (lane & 31)];
+            if (tb >= row.context) {
+                bits = tree_bits(row, tb - row.context);
+            } else {
+                const uint32_t left = row.context - tb;
+                bits = left >= 64 ? ~0ull : ((1ull << left) - 1) | row.low << left;
+            }
+        }
+        tree_block<D, RW>(a, stage + T::STAGE * (k & 1), qf, bits, masked, lane, gw % T::SHARE, st);
+    }
+    for (uint32_t k = mine; k < nb; ++k) next(k);
+    tree_wait<0>();  // (rows behind the last block, too)
+}
+
+// The first query of the launch whose request index is at least x[0], and x[1]:
+// each step, the wave's lanes look at 64 places of what is left.
+__device__ __forceinline__ void tree_find(const sglkv_attn_params &a, uint32_t lane, uint32_t request, uint32_t *first, uint32_t *end) {
+    const uint32_t count = static_cast<uint32_t>(a.query_count);  // (host: below 2^31)
+    uint32_t lo[2] = {0, 0}, hi[2] = {count, count};
+    while (lo[0] < hi[0] || lo[1] < hi[1]) {
+#pragma unroll
+        for (uint32_t x = 0; x < 2; ++x) {
+            const uint32_t step = (hi[x] - lo[x] + 63) / 64, at = lo[x] + lane * step;
+            const bool in = step && at < hi[x];
+            const uint32_t v = in ? a.query_request_indices[at] : 0xFFFFFFFFu;
+            const uint32_t c = __popcll(__ballot(in && v < request + x));
+            hi[x] = lo[x] + c * step < hi[x] ? lo[x] + c * step : hi[x];
+            if (c) lo[x] += (c - 1) * step + 1;
+        }
+    }
+    *first = lo[0];
+    *end = lo[1] > lo[0] ? lo[1] : lo[0];
+}
+
+// The lane's row number among the tile's and its head: worked out anew (the lane
+// passes through an empty asm) rather than held across the loop.
+template <uint32_t D, uint32_t RW>
+__device__ __forceinline__ uint32_t tree_place(const sglkv_attn_params &a, uint32_t w, uint32_t lane, uint32_t *head) {
+    typedef tree_tl<D, RW> T;
+    asm volatile("" : "+v"(lane));
+    const uint32_t r = 32 * (w % T::GW / T::SHARE) + (lane & 31), number = r / a.group;
+    *head = r - number * a.group;
+    return number;
+}
+
+// The rows' outputs (one split) or records, the token groups joined; rows that do
+// not reach past t0, or whose query is not number `only` (if any), write nothing.
+template <uint32_t D, uint32_t RW>
+__device__ __forceinline__ void tree_write(uint32_t w, uint32_t lane, uint8_t *lds, uint32_t kvh, uint32_t split, uint32_t t0,
+                                           uint32_t only, const tree_state<D, RW> &st) {
+    typedef tree_tl<D, RW> T;
+    const sglkv_attn_params &a = tree_params().a;
+    const uint32_t tw = w / T::GW, gw = w % T::GW, part = gw % T::SHARE;
+    float l = st.l_part + __shfl_xor(st.l_part, 32), m = st.m_run;
+    float v[T::OWN];
+    if constexpr (T::TW > 1) {
+        // The groups' statistics, then their outputs, at one maximum.
+        float2 *ml = reinterpret_cast<float2 *>(lds + T::RING);
+        float *outs = reinterpret_cast<float *>(lds);
+        __syncthreads();  // (the stages and rings are no longer read)
+        if (lane < 32) ml[32 * w + lane] = make_float2(m, l);
+        __syncthreads();
+        float top = m, sum = 0.0f;
+        float2 group[T::TW];
+#pragma unroll
+        for (uint32_t g = 0; g < T::TW; ++g) {
+            group[g] = ml[32 * (T::GW * g + gw) + (lane & 31)];
+            top = fmaxf(top, group[g].x);
+        }
+#pragma unroll
+        for (uint32_t g = 0; g < T::TW; ++g) sum += group[g].y * exp2f(group[g].x - top);
+        const float scale = exp2f(m - top);
+#pragma unroll
+        for (uint32_t n = 0; n < T::NT; ++n)
+#pragma unroll
+            for (uint32_t i = 0; i < 16; ++i) outs[64 * (16 * (T::NT * w + n) + i) + lane] = st.o[n][i] * scale;
+        __syncthreads();
+#pragma unroll
+        for (uint32_t i = 0; i < T::OWN; ++i) {
+            v[i] = 0.0f;
+#pragma unroll
+            for (uint32_t g = 0; g < T::TW; ++g) v[i] += outs[64 * (16 * T::NT * (T::GW * g + gw) + T::OWN * tw + i) + lane];
+        }
+        m = top;
+        l = sum;
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < T::OWN; ++i) v[i] = st.o[i / 16][i % 16];
+    }
+    uint32_t rh;
+    const uint32_t number = tree_place<D, RW>(a, w, lane, &rh);
+    const tree_row &row = reinterpret_cast<const tree_row *>(lds + T::TABLE)[32 * w + (lane & 31)];
+    if (row.reach <= t0 || (only != 0xFFFFFFFFu && number != only)) return;
+    const uint64_t qrow = static_cast<uint64_t>(row.query) * a.query_heads + kvh * a.group + rh;
+    // Value 4 i + e of the lane: dim 8 (i + OWN tw / 4) + 4 (lane / 32) + e of the wave's dims.
+    const uint32_t dim = D / T::SHARE * part + 2 * T::OWN * tw + 4 * (lane >> 5);
+    if (a.splits == 1) {
+        const float linv = 1.0f / l;
+        uint16_t *out = a.output + qrow * D + dim;
+#pragma unroll
+        for (uint32_t i = 0; i < T::OWN / 4; ++i) {
+            sglkv_u16x4 x;
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) x[e] = attn_to_bf16(v[4 * i + e] * linv);
+            *reinterpret_cast<sglkv_u16x4 *>(out + 8 * i) = x;  // (host: 8-byte aligned output)
+        }
+        return;
+    }
+    const uint64_t rec = qrow * a.splits + split;
+    if (lane < 32 && part == 0 && tw == 0) {
+        float *ml = attn_rec_ml(a, rec);
+        ml[0] = m;
+        ml[1] = l;
+    }
+    float *out = attn_rec_o(a, rec) + dim;
+#pragma unroll
+    for (uint32_t i = 0; i < T::OWN / 4; ++i)
+        *reinterpret_cast<sglkv_f32x4 *>(out + 8 * i) = sglkv_f32x4{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
+}
+
+template <uint32_t D, uint32_t RW>
+__device__ __forceinline__ void tree_tile_body() {
+    typedef tree_tl<D, RW> T;
+    extern __shared__ __attribute__((aligned(16))) uint8_t tree_tile_lds[];
+    const sglkv_tree_params &p = tree_params();
+    const sglkv_attn_params &a = p.a;
+    uint8_t *lds = tree_tile_lds;
+    uint32_t *words = reinterpret_cast<uint32_t *>(lds + T::WORDS);
+    const uint32_t lds_at = attn_lat_lds_at(lds);
+    const uint32_t tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // Eight (split, request, KV head)s go side by side, one to an XCD, the tiles of each one after another: they
+    // read the same rows.
+    const uint32_t eight = blockIdx.x / 8 / p.tile_slots, slot = blockIdx.x / 8 - eight * p.tile_slots;
+    const uint32_t item = 8 * eight + blockIdx.x % 8, requests = static_cast<uint32_t>(a.request_count);
+    const uint32_t kvh = item % a.kv_heads, of = item / a.kv_heads, split = of / (requests + 1), req = of - split * (requests + 1);
+    if (split >= a.splits) return;
+    const bool known = req < requests, report = (split | kvh) == 0;  // (the request behind the last: queries of no request)
+    uint32_t first, end;
+    tree_find(a, lane, req, &first, &end);
+    if (!known) end = static_cast<uint32_t>(a.query_count);
+    if (report && slot == 0 && known) {
+        // This request's share of the check that the indices never fall.
+        const uint64_t q0 = a.query_count * req / requests, q1 = a.query_count * (req + 1) / requests;
+        for (uint64_t q = q0 + tid; q < q1; q += 256)
+            if (q && a.query_request_indices[q - 1] > a.query_request_indices[q]) atomicOr(a.flag, SGLKV_FLAG_ATTN_REQUEST);
+    }
+    const uint32_t t0 = split * static_cast<uint32_t>(a.chunk_tokens);
+    for (uint32_t q0 = first + slot * p.tile_queries; q0 < end;) {
+        sglkv_u16x8 qf[T::KC];
+        uint32_t nq;
+        {
+            // The lane's row: its query, head, mask and reach.
+            const sglkv_tree_params &p = tree_params();
+            const sglkv_attn_params &a = p.a;
+            nq = end - q0 < p.tile_queries ? end - q0 : p.tile_queries;
+            const uint64_t from = known ? a.request_slot_offsets[req] : 0, to = known ? a.request_slot_offsets[req + 1] : 0;
+            uint32_t rh;
+            tree_row row;
+            row.number = tree_place<D, RW>(a, w, lane, &rh);
+            const bool has = row.number < nq;
+            row.query = q0 + (has ? row.number : 0);
+            const uint64_t qrow = static_cast<uint64_t>(row.query) * a.query_heads + kvh * a.group + rh;
+            const uint64_t *mask = p.masks + static_cast<uint64_t>(row.query) * p.mask_words;
+            row.low = mask[0];
+            row.high = p.mask_words > 1 ? mask[1] : 0;
+            const uint64_t length = a.query_sequence_lengths[row.query];
+            const uint32_t index = a.query_request_indices[row.query];
+#pragma unroll
+            for (uint32_t c = 0; c < T::KC; ++c)
+                qf[c] = *reinterpret_cast<const sglkv_u16x8 *>(a.queries + qrow * D + 16 * c + 8 * (lane >> 5));
+            uint32_t drafts = row.high ? 128 - __builtin_clzll(row.high) : row.low ? 64 - __builtin_clzll(row.low) : 0;
+            for (uint32_t i = 2; i < p.mask_words; ++i) {
+                const uint64_t m = mask[i];
+                if (m) drafts = 64 * i + 64 - __builtin_clzll(m);
+            }
+            const bool any = has && (length != 0 || drafts != 0);
+            uint32_t bad = 0;
+            if (any) {
+                if (!known || index != req)
+                    bad = SGLKV_FLAG_ATTN_REQUEST;
+                else if (from > to || to > a.sequence_slot_count || length > to - from || length + drafts > to - from ||
+                         length + drafts > p.max_length)
+                    bad = SGLKV_FLAG_ATTN_SEQUENCE;
+                if (bad && report) atomicOr(a.flag, bad);
+            }
+            const bool live = any && !bad;
+            row.context = live ? static_cast<uint32_t>(length) : 0;
+            row.reach = live ? row.context + drafts : 0;
+            reinterpret_cast<tree_row *>(lds + T::TABLE)[32 * w + (lane & 31)] = row;  // (the wave's own: no barrier)
+            if (has && !live && a.splits == 1 && w < T::GW) {
+                // Nothing attended: zeros (with several splits the merge writes them).
+                uint16_t *out = a.output + qrow * D + D / T::SHARE * (w % T::SHARE) + 4 * (lane >> 5);
+#pragma unroll
+                for (uint32_t i = 0; i < 4 * T::NT; ++i) *reinterpret_cast<sglkv_u16x4 *>(out + 8 * i) = sglkv_u16x4{0, 0, 0, 0};
+            }
+        }
+        auto wave_most = [&](uint32_t v) {
+#pragma unroll
+            for (uint32_t d = 1; d < 32; d <<= 1) {
+                const uint32_t x = __shfl_xor(v, d);
+                v = x > v ? x : v;
+            }
+            return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(v));
+        };
+        auto tile_most = [&](uint32_t v) {
+            __syncthreads();  // (the words are no longer read)
+            if (lane == 0) words[w] = v;
+            __syncthreads();
+            uint32_t x = words[0];
+#pragma unroll
+            for (uint32_t i = 1; i < 4; ++i) x = words[i] > x ? words[i] : x;
+            return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(x));
+        };
+        // One pass with every row; the tile is done unless its values are not finite. A token that one row attends
+        // and another does not has weight 0 in the other's product, and 0 times an infinite or NaN value is NaN. So
+        // when a wave whose rows attend different tokens holds an output that is not finite, the queries are done
+        // again one by one: no row then meets a token that it does not attend.
+        for (uint32_t only = 0xFFFFFFFFu;;) {
+            const sglkv_tree_params &p = tree_params();
+            const sglkv_attn_params &a = p.a;
+            const uint32_t chunk = static_cast<uint32_t>(a.chunk_tokens);
+            tree_pass pass;
+            uint32_t wave_reach, wave_least;
+            {
+                const tree_row &row = reinterpret_cast<const tree_row *>(lds + T::TABLE)[32 * w + (lane & 31)];
+                const bool on = row.reach != 0 && (only == 0xFFFFFFFFu || row.number == only);
+                const uint32_t context = row.context;
+                wave_reach = wave_most(on ? row.reach : 0);
+                wave_least = ~wave_most(on ? ~context : 0);
+                const uint32_t farthest = tile_most(wave_reach);
+                pass.t0 = t0;
+                pass.t1 = farthest <= t0 ? t0 : farthest - t0 < chunk ? farthest : t0 + chunk;
+                if (pass.t1 > t0) {
+                    pass.start = a.request_slot_offsets[req];  // (a row reaches into it: the request is one, its range holds)
+                    const uint64_t slots = a.request_slot_offsets[req + 1] - pass.start;
+                    pass.last = static_cast<uint32_t>(slots < 1ull << 31 ? slots : 1ull << 31) - 1;  // (none behind 2^31 are reached)
+                    pass.whole = tile_most(wave_most(on ? context : 0));
+                    pass.common = ~tile_most(~wave_least);
+                    // The drafts behind `whole` that some row attends.
+                    uint64_t *seen = reinterpret_cast<uint64_t *>(lds + T::UNION);
+                    if (tid < SGLKV_TREE_MAX_WORDS) seen[tid] = 0;
+                    __syncthreads();
+                    if (on && pass.whole - context < 64 * p.mask_words)
+                        for (uint32_t i = 0; i < p.mask_words; ++i) {
+                            const uint64_t m = tree_bits(row, pass.whole - context + 64 * i);
+                            if (m) atomicOr(reinterpret_cast<unsigned long long *>(seen + i), static_cast<unsigned long long>(m));
+                        }
+                    __syncthreads();
+                }
+            }
+            bool redo = false;
+            if (pass.t1 > t0) {
+                tree_state<D, RW> st;
+                const uint64_t pool = reinterpret_cast<uint64_t>(a.pool);
+                tree_run<D, RW>(tree_params(), pass, pool + a.key_offset + kvh * a.key_head_stride,
+                                pool + a.value_offset + kvh * a.value_head_stride, w, lane, lds, lds_at, wave_least, wave_reach, qf,
+                                st);
+                if (only == 0xFFFFFFFFu && pass.t1 > pass.common) {
+                    float odd = 0.0f;
+#pragma unroll
+                    for (uint32_t n = 0; n < T::NT; ++n)
+#pragma unroll
+                        for (uint32_t i = 0; i < 16; ++i) odd = __builtin_fmaf(st.o[n][i], 0.0f, odd);
+                    const tree_row &row = reinterpret_cast<const tree_row *>(lds + T::TABLE)[32 * w + (lane & 31)];
+                    redo = tile_most(__ballot(odd != 0.0f && row.reach > t0) != 0 ? 1 : 0) != 0;  // (NaN != 0)
+                }
+                if (!redo) tree_write<D, RW>(w, lane, lds, kvh, split, t0, only, st);
+            }
+            if (only == 0xFFFFFFFFu && !redo) break;
+            if (++only == nq) break;  // (from the whole tile to query 0)
+        }
+        __syncthreads();  // (the next tile's loads go where this one's outputs were joined)
+        const sglkv_tree_params &p = tree_params();
+        q0 += p.tile_slots * p.tile_queries;
+    }
+}
+
 }  // namespace
 
 extern "C" __global__ __launch_bounds__(64) void sglkv_tree_attention_v16(sglkv_tree_params p) { tree_body<true>(p); }
@@ -143,6 +745,20 @@ extern "C" __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2
     sglkv_tree_params p) {
     tree_body<false>(p);
 }
+
+#define SGLKV_TREE_TILE(D, RW, WAVES)                                                                              \
+    extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WAVES))) void                 \
+    sglkv_tree_tile##D##_##RW(sglkv_tree_params) {                                                                 \
+        tree_tile_body<D, RW>();                                                                                   \
+    }
+SGLKV_TREE_TILE(64, 1, 2)
+SGLKV_TREE_TILE(64, 2, 2)
+SGLKV_TREE_TILE(64, 4, 2)
+SGLKV_TREE_TILE(128, 1, 1)
+SGLKV_TREE_TILE(128, 2, 2)
+SGLKV_TREE_TILE(128, 4, 2)
+SGLKV_TREE_TILE(256, 1, 1)
+SGLKV_TREE_TILE(256, 2, 2)
 
 // Merges the split records of each (query, head), as
 // sglkv_paged_attention_combine does for queries that attend all tokens up to

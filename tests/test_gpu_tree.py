@@ -217,7 +217,7 @@ def test_bad_metadata(k, dk):
 
 @pytest.mark.parametrize("dk", [128, 40])
 def test_a_slot_outside_the_pool(k, dk):
-    """Reported where it is attended and left out; not looked at where nobody attends it."""
+    """Reported where it is attended, and what does not attend it is right; not looked at where nobody attends it."""
     _, trees = _make(6, dk=dk, contexts=(50,), drafts=(10,))
     trees.masks[:, 7] = False
     trees.masks[7, 6] = True
@@ -228,18 +228,23 @@ def test_a_slot_outside_the_pool(k, dk):
     _check(got, want, absolute)
     bad = _make(6, dk=dk, contexts=(50,), drafts=(10,))[1]
     bad.masks[:, 7] = trees.masks[:, 7]
+    bad.masks[:, 8] = False
+    bad.masks[2:5, 8] = True
     bad.masks[7, 6] = True
     bad.slots[57] = bad.pool.pages * bad.pool.page
-    bad.slots[20] = 2 ** 63
+    slot = bad.slots[58]
+    want, absolute = bad.attend()
+    bad.slots[58] = 2 ** 63
     got = _run(k, bad)
     with pytest.raises(kv.KvError) as e:
         k.check_errors()
     assert e.value.fields[0] == 4
-    # As if token 20 were not there.
-    out = Trees.__new__(Trees)
-    out.__dict__.update(bad.__dict__)
-    out.attended = lambda q: np.delete(Trees.attended(bad, q), 20)
-    _check(got, *out.attend())
+    rest = np.delete(np.arange(10), [2, 3, 4])
+    _check(got[rest], want[rest], absolute[rest])
+    bad.slots[58] = slot
+    got = _run(k, bad)
+    k.check_errors()
+    _check(got, want, absolute)
 
 
 def test_queries_out_of_order_are_reported(k):
