@@ -530,6 +530,8 @@ typedef struct sglkv_keep_params {
 #define SGLKV_BEAM_JOIN_THREADS 256u
 #define SGLKV_BEAM_OWN 32u    /* logits of a thread */
 #define SGLKV_BEAM_CHUNK (SGLKV_BEAM_THREADS * SGLKV_BEAM_OWN)
+#define SGLKV_BEAM_LIST 512u     /* tokens that are ranked among each other */
+#define SGLKV_BEAM_FINALS 256u   /* beams' continuations, likewise */
 #define SGLKV_BEAM_MAX_SPLITS 64u  /* a lane each */
 #define SGLKV_BEAM_MAX_BEAMS 1024u
 typedef struct sglkv_beam_params {
