@@ -12,7 +12,7 @@ using namespace sglkv;
 namespace {
 
 struct BeamShape {
-    uint64_t rows, stride, splits;
+    uint64_t rows, stride, rounds, splits;
     uint64_t partial_bytes, candidate_bytes, list_bytes;
 };
 
@@ -39,7 +39,11 @@ int32_t beam_shape(const sgl_kv_beam_config &c, BeamShape *out) {
     BeamShape &h = *out;
     h.rows = c.request_count * c.beam_count;  // (below 2^42)
     h.stride = c.row_stride ? c.row_stride : c.vocab_size;
-    h.splits = divide_up(c.vocab_size, SGLKV_BEAM_CHUNK);
+    // Several rounds a workgroup where there are more than fill the card: what a workgroup does once is shared by them.
+    const uint64_t chunks = divide_up(c.vocab_size, SGLKV_BEAM_CHUNK);
+    h.rounds = h.rows * chunks / 2048;
+    h.rounds = h.rounds < 1 ? 1 : h.rounds > chunks ? chunks : h.rounds;
+    h.splits = divide_up(chunks, h.rounds);
     // A dispatch counts its work-items in 32 bits; parents are numbered in 32 bits, too.
     const uint64_t limit = UINT32_MAX / SGLKV_BEAM_THREADS;
     if (h.rows * h.splits > limit) return too_large_dim("workgroups", h.rows * h.splits, limit);
@@ -106,6 +110,7 @@ extern "C" int32_t sgl_rocm_kv_select_beams(sgl_rocm_kv_ctx *ctx, const sgl_kv_b
     p.vocab = (uint32_t)c.vocab_size;
     p.kept = (uint32_t)c.max_kept;
     p.splits = (uint32_t)h.splits;
+    p.rounds = (uint32_t)h.rounds;
     DeviceScope scope(ctx->device);
     if (scope.status() != hipSuccess) return hip_fail(scope.status(), "hipSetDevice");
     hipStream_t s = static_cast<hipStream_t>(stream);

@@ -523,12 +523,13 @@ typedef struct sglkv_keep_params {
     uint32_t groups;          /* workgroups of a (request, layer) */
 } sglkv_keep_params;
 
-/* Beam selection. A workgroup reads SGLKV_BEAM_THREADS * SGLKV_BEAM_OWN logits of
- * a row (a split), and leaves their maximum, the sum of their exponentials and
- * the `kept` largest in order; one workgroup a request joins them. */
+/* Beam selection. A workgroup reads a split of a row, SGLKV_BEAM_THREADS *
+ * SGLKV_BEAM_OWN logits a round, and leaves their maximum, the sum of their
+ * exponentials and the `kept` largest in order; one workgroup a request joins
+ * them. */
 #define SGLKV_BEAM_THREADS 256u
-#define SGLKV_BEAM_JOIN_THREADS 256u
-#define SGLKV_BEAM_OWN 32u    /* logits of a thread */
+#define SGLKV_BEAM_JOIN_THREADS 512u
+#define SGLKV_BEAM_OWN 32u    /* logits of a thread in a round */
 #define SGLKV_BEAM_CHUNK (SGLKV_BEAM_THREADS * SGLKV_BEAM_OWN)
 #define SGLKV_BEAM_LIST 512u     /* tokens that are ranked among each other */
 #define SGLKV_BEAM_FINALS 256u   /* beams' continuations, likewise */
@@ -548,7 +549,7 @@ typedef struct sglkv_beam_params {
     uint32_t vocab;
     uint32_t kept;
     uint32_t splits;
-    uint32_t reserved;
+    uint32_t rounds;          /* of a split */
 } sglkv_beam_params;
 
 /* Forks. The workspace: word 0 is the plan's verdict (1: carried out), word 1 the
