@@ -115,18 +115,19 @@ namespace {
 
 // The workspace's parts, each a multiple of 64 bytes.
 struct ForkParts {
-    uint64_t first, children, before, freed, bytes;
+    uint64_t first, children, before, copies, freed, bytes;
 };
 
-int32_t fork_parts(const sgl_kv_fork_config &c, ForkParts *out) {
+ForkParts fork_parts(const sgl_kv_fork_config &c) {
     auto lines = [](uint64_t words) { return divide_up(4 * words, 64) * 64; };
-    ForkParts &f = *out;
+    ForkParts f;
     f.first = 4 * SGLKV_FORK_HEAD_WORDS;
     f.children = f.first + lines(c.parent_count);
     f.before = f.children + lines(c.parent_count);
-    f.freed = f.before + lines(c.sequence_count);
+    f.copies = f.before + lines(c.sequence_count);
+    f.freed = f.copies + sizeof(sglkv_page_copy) / 4 * lines(c.sequence_count);
     f.bytes = f.freed + lines(divide_up(c.page_count, 32));
-    return SGL_KV_OK;
+    return f;
 }
 
 bool overlap(uint64_t a, uint64_t an, uint64_t b, uint64_t bn) { return an && bn && a < b + bn && b < a + an; }
@@ -150,8 +151,7 @@ extern "C" int32_t sgl_kv_fork_plan_new(const sgl_kv_fork_config *config, sgl_kv
     sgl_kv_fork_plan p;
     memset(&p, 0, sizeof p);
     p.config = c;
-    ForkParts parts;
-    fork_parts(c, &parts);
+    const ForkParts parts = fork_parts(c);
     p.parents_required_bytes = 4 * c.sequence_count;
     p.lengths_required_bytes = 8 * c.parent_count;
     p.forked_lengths_required_bytes = 8 * c.sequence_count;
@@ -198,8 +198,7 @@ extern "C" int32_t sgl_rocm_kv_fork_sequences(sgl_rocm_kv_ctx *ctx, const sgl_kv
         return fail(SGL_KV_INVALID_ARGUMENT, "pool", pool->page_size, pool->page_count, 0,
                     "the pool has %llu pages of %llu tokens, the plan %llu of %llu", (unsigned long long)pool->page_count,
                     (unsigned long long)pool->page_size, (unsigned long long)c.page_count, (unsigned long long)c.page_size);
-    ForkParts parts;
-    fork_parts(c, &parts);
+    const ForkParts parts = fork_parts(c);
     p.parents = reinterpret_cast<const uint32_t *>(parents);
     p.lengths = reinterpret_cast<const uint64_t *>(lengths);
     p.tables = reinterpret_cast<const int32_t *>(tables);
@@ -212,6 +211,7 @@ extern "C" int32_t sgl_rocm_kv_fork_sequences(sgl_rocm_kv_ctx *ctx, const sgl_kv
     p.first = reinterpret_cast<uint32_t *>(workspace + parts.first);
     p.children = reinterpret_cast<uint32_t *>(workspace + parts.children);
     p.before = reinterpret_cast<uint32_t *>(workspace + parts.before);
+    p.copies = reinterpret_cast<sglkv_page_copy *>(workspace + parts.copies);
     p.freed = reinterpret_cast<uint32_t *>(workspace + parts.freed);
     p.flag = ctx->flag;
     p.table_pages = c.table_pages;
@@ -221,22 +221,37 @@ extern "C" int32_t sgl_rocm_kv_fork_sequences(sgl_rocm_kv_ctx *ctx, const sgl_kv
     p.append = (uint32_t)c.append_tokens;
     p.tensors = pool->tensor_count;
     p.layers = layer_count;
-    uint64_t apart = p.pool.stride[0];
+    uint64_t bits = layer_count > 1 ? layer_stride : 0, most = 0;
     for (uint32_t t = 0; t < p.tensors; ++t) {
         const uint64_t chunk = view_row_bytes(*pool, t) / p.heads;
         if (chunk > UINT32_MAX) return too_large_dim("row_bytes", chunk * p.heads, UINT32_MAX * (uint64_t)p.heads);
         p.chunk[t] = (uint32_t)chunk;
+        bits |= chunk | p.pool.plane[t] | p.pool.head_stride[t];
+        if (view_row_bytes(*pool, t) > most) most = view_row_bytes(*pool, t);
     }
-    p.wide = apart % 16 == 0;
+    uint64_t region;
+    p.wide = p.pool.stride[0] % 16 != 0 ? 0 : bits % 16 != 0 || mul_ovf(most, c.page_size, &region) || region > UINT32_MAX ? 1 : 2;
+    const uint64_t groups = (uint64_t)p.sequences * p.layers * p.tensors, limit = UINT32_MAX / SGLKV_FORK_THREADS;
+    if (groups > limit) return too_large_dim("workgroups", groups, limit);
+    // One workgroup takes as long as the other way's three launches where it goes through some 16,384 entries.
+    const bool small = c.sequence_count <= SGLKV_FORK_SMALL_SEQUENCES && c.parent_count <= SGLKV_FORK_SMALL_SEQUENCES &&
+                       c.table_pages <= SGLKV_FORK_SMALL_ENTRIES && c.page_count <= SGLKV_FORK_SMALL_PAGES &&
+                       c.sequence_count * c.table_pages <= SGLKV_FORK_SMALL_ENTRIES &&
+                       c.parent_count * c.table_pages <= SGLKV_FORK_SMALL_ENTRIES && c.table_pages * c.page_size < 1ull << 31;
     DeviceScope scope(ctx->device);
     if (scope.status() != hipSuccess) return hip_fail(scope.status(), "hipSetDevice");
     hipStream_t s = static_cast<hipStream_t>(stream);
-    rc = launch_kernel(ctx->fork_plan, 1, 1, 1, SGLKV_FORK_PLAN_THREADS, 0, s, &p, "fork plan launch");
+    if (small) {
+        rc = launch_kernel(ctx->fork_small, 1, 1, 1, SGLKV_FORK_PLAN_THREADS, 4 * (unsigned)divide_up(c.page_count, 32), s, &p,
+                           "fork plan launch");
+    } else {
+        rc = launch_kernel(ctx->fork_plan, 1, 1, 1, SGLKV_FORK_PLAN_THREADS, 0, s, &p, "fork plan launch");
+        if (!rc)
+            rc = launch_kernel(ctx->fork_tables, p.sequences + p.old_sequences, 1, 1, SGLKV_FORK_THREADS, 0, s, &p,
+                               "fork tables launch");
+        if (!rc) rc = launch_kernel(ctx->fork_free, 1, 1, 1, SGLKV_FORK_PLAN_THREADS, 0, s, &p, "fork free pages launch");
+    }
     if (!rc)
-        rc = launch_kernel(ctx->fork_copy, p.sequences, p.layers, p.tensors, SGLKV_FORK_THREADS, 0, s, &p, "fork copy launch");
-    if (!rc)
-        rc = launch_kernel(ctx->fork_tables, p.sequences + p.old_sequences, 1, 1, SGLKV_FORK_THREADS, 0, s, &p,
-                           "fork tables launch");
-    if (!rc) rc = launch_kernel(ctx->fork_free, 1, 1, 1, SGLKV_FORK_PLAN_THREADS, 0, s, &p, "fork free pages launch");
+        rc = launch_kernel(ctx->fork_copy, groups, 1, 1, SGLKV_FORK_THREADS, 0, s, &p, "fork copy launch");
     return rc ? rc : ok();
 }

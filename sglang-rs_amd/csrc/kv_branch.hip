@@ -92,45 +92,262 @@ __device__ __forceinline__ void brn_keep_body(const sglkv_keep_params &p) {
 }
 
 // ---- fork_sequences ---------------------------------------------------------
+//
+// The book-keeping is a chain of short steps: who has which children, how many new
+// pages come before each sequence's (a sum), the tables, the references, the freed
+// pages in order. Few sequences take one workgroup, which has all of it in LDS;
+// many take three launches. The copies are a launch of their own: bytes.
 
-// What sequence s needs: its parent's tokens, pages of these, new pages.
+// What a sequence needs: its parent's tokens, pages of these, new pages.
 struct brn_need {
-    uint32_t parent;
     uint64_t length, full, pages, need;
-    uint32_t fresh;  // new pages, a copied last page first among them
+    uint32_t parent, fresh;  // fresh: new pages, a copied last page first among them
     bool copies;
 };
-__device__ __forceinline__ brn_need brn_sequence(const sglkv_fork_params &p, uint32_t s, const uint32_t *first) {
+// `first`: the sequence is its parent's lowest child.
+__device__ __forceinline__ brn_need brn_sequence(const sglkv_fork_params &p, uint32_t parent, uint64_t length, bool first) {
     brn_need n;
-    n.parent = p.parents[s];
-    const bool live = n.parent != SGLKV_FORK_NONE;
-    n.length = live ? p.lengths[n.parent] : 0;
-    n.full = n.length / p.pool.page_size;
-    n.pages = n.full + (n.length % p.pool.page_size != 0);
+    const bool live = parent != SGLKV_FORK_NONE;
+    n.parent = parent;
+    n.length = live ? length : 0;
     const uint64_t end = n.length + p.append;
-    n.need = live ? end / p.pool.page_size + (end % p.pool.page_size != 0) : 0;
-    n.copies = live && n.pages > n.full && __hip_atomic_load(first + n.parent, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != s;
+    if (end >> 32 == 0) {  // (a 64-bit division takes a hundred instructions)
+        const uint32_t size = p.pool.page_size, l = static_cast<uint32_t>(n.length), e = static_cast<uint32_t>(end);
+        n.full = l / size;
+        n.pages = n.full + (l % size != 0);
+        n.need = live ? e / size + (e % size != 0) : 0;
+    } else {
+        n.full = n.length / p.pool.page_size;
+        n.pages = n.full + (n.length % p.pool.page_size != 0);
+        n.need = live ? end / p.pool.page_size + (end % p.pool.page_size != 0) : 0;
+    }
+    n.copies = n.pages > n.full && !first;
     n.fresh = static_cast<uint32_t>(n.need - n.pages) + (n.copies ? 1u : 0u);
     return n;
 }
 
-// One workgroup: who is whose first child, how many new pages come before each
-// sequence's, and whether all of that holds.
+// Exclusive sums over a workgroup of 1,024 threads in their order, and the total.
+// `sums`: a word for each wave; a barrier before and behind.
+__device__ __forceinline__ uint64_t brn_sum(uint64_t own, uint64_t *sums, uint64_t *all) {
+    constexpr uint32_t W = SGLKV_FORK_PLAN_THREADS / 64;
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    uint64_t sum = own;
+#pragma unroll
+    for (uint32_t d = 1; d < 64; d <<= 1) {
+        const uint64_t x = __shfl_up(sum, d);
+        sum += lane >= d ? x : 0;
+    }
+    if (lane == 63) sums[wave] = sum;
+    __syncthreads();
+    uint64_t before = 0, total = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < W; ++w) {
+        before += w < wave ? sums[w] : 0;
+        total += sums[w];
+    }
+    *all = total;
+    __syncthreads();
+    return before + sum - own;
+}
+
+// New page number k of the call.
+__device__ __forceinline__ uint32_t brn_fresh(const sglkv_fork_params &p, uint64_t free_count, uint32_t k) {
+    return static_cast<uint32_t>(p.free_pages[free_count - 1 - k]);
+}
+
+// Entry j of sequence s's new row. `old`: its parent's entry j.
+__device__ __forceinline__ int32_t brn_entry(const sglkv_fork_params &p, const brn_need &n, uint64_t j, int32_t old,
+                                             uint64_t free_count, uint32_t before) {
+    const uint64_t begin = n.copies ? n.full : n.pages;  // new pages from here on
+    if (j >= begin && j < n.need) {
+        const uint32_t page = brn_fresh(p, free_count, before + static_cast<uint32_t>(j - begin));
+        p.references[page] = 1;
+        return static_cast<int32_t>(page);
+    }
+    if (j >= n.pages) return -1;
+    if (static_cast<uint32_t>(old) < p.page_count) return old;
+    atomicOr(p.flag, SGLKV_FLAG_PAGE);
+    return -1;
+}
+
+// Entry j of an old row of `length` tokens that `children` go on from: a row of its
+// own less, and one more for each child that shares the page. True: the page is
+// held by nothing any more. (No other row's change can follow the one that reaches
+// 0: a row that goes on holds its own reference until then.)
+__device__ __forceinline__ bool brn_release(const sglkv_fork_params &p, uint64_t length, uint64_t j, uint32_t children, int32_t entry) {
+    const uint64_t next = (j + 1) * p.pool.page_size;
+    const int32_t change = static_cast<int32_t>(next <= length ? children : children ? 1 : 0) - 1;
+    if (change == 0) return false;
+    const uint32_t page = static_cast<uint32_t>(entry);
+    if (page >= p.page_count) {
+        atomicOr(p.flag, SGLKV_FLAG_PAGE);
+        return false;
+    }
+    return atomicAdd(p.references + page, static_cast<uint32_t>(change)) + static_cast<uint32_t>(change) == 0;
+}
+
+// The copy of a last page, if its source is one.
+__device__ __forceinline__ sglkv_page_copy brn_copy_of(const sglkv_fork_params &p, const brn_need &n, uint64_t free_count, uint32_t before) {
+    sglkv_page_copy c;
+    c.source = static_cast<uint32_t>(p.tables[n.parent * p.table_pages + n.full]);
+    c.to = brn_fresh(p, free_count, before);
+    c.rows = c.source < p.page_count ? static_cast<uint32_t>(n.length - n.full * p.pool.page_size) : 0;
+    return c;
+}
+
+// The freed pages of 32 for each thread behind the `end` free ones, ascending.
+__device__ __forceinline__ void brn_append(const sglkv_fork_params &p, uint32_t word, uint32_t bits, uint64_t at) {
+    for (; bits; bits &= bits - 1, ++at)
+        if (at < p.page_count) p.free_pages[at] = static_cast<int32_t>(32 * word + __builtin_ctz(bits));
+}
+__device__ __forceinline__ void brn_free_count(const sglkv_fork_params &p, uint64_t end) {
+    // (More than the pool has: the caller's counts and its free pages contradict each other.)
+    if (end > p.page_count) atomicOr(p.flag, SGLKV_FLAG_PAGE);
+    *p.free_count = end < p.page_count ? end : p.page_count;
+}
+
+// Everything but the copies of few sequences, in one workgroup.
+__device__ __forceinline__ void brn_small_body(const sglkv_fork_params &p) {
+    constexpr uint32_t T = SGLKV_FORK_PLAN_THREADS, N = SGLKV_FORK_SMALL_SEQUENCES, U = 4;
+    extern __shared__ uint32_t brn_bits[];  // a bit for each page that is freed
+    __shared__ uint64_t sums[T / 64];
+    __shared__ uint32_t parents[N], lengths[N], first[N], children[N], before[N], place[N];
+    const uint32_t tid = threadIdx.x, words = (p.page_count + 31) / 32;
+    const uint32_t width = static_cast<uint32_t>(p.table_pages), room = width * p.pool.page_size;  // (host: below 2^31)
+    const uint32_t old_entries = p.old_sequences * width, new_entries = p.sequences * width;
+    // The first entries of the old tables, ahead of what says which of them count.
+    int32_t early[U];
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) early[u] = p.tables[tid + T * u < old_entries ? tid + T * u : 0];
+    const uint64_t free_count = *p.free_count;
+    uint32_t bad = free_count > p.page_count ? SGLKV_FLAG_ATTN_SEQUENCE : 0u;
+    for (uint32_t i = tid; i < p.old_sequences; i += T) {
+        const uint64_t length = p.lengths[i];
+        if (length > room) bad |= SGLKV_FLAG_ATTN_SEQUENCE;
+        lengths[i] = static_cast<uint32_t>(length);
+        first[i] = SGLKV_FORK_NONE;
+        children[i] = 0;
+    }
+    for (uint32_t s = tid; s < p.sequences; s += T) parents[s] = p.parents[s];
+    for (uint32_t i = tid; i < words; i += T) brn_bits[i] = 0;
+    __syncthreads();
+    for (uint32_t s = tid; s < p.sequences; s += T) {
+        const uint32_t parent = parents[s];
+        if (parent == SGLKV_FORK_NONE) continue;
+        if (parent >= p.old_sequences) {
+            bad |= SGLKV_FLAG_ATTN_REQUEST;
+            continue;
+        }
+        atomicMin(first + parent, s);
+        atomicAdd(children + parent, 1u);
+        if (lengths[parent] > room || p.append > room - lengths[parent]) bad |= SGLKV_FLAG_ATTN_SEQUENCE;
+    }
+    if (__syncthreads_or(bad)) {
+        if (bad) atomicOr(p.flag, bad);
+        if (tid == 0) p.head[0] = p.head[2] = 0;
+        return;
+    }
+    auto need = [&](uint32_t s) {
+        const uint32_t parent = parents[s];
+        const bool live = parent != SGLKV_FORK_NONE;
+        return brn_sequence(p, parent, live ? lengths[parent] : 0, !live || first[parent] == s);
+    };
+    // New pages, and copies, before each sequence's.
+    uint64_t done = 0;
+    for (uint32_t s0 = 0; s0 < p.sequences; s0 += T) {
+        const uint32_t s = s0 + tid;
+        uint64_t own = 0, all;
+        if (s < p.sequences) {
+            const brn_need n = need(s);
+            own = n.fresh | static_cast<uint64_t>(n.copies) << 32;
+        }
+        const uint64_t at = done + brn_sum(own, sums, &all);
+        if (s < p.sequences) {
+            before[s] = static_cast<uint32_t>(at);
+            place[s] = static_cast<uint32_t>(at >> 32);
+        }
+        done += all;
+    }
+    const uint32_t taken = static_cast<uint32_t>(done), copies = static_cast<uint32_t>(done >> 32);
+    if (taken > free_count) {
+        bad = SGLKV_FLAG_OUT_OF_PAGES;
+    } else {
+        for (uint32_t i = tid; i < taken; i += T)
+            if (static_cast<uint32_t>(p.free_pages[free_count - 1 - i]) >= p.page_count) bad |= SGLKV_FLAG_PAGE;
+    }
+    const bool refused = __syncthreads_or(bad) != 0;
+    if (tid == 0) {
+        p.head[0] = refused ? 0 : 1;
+        p.head[2] = refused ? 0 : copies;
+    }
+    if (refused) {
+        if (bad) atomicOr(p.flag, bad);
+        return;
+    }
+    for (uint32_t s = tid; s < p.sequences; s += T) {
+        const brn_need n = need(s);
+        p.forked_lengths[s] = n.length;
+        if (n.copies) p.copies[place[s]] = brn_copy_of(p, n, free_count, before[s]);
+    }
+    for (uint32_t i0 = 0; i0 < new_entries; i0 += U * T) {
+        int32_t old[U];
+        brn_need n[U];
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) {
+            const uint32_t i = i0 + T * u + tid, s = i < new_entries ? i / width : 0, j = i - s * width;
+            n[u] = need(s);
+            old[u] = i < new_entries && j < n[u].pages ? p.tables[n[u].parent * width + j] : -1;
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) {
+            const uint32_t i = i0 + T * u + tid, s = i / width;
+            if (i < new_entries) p.forked_tables[i] = brn_entry(p, n[u], i - s * width, old[u], free_count, before[s]);
+        }
+    }
+    for (uint32_t i0 = 0; i0 < old_entries; i0 += U * T)
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) {
+            const uint32_t i = i0 + T * u + tid, r = i / width, j = i - r * width;
+            if (i >= old_entries || j * p.pool.page_size >= lengths[r]) continue;
+            const int32_t entry = i0 == 0 ? early[u] : p.tables[i];
+            if (brn_release(p, lengths[r], j, children[r], entry)) atomicOr(brn_bits + entry / 32, 1u << (entry % 32));
+        }
+    __syncthreads();
+    uint64_t end = free_count - taken;
+    for (uint32_t w0 = 0; w0 < words; w0 += T) {
+        const uint32_t bits = w0 + tid < words ? brn_bits[w0 + tid] : 0;
+        uint64_t all;
+        const uint64_t at = end + brn_sum(__popc(bits), sums, &all);
+        brn_append(p, w0 + tid, bits, at);
+        end += all;
+    }
+    if (tid == 0) brn_free_count(p, end);
+}
+
+// The same in three launches. One workgroup: who is whose first child, how many new
+// pages come before each sequence's, and whether all of that holds.
+__device__ __forceinline__ uint32_t brn_first(const sglkv_fork_params &p, uint32_t parent) {
+    return __hip_atomic_load(p.first + parent, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ brn_need brn_sequence(const sglkv_fork_params &p, uint32_t s) {
+    const uint32_t parent = p.parents[s];
+    const bool live = parent != SGLKV_FORK_NONE;
+    return brn_sequence(p, parent, live ? p.lengths[parent] : 0, !live || brn_first(p, parent) == s);
+}
 __device__ __forceinline__ void brn_plan_body(const sglkv_fork_params &p) {
     constexpr uint32_t T = SGLKV_FORK_PLAN_THREADS;
     __shared__ uint64_t sums[T / 64];
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const uint32_t tid = threadIdx.x;
     const uint64_t room = p.table_pages * p.pool.page_size;  // (host: no overflow)
-    for (uint32_t i = tid; i < p.old_sequences; i += T) {
-        __hip_atomic_store(p.first + i, SGLKV_FORK_NONE, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __hip_atomic_store(p.children + i, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    for (uint32_t i = tid; i < (p.page_count + 31) / 32; i += T) p.freed[i] = 0;
     uint32_t bad = 0;
     const uint64_t free_count = *p.free_count;
     if (free_count > p.page_count) bad |= SGLKV_FLAG_ATTN_SEQUENCE;
-    for (uint32_t i = tid; i < p.old_sequences; i += T)
+    for (uint32_t i = tid; i < p.old_sequences; i += T) {
+        __hip_atomic_store(p.first + i, SGLKV_FORK_NONE, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(p.children + i, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         if (p.lengths[i] > room) bad |= SGLKV_FLAG_ATTN_SEQUENCE;
+    }
+    for (uint32_t i = tid; i < (p.page_count + 31) / 32; i += T) p.freed[i] = 0;
     __threadfence();
     __syncthreads();
     for (uint32_t s = tid; s < p.sequences; s += T) {
@@ -148,46 +365,42 @@ __device__ __forceinline__ void brn_plan_body(const sglkv_fork_params &p) {
     __threadfence();
     if (__syncthreads_or(bad)) {
         if (bad) atomicOr(p.flag, bad);
-        if (tid == 0) p.head[0] = 0;
+        if (tid == 0) p.head[0] = p.head[2] = 0;
         return;
     }
-    // New pages before each sequence's: sums over the waves, round by round.
+    // (Numbers past the free pages' are not used: the call is refused.)
     uint64_t taken = 0;
     for (uint32_t s0 = 0; s0 < p.sequences; s0 += T) {
-        const uint32_t s = s0 + tid, own = s < p.sequences ? brn_sequence(p, s, p.first).fresh : 0;
-        uint64_t sum = own;
-#pragma unroll
-        for (uint32_t d = 1; d < 64; d <<= 1) {
-            const uint64_t x = __shfl_up(sum, d);
-            sum += lane >= d ? x : 0;
-        }
-        if (lane == 63) sums[wave] = sum;
-        __syncthreads();
-        uint64_t before = taken, all = 0;
-        for (uint32_t w = 0; w < T / 64; ++w) {
-            if (w < wave) before += sums[w];
-            all += sums[w];
-        }
-        // (Numbers past the free ones are not used: the call is refused.)
-        if (s < p.sequences) p.before[s] = static_cast<uint32_t>(before + sum - own);
+        const uint32_t s = s0 + tid;
+        uint64_t all;
+        const uint64_t at = taken + brn_sum(s < p.sequences ? brn_sequence(p, s).fresh : 0, sums, &all);
+        if (s < p.sequences) p.before[s] = static_cast<uint32_t>(at);
         taken += all;
-        __syncthreads();
     }
-    if (taken > free_count) bad |= SGLKV_FLAG_OUT_OF_PAGES;
-    else
+    if (taken > free_count) {
+        bad |= SGLKV_FLAG_OUT_OF_PAGES;
+    } else {
         for (uint64_t i = free_count - taken + tid; i < free_count; i += T)
             if (static_cast<uint32_t>(p.free_pages[i]) >= p.page_count) bad |= SGLKV_FLAG_PAGE;
+    }
     const bool refused = __syncthreads_or(bad) != 0;
     if (bad) atomicOr(p.flag, bad);
+    uint64_t copies = 0;
+    if (!refused)
+        for (uint32_t s0 = 0; s0 < p.sequences; s0 += T) {
+            const uint32_t s = s0 + tid;
+            const brn_need n = brn_sequence(p, s < p.sequences ? s : 0);
+            const bool own = s < p.sequences && n.copies;
+            uint64_t all;
+            const uint64_t at = copies + brn_sum(own, sums, &all);
+            if (own) p.copies[at] = brn_copy_of(p, n, free_count, p.before[s]);
+            copies += all;
+        }
     if (tid == 0) {
         p.head[0] = refused ? 0 : 1;
         p.head[1] = static_cast<uint32_t>(taken);
+        p.head[2] = static_cast<uint32_t>(copies);
     }
-}
-
-// New page number k of the call.
-__device__ __forceinline__ uint32_t brn_fresh(const sglkv_fork_params &p, uint64_t free_count, uint32_t k) {
-    return static_cast<uint32_t>(p.free_pages[free_count - 1 - k]);
 }
 
 // The new tables, the references, the pages that are freed: a workgroup to each
@@ -197,110 +410,84 @@ __device__ __forceinline__ void brn_tables_body(const sglkv_fork_params &p) {
     const uint32_t tid = threadIdx.x;
     if (blockIdx.x < p.sequences) {
         const uint32_t s = blockIdx.x;
-        const brn_need n = brn_sequence(p, s, p.first);
+        const brn_need n = brn_sequence(p, s);
         const uint64_t free_count = *p.free_count;
-        const uint64_t begin = n.copies ? n.full : n.pages;  // new pages from here on
         if (tid == 0) p.forked_lengths[s] = n.length;
         for (uint64_t j = tid; j < p.table_pages; j += SGLKV_FORK_THREADS) {
-            int32_t page = -1;
-            if (j >= begin && j < n.need) {
-                page = static_cast<int32_t>(brn_fresh(p, free_count, p.before[s] + static_cast<uint32_t>(j - begin)));
-                p.references[page] = 1;
-            } else if (j < n.pages) {
-                page = p.tables[n.parent * p.table_pages + j];
-                if (static_cast<uint32_t>(page) >= p.page_count) {
-                    atomicOr(p.flag, SGLKV_FLAG_PAGE);
-                    page = -1;
-                }
-            }
-            p.forked_tables[s * p.table_pages + j] = page;
+            const int32_t old = j < n.pages ? p.tables[n.parent * p.table_pages + j] : -1;
+            p.forked_tables[s * p.table_pages + j] = brn_entry(p, n, j, old, free_count, p.before[s]);
         }
         return;
     }
-    const uint32_t old = blockIdx.x - p.sequences, children = p.children[old];
-    const uint64_t length = p.lengths[old], full = length / p.pool.page_size, pages = full + (length % p.pool.page_size != 0);
-    for (uint64_t j = tid; j < pages; j += SGLKV_FORK_THREADS) {
-        const uint32_t page = static_cast<uint32_t>(p.tables[old * p.table_pages + j]);
-        // A row of its own less; one more for each child that shares the page.
-        const int32_t change = static_cast<int32_t>(j < full ? children : children ? 1 : 0) - 1;
-        if (change == 0) continue;
-        if (page >= p.page_count) {
-            atomicOr(p.flag, SGLKV_FLAG_PAGE);
-            continue;
-        }
-        const uint32_t was = atomicAdd(p.references + page, static_cast<uint32_t>(change));
-        // (No other row's change can follow the one that reaches 0: a row that goes on adds before
-        // or after, and its own reference keeps the count above 0 until it is subtracted.)
-        if (was + static_cast<uint32_t>(change) == 0) atomicOr(p.freed + page / 32, 1u << (page % 32));
-    }
-}
-
-// The last pages' rows: a workgroup to each (sequence, layer, tensor), which
-// copies the chunks of the heads (head-major pages) or all rows at once.
-__device__ __forceinline__ void brn_copy_body(const sglkv_fork_params &p) {
-    if (p.head[0] == 0) return;
-    const uint32_t s = blockIdx.x, layer = blockIdx.y, t = blockIdx.z, tid = threadIdx.x;
-    const brn_need n = brn_sequence(p, s, p.first);
-    if (!n.copies) return;
-    const uint32_t source = static_cast<uint32_t>(p.tables[n.parent * p.table_pages + n.full]);
-    if (source >= p.page_count) return;  // (reported with the tables)
-    const uint32_t to = brn_fresh(p, *p.free_count, p.before[s]);
-    const uint64_t base = p.pool.plane[t] + layer * p.pool.layer_stride;
-    const uint64_t rows = n.length - n.full * p.pool.page_size;
-    // A head's rows lie together, and so do a token-major page's whole rows.
-    const uint64_t bytes = rows * p.chunk[t];
-    for (uint32_t h = 0; h < p.heads; ++h) {
-        const uint64_t from_at = base + source * p.pool.stride[t] + h * p.pool.head_stride[t];
-        const uint64_t to_at = base + to * p.pool.stride[t] + h * p.pool.head_stride[t];
-        uint64_t done = 0;
-        if (p.wide) {
-            // Both are misaligned alike: 16 bytes at a time from the first multiple of 16.
-            const uint64_t lead = (16 - from_at % 16) % 16, head = lead < bytes ? lead : bytes;
-            const uint64_t vectors = (bytes - head) / 16;
-            for (uint64_t i = tid; i < head; i += SGLKV_FORK_THREADS)
-                reinterpret_cast<sglkv_gdst *>(to_at)[i] = reinterpret_cast<sglkv_gsrc *>(from_at)[i];
-            for (uint64_t i = tid; i < vectors; i += SGLKV_FORK_THREADS)
-                reinterpret_cast<brn_dst16 *>(to_at + head)[i] = reinterpret_cast<brn_src16 *>(from_at + head)[i];
-            done = head + 16 * vectors;
-        }
-        for (uint64_t i = done + tid; i < bytes; i += SGLKV_FORK_THREADS)
-            reinterpret_cast<sglkv_gdst *>(to_at)[i] = reinterpret_cast<sglkv_gsrc *>(from_at)[i];
+    const uint32_t r = blockIdx.x - p.sequences, children = p.children[r];
+    const uint64_t length = p.lengths[r];
+    for (uint64_t j = tid; j * p.pool.page_size < length; j += SGLKV_FORK_THREADS) {
+        const int32_t entry = p.tables[r * p.table_pages + j];
+        if (brn_release(p, length, j, children, entry)) atomicOr(p.freed + entry / 32, 1u << (entry % 32));
     }
 }
 
 // One workgroup: the freed pages behind what is left of the free ones, ascending.
 __device__ __forceinline__ void brn_free_body(const sglkv_fork_params &p) {
     constexpr uint32_t T = SGLKV_FORK_PLAN_THREADS;
-    __shared__ uint32_t sums[T / 64];
+    __shared__ uint64_t sums[T / 64];
     if (p.head[0] == 0) return;
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, words = (p.page_count + 31) / 32;
+    const uint32_t tid = threadIdx.x, words = (p.page_count + 31) / 32;
     uint64_t end = *p.free_count - p.head[1];
     for (uint32_t w0 = 0; w0 < words; w0 += T) {
-        uint32_t bits = w0 + tid < words ? p.freed[w0 + tid] : 0;
-        const uint32_t own = __popc(bits);
-        uint32_t sum = own;
-#pragma unroll
-        for (uint32_t d = 1; d < 64; d <<= 1) {
-            const uint32_t x = __shfl_up(sum, d);
-            sum += lane >= d ? x : 0;
-        }
-        if (lane == 63) sums[wave] = sum;
-        __syncthreads();
-        uint64_t at = end + sum - own;
-        uint32_t all = 0;
-        for (uint32_t w = 0; w < T / 64; ++w) {
-            if (w < wave) at += sums[w];
-            all += sums[w];
-        }
-        for (; bits; bits &= bits - 1, ++at)
-            if (at < p.page_count) p.free_pages[at] = static_cast<int32_t>(32 * (w0 + tid) + __builtin_ctz(bits));
+        const uint32_t bits = w0 + tid < words ? p.freed[w0 + tid] : 0;
+        uint64_t all;
+        const uint64_t at = end + brn_sum(__popc(bits), sums, &all);
+        brn_append(p, w0 + tid, bits, at);
         end += all;
-        __syncthreads();
     }
-    // (More than the pool has: the caller's counts and its free pages contradict each other.)
-    if (tid == 0) {
-        if (end > p.page_count) atomicOr(p.flag, SGLKV_FLAG_PAGE);
-        *p.free_count = end < p.page_count ? end : p.page_count;
+    if (tid == 0) brn_free_count(p, end);
+}
+
+// The last pages' rows: a workgroup to each (copy, layer, tensor). A head's rows lie
+// together on head-major pages, all heads' on token-major ones: `heads` stretches.
+__device__ __forceinline__ void brn_copy_body(const sglkv_fork_params &p) {
+    constexpr uint32_t T = SGLKV_FORK_THREADS, U = 8;
+    // (A page's layers and tensors one after another; the workgroups without a copy come last.)
+    const uint32_t parts = p.layers * p.tensors, number = blockIdx.x / parts, part = blockIdx.x - number * parts;
+    const uint32_t layer = part / p.tensors, t = part - layer * p.tensors, tid = threadIdx.x;
+    const sglkv_page_copy c = p.copies[number];
+    if (number >= p.head[2]) return;
+    const uint64_t base = p.pool.plane[t] + layer * p.pool.layer_stride, bytes = static_cast<uint64_t>(c.rows) * p.chunk[t];
+    const uint64_t source = base + c.source * p.pool.stride[t], to = base + c.to * p.pool.stride[t];
+    if (p.wide == 2) {
+        // (Host: a page's part of a tensor is below 2^32 bytes.)
+        const uint32_t vectors = static_cast<uint32_t>(bytes / 16), all = vectors * p.heads;
+        for (uint32_t i0 = tid; i0 < all; i0 += U * T) {
+            sglkv_v4u x[U];
+            uint64_t at[U];
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u) {
+                const uint32_t i = i0 + T * u < all ? i0 + T * u : i0, h = p.heads > 1 ? i / vectors : 0;
+                at[u] = h * p.pool.head_stride[t] + 16ull * (i - h * vectors);
+                x[u] = __builtin_nontemporal_load(reinterpret_cast<brn_src16 *>(source + at[u]));
+            }
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u)
+                if (i0 + T * u < all) __builtin_nontemporal_store(x[u], reinterpret_cast<brn_dst16 *>(to + at[u]));
+        }
+        return;
+    }
+    for (uint32_t h = 0; h < p.heads; ++h) {
+        const uint64_t from_at = source + h * p.pool.head_stride[t], to_at = to + h * p.pool.head_stride[t];
+        uint64_t done = 0;
+        if (p.wide) {
+            // Both are misaligned alike: 16 bytes at a time from the first multiple of 16.
+            const uint64_t lead = (16 - from_at % 16) % 16, head = lead < bytes ? lead : bytes;
+            const uint64_t vectors = (bytes - head) / 16;
+            for (uint64_t i = tid; i < head; i += T)
+                reinterpret_cast<sglkv_gdst *>(to_at)[i] = reinterpret_cast<sglkv_gsrc *>(from_at)[i];
+            for (uint64_t i = tid; i < vectors; i += T)
+                reinterpret_cast<brn_dst16 *>(to_at + head)[i] = reinterpret_cast<brn_src16 *>(from_at + head)[i];
+            done = head + 16 * vectors;
+        }
+        for (uint64_t i = done + tid; i < bytes; i += T)
+            reinterpret_cast<sglkv_gdst *>(to_at)[i] = reinterpret_cast<sglkv_gsrc *>(from_at)[i];
     }
 }
 
@@ -316,6 +503,7 @@ extern "C" __global__ __launch_bounds__(SGLKV_KEEP_THREADS) void sglkv_keep_draf
     brn_keep_body<uint8_t>(p);
 }
 
+extern "C" __global__ __launch_bounds__(SGLKV_FORK_PLAN_THREADS) void sglkv_fork_small(sglkv_fork_params p) { brn_small_body(p); }
 extern "C" __global__ __launch_bounds__(SGLKV_FORK_PLAN_THREADS) void sglkv_fork_plan(sglkv_fork_params p) { brn_plan_body(p); }
 extern "C" __global__ __launch_bounds__(SGLKV_FORK_THREADS) void sglkv_fork_tables(sglkv_fork_params p) { brn_tables_body(p); }
 extern "C" __global__ __launch_bounds__(SGLKV_FORK_THREADS) void sglkv_fork_copy(sglkv_fork_params p) { brn_copy_body(p); }

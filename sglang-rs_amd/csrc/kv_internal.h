@@ -175,7 +175,7 @@ struct sgl_rocm_kv_ctx {
     hipFunction_t tree_tile[3][3];        // dims 64, 128, 256; 1, 2, 4 row waves (2 at dims 256)
     hipFunction_t tree_combine;
     hipFunction_t keep_drafts[3];         // pieces of 16, 4 and 1 bytes
-    hipFunction_t fork_plan, fork_tables, fork_copy, fork_free;
+    hipFunction_t fork_small, fork_plan, fork_tables, fork_copy, fork_free;
     hipFunction_t beam_rows[2];           // bf16, f32
     hipFunction_t beam_join;
     uint32_t attention_occupancy[15];     // resident workgroups per CU of attention[i] ...

@@ -553,12 +553,22 @@ typedef struct sglkv_beam_params {
 } sglkv_beam_params;
 
 /* Forks. The workspace: word 0 is the plan's verdict (1: carried out), word 1 the
- * pages taken; then each parent's lowest child and number of children, each
- * sequence's first new page's number, and a bit for each page that is freed. */
+ * pages taken, word 2 the copies; then each parent's lowest child and number of
+ * children, each sequence's first new page's number, the copies, and a bit for
+ * each page that is freed. Few sequences and pages (SGLKV_FORK_SMALL_*) are kept
+ * in one workgroup's LDS instead. */
 #define SGLKV_FORK_THREADS 256u
 #define SGLKV_FORK_PLAN_THREADS 1024u
 #define SGLKV_FORK_HEAD_WORDS 32u
 #define SGLKV_FORK_NONE 0xFFFFFFFFu
+#define SGLKV_FORK_SMALL_SEQUENCES 2048u  /* old or new */
+#define SGLKV_FORK_SMALL_ENTRIES 16384u   /* of the old or the new tables */
+#define SGLKV_FORK_SMALL_PAGES 262144u
+typedef struct sglkv_page_copy {
+    uint32_t source, to;      /* pages */
+    uint32_t rows;
+    uint32_t reserved;
+} sglkv_page_copy;
 typedef struct sglkv_fork_params {
     const uint32_t *parents;
     const uint64_t *lengths;
@@ -572,6 +582,7 @@ typedef struct sglkv_fork_params {
     uint32_t *first;          /* [parent] */
     uint32_t *children;       /* [parent] */
     uint32_t *before;         /* [sequence] */
+    sglkv_page_copy *copies;  /* [sequence] */
     uint32_t *freed;          /* [ceil(page_count / 32)] */
     uint32_t *flag;
     sglkv_side pool;
@@ -583,7 +594,7 @@ typedef struct sglkv_fork_params {
     uint32_t heads;           /* chunks of a token's row: the heads of head-major pages, else 1 */
     uint32_t layers;
     uint32_t chunk[2];        /* bytes of tensor t's chunk */
-    uint32_t wide;            /* pages and regions are 16-byte aligned alike: 16-byte accesses */
+    uint32_t wide;            /* 2: every chunk and address is a multiple of 16; 1: pages lie a multiple of 16 apart */
 } sglkv_fork_params;
 
 /* Bytes of zeros the context keeps for reads that must contribute nothing

@@ -632,6 +632,7 @@ extern "C" int32_t sgl_rocm_kv_init(int32_t device, const char *code_object_path
                      {"sglkv_keep_drafts_v16", &ctx->keep_drafts[0]},
                      {"sglkv_keep_drafts_v4", &ctx->keep_drafts[1]},
                      {"sglkv_keep_drafts_v1", &ctx->keep_drafts[2]},
+                     {"sglkv_fork_small", &ctx->fork_small},
                      {"sglkv_fork_plan", &ctx->fork_plan},
                      {"sglkv_fork_tables", &ctx->fork_tables},
                      {"sglkv_fork_copy", &ctx->fork_copy},
