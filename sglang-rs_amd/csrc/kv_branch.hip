@@ -26,52 +26,61 @@ __device__ __forceinline__ void brn_keep_body(const sglkv_keep_params &p) {
     typedef __attribute__((address_space(1))) const V src_t;
     typedef __attribute__((address_space(1))) V dst_t;
     constexpr uint32_t U = 8;
-    __shared__ uint64_t from[2][SGLKV_KEEP_ROWS], to[2][SGLKV_KEEP_ROWS];
+    __shared__ uint64_t from[2][SGLKV_KEEP_ROWS], to[2][SGLKV_KEEP_ROWS];  // (an entry that stays: from[0] says so)
+    __shared__ uint32_t most;
     const uint32_t tid = threadIdx.x, layer = blockIdx.y;
     const uint64_t req = blockIdx.x / p.groups;
     const uint32_t group = blockIdx.x % p.groups;
     const bool report = layer == 0 && group == 0;
     const uint32_t *list = p.kept + req * p.max_kept;
+    // (The list does not wait for the request's range, so that the slots are a second step and the rows a third.)
+    uint32_t k = tid < p.max_kept ? list[tid] : SGLKV_SELECT_NONE, before = tid && tid < p.max_kept ? list[tid - 1] : 0;
     const uint64_t s = p.request_slot_offsets[req], e = p.request_slot_offsets[req + 1], context = p.request_lengths[req];
-    // The whole list first: a request moves all of its rows or none.
+    if (tid == 0) most = 0;
     uint32_t bad = s > e || e > p.sequence_slot_count || context > e - s ? SGLKV_FLAG_ATTN_SEQUENCE : 0u;
     const uint64_t room = bad ? 0 : e - s - context;
-    uint32_t count = 0;
-    if (!bad)
-        for (uint32_t i = tid; i < p.max_kept; i += SGLKV_KEEP_THREADS) {
-            const uint32_t k = list[i], before = i ? list[i - 1] : 0;
-            if (k == SGLKV_SELECT_NONE) continue;
-            count = i + 1;
-            if (k >= room || (i && before >= k)) {
-                bad |= SGLKV_FLAG_ATTN_SEQUENCE;
-            } else if (k != i) {
-                if (p.sequence_slots[s + context + k] >= p.pool.slot_count ||
-                    p.sequence_slots[s + context + i] >= p.pool.slot_count)
-                    bad |= SGLKV_FLAG_ATTN_SLOT;
+    // Where entry i's row goes from and to, if it moves; what is wrong with it.
+    auto place = [&](uint32_t i, uint32_t k, uint32_t before) {
+        const uint32_t at = i % SGLKV_KEEP_ROWS;
+        from[0][at] = SGLKV_INVALID_OFFSET;
+        if (k == SGLKV_SELECT_NONE) return 0u;
+        if (k >= room || (i && before >= k)) return SGLKV_FLAG_ATTN_SEQUENCE;
+        if (k == i) return 0u;
+        const uint64_t source = p.sequence_slots[s + context + k], dest = p.sequence_slots[s + context + i];
+        if (source >= p.pool.slot_count || dest >= p.pool.slot_count) return SGLKV_FLAG_ATTN_SLOT;
+#pragma unroll
+        for (uint32_t t = 0; t < 2; ++t)
+            if (t < p.tensors) {
+                from[t][at] = brn_row(p.pool, t, static_cast<uint32_t>(source));
+                to[t][at] = brn_row(p.pool, t, static_cast<uint32_t>(dest));
             }
-        }
-    if (bad && report) atomicOr(p.flag, bad);
+        return 0u;
+    };
+    // The whole list first, from its end: a request moves all of its rows or none, and the first entries' places stay.
     // (Entries behind NONE do not ascend: the last entry's place is the count.)
-    uint32_t *const most = reinterpret_cast<uint32_t *>(from);
-    if (tid == 0) *most = 0;
+    uint32_t count = 0;
+    for (uint32_t i0 = p.max_kept > SGLKV_KEEP_ROWS ? (p.max_kept - 1) / SGLKV_KEEP_ROWS * SGLKV_KEEP_ROWS : 0; i0; i0 -= SGLKV_KEEP_ROWS) {
+        const uint32_t i = i0 + tid;
+        if (i >= p.max_kept) continue;
+        const uint32_t own = list[i];
+        bad |= place(i, own, list[i - 1]);
+        if (own != SGLKV_SELECT_NONE && i >= count) count = i + 1;
+    }
+    bad |= place(tid, k, before);
+    if (k != SGLKV_SELECT_NONE && tid >= count) count = tid + 1;
+    if (bad && report) atomicOr(p.flag, bad);
     if (__syncthreads_or(bad)) return;
-    atomicMax(most, count);
+    if (count) atomicMax(&most, count);
     __syncthreads();
-    count = *most;
+    count = most;
     const uint64_t base = layer * p.pool.layer_stride;
     for (uint32_t r0 = 0; r0 < count; r0 += SGLKV_KEEP_ROWS) {
         const uint32_t rows = count - r0 < SGLKV_KEEP_ROWS ? count - r0 : SGLKV_KEEP_ROWS;
-        __syncthreads();
-        if (tid < rows) {
-            const uint32_t i = r0 + tid, k = list[i];
-#pragma unroll
-            for (uint32_t t = 0; t < 2; ++t) {
-                const bool moves = t < p.tensors && k != i;
-                from[t][tid] = moves ? brn_row(p.pool, t, static_cast<uint32_t>(p.sequence_slots[s + context + k])) : SGLKV_INVALID_OFFSET;
-                to[t][tid] = moves ? brn_row(p.pool, t, static_cast<uint32_t>(p.sequence_slots[s + context + i])) : 0;
-            }
+        if (r0) {
+            __syncthreads();
+            if (tid < rows) (void)place(r0 + tid, list[r0 + tid], 0);
+            __syncthreads();
         }
-        __syncthreads();
         const uint32_t first = p.heads * p.chunk_pieces[0];
         for (uint32_t piece = group * SGLKV_KEEP_THREADS + tid; piece < p.pieces; piece += p.groups * SGLKV_KEEP_THREADS) {
             const uint32_t t = piece >= first, x = t ? piece - first : piece, h = x / p.chunk_pieces[t];
@@ -80,12 +89,13 @@ __device__ __forceinline__ void brn_keep_body(const sglkv_keep_params &p) {
                 V v[U];
 #pragma unroll
                 for (uint32_t u = 0; u < U; ++u) {
-                    const uint64_t o = r + u < rows ? from[t][r + u] : SGLKV_INVALID_OFFSET;
-                    if (o != SGLKV_INVALID_OFFSET) v[u] = *reinterpret_cast<src_t *>(at + o);
+                    if (r + u < rows && from[0][r + u] != SGLKV_INVALID_OFFSET)
+                        v[u] = __builtin_nontemporal_load(reinterpret_cast<src_t *>(at + from[t][r + u]));
                 }
 #pragma unroll
                 for (uint32_t u = 0; u < U; ++u)
-                    if (r + u < rows && from[t][r + u] != SGLKV_INVALID_OFFSET) *reinterpret_cast<dst_t *>(at + to[t][r + u]) = v[u];
+                    if (r + u < rows && from[0][r + u] != SGLKV_INVALID_OFFSET)
+                        __builtin_nontemporal_store(v[u], reinterpret_cast<dst_t *>(at + to[t][r + u]));
             }
         }
     }
@@ -155,12 +165,14 @@ __device__ __forceinline__ uint32_t brn_fresh(const sglkv_fork_params &p, uint64
     return static_cast<uint32_t>(p.free_pages[free_count - 1 - k]);
 }
 
-// Entry j of sequence s's new row. `old`: its parent's entry j.
-__device__ __forceinline__ int32_t brn_entry(const sglkv_fork_params &p, const brn_need &n, uint64_t j, int32_t old,
-                                             uint64_t free_count, uint32_t before) {
+// Entry j of sequence s's new row. `old`: its parent's entry j; fresh(k): new page
+// number k of the call.
+template <typename F>
+__device__ __forceinline__ int32_t brn_entry(const sglkv_fork_params &p, const brn_need &n, uint64_t j, int32_t old, F fresh,
+                                             uint32_t before) {
     const uint64_t begin = n.copies ? n.full : n.pages;  // new pages from here on
     if (j >= begin && j < n.need) {
-        const uint32_t page = brn_fresh(p, free_count, before + static_cast<uint32_t>(j - begin));
+        const uint32_t page = fresh(before + static_cast<uint32_t>(j - begin));
         p.references[page] = 1;
         return static_cast<int32_t>(page);
     }
@@ -186,11 +198,11 @@ __device__ __forceinline__ bool brn_release(const sglkv_fork_params &p, uint64_t
     return atomicAdd(p.references + page, static_cast<uint32_t>(change)) + static_cast<uint32_t>(change) == 0;
 }
 
-// The copy of a last page, if its source is one.
-__device__ __forceinline__ sglkv_page_copy brn_copy_of(const sglkv_fork_params &p, const brn_need &n, uint64_t free_count, uint32_t before) {
+// The copy of a last page to page `to`, if its source is one.
+__device__ __forceinline__ sglkv_page_copy brn_copy_of(const sglkv_fork_params &p, const brn_need &n, uint32_t to) {
     sglkv_page_copy c;
     c.source = static_cast<uint32_t>(p.tables[n.parent * p.table_pages + n.full]);
-    c.to = brn_fresh(p, free_count, before);
+    c.to = to;
     c.rows = c.source < p.page_count ? static_cast<uint32_t>(n.length - n.full * p.pool.page_size) : 0;
     return c;
 }
@@ -211,7 +223,7 @@ __device__ __forceinline__ void brn_small_body(const sglkv_fork_params &p) {
     constexpr uint32_t T = SGLKV_FORK_PLAN_THREADS, N = SGLKV_FORK_SMALL_SEQUENCES, U = 4;
     extern __shared__ uint32_t brn_bits[];  // a bit for each page that is freed
     __shared__ uint64_t sums[T / 64];
-    __shared__ uint32_t parents[N], lengths[N], first[N], children[N], before[N], place[N];
+    __shared__ uint32_t parents[N], lengths[N], first[N], children[N], before[N], place[N], top[T];  // top: the first new pages
     const uint32_t tid = threadIdx.x, words = (p.page_count + 31) / 32;
     const uint32_t width = static_cast<uint32_t>(p.table_pages), room = width * p.pool.page_size;  // (host: below 2^31)
     const uint32_t old_entries = p.old_sequences * width, new_entries = p.sequences * width;
@@ -230,7 +242,17 @@ __device__ __forceinline__ void brn_small_body(const sglkv_fork_params &p) {
     }
     for (uint32_t s = tid; s < p.sequences; s += T) parents[s] = p.parents[s];
     for (uint32_t i = tid; i < words; i += T) brn_bits[i] = 0;
+    if (free_count <= p.page_count && tid < free_count) top[tid] = static_cast<uint32_t>(p.free_pages[free_count - 1 - tid]);
     __syncthreads();
+    // (The new tables' first entries, too.)
+    int32_t old[U];
+    auto parent_entry = [&](uint32_t i) {
+        const uint32_t s = i < new_entries ? i / width : 0, parent = parents[s];
+        return i < new_entries && parent < p.old_sequences ? p.tables[parent * width + (i - s * width)] : -1;
+    };
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) old[u] = parent_entry(T * u + tid);
+    auto fresh = [&](uint32_t k) { return k < T ? top[k] : brn_fresh(p, free_count, k); };
     for (uint32_t s = tid; s < p.sequences; s += T) {
         const uint32_t parent = parents[s];
         if (parent == SGLKV_FORK_NONE) continue;
@@ -273,7 +295,7 @@ __device__ __forceinline__ void brn_small_body(const sglkv_fork_params &p) {
         bad = SGLKV_FLAG_OUT_OF_PAGES;
     } else {
         for (uint32_t i = tid; i < taken; i += T)
-            if (static_cast<uint32_t>(p.free_pages[free_count - 1 - i]) >= p.page_count) bad |= SGLKV_FLAG_PAGE;
+            if (fresh(i) >= p.page_count) bad |= SGLKV_FLAG_PAGE;
     }
     const bool refused = __syncthreads_or(bad) != 0;
     if (tid == 0) {
@@ -287,21 +309,16 @@ __device__ __forceinline__ void brn_small_body(const sglkv_fork_params &p) {
     for (uint32_t s = tid; s < p.sequences; s += T) {
         const brn_need n = need(s);
         p.forked_lengths[s] = n.length;
-        if (n.copies) p.copies[place[s]] = brn_copy_of(p, n, free_count, before[s]);
+        if (n.copies) p.copies[place[s]] = brn_copy_of(p, n, fresh(before[s]));
     }
     for (uint32_t i0 = 0; i0 < new_entries; i0 += U * T) {
-        int32_t old[U];
-        brn_need n[U];
+        if (i0)
 #pragma unroll
-        for (uint32_t u = 0; u < U; ++u) {
-            const uint32_t i = i0 + T * u + tid, s = i < new_entries ? i / width : 0, j = i - s * width;
-            n[u] = need(s);
-            old[u] = i < new_entries && j < n[u].pages ? p.tables[n[u].parent * width + j] : -1;
-        }
+            for (uint32_t u = 0; u < U; ++u) old[u] = parent_entry(i0 + T * u + tid);
 #pragma unroll
         for (uint32_t u = 0; u < U; ++u) {
             const uint32_t i = i0 + T * u + tid, s = i / width;
-            if (i < new_entries) p.forked_tables[i] = brn_entry(p, n[u], i - s * width, old[u], free_count, before[s]);
+            if (i < new_entries) p.forked_tables[i] = brn_entry(p, need(s), i - s * width, old[u], fresh, before[s]);
         }
     }
     for (uint32_t i0 = 0; i0 < old_entries; i0 += U * T)
@@ -393,7 +410,7 @@ __device__ __forceinline__ void brn_plan_body(const sglkv_fork_params &p) {
             const bool own = s < p.sequences && n.copies;
             uint64_t all;
             const uint64_t at = copies + brn_sum(own, sums, &all);
-            if (own) p.copies[at] = brn_copy_of(p, n, free_count, p.before[s]);
+            if (own) p.copies[at] = brn_copy_of(p, n, brn_fresh(p, free_count, p.before[s]));
             copies += all;
         }
     if (tid == 0) {
@@ -415,7 +432,8 @@ __device__ __forceinline__ void brn_tables_body(const sglkv_fork_params &p) {
         if (tid == 0) p.forked_lengths[s] = n.length;
         for (uint64_t j = tid; j < p.table_pages; j += SGLKV_FORK_THREADS) {
             const int32_t old = j < n.pages ? p.tables[n.parent * p.table_pages + j] : -1;
-            p.forked_tables[s * p.table_pages + j] = brn_entry(p, n, j, old, free_count, p.before[s]);
+            p.forked_tables[s * p.table_pages + j] =
+                brn_entry(p, n, j, old, [&](uint32_t k) { return brn_fresh(p, free_count, k); }, p.before[s]);
         }
         return;
     }
