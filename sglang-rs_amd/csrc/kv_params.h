@@ -486,10 +486,16 @@ typedef struct sglkv_tree_params {
     uint64_t max_length;      /* the farthest that a query of the launch reaches */
     uint32_t mask_words;
     uint32_t tile_queries;    /* tiles: queries of one */
-    uint32_t tile_slots;      /* tiles: workgroups of a (split, request, KV head) */
-    uint32_t reserved;
+    uint32_t tile_slots;      /* tiles: workgroups of a (request, split) and KV head, unless `balanced` */
+    uint32_t pairs;           /* tiles: (request, split, tile)s that make up the workgroups resident at once */
+    uint32_t balanced;        /* tiles: the workgroups find the splits themselves */
+    uint32_t unit;            /* tiles: tokens of a block for each token group (0: the generic body) */
+    uint32_t least;           /* tiles: units of a split or more */
+    uint32_t *chunk_word;     /* tiles: the tokens of a split that the workgroups found */
 } sglkv_tree_params;
 #define SGLKV_TREE_MAX_WORDS 16u
+#define SGLKV_TREE_BALANCED 64u   /* most requests whose splits are found on the device ... */
+#define SGLKV_TREE_LISTED 4096u   /* ... and most queries */
 /* Tiles: head dims d, `rows` row waves (32 rows each) of the workgroup's four.
  * Tokens of a block; LDS: two stages of K and V rows for each token group, the
  * raw slots of two blocks a wave (2 KiB), the drafts that the tile attends, a
@@ -498,7 +504,7 @@ typedef struct sglkv_tree_params {
 #define SGLKV_TREE_BLOCK(d, rows) ((rows) == 4u ? 64u : 32u)
 #define SGLKV_TREE_LDS_BYTES(d, rows)                                                              \
     (2u * (4u / ((rows) * SGLKV_TREE_SHARE(d))) * 4u * (d) * SGLKV_TREE_BLOCK(d, rows) + 2048u +   \
-     8u * (SGLKV_TREE_MAX_WORDS + 2u) + 64u + 4096u)
+     8u * (SGLKV_TREE_MAX_WORDS + 2u) + 80u + 4096u)
 
 /* Accepted drafts' rows, moved together in place. Thread t of a workgroup owns
  * piece t, t + 256, ... of every row of a (request, layer): rows go in the order

@@ -26,15 +26,16 @@ struct TreeShape {
     // Tiles: head dims 64, 128 or 256 on rows that the buffers' alignment, which is the call's to see, lets 16-byte
     // accesses read.
     bool tiles;
-    uint32_t row_waves, tile_queries, tile_slots;
+    uint32_t row_waves, tile_queries, tile_slots, unit, least;
+    bool balanced;
+    uint64_t pairs;
     TreeWay tile;
 };
 
-// Splits of `chunk` tokens, their records and their merge.
-int32_t split_records(const sgl_kv_attention_plan_config &c, uint64_t max_length, TreeWay *w) {
+// The records of a query head's `splits` splits, and their merge.
+int32_t split_records(const sgl_kv_attention_plan_config &c, TreeWay *w) {
     uint64_t heads;
     if (mul_ovf(c.query_count, c.query_head_count, &heads)) return attention_overflow();
-    w->splits = divide_up(max_length, w->chunk);
     w->record_bytes = w->combine_grid = 0;
     if (w->splits > 1) {
         if (mul_ovf(heads, w->splits, &w->record_bytes) ||
@@ -62,28 +63,38 @@ int32_t tile_shape(const sgl_kv_attention_plan_config &c, const sgl_kv_tree_atte
     h.row_waves = rows <= 32 ? 1 : rows <= 64 || most == 2 ? 2 : 4;
     while (group > 32 * h.row_waves) h.row_waves *= 2;
     h.tile_queries = 32 * h.row_waves / (uint32_t)group;
-    // Workgroups for trees of up to twice the average; larger ones go on by their number.
-    const uint64_t drafts = 64 * t.mask_words < 2 * mean ? 64 * t.mask_words : 2 * mean;
-    h.tile_slots = (uint32_t)divide_up(drafts < c.query_count ? drafts : c.query_count, h.tile_queries);
-    // As many workgroups as stay resident at once, each with two blocks of each of its token groups or more. The
-    // sequences have sequence_slot_count tokens together; each ends inside a split.
-    const uint64_t groups = 4 / (h.row_waves * SGLKV_TREE_SHARE(d));
-    const uint64_t resident = 256 * (d == 64 ? (h.row_waves == 2 ? 3 : 2) : h.row_waves == 1 ? 1 : 2);
-    const uint64_t tiles = divide_up(mean, h.tile_queries), alike = c.kv_head_count * tiles;
-    const uint64_t total = c.sequence_slot_count, half = divide_up(c.request_count, 2);
-    const uint64_t live = resident / alike > c.request_count ? resident / alike - half : half;
-    const uint64_t least = 2 * groups * SGLKV_TREE_BLOCK(d, h.row_waves);
+    // (Request, split, tile)s: as many as make the workgroups that stay resident at once, or half as many again as the
+    // requests' tiles, so that ragged ones even out. A request has at most twice its even share of splits and two more,
+    // which bounds the records.
+    const uint64_t groups = 4 / (h.row_waves * SGLKV_TREE_SHARE(d)), count = c.request_count;
+    const uint64_t resident = 256 * (d == 128 && h.row_waves == 1 ? 1 : d == 256 && h.row_waves == 1 ? 1 : 2);
+    const uint64_t tiles = divide_up(mean, h.tile_queries), most_tiles = c.query_count / h.tile_queries + count;
+    h.unit = (uint32_t)(groups * SGLKV_TREE_BLOCK(d, h.row_waves));
+    h.least = 2;
+    h.balanced = count <= SGLKV_TREE_BALANCED && c.query_count <= SGLKV_TREE_LISTED;
     TreeWay &w = h.tile;
-    w.chunk = divide_up(total, live);
-    if (w.chunk > h.max_length) w.chunk = h.max_length;
-    if (w.chunk < least) w.chunk = least;
-    w.chunk = divide_up(w.chunk, least) * least;
-    int32_t rc = split_records(c, h.max_length, &w);
+    h.pairs = resident / c.kv_head_count > 1 ? resident / c.kv_head_count : 1;
+    uint64_t pieces = 2 * divide_up(h.pairs, count * tiles) + 2, numbers = most_tiles + most_tiles / 2;
+    if (numbers < h.pairs) numbers = h.pairs;
+    if (!h.balanced) {
+        // One length of splits for all, twice the average request's; workgroups for the tiles of twice the average one.
+        const uint64_t drafts = 64 * t.mask_words < 2 * mean ? 64 * t.mask_words : 2 * mean;
+        h.tile_slots = (uint32_t)divide_up(drafts < c.query_count ? drafts : c.query_count, h.tile_queries);
+        w.chunk = 2 * divide_up(c.sequence_slot_count, count);
+        if (w.chunk > h.max_length) w.chunk = h.max_length;
+        if (w.chunk < h.unit * h.least) w.chunk = h.unit * h.least;
+        pieces = divide_up(h.max_length, w.chunk);
+        if (mul_ovf(count, pieces, &numbers) || mul_ovf(numbers, h.tile_slots, &numbers)) return attention_overflow();
+    }
+    w.splits = divide_up(h.max_length, h.unit * h.least);
+    if (w.splits > pieces) w.splits = pieces;
+    int32_t rc = split_records(c, &w);
     if (rc) return rc;
-    uint64_t items;
-    if (mul_ovf(c.request_count + 1, c.kv_head_count, &items) || mul_ovf(items, w.splits, &items) || items > UINT64_MAX - 7 ||
-        mul_ovf(divide_up(items, 8) * 8, h.tile_slots, &w.base))
-        return attention_overflow();
+    if (h.pairs > UINT32_MAX / 2 || w.splits > UINT32_MAX || mul_ovf(numbers, c.kv_head_count, &w.base)) {
+        h.tiles = false;
+        return SGL_KV_OK;
+    }
+    w.record_bytes += 64;  // the word that the workgroups leave for the merge
     h.tiles = w.base <= UINT32_MAX / 256;
     return SGL_KV_OK;
 }
@@ -113,7 +124,8 @@ int32_t tree_shape(const sgl_kv_attention_plan_config &c, const sgl_kv_tree_atte
     w.chunk = divide_up(w.chunk, SGLKV_ATTN_TOKENS) * SGLKV_ATTN_TOKENS;
     const uint64_t limit = UINT32_MAX / 64;  // a dispatch counts its work-items in 32 bits
     if (w.base > limit) return too_large_dim("workgroups", w.base, limit);
-    int32_t rc = split_records(c, h.max_length, &w);
+    w.splits = divide_up(h.max_length, w.chunk);
+    int32_t rc = split_records(c, &w);
     return rc ? rc : tile_shape(c, t, out);
 }
 
@@ -201,6 +213,11 @@ extern "C" int32_t sgl_rocm_kv_tree_attention(sgl_rocm_kv_ctx *ctx, const sgl_kv
         p.a.key_token_stride32 = p.a.value_token_stride32 = (uint32_t)p.a.key_token_stride;
         p.tile_queries = shape.tile_queries;
         p.tile_slots = shape.tile_slots;
+        p.pairs = (uint32_t)shape.pairs;
+        p.balanced = shape.balanced;
+        p.unit = shape.unit;
+        p.least = shape.least;
+        p.chunk_word = reinterpret_cast<uint32_t *>(workspace + way.record_bytes - 64);
         const int dims = p.a.dk == 64 ? 0 : p.a.dk == 128 ? 1 : 2, rows = shape.row_waves == 1 ? 0 : shape.row_waves == 2 ? 1 : 2;
         rc = launch_kernel(ctx->tree_tile[dims][rows], way.base, 1, 1, 256, SGLKV_TREE_LDS_BYTES(p.a.dk, shape.row_waves), s, &p,
                            "tree attention launch");

@@ -165,8 +165,8 @@ struct tree_tl {
     static constexpr uint32_t OWN = 16 * NT / TW;         // outputs of a lane after the groups are joined
     static constexpr uint32_t RING = 2 * TW * STAGE;      // 256 bytes of raw slots for each wave and stage
     static constexpr uint32_t UNION = RING + 2048;        // which drafts the tile attends at all
-    static constexpr uint32_t WORDS = UNION + 8 * (SGLKV_TREE_MAX_WORDS + 2);  // a word for each wave
-    static constexpr uint32_t TABLE = WORDS + 64;         // each wave's rows (tree_row)
+    static constexpr uint32_t WORDS = UNION + 8 * (SGLKV_TREE_MAX_WORDS + 2);  // four words for each wave, and four held
+    static constexpr uint32_t TABLE = WORDS + 80;         // each wave's rows (tree_row)
     static constexpr uint32_t VBUF = D > 128 && TW == 1 ? 1 : 2;  // steps whose values there are registers for
     static_assert(TABLE + 4096 == SGLKV_TREE_LDS_BYTES(D, RW), "the host sizes the same LDS");
     static_assert(N <= 32 && LPW * TPL == N && TW * GW == 4 && OWN * TW == 16 * NT && OWN % 4 == 0, "whole loads and shares");
@@ -183,6 +183,14 @@ __device__ __forceinline__ void tree_load_slots(uint64_t address, uint32_t at) {
         : "=&s"(save)
         : "s"(at), "v"(address)
         : "memory");
+}
+// A wave's slots of the block from token `tb` on; `base`: the request's first slot
+// and the lane's word of it.
+template <uint32_t D, uint32_t RW>
+__device__ __forceinline__ void tree_slots(uint64_t base, uint32_t last, uint32_t tb, uint32_t gw, uint32_t lane, uint32_t at) {
+    typedef tree_tl<D, RW> T;
+    const uint32_t tok = tb + T::N * gw + lane % T::N;
+    tree_load_slots(base + 8ull * (tok < last ? tok : last), at);
 }
 template <uint32_t COUNT>
 __device__ __forceinline__ void tree_wait() {
@@ -251,11 +259,12 @@ struct tree_state {
 // ring. A token that no row attends, or whose slot is outside the pool, reads the
 // zero row.
 template <uint32_t D, uint32_t RW>
-__device__ __forceinline__ void tree_issue(const sglkv_attn_params &p, const tree_pass &pass, uint64_t kbase, uint64_t vbase,
+__device__ __forceinline__ void tree_issue(const sglkv_attn_params &held, const tree_pass &pass, uint64_t kbase, uint64_t vbase,
                                            const uint32_t *ring, const uint64_t *seen, uint32_t tb, uint32_t gw, uint32_t lane,
                                            uint32_t stage_at) {
     typedef tree_tl<D, RW> T;
-    if (T::VBUF == 1) asm volatile("" : "+v"(lane));  // (what it computes from the lane is not held across the block)
+    const sglkv_attn_params &p = D > 128 && T::TW > 1 ? tree_params().a : held;  // (no scalar registers left to hold them)
+    if (D > 64) asm volatile("" : "+v"(lane));  // (what it computes from the lane is not held across the block)
     const uint32_t c = lane / T::PIECES, pos = lane % T::PIECES;
     const uint64_t zero = reinterpret_cast<uint64_t>(p.zero_row) + 16 * pos;
     const uint32_t mask = (1u << p.page_shift) - 1, slots = static_cast<uint32_t>(p.slot_count);  // (host: below 2^32)
@@ -271,7 +280,7 @@ __device__ __forceinline__ void tree_issue(const sglkv_attn_params &p, const tre
             ok = tok < pass.t1 && (tok < pass.whole || (place < 64 * SGLKV_TREE_MAX_WORDS && (seen[place >> 6] >> (place & 63)) & 1));
         }
         if (ok && (high != 0 || low >= slots)) {
-            atomicOr(p.flag, SGLKV_FLAG_ATTN_SLOT);
+            atomicOr(tree_params().a.flag, SGLKV_FLAG_ATTN_SLOT);
             ok = false;
         }
         const uint32_t s = ok ? low : 0u;
@@ -423,10 +432,7 @@ __device__ __forceinline__ void tree_run(const sglkv_tree_params &p, const tree_
     const uint32_t end = reach < pass.t1 ? reach : pass.t1;
     const uint32_t mine = end <= first ? 0 : (end - first + T::B * T::TW - 1) / (T::B * T::TW);
     auto block = [&](uint32_t k) { return first + k * T::B * T::TW; };
-    auto slots = [&](uint32_t k) {
-        const uint32_t tok = block(k) + T::N * gw + lane % T::N;
-        tree_load_slots(slot_base + 8ull * (tok < pass.last ? tok : pass.last), ring_at + 256 * (k & 1));
-    };
+    auto slots = [&](uint32_t k) { tree_slots<D, RW>(slot_base, pass.last, block(k), gw, lane, ring_at + 256 * (k & 1)); };
     auto rows = [&](uint32_t k) {
         tree_issue<D, RW>(a, pass, kbase, vbase, ring + 64 * (k & 1), seen, block(k), gw, lane, stage_at + T::STAGE * (k & 1));
     };
@@ -434,21 +440,26 @@ __device__ __forceinline__ void tree_run(const sglkv_tree_params &p, const tree_
     st.l_part = 0.0f;
 #pragma unroll
     for (uint32_t n = 0; n < T::NT; ++n) st.o[n] = sglkv_f32x16{};
-    // Everything that the compiler loaded has arrived: it puts no wait into the loop, where rows are in flight.
+    // The first two blocks' slots have arrived (the caller's tree_slots), and everything that the compiler loaded: it
+    // puts no wait into the loop, where rows are in flight.
     __builtin_amdgcn_s_waitcnt(0x0F70);
-    slots(0);
-    tree_wait<0>();
-    slots(1);
     rows(0);
-    // Block k's rows have landed; block k + 1's are on their way.
+    slots(2);
+    rows(1);
+    // Block k's rows have landed; block k + 1's are on their way (the first two blocks' both from the start).
     auto next = [&](uint32_t k) {
         if constexpr (T::GW == 1) {
             // The wave's own stages: the slots of k + 1 are older than the rows of k.
-            tree_wait<2 * T::LPW>();
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // block k - 1's stage is read
-            slots(k + 2);
-            rows(k + 1);
+            if (k) {
+                tree_wait<2 * T::LPW>();
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // block k - 1's stage is read
+                slots(k + 2);
+                rows(k + 1);
+            }
             tree_wait<2 * T::LPW + 1>();
+        } else if (k == 0) {
+            tree_wait<2 * T::LPW + 1>();
+            asm volatile("s_barrier" ::: "memory");
         } else {
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
             slots(k + 2);
@@ -495,10 +506,159 @@ __device__ __forceinline__ void tree_find(const sglkv_attn_params &a, uint32_t l
     *end = lo[1] > lo[0] ? lo[1] : lo[0];
 }
 
+// x joined over 32 lanes whose halves of the wave are alike.
+template <typename F>
+__device__ __forceinline__ uint32_t tree_join(uint32_t x, F join) {
+    x = join(x, sel_join<1>(x));
+    x = join(x, sel_join<2>(x));
+    x = join(x, sel_join<4>(x));
+    x = join(x, sel_join<8>(x));
+    return __builtin_amdgcn_readfirstlane(join(x, sel_join<16>(x)));
+}
+__device__ __forceinline__ uint32_t tree_most(uint32_t x) {
+    return tree_join(x, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+}
+
+// ---- A launch's tiles ----
+//
+// Request r has T_r tiles of its queries and n_r tokens, cut into ceil(n_r / c) even
+// splits, with the smallest c (whole units: a block for each token group) that leaves
+// at most as many (request, split, tile)s as workgroups are resident at once, whatever
+// the lengths, which the host does not know; they are numbered without a gap, since a
+// workgroup that finds nothing to do holds its place until the ones before it on its
+// CU are done: 32 requests of 300 to 8,192 tokens took 265 us with every other
+// workgroup empty, 163 us without; with half as many pairs 209, with twice 167.
+// Each workgroup finds c and its own place, a lane to a request. Past
+// SGLKV_TREE_BALANCED requests or SGLKV_TREE_LISTED queries c is the host's, and
+// tiles beyond the average request's are taken by the same workgroups.
+
+// The tokens of request r that the launch can reach (its slots, at most max_length).
+__device__ __forceinline__ uint32_t tree_tokens(const sglkv_tree_params &p, uint32_t r) {
+    const uint64_t s = p.a.request_slot_offsets[r], e = p.a.request_slot_offsets[r + 1];
+    const uint64_t n = s <= e && e <= p.a.sequence_slot_count ? e - s : 0;
+    return static_cast<uint32_t>(n < p.max_length ? n : p.max_length);
+}
+__device__ __forceinline__ uint32_t tree_splits(uint32_t n, uint32_t c) { return n > c ? (n + c - 1) / c : 1; }
+// Tokens of a split of a request of n tokens.
+__device__ __forceinline__ uint32_t tree_chunk(const sglkv_tree_params &p, uint32_t n, uint32_t c) {
+    const uint32_t k = tree_splits(n, c);
+    return ((n + k - 1) / k + p.unit - 1) / p.unit * p.unit;
+}
+
+// A workgroup's place: its request's queries [first, end) from tile `tile` on, every
+// tile_step-th, and the split. Queries [loose, loose_end) belong to no request.
+struct tree_place {
+    uint32_t request, split, chunk, first, end, tile, tile_step, loose, loose_end;
+};
+
+// Where each request's queries begin and end, in LDS (the last entry: those of no
+// request), and whether the indices ever fall.
+__device__ __forceinline__ void tree_list(const sglkv_attn_params &a, uint32_t tid, uint32_t *begins, uint32_t *ends) {
+    const uint32_t count = static_cast<uint32_t>(a.query_count), requests = static_cast<uint32_t>(a.request_count);
+    if (tid <= requests) begins[tid] = ends[tid] = 0;
+    __syncthreads();
+    for (uint32_t i = tid; i < count; i += 256) {
+        const uint32_t x = a.query_request_indices[i], y = a.query_request_indices[i ? i - 1 : 0];
+        const uint32_t own = x < requests ? x : requests, before = y < requests ? y : requests;
+        if (i == 0 || own != before) {
+            begins[own] = i;
+            if (i) ends[before] = i;
+        }
+        if (i + 1 == count) ends[own] = count;
+        if (y > x && blockIdx.x == 0) atomicOr(a.flag, SGLKV_FLAG_ATTN_REQUEST);
+    }
+    __syncthreads();
+}
+
+// False: no (request, split, tile) has this number. (Loose queries are there all the same.)
+__device__ __forceinline__ bool tree_balance(const sglkv_tree_params &p, uint32_t number, uint32_t tid, uint32_t lane,
+                                             uint32_t *begins, tree_place *at) {
+    const sglkv_attn_params &a = p.a;
+    uint32_t *const ends = begins + SGLKV_TREE_BALANCED + 1;
+    const uint32_t requests = static_cast<uint32_t>(a.request_count), unit = p.unit;
+    const uint32_t n = lane < requests ? tree_tokens(p, lane) : 0;
+    tree_list(a, tid, begins, ends);
+    auto sum = [](uint32_t x) {
+        x += sel_join<1>(x);
+        x += sel_join<2>(x);
+        x += sel_join<4>(x);
+        x += sel_join<8>(x);
+        x += sel_join<16>(x);
+        return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(x + sel_join<32>(x)));
+    };
+    const uint32_t first = lane < requests ? begins[lane] : 0, end = lane < requests ? ends[lane] : 0;
+    const uint32_t tiles = end > first ? (end - first + p.tile_queries - 1) / p.tile_queries : 0;
+    at->loose = __builtin_amdgcn_readfirstlane(begins[requests]);
+    at->loose_end = __builtin_amdgcn_readfirstlane(ends[requests]);
+    const uint32_t least_pairs = sum(tiles), most_pairs = p.pairs > least_pairs + least_pairs / 2 ? p.pairs : least_pairs + least_pairs / 2;
+    // From what an even share would be (in floats: an estimate), in steps of a sixteenth.
+    float work = static_cast<float>(tiles) * static_cast<float>(n);
+    work += __uint_as_float(sel_join<1>(__float_as_uint(work)));
+    work += __uint_as_float(sel_join<2>(__float_as_uint(work)));
+    work += __uint_as_float(sel_join<4>(__float_as_uint(work)));
+    work += __uint_as_float(sel_join<8>(__float_as_uint(work)));
+    work += __uint_as_float(sel_join<16>(__float_as_uint(work)));
+    work += __uint_as_float(sel_join<32>(__float_as_uint(work)));
+    uint32_t most = n;
+    most = most > sel_join<32>(most) ? most : sel_join<32>(most);
+    most = tree_most(most);
+    const uint32_t by_records = (most + a.splits - 1) / a.splits;
+    uint32_t c = static_cast<uint32_t>(work / static_cast<float>(most_pairs ? most_pairs : 1));
+    c = (c > by_records ? c : by_records) / unit + 1;
+    c = c > p.least ? c : p.least;
+    uint32_t own = 0, all;
+    for (;; c += c / 16 + 1) {
+        own = tiles * tree_splits(n, c * unit);
+        all = sum(own);
+        if (all <= most_pairs) break;  // (at c past the longest request: its tiles alone)
+    }
+    c *= unit;
+    if (number == 0 && lane == 0) *p.chunk_word = c;  // (every workgroup finds the same)
+    uint32_t upto = own;
+#pragma unroll 1
+    for (uint32_t d = 1; d < 64; d <<= 1) {
+        const uint32_t x = __shfl_up(upto, d);
+        upto += lane >= d ? x : 0u;
+    }
+    const uint64_t here = __ballot(number < upto);
+    if (!here) return false;
+    const uint32_t l = __builtin_ctzll(here), within = number - __builtin_amdgcn_readlane(upto - own, l);
+    const uint32_t of = __builtin_amdgcn_readlane(tiles, l);
+    at->request = l;
+    at->split = within / of;
+    at->tile = within - at->split * of;
+    at->tile_step = 1u << 30;  // (one tile each)
+    at->first = __builtin_amdgcn_readlane(first, l);
+    at->end = __builtin_amdgcn_readlane(end, l);
+    at->chunk = tree_chunk(p, __builtin_amdgcn_readlane(n, l), c);
+    return true;
+}
+
+// The same where there are too many for that.
+__device__ __forceinline__ bool tree_number(const sglkv_tree_params &p, uint32_t number, uint32_t tid, uint32_t lane, tree_place *at) {
+    const sglkv_attn_params &a = p.a;
+    const uint32_t requests = static_cast<uint32_t>(a.request_count), of_slot = requests * a.splits, count = static_cast<uint32_t>(a.query_count);
+    const uint32_t slot = number / of_slot, u = number - slot * of_slot, every = gridDim.x / a.kv_heads;
+    // The workgroup's share of the check that the indices never fall.
+    if (blockIdx.x % a.kv_heads == 0)
+        for (uint64_t q = static_cast<uint64_t>(number) * 256 + tid; q < count; q += static_cast<uint64_t>(every) * 256)
+            if (q && a.query_request_indices[q - 1] > a.query_request_indices[q]) atomicOr(a.flag, SGLKV_FLAG_ATTN_REQUEST);
+    tree_find(a, lane, requests, &at->loose, &at->loose_end);
+    at->loose_end = count;
+    if (slot >= p.tile_slots) return false;
+    at->split = u / requests;
+    at->request = u - at->split * requests;
+    at->tile = slot;
+    at->tile_step = p.tile_slots;
+    at->chunk = tree_chunk(p, tree_tokens(p, at->request), static_cast<uint32_t>(a.chunk_tokens));
+    tree_find(a, lane, at->request, &at->first, &at->end);
+    return true;
+}
+
 // The lane's row number among the tile's and its head: worked out anew (the lane
 // passes through an empty asm) rather than held across the loop.
 template <uint32_t D, uint32_t RW>
-__device__ __forceinline__ uint32_t tree_place(const sglkv_attn_params &a, uint32_t w, uint32_t lane, uint32_t *head) {
+__device__ __forceinline__ uint32_t tree_row_of(const sglkv_attn_params &a, uint32_t w, uint32_t lane, uint32_t *head) {
     typedef tree_tl<D, RW> T;
     asm volatile("" : "+v"(lane));
     const uint32_t r = 32 * (w % T::GW / T::SHARE) + (lane & 31), number = r / a.group;
@@ -551,7 +711,7 @@ __device__ __forceinline__ void tree_write(uint32_t w, uint32_t lane, uint8_t *l
         for (uint32_t i = 0; i < T::OWN; ++i) v[i] = st.o[i / 16][i % 16];
     }
     uint32_t rh;
-    const uint32_t number = tree_place<D, RW>(a, w, lane, &rh);
+    const uint32_t number = tree_row_of<D, RW>(a, w, lane, &rh);
     const tree_row &row = reinterpret_cast<const tree_row *>(lds + T::TABLE)[32 * w + (lane & 31)];
     if (row.reach <= t0 || (only != 0xFFFFFFFFu && number != only)) return;
     const uint64_t qrow = static_cast<uint64_t>(row.query) * a.query_heads + kvh * a.group + rh;
@@ -581,6 +741,35 @@ __device__ __forceinline__ void tree_write(uint32_t w, uint32_t lane, uint8_t *l
         *reinterpret_cast<sglkv_f32x4 *>(out + 8 * i) = sglkv_f32x4{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
 }
 
+// The first two blocks' slots of a wave, into its ring.
+template <uint32_t D, uint32_t RW>
+__device__ __forceinline__ void tree_first_slots(const sglkv_attn_params &a, uint64_t from, uint64_t to, uint32_t t0, uint32_t w,
+                                                 uint32_t lane, uint32_t lds_at) {
+    typedef tree_tl<D, RW> T;
+    const uint64_t base = reinterpret_cast<uint64_t>(a.sequence_slots + from) + 4 * (lane / T::N % 2);
+    const uint32_t last = static_cast<uint32_t>(to - from < 1ull << 31 ? to - from : 1ull << 31) - 1;
+    const uint32_t tb = t0 + w / T::GW * T::B, at = lds_at + T::RING + 512 * w;
+    tree_slots<D, RW>(base, last, tb, w % T::GW, lane, at);
+    tree_slots<D, RW>(base, last, tb + T::B * T::TW, w % T::GW, lane, at + 256);
+}
+
+// The queries of no request: those that attend something are reported, and all give
+// zeros (with several splits the merge writes them). Every workgroup takes a share.
+__device__ __forceinline__ void tree_loose(uint32_t number, uint32_t kvh, uint32_t tid, uint32_t first, uint32_t end) {
+    const sglkv_tree_params &p = tree_params();
+    const sglkv_attn_params &a = p.a;
+    for (uint32_t q = first + number; q < end; q += gridDim.x / a.kv_heads) {
+        if (kvh == 0 && tid == 0) {
+            uint64_t any = a.query_sequence_lengths[q];
+            for (uint32_t i = 0; i < p.mask_words; ++i) any |= p.masks[static_cast<uint64_t>(q) * p.mask_words + i];
+            if (any) atomicOr(a.flag, SGLKV_FLAG_ATTN_REQUEST);
+        }
+        if (a.splits > 1) continue;
+        uint16_t *out = a.output + (static_cast<uint64_t>(q) * a.query_heads + kvh * a.group) * a.dv;
+        for (uint32_t i = 4 * tid; i < a.group * a.dv; i += 1024) *reinterpret_cast<sglkv_u16x4 *>(out + i) = sglkv_u16x4{0, 0, 0, 0};
+    }
+}
+
 template <uint32_t D, uint32_t RW>
 __device__ __forceinline__ void tree_tile_body() {
     typedef tree_tl<D, RW> T;
@@ -589,37 +778,40 @@ __device__ __forceinline__ void tree_tile_body() {
     const sglkv_attn_params &a = p.a;
     uint8_t *lds = tree_tile_lds;
     uint32_t *words = reinterpret_cast<uint32_t *>(lds + T::WORDS);
+    uint64_t *seen = reinterpret_cast<uint64_t *>(lds + T::UNION);
     const uint32_t lds_at = attn_lat_lds_at(lds);
     const uint32_t tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    // Eight (split, request, KV head)s go side by side, one to an XCD, the tiles of each one after another: they
-    // read the same rows.
-    const uint32_t eight = blockIdx.x / 8 / p.tile_slots, slot = blockIdx.x / 8 - eight * p.tile_slots;
-    const uint32_t item = 8 * eight + blockIdx.x % 8, requests = static_cast<uint32_t>(a.request_count);
-    const uint32_t kvh = item % a.kv_heads, of = item / a.kv_heads, split = of / (requests + 1), req = of - split * (requests + 1);
-    if (split >= a.splits) return;
-    const bool known = req < requests, report = (split | kvh) == 0;  // (the request behind the last: queries of no request)
-    uint32_t first, end;
-    tree_find(a, lane, req, &first, &end);
-    if (!known) end = static_cast<uint32_t>(a.query_count);
-    if (report && slot == 0 && known) {
-        // This request's share of the check that the indices never fall.
-        const uint64_t q0 = a.query_count * req / requests, q1 = a.query_count * (req + 1) / requests;
-        for (uint64_t q = q0 + tid; q < q1; q += 256)
-            if (q && a.query_request_indices[q - 1] > a.query_request_indices[q]) atomicOr(a.flag, SGLKV_FLAG_ATTN_REQUEST);
-    }
-    const uint32_t t0 = split * static_cast<uint32_t>(a.chunk_tokens);
-    for (uint32_t q0 = first + slot * p.tile_queries; q0 < end;) {
+    // The KV heads of a tile side by side, one to an XCD where there are eight.
+    const uint32_t number = blockIdx.x / a.kv_heads, kvh = blockIdx.x - number * a.kv_heads;
+    tree_place at = {};
+    const bool any = __builtin_amdgcn_readfirstlane(p.balanced ? tree_balance(p, number, tid, lane, reinterpret_cast<uint32_t *>(lds), &at)
+                                                               : tree_number(p, number, tid, lane, &at));
+    __syncthreads();  // (the list is read: rows go there)
+    if (at.loose < at.loose_end) tree_loose(number, kvh, tid, at.loose, at.loose_end);
+    if (!any) return;
+    auto uniform = [](uint32_t x) { return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(x)); };
+    const uint32_t req = uniform(at.request), split = uniform(at.split), chunk = uniform(at.chunk);
+    const uint32_t t0 = split * chunk;
+    words[19] = chunk;
+    // Held in LDS, not in registers that the loops need; every wave writes them and reads its own.
+    words[16] = uniform(at.end);
+    words[17] = uniform(at.tile_step);
+    for (uint32_t q0 = uniform(at.first + at.tile * p.tile_queries); q0 < uniform(words[16]);) {
         sglkv_u16x8 qf[T::KC];
-        uint32_t nq;
         {
             // The lane's row: its query, head, mask and reach.
             const sglkv_tree_params &p = tree_params();
             const sglkv_attn_params &a = p.a;
-            nq = end - q0 < p.tile_queries ? end - q0 : p.tile_queries;
-            const uint64_t from = known ? a.request_slot_offsets[req] : 0, to = known ? a.request_slot_offsets[req + 1] : 0;
+            const uint32_t left = uniform(words[16]) - q0;
+            const uint32_t nq = left < p.tile_queries ? left : p.tile_queries;
+            words[18] = nq;
+            const uint64_t from = a.request_slot_offsets[req], to = a.request_slot_offsets[req + 1];
+            // The first two blocks' slots, on their way with what says which of them count.
+            if (from < to && to <= a.sequence_slot_count) tree_first_slots<D, RW>(a, from, to, t0, w, lane, lds_at);
+            if (tid < SGLKV_TREE_MAX_WORDS) seen[tid] = 0;
             uint32_t rh;
             tree_row row;
-            row.number = tree_place<D, RW>(a, w, lane, &rh);
+            row.number = tree_row_of<D, RW>(a, w, lane, &rh);
             const bool has = row.number < nq;
             row.query = q0 + (has ? row.number : 0);
             const uint64_t qrow = static_cast<uint64_t>(row.query) * a.query_heads + kvh * a.group + rh;
@@ -639,12 +831,12 @@ __device__ __forceinline__ void tree_tile_body() {
             const bool any = has && (length != 0 || drafts != 0);
             uint32_t bad = 0;
             if (any) {
-                if (!known || index != req)
+                if (index != req)
                     bad = SGLKV_FLAG_ATTN_REQUEST;
                 else if (from > to || to > a.sequence_slot_count || length > to - from || length + drafts > to - from ||
                          length + drafts > p.max_length)
                     bad = SGLKV_FLAG_ATTN_SEQUENCE;
-                if (bad && report) atomicOr(a.flag, bad);
+                if (bad && (split | kvh) == 0) atomicOr(a.flag, bad);
             }
             const bool live = any && !bad;
             row.context = live ? static_cast<uint32_t>(length) : 0;
@@ -657,23 +849,6 @@ __device__ __forceinline__ void tree_tile_body() {
                 for (uint32_t i = 0; i < 4 * T::NT; ++i) *reinterpret_cast<sglkv_u16x4 *>(out + 8 * i) = sglkv_u16x4{0, 0, 0, 0};
             }
         }
-        auto wave_most = [&](uint32_t v) {
-#pragma unroll
-            for (uint32_t d = 1; d < 32; d <<= 1) {
-                const uint32_t x = __shfl_xor(v, d);
-                v = x > v ? x : v;
-            }
-            return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(v));
-        };
-        auto tile_most = [&](uint32_t v) {
-            __syncthreads();  // (the words are no longer read)
-            if (lane == 0) words[w] = v;
-            __syncthreads();
-            uint32_t x = words[0];
-#pragma unroll
-            for (uint32_t i = 1; i < 4; ++i) x = words[i] > x ? words[i] : x;
-            return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(x));
-        };
         // One pass with every row; the tile is done unless its values are not finite. A token that one row attends
         // and another does not has weight 0 in the other's product, and 0 times an infinite or NaN value is NaN. So
         // when a wave whose rows attend different tokens holds an output that is not finite, the queries are done
@@ -681,33 +856,41 @@ __device__ __forceinline__ void tree_tile_body() {
         for (uint32_t only = 0xFFFFFFFFu;;) {
             const sglkv_tree_params &p = tree_params();
             const sglkv_attn_params &a = p.a;
-            const uint32_t chunk = static_cast<uint32_t>(a.chunk_tokens);
             tree_pass pass;
             uint32_t wave_reach, wave_least;
             {
                 const tree_row &row = reinterpret_cast<const tree_row *>(lds + T::TABLE)[32 * w + (lane & 31)];
                 const bool on = row.reach != 0 && (only == 0xFFFFFFFFu || row.number == only);
                 const uint32_t context = row.context;
-                wave_reach = wave_most(on ? row.reach : 0);
-                wave_least = ~wave_most(on ? ~context : 0);
-                const uint32_t farthest = tile_most(wave_reach);
+                // The waves' extremes, exchanged.
+                wave_reach = tree_most(on ? row.reach : 0);
+                const uint32_t most = tree_most(on ? context : 0), least = tree_most(on ? ~context : 0);
+                wave_least = ~least;
+                if (lane == 0) *reinterpret_cast<sglkv_v4u *>(words + 4 * w) = sglkv_v4u{wave_reach, most, least, 0};
+                __syncthreads();
+                sglkv_v4u x = *reinterpret_cast<const sglkv_v4u *>(words);
+#pragma unroll
+                for (uint32_t i = 1; i < 4; ++i) {
+                    const sglkv_v4u y = *reinterpret_cast<const sglkv_v4u *>(words + 4 * i);
+#pragma unroll
+                    for (uint32_t e = 0; e < 3; ++e) x[e] = y[e] > x[e] ? y[e] : x[e];
+                }
+                const uint32_t farthest = __builtin_amdgcn_readfirstlane(x[0]);
+                pass.whole = __builtin_amdgcn_readfirstlane(x[1]);
+                pass.common = ~__builtin_amdgcn_readfirstlane(x[2]);
                 pass.t0 = t0;
-                pass.t1 = farthest <= t0 ? t0 : farthest - t0 < chunk ? farthest : t0 + chunk;
+                pass.t1 = farthest <= t0 ? t0 : farthest - t0 < uniform(words[19]) ? farthest : t0 + uniform(words[19]);
                 if (pass.t1 > t0) {
                     pass.start = a.request_slot_offsets[req];  // (a row reaches into it: the request is one, its range holds)
                     const uint64_t slots = a.request_slot_offsets[req + 1] - pass.start;
                     pass.last = static_cast<uint32_t>(slots < 1ull << 31 ? slots : 1ull << 31) - 1;  // (none behind 2^31 are reached)
-                    pass.whole = tile_most(wave_most(on ? context : 0));
-                    pass.common = ~tile_most(~wave_least);
                     // The drafts behind `whole` that some row attends.
-                    uint64_t *seen = reinterpret_cast<uint64_t *>(lds + T::UNION);
-                    if (tid < SGLKV_TREE_MAX_WORDS) seen[tid] = 0;
-                    __syncthreads();
                     if (on && pass.whole - context < 64 * p.mask_words)
                         for (uint32_t i = 0; i < p.mask_words; ++i) {
                             const uint64_t m = tree_bits(row, pass.whole - context + 64 * i);
                             if (m) atomicOr(reinterpret_cast<unsigned long long *>(seen + i), static_cast<unsigned long long>(m));
                         }
+                    if (only != 0xFFFFFFFFu) tree_first_slots<D, RW>(a, pass.start, pass.start + pass.last + 1, t0, w, lane, lds_at);
                     __syncthreads();
                 }
             }
@@ -725,16 +908,20 @@ __device__ __forceinline__ void tree_tile_body() {
 #pragma unroll
                         for (uint32_t i = 0; i < 16; ++i) odd = __builtin_fmaf(st.o[n][i], 0.0f, odd);
                     const tree_row &row = reinterpret_cast<const tree_row *>(lds + T::TABLE)[32 * w + (lane & 31)];
-                    redo = tile_most(__ballot(odd != 0.0f && row.reach > t0) != 0 ? 1 : 0) != 0;  // (NaN != 0)
+                    redo = __syncthreads_or(odd != 0.0f && row.reach > t0) != 0;  // (NaN != 0)
                 }
                 if (!redo) tree_write<D, RW>(w, lane, lds, kvh, split, t0, only, st);
             }
             if (only == 0xFFFFFFFFu && !redo) break;
-            if (++only == nq) break;  // (from the whole tile to query 0)
+            if (++only == uniform(words[18])) break;  // (from the whole tile to query 0)
+            __syncthreads();
+            if (tid < SGLKV_TREE_MAX_WORDS) seen[tid] = 0;
         }
+        tree_wait<0>();  // (slots that nothing was read for)
         __syncthreads();  // (the next tile's loads go where this one's outputs were joined)
-        const sglkv_tree_params &p = tree_params();
-        q0 += p.tile_slots * p.tile_queries;
+        const uint32_t left = uniform(words[16]) - q0, step = uniform(words[17]);
+        if (step >= left) break;  // (a tile has a query or more)
+        q0 += step * tree_params().tile_queries;
     }
 }
 
@@ -772,7 +959,13 @@ extern "C" __global__ __launch_bounds__(SGLKV_ATTN_COMBINE_THREADS) void sglkv_t
     const bool inside = place.own < place.items && item < a.query_count * a.query_heads;
     tree_query t;
     const bool any = inside && tree_metadata(p, item / a.query_heads, false, &t);
-    const uint32_t used = any ? static_cast<uint32_t>((t.reach + a.chunk_tokens - 1) / a.chunk_tokens) : 0;
+    uint64_t chunk = a.chunk_tokens;
+    if (p.unit && any) {
+        const uint32_t c = p.balanced ? *p.chunk_word : static_cast<uint32_t>(a.chunk_tokens);
+        chunk = tree_chunk(p, tree_tokens(p, a.query_request_indices[item / a.query_heads]), c);
+    }
+    uint32_t used = any ? static_cast<uint32_t>((t.reach + chunk - 1) / chunk) : 0;
+    if (used > a.splits) used = a.splits;  // (indices that fall, which are reported: never past the records)
     const uint64_t i0 = inside ? item * a.splits : 0;
     const float2 *ml = reinterpret_cast<const float2 *>(attn_rec_ml(a, i0));
     const float *o = attn_rec_o(a, i0);

@@ -67,6 +67,11 @@ SHAPES = [
     dict(heads=2, qheads=6, dk=97, contexts=(333, 1), drafts=(11, 3)),
     dict(heads=2, qheads=8, dk=128, shift=2, contexts=(300,), drafts=(16,)),                  # a pool that is not 16-byte aligned
     dict(heads=2, qheads=8, dk=40, hnd=True, contexts=(300, 100), drafts=(16, 2)),
+    dict(heads=2, qheads=8, contexts=(400, 3) * 32, drafts=(7, 2) * 32, padding=3),           # as many requests as one wave has lanes
+    dict(heads=2, qheads=8, contexts=(400, 3, 0, 17, 200) * 14, drafts=(7, 2, 1, 1, 61) * 14, padding=9),      # and more
+    dict(heads=1, qheads=8, dk=64, contexts=(900,) + (1,) * 129, drafts=(120,) + (1,) * 129, hnd=True, spare=1),
+    dict(heads=1, qheads=4, dk=256, contexts=(1,) * 99 + (700,), drafts=(1,) * 99 + (64,)),
+    dict(heads=1, qheads=1, dk=64, contexts=(30, 0, 7, 64, 1), drafts=(1000, 1020, 800, 1024, 700), words=16, spare=1),  # long lists
 ]
 
 
