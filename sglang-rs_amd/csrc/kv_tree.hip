@@ -255,6 +255,24 @@ struct tree_state {
     sglkv_f32x16 o[tree_tl<D, RW>::NT];  // o[n][i]: dim 32n + 8(i/4) + 4(l/32) + i%4 of the wave's dims of the row
 };
 
+// x of lane J of each PIECES lanes.
+template <uint32_t PIECES, uint32_t J>
+__device__ __forceinline__ uint64_t tree_of_lane(uint64_t x) {
+    uint32_t half[2];
+#pragma unroll
+    for (uint32_t e = 0; e < 2; ++e) {
+        const int v = static_cast<int>(x >> (32 * e));
+        if constexpr (PIECES < 16) half[e] = __builtin_amdgcn_ds_swizzle(v, (J << 5) | (32 - PIECES));
+        else half[e] = __builtin_amdgcn_update_dpp(v, v, 0x150 + J, 0xF, 0xF, false);  // (row_newbcast: within 16 lanes)
+    }
+    return static_cast<uint64_t>(half[1]) << 32 | half[0];
+}
+template <uint32_t N, typename F, uint32_t J = 0>
+__device__ __forceinline__ void tree_each(F &f) {
+    f(std::integral_constant<uint32_t, J>());
+    if constexpr (J + 1 < N) tree_each<N, F, J + 1>(f);
+}
+
 // A wave's share of a block's rows into its group's stage, from the slots in its
 // ring. A token that no row attends, or whose slot is outside the pool, reads the
 // zero row.
@@ -263,31 +281,35 @@ __device__ __forceinline__ void tree_issue(const sglkv_attn_params &held, const 
                                            const uint32_t *ring, const uint64_t *seen, uint32_t tb, uint32_t gw, uint32_t lane,
                                            uint32_t stage_at) {
     typedef tree_tl<D, RW> T;
-    const sglkv_attn_params &p = D > 128 && T::TW > 1 ? tree_params().a : held;  // (no scalar registers left to hold them)
+    const sglkv_attn_params &p = D > 64 ? tree_params().a : held;  // (no scalar registers left to hold them)
     if (D > 64) asm volatile("" : "+v"(lane));  // (what it computes from the lane is not held across the block)
-    const uint32_t c = lane / T::PIECES, pos = lane % T::PIECES;
-    const uint64_t zero = reinterpret_cast<uint64_t>(p.zero_row) + 16 * pos;
-    const uint32_t mask = (1u << p.page_shift) - 1, slots = static_cast<uint32_t>(p.slot_count);  // (host: below 2^32)
-    const bool inside = tb + T::B <= pass.t1 && tb + T::B <= pass.whole;
-    uint64_t ka[T::LPW], va[T::LPW];
-#pragma unroll
-    for (uint32_t j = 0; j < T::LPW; ++j) {
-        const uint32_t i = T::TPL * j + c, t = T::N * gw + i, tok = tb + t;
-        const uint32_t low = ring[i], high = ring[T::N + i];
-        bool ok = true;
-        if (!inside) {
-            const uint32_t place = tok - pass.whole;
-            ok = tok < pass.t1 && (tok < pass.whole || (place < 64 * SGLKV_TREE_MAX_WORDS && (seen[place >> 6] >> (place & 63)) & 1));
-        }
-        if (ok && (high != 0 || low >= slots)) {
-            atomicOr(tree_params().a.flag, SGLKV_FLAG_ATTN_SLOT);
-            ok = false;
-        }
-        const uint32_t s = ok ? low : 0u;
-        // K and V share the token's offset (the host's rule, as for paged attention's tiles).
-        const uint64_t off = static_cast<uint64_t>(s >> p.page_shift) * p.page_stride32 + __umul24(s & mask, p.key_token_stride32);
-        attn_sel64x2(ok, kbase + off + 16 * (pos ^ T::A::kswz(t)), vbase + off + 16 * (pos ^ T::A::vswz(t)), zero, ka[j], va[j]);
+    static_assert((T::LPW & (T::LPW - 1)) == 0 && T::LPW <= T::PIECES && T::LPW <= 16, "a lane for each load of a token's lanes");
+    // Load j of a token's PIECES lanes reads the place that lane j of them has worked out.
+    const uint32_t c = lane / T::PIECES, pos = lane % T::PIECES, own = T::TPL * (pos % T::LPW) + c;
+    uint32_t low = ring[own];
+    const uint32_t high = ring[T::N + own], tok = tb + T::N * gw + own;
+    bool ok = true;
+    if (!(tb + T::B <= pass.t1 && tb + T::B <= pass.whole)) {
+        const uint32_t place = tok - pass.whole;
+        ok = tok < pass.t1 && (tok < pass.whole || (place < 64 * SGLKV_TREE_MAX_WORDS && (seen[place >> 6] >> (place & 63)) & 1));
     }
+    if (ok && (high != 0 || low >= static_cast<uint32_t>(p.slot_count))) {  // (host: below 2^32)
+        atomicOr(tree_params().a.flag, SGLKV_FLAG_ATTN_SLOT);
+        ok = false;
+    }
+    low = ok ? low : 0u;
+    // K and V share the token's offset (the host's rule, as for paged attention's tiles).
+    const uint64_t off = static_cast<uint64_t>(low >> p.page_shift) * p.page_stride32 +
+                         __umul24(low & ((1u << p.page_shift) - 1), p.key_token_stride32);
+    const uint64_t zero = reinterpret_cast<uint64_t>(p.zero_row);
+    uint64_t kat, vat, ka[T::LPW], va[T::LPW];
+    attn_sel64x2(ok, kbase + off, vbase + off, zero, kat, vat);
+    auto each = [&](auto j) {
+        const uint32_t t = T::N * gw + T::TPL * j() + c;
+        ka[j()] = tree_of_lane<T::PIECES, j()>(kat) + 16 * (pos ^ T::A::kswz(t));
+        va[j()] = tree_of_lane<T::PIECES, j()>(vat) + 16 * (pos ^ T::A::vswz(t));
+    };
+    tree_each<T::LPW>(each);
     const uint32_t at = stage_at + 1024 * T::LPW * gw;
     tree_load_rows<T::LPW>(ka, at);
     tree_load_rows<T::LPW>(va, at + T::V);
@@ -402,7 +424,7 @@ __device__ __forceinline__ void tree_block(const sglkv_attn_params &p, const uin
             for (uint32_t n = 0; n < 2 * T::NT; ++n) {
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                      // a product
                 __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);                      // an LDS read
-                __builtin_amdgcn_sched_group_barrier(0x402, T::NT == 4 ? 8 : 16, 0);  // vector and exp instructions
+                __builtin_amdgcn_sched_group_barrier(0x402, T::NT == 4 ? 6 : 16, 0);  // vector and exp instructions
             }
         }
     }
@@ -446,43 +468,38 @@ __device__ __forceinline__ void tree_run(const sglkv_tree_params &p, const tree_
     rows(0);
     slots(2);
     rows(1);
-    // Block k's rows have landed; block k + 1's are on their way (the first two blocks' both from the start).
-    auto next = [&](uint32_t k) {
+    tree_wait<2 * T::LPW + 1>();  // block 0's rows have landed; block 1's are on their way
+    if constexpr (T::GW > 1) asm volatile("s_barrier" ::: "memory");
+    for (uint32_t k = 0;;) {
+        if (k < mine) {
+            const uint32_t tb = block(k);
+            const bool masked = tb + T::B > least;
+            uint64_t bits = 0;
+            if (masked) {
+                const tree_row &row = reinterpret_cast<const tree_row *>(lds + T::TABLE)[32 * w + (lane & 31)];
+                if (tb >= row.context) {
+                    bits = tree_bits(row, tb - row.context);
+                } else {
+                    const uint32_t left = row.context - tb;
+                    bits = left >= 64 ? ~0ull : ((1ull << left) - 1) | row.low << left;
+                }
+            }
+            tree_block<D, RW>(a, stage + T::STAGE * (k & 1), qf, bits, masked, lane, gw % T::SHARE, st);
+        }
+        if (++k >= nb) break;
         if constexpr (T::GW == 1) {
             // The wave's own stages: the slots of k + 1 are older than the rows of k.
-            if (k) {
-                tree_wait<2 * T::LPW>();
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // block k - 1's stage is read
-                slots(k + 2);
-                rows(k + 1);
-            }
+            tree_wait<2 * T::LPW>();
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // block k - 1's stage is read
+            slots(k + 2);
+            rows(k + 1);
             tree_wait<2 * T::LPW + 1>();
-        } else if (k == 0) {
-            tree_wait<2 * T::LPW + 1>();
-            asm volatile("s_barrier" ::: "memory");
         } else {
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
             slots(k + 2);
             rows(k + 1);
         }
-    };
-    for (uint32_t k = 0; k < mine; ++k) {
-        next(k);
-        const uint32_t tb = block(k);
-        const bool masked = tb + T::B > least;
-        uint64_t bits = 0;
-        if (masked) {
-            const tree_row &row = reinterpret_cast<const tree_row *>(lds + T::TABLE)[32 * w + (lane & 31)];
-            if (tb >= row.context) {
-                bits = tree_bits(row, tb - row.context);
-            } else {
-                const uint32_t left = row.context - tb;
-                bits = left >= 64 ? ~0ull : ((1ull << left) - 1) | row.low << left;
-            }
-        }
-        tree_block<D, RW>(a, stage + T::STAGE * (k & 1), qf, bits, masked, lane, gw % T::SHARE, st);
     }
-    for (uint32_t k = mine; k < nb; ++k) next(k);
     tree_wait<0>();  // (rows behind the last block, too)
 }
 
@@ -836,13 +853,17 @@ __device__ __forceinline__ void tree_tile_body() {
                 else if (from > to || to > a.sequence_slot_count || length > to - from || length + drafts > to - from ||
                          length + drafts > p.max_length)
                     bad = SGLKV_FLAG_ATTN_SEQUENCE;
-                if (bad && (split | kvh) == 0) atomicOr(a.flag, bad);
+                uint32_t place = split | kvh;
+                asm volatile("" : "+s"(place));  // (no comparison of it held across the loops, nor of w below)
+                if (bad && place == 0) atomicOr(a.flag, bad);
             }
             const bool live = any && !bad;
             row.context = live ? static_cast<uint32_t>(length) : 0;
             row.reach = live ? row.context + drafts : 0;
             reinterpret_cast<tree_row *>(lds + T::TABLE)[32 * w + (lane & 31)] = row;  // (the wave's own: no barrier)
-            if (has && !live && a.splits == 1 && w < T::GW) {
+            uint32_t wave = w;
+            asm volatile("" : "+s"(wave));
+            if (has && !live && a.splits == 1 && wave < T::GW) {
                 // Nothing attended: zeros (with several splits the merge writes them).
                 uint16_t *out = a.output + qrow * D + D / T::SHARE * (w % T::SHARE) + 4 * (lane >> 5);
 #pragma unroll
