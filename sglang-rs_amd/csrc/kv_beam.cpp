@@ -47,6 +47,8 @@ int32_t beam_shape(const sgl_kv_beam_config &c, BeamShape *out) {
     // A dispatch counts its work-items in 32 bits; parents are numbered in 32 bits, too.
     const uint64_t limit = UINT32_MAX / SGLKV_BEAM_THREADS;
     if (h.rows * h.splits > limit) return too_large_dim("workgroups", h.rows * h.splits, limit);
+    const uint64_t joins = UINT32_MAX / SGLKV_BEAM_JOIN_THREADS;
+    if (c.request_count > joins) return too_large_dim("workgroups", c.request_count, joins);
     h.partial_bytes = divide_up(8 * h.rows * h.splits, 64) * 64;
     h.candidate_bytes = 8 * h.rows * h.splits * c.max_kept;
     h.list_bytes = 8 * h.rows * c.max_kept;

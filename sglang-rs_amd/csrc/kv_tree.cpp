@@ -77,11 +77,13 @@ int32_t tile_shape(const sgl_kv_attention_plan_config &c, const sgl_kv_tree_atte
     uint64_t pieces = 2 * divide_up(h.pairs, count * tiles) + 2, numbers = most_tiles + most_tiles / 2;
     if (numbers < h.pairs) numbers = h.pairs;
     if (!h.balanced) {
-        // One length of splits for all, twice the average request's; workgroups for the tiles of twice the average one.
+        // One length of splits for all, twice the average request's and an eighth of the longest's at least; workgroups
+        // for the tiles of twice the average one.
         const uint64_t drafts = 64 * t.mask_words < 2 * mean ? 64 * t.mask_words : 2 * mean;
         h.tile_slots = (uint32_t)divide_up(drafts < c.query_count ? drafts : c.query_count, h.tile_queries);
         w.chunk = 2 * divide_up(c.sequence_slot_count, count);
         if (w.chunk > h.max_length) w.chunk = h.max_length;
+        if (w.chunk < divide_up(h.max_length, 8)) w.chunk = divide_up(h.max_length, 8);
         if (w.chunk < h.unit * h.least) w.chunk = h.unit * h.least;
         pieces = divide_up(h.max_length, w.chunk);
         if (mul_ovf(count, pieces, &numbers) || mul_ovf(numbers, h.tile_slots, &numbers)) return attention_overflow();

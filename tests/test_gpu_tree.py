@@ -75,7 +75,7 @@ SHAPES = [
 ]
 
 
-@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "-".join(f"{a}{b}" for a, b in s.items()).replace(" ", ""))
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "-".join(f"{a}{b}" for a, b in s.items()).replace(" ", "")[:80])
 @pytest.mark.parametrize("hint", [True, False])
 def test_against_the_definition(k, shape, hint):
     """Random trees; the longest reach given or not."""
