@@ -504,7 +504,7 @@ typedef struct sglkv_tree_params {
 #define SGLKV_TREE_BLOCK(d, rows) ((rows) == 4u ? 64u : 32u)
 #define SGLKV_TREE_LDS_BYTES(d, rows)                                                              \
     (2u * (4u / ((rows) * SGLKV_TREE_SHARE(d))) * 4u * (d) * SGLKV_TREE_BLOCK(d, rows) + 2048u +   \
-     8u * (SGLKV_TREE_MAX_WORDS + 2u) + 80u + 4096u)
+     8u * (SGLKV_TREE_MAX_WORDS + 2u) + 96u + 4096u)
 
 /* Accepted drafts' rows, moved together in place. Thread t of a workgroup owns
  * piece t, t + 256, ... of every row of a (request, layer): rows go in the order

@@ -165,8 +165,8 @@ struct tree_tl {
     static constexpr uint32_t OWN = 16 * NT / TW;         // outputs of a lane after the groups are joined
     static constexpr uint32_t RING = 2 * TW * STAGE;      // 256 bytes of raw slots for each wave and stage
     static constexpr uint32_t UNION = RING + 2048;        // which drafts the tile attends at all
-    static constexpr uint32_t WORDS = UNION + 8 * (SGLKV_TREE_MAX_WORDS + 2);  // four words for each wave, and four held
-    static constexpr uint32_t TABLE = WORDS + 80;         // each wave's rows (tree_row)
+    static constexpr uint32_t WORDS = UNION + 8 * (SGLKV_TREE_MAX_WORDS + 2);  // four words for each wave, and eight held
+    static constexpr uint32_t TABLE = WORDS + 96;         // each wave's rows (tree_row)
     static constexpr uint32_t VBUF = D > 128 && TW == 1 ? 1 : 2;  // steps whose values there are registers for
     static_assert(TABLE + 4096 == SGLKV_TREE_LDS_BYTES(D, RW), "the host sizes the same LDS");
     static_assert(N <= 32 && LPW * TPL == N && TW * GW == 4 && OWN * TW == 16 * NT && OWN % 4 == 0, "whole loads and shares");
@@ -215,6 +215,18 @@ __device__ __forceinline__ const sglkv_tree_params &tree_params() {
     kernarg *k = (kernarg *)__builtin_amdgcn_kernarg_segment_ptr();
     asm volatile("" : "+s"(k));
     return *(const sglkv_tree_params *)k;
+}
+
+// Every line of them on its way into the scalar cache at once, where the first use
+// of each would wait for memory by itself.
+__device__ __forceinline__ void tree_touch() {
+    uint32_t x[6];
+    static_assert(sizeof(sglkv_tree_params) > 320 && sizeof(sglkv_tree_params) <= 384, "six lines of 64 bytes");
+    asm volatile(
+        "s_load_dword %0, %6, 0\n\ts_load_dword %1, %6, 64\n\ts_load_dword %2, %6, 128\n\ts_load_dword %3, %6, 192\n\t"
+        "s_load_dword %4, %6, 256\n\ts_load_dword %5, %6, 320\n\ts_waitcnt lgkmcnt(0)"
+        : "=&s"(x[0]), "=&s"(x[1]), "=&s"(x[2]), "=&s"(x[3]), "=&s"(x[4]), "=&s"(x[5])
+        : "s"(__builtin_amdgcn_kernarg_segment_ptr()));
 }
 
 // What a pass over the tile's tokens needs: [t0, t1) of the request, all tokens
@@ -536,6 +548,20 @@ __device__ __forceinline__ uint32_t tree_most(uint32_t x) {
     return tree_join(x, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
 }
 
+__device__ __forceinline__ uint32_t tree_any(uint32_t x) {
+    return tree_join(x, [](uint32_t a, uint32_t b) { return a | b; });
+}
+
+// The sum of x over the lanes up to this one.
+__device__ __forceinline__ uint32_t tree_upto(uint32_t x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);  // (row_shr: within 16 lanes)
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // (the last lane of 16 to the next 16)
+    return x + __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // (lane 31 to the upper half)
+}
+
 // ---- A launch's tiles ----
 //
 // Request r has T_r tiles of its queries and n_r tokens, cut into ceil(n_r / c) even
@@ -549,9 +575,8 @@ __device__ __forceinline__ uint32_t tree_most(uint32_t x) {
 // SGLKV_TREE_BALANCED requests or SGLKV_TREE_LISTED queries c is the host's, and
 // tiles beyond the average request's are taken by the same workgroups.
 
-// The tokens of request r that the launch can reach (its slots, at most max_length).
-__device__ __forceinline__ uint32_t tree_tokens(const sglkv_tree_params &p, uint32_t r) {
-    const uint64_t s = p.a.request_slot_offsets[r], e = p.a.request_slot_offsets[r + 1];
+// The tokens of a request with slots [s, e) that the launch can reach (at most max_length).
+__device__ __forceinline__ uint32_t tree_tokens(const sglkv_tree_params &p, uint64_t s, uint64_t e) {
     const uint64_t n = s <= e && e <= p.a.sequence_slot_count ? e - s : 0;
     return static_cast<uint32_t>(n < p.max_length ? n : p.max_length);
 }
@@ -572,10 +597,11 @@ struct tree_place {
 // request), and whether the indices ever fall.
 __device__ __forceinline__ void tree_list(const sglkv_attn_params &a, uint32_t tid, uint32_t *begins, uint32_t *ends) {
     const uint32_t count = static_cast<uint32_t>(a.query_count), requests = static_cast<uint32_t>(a.request_count);
+    uint32_t i = tid < count ? tid : count - 1;
+    uint32_t x = a.query_request_indices[i], y = a.query_request_indices[i ? i - 1 : 0];  // (on their way over the barrier)
     if (tid <= requests) begins[tid] = ends[tid] = 0;
     __syncthreads();
-    for (uint32_t i = tid; i < count; i += 256) {
-        const uint32_t x = a.query_request_indices[i], y = a.query_request_indices[i ? i - 1 : 0];
+    for (i = tid; i < count;) {
         const uint32_t own = x < requests ? x : requests, before = y < requests ? y : requests;
         if (i == 0 || own != before) {
             begins[own] = i;
@@ -583,6 +609,10 @@ __device__ __forceinline__ void tree_list(const sglkv_attn_params &a, uint32_t t
         }
         if (i + 1 == count) ends[own] = count;
         if (y > x && blockIdx.x == 0) atomicOr(a.flag, SGLKV_FLAG_ATTN_REQUEST);
+        i += 256;
+        if (i >= count) break;
+        x = a.query_request_indices[i];
+        y = a.query_request_indices[i - 1];
     }
     __syncthreads();
 }
@@ -593,8 +623,10 @@ __device__ __forceinline__ bool tree_balance(const sglkv_tree_params &p, uint32_
     const sglkv_attn_params &a = p.a;
     uint32_t *const ends = begins + SGLKV_TREE_BALANCED + 1;
     const uint32_t requests = static_cast<uint32_t>(a.request_count), unit = p.unit;
-    const uint32_t n = lane < requests ? tree_tokens(p, lane) : 0;
+    const uint64_t *const range = a.request_slot_offsets + (lane < requests ? lane : requests - 1);
+    const uint64_t from = range[0], to = range[1];
     tree_list(a, tid, begins, ends);
+    const uint32_t n = lane < requests ? tree_tokens(p, from, to) : 0;
     auto sum = [](uint32_t x) {
         x += sel_join<1>(x);
         x += sel_join<2>(x);
@@ -631,12 +663,7 @@ __device__ __forceinline__ bool tree_balance(const sglkv_tree_params &p, uint32_
     }
     c *= unit;
     if (number == 0 && lane == 0) *p.chunk_word = c;  // (every workgroup finds the same)
-    uint32_t upto = own;
-#pragma unroll 1
-    for (uint32_t d = 1; d < 64; d <<= 1) {
-        const uint32_t x = __shfl_up(upto, d);
-        upto += lane >= d ? x : 0u;
-    }
+    const uint32_t upto = tree_upto(own);
     const uint64_t here = __ballot(number < upto);
     if (!here) return false;
     const uint32_t l = __builtin_ctzll(here), within = number - __builtin_amdgcn_readlane(upto - own, l);
@@ -667,7 +694,8 @@ __device__ __forceinline__ bool tree_number(const sglkv_tree_params &p, uint32_t
     at->request = u - at->split * requests;
     at->tile = slot;
     at->tile_step = p.tile_slots;
-    at->chunk = tree_chunk(p, tree_tokens(p, at->request), static_cast<uint32_t>(a.chunk_tokens));
+    const uint64_t *const range = a.request_slot_offsets + at->request;
+    at->chunk = tree_chunk(p, tree_tokens(p, range[0], range[1]), static_cast<uint32_t>(a.chunk_tokens));
     tree_find(a, lane, at->request, &at->first, &at->end);
     return true;
 }
@@ -747,7 +775,9 @@ __device__ __forceinline__ void tree_write(uint32_t w, uint32_t lane, uint8_t *l
         return;
     }
     const uint64_t rec = qrow * a.splits + split;
-    if (lane < 32 && part == 0 && tw == 0) {
+    uint32_t wave = w;
+    asm volatile("" : "+v"(lane), "+s"(wave));  // (no comparison of them held across the loops)
+    if (lane < 32 && wave < T::GW && wave % T::SHARE == 0) {
         float *ml = attn_rec_ml(a, rec);
         ml[0] = m;
         ml[1] = l;
@@ -791,6 +821,7 @@ template <uint32_t D, uint32_t RW>
 __device__ __forceinline__ void tree_tile_body() {
     typedef tree_tl<D, RW> T;
     extern __shared__ __attribute__((aligned(16))) uint8_t tree_tile_lds[];
+    tree_touch();
     const sglkv_tree_params &p = tree_params();
     const sglkv_attn_params &a = p.a;
     uint8_t *lds = tree_tile_lds;
@@ -822,9 +853,15 @@ __device__ __forceinline__ void tree_tile_body() {
             const uint32_t left = uniform(words[16]) - q0;
             const uint32_t nq = left < p.tile_queries ? left : p.tile_queries;
             words[18] = nq;
-            const uint64_t from = a.request_slot_offsets[req], to = a.request_slot_offsets[req + 1];
+            const uint64_t *const range = a.request_slot_offsets + req;
+            const uint64_t from = range[0], to = range[1];
             // The first two blocks' slots, on their way with what says which of them count.
             if (from < to && to <= a.sequence_slot_count) tree_first_slots<D, RW>(a, from, to, t0, w, lane, lds_at);
+            // For the passes, which look at them where a row reaches into the range, so that it is one. (No slot behind
+            // 2^31 is reached.)
+            words[20] = static_cast<uint32_t>(from);
+            words[21] = static_cast<uint32_t>(from >> 32);
+            words[22] = static_cast<uint32_t>(to - from < 1ull << 31 ? to - from : 1ull << 31) - 1;
             if (tid < SGLKV_TREE_MAX_WORDS) seen[tid] = 0;
             uint32_t rh;
             tree_row row;
@@ -853,9 +890,9 @@ __device__ __forceinline__ void tree_tile_body() {
                 else if (from > to || to > a.sequence_slot_count || length > to - from || length + drafts > to - from ||
                          length + drafts > p.max_length)
                     bad = SGLKV_FLAG_ATTN_SEQUENCE;
-                uint32_t place = split | kvh;
-                asm volatile("" : "+s"(place));  // (no comparison of it held across the loops, nor of w below)
-                if (bad && place == 0) atomicOr(a.flag, bad);
+                uint32_t own = split;
+                asm volatile("" : "+s"(own));  // (no comparison of it held across the loops, nor of w below)
+                if (bad && (own | kvh) == 0) atomicOr(a.flag, bad);
             }
             const bool live = any && !bad;
             row.context = live ? static_cast<uint32_t>(length) : 0;
@@ -902,15 +939,20 @@ __device__ __forceinline__ void tree_tile_body() {
                 pass.t0 = t0;
                 pass.t1 = farthest <= t0 ? t0 : farthest - t0 < uniform(words[19]) ? farthest : t0 + uniform(words[19]);
                 if (pass.t1 > t0) {
-                    pass.start = a.request_slot_offsets[req];  // (a row reaches into it: the request is one, its range holds)
-                    const uint64_t slots = a.request_slot_offsets[req + 1] - pass.start;
-                    pass.last = static_cast<uint32_t>(slots < 1ull << 31 ? slots : 1ull << 31) - 1;  // (none behind 2^31 are reached)
+                    pass.start = static_cast<uint64_t>(uniform(words[21])) << 32 | uniform(words[20]);
+                    pass.last = uniform(words[22]);
                     // The drafts behind `whole` that some row attends.
-                    if (on && pass.whole - context < 64 * p.mask_words)
-                        for (uint32_t i = 0; i < p.mask_words; ++i) {
-                            const uint64_t m = tree_bits(row, pass.whole - context + 64 * i);
-                            if (m) atomicOr(reinterpret_cast<unsigned long long *>(seen + i), static_cast<unsigned long long>(m));
-                        }
+                    for (uint32_t i = 0; i < p.mask_words; ++i) {
+                        uint64_t m = 0;
+                        if (on && pass.whole - context < 64 * p.mask_words) m = tree_bits(row, pass.whole - context + 64 * i);
+                        // (joined over the wave first: the compiler's own way, lane by lane, took 1.5 us)
+                        const uint64_t any = static_cast<uint64_t>(tree_any(static_cast<uint32_t>(m >> 32))) << 32 |
+                                             tree_any(static_cast<uint32_t>(m));
+                        uint32_t l = lane;
+                        asm volatile("" : "+v"(l));
+                        if (any && l == 0)
+                            atomicOr(reinterpret_cast<unsigned long long *>(seen + i), static_cast<unsigned long long>(any));
+                    }
                     if (only != 0xFFFFFFFFu) tree_first_slots<D, RW>(a, pass.start, pass.start + pass.last + 1, t0, w, lane, lds_at);
                     __syncthreads();
                 }
@@ -983,7 +1025,8 @@ extern "C" __global__ __launch_bounds__(SGLKV_ATTN_COMBINE_THREADS) void sglkv_t
     uint64_t chunk = a.chunk_tokens;
     if (p.unit && any) {
         const uint32_t c = p.balanced ? *p.chunk_word : static_cast<uint32_t>(a.chunk_tokens);
-        chunk = tree_chunk(p, tree_tokens(p, a.query_request_indices[item / a.query_heads]), c);
+        const uint64_t *const range = a.request_slot_offsets + a.query_request_indices[item / a.query_heads];
+        chunk = tree_chunk(p, tree_tokens(p, range[0], range[1]), c);
     }
     uint32_t used = any ? static_cast<uint32_t>((t.reach + chunk - 1) / chunk) : 0;
     if (used > a.splits) used = a.splits;  // (indices that fall, which are reported: never past the records)
