@@ -1273,8 +1273,10 @@ typedef struct sgl_kv_tree_attention_buffers {
  * which reaches past its request's slots or past max_sequence_length (SEQUENCE),
  * gives zeros; a token whose slot is outside the pool is reported (SLOT), and the
  * outputs of the queries that attend it are unspecified. Keys and values of tokens
- * that a query does not attend never reach its output, whatever they hold. Softmax
- * statistics and sums are held in 32 bits; the output is rounded to bf16. */
+ * that a query does not attend never reach its output, whatever they hold. An
+ * infinite value that it does attend gives an infinity or NaN (a weight's lo part
+ * may be 0 or negative). Softmax statistics and sums are held in 32 bits; the
+ * output is rounded to bf16. */
 int32_t sgl_rocm_kv_tree_attention(sgl_rocm_kv_ctx *ctx, const sgl_kv_tree_attention_plan *plan,
                                    const sgl_kv_tree_attention_buffers *buffers, void *stream);
 

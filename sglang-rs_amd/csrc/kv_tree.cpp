@@ -58,14 +58,21 @@ int32_t tile_shape(const sgl_kv_attention_plan_config &c, const sgl_kv_tree_atte
               group <= 32 * most && c.slot_count < 1ull << 32 && c.layout.page_stride_bytes <= UINT32_MAX &&
               c.layout.key_row_bytes < 1u << 24 && c.query_count < 1ull << 31;
     if (!h.tiles) return SGL_KV_OK;
-    // Row waves for the rows that a request has on average: fewer leave more token groups.
+    // Row waves: one, with four (at head dim 256 two) token groups, where the launch has few tiles anyway and each is to
+    // be done sooner (one request of up to 4,096 tokens with up to 16 drafts, head dims 64, 128 and 256: 15.4, 19.8 and
+    // 26.5 us, with two 16.6, 22.1 and 30.6; 16 such with 4: 27.7, 41.5 and 87.8, with two 26.2, 38.2 and 65.6). Else two
+    // or four by the rows that a request has on average (64 requests with up to 12 drafts of 4 heads: 76 and 156 us with
+    // two, 82 and 159 with four; with up to 24: 103 and 185 with two, 91 and 171 with four).
     const uint64_t mean = divide_up(c.query_count, c.request_count), rows = mean * group;
-    h.row_waves = rows <= 32 ? 1 : rows <= 64 || most == 2 ? 2 : 4;
+    uint64_t few;
+    h.row_waves = rows <= 32 || most == 2 ? 2 : 4;
+    if (!mul_ovf(c.request_count, divide_up(rows, 32) * c.kv_head_count, &few) && few <= (d > 128 ? 16 : 64)) h.row_waves = 1;
     while (group > 32 * h.row_waves) h.row_waves *= 2;
     h.tile_queries = 32 * h.row_waves / (uint32_t)group;
-    // (Request, split, tile)s: as many as make the workgroups that stay resident at once, or half as many again as the
-    // requests' tiles, so that ragged ones even out. A request has at most twice its even share of splits and two more,
-    // which bounds the records.
+    // (Request, split, tile)s: as many as make the workgroups that stay resident at once, or the multiple of that which
+    // is half as many again as the requests' tiles, so that ragged ones even out (40 requests of 300 to 4,096 tokens: 107
+    // us with 64 a KV head, 128 with 80; 64 requests: 150 with 128, 164 with 96, 173 with 64). A request has at most
+    // twice its even share of splits and two more, which bounds the records.
     const uint64_t groups = 4 / (h.row_waves * SGLKV_TREE_SHARE(d)), count = c.request_count;
     const uint64_t resident = 256 * (d == 128 && h.row_waves == 1 ? 1 : d == 256 && h.row_waves == 1 ? 1 : 2);
     const uint64_t tiles = divide_up(mean, h.tile_queries), most_tiles = c.query_count / h.tile_queries + count;
@@ -74,8 +81,7 @@ int32_t tile_shape(const sgl_kv_attention_plan_config &c, const sgl_kv_tree_atte
     h.balanced = count <= SGLKV_TREE_BALANCED && c.query_count <= SGLKV_TREE_LISTED;
     TreeWay &w = h.tile;
     h.pairs = resident / c.kv_head_count > 1 ? resident / c.kv_head_count : 1;
-    uint64_t pieces = 2 * divide_up(h.pairs, count * tiles) + 2, numbers = most_tiles + most_tiles / 2;
-    if (numbers < h.pairs) numbers = h.pairs;
+    uint64_t pieces = 2 * divide_up(h.pairs, count * tiles) + 2, numbers = divide_up(most_tiles + most_tiles / 2, h.pairs) * h.pairs;
     if (!h.balanced) {
         // One length of splits for all, twice the average request's and an eighth of the longest's at least; workgroups
         // for the tiles of twice the average one.

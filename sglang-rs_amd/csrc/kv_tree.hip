@@ -566,9 +566,9 @@ __device__ __forceinline__ uint32_t tree_upto(uint32_t x) {
 //
 // Request r has T_r tiles of its queries and n_r tokens, cut into ceil(n_r / c) even
 // splits, with the smallest c (whole units: a block for each token group) that leaves
-// at most as many (request, split, tile)s as workgroups are resident at once, whatever
-// the lengths, which the host does not know; they are numbered without a gap, since a
-// workgroup that finds nothing to do holds its place until the ones before it on its
+// at most as many (request, split, tile)s as workgroups are resident at once, or a
+// multiple of that with half as many again as the tiles. The host does not know the
+// lengths. They are numbered without a gap, since a workgroup that finds nothing to do holds its place until the ones before it on its
 // CU are done: 32 requests of 300 to 8,192 tokens took 265 us with every other
 // workgroup empty, 163 us without; with half as many pairs 209, with twice 167.
 // Each workgroup finds c and its own place, a lane to a request. Past
@@ -639,7 +639,8 @@ __device__ __forceinline__ bool tree_balance(const sglkv_tree_params &p, uint32_
     const uint32_t tiles = end > first ? (end - first + p.tile_queries - 1) / p.tile_queries : 0;
     at->loose = __builtin_amdgcn_readfirstlane(begins[requests]);
     at->loose_end = __builtin_amdgcn_readfirstlane(ends[requests]);
-    const uint32_t least_pairs = sum(tiles), most_pairs = p.pairs > least_pairs + least_pairs / 2 ? p.pairs : least_pairs + least_pairs / 2;
+    const uint32_t least_pairs = sum(tiles), fills = (least_pairs + least_pairs / 2 + p.pairs - 1) / p.pairs;
+    const uint32_t most_pairs = p.pairs * (fills ? fills : 1);
     // From what an even share would be (in floats: an estimate), in steps of a sixteenth.
     float work = static_cast<float>(tiles) * static_cast<float>(n);
     work += __uint_as_float(sel_join<1>(__float_as_uint(work)));
@@ -652,7 +653,7 @@ __device__ __forceinline__ bool tree_balance(const sglkv_tree_params &p, uint32_
     most = most > sel_join<32>(most) ? most : sel_join<32>(most);
     most = tree_most(most);
     const uint32_t by_records = (most + a.splits - 1) / a.splits;
-    uint32_t c = static_cast<uint32_t>(work / static_cast<float>(most_pairs ? most_pairs : 1));
+    uint32_t c = static_cast<uint32_t>(work / static_cast<float>(most_pairs));
     c = (c > by_records ? c : by_records) / unit + 1;
     c = c > p.least ? c : p.least;
     uint32_t own = 0, all;
