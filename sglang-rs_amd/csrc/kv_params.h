@@ -568,7 +568,7 @@ typedef struct sglkv_beam_params {
 #define SGLKV_FORK_HEAD_WORDS 32u
 #define SGLKV_FORK_NONE 0xFFFFFFFFu
 #define SGLKV_FORK_SMALL_SEQUENCES 2048u  /* old or new */
-#define SGLKV_FORK_SMALL_ENTRIES 16384u   /* of the old or the new tables */
+#define SGLKV_FORK_SMALL_ENTRIES 8192u    /* of the old or the new tables */
 #define SGLKV_FORK_SMALL_PAGES 262144u
 typedef struct sglkv_page_copy {
     uint32_t source, to;      /* pages */

@@ -69,10 +69,9 @@ int32_t tile_shape(const sgl_kv_attention_plan_config &c, const sgl_kv_tree_atte
     if (!mul_ovf(c.request_count, divide_up(rows, 32) * c.kv_head_count, &few) && few <= (d > 128 ? 16 : 64)) h.row_waves = 1;
     while (group > 32 * h.row_waves) h.row_waves *= 2;
     h.tile_queries = 32 * h.row_waves / (uint32_t)group;
-    // (Request, split, tile)s: as many as make the workgroups that stay resident at once, or the multiple of that which
-    // is half as many again as the requests' tiles, so that ragged ones even out (40 requests of 300 to 4,096 tokens: 107
-    // us with 64 a KV head, 128 with 80; 64 requests: 150 with 128, 164 with 96, 173 with 64). A request has at most
-    // twice its even share of splits and two more, which bounds the records.
+    // (Request, split, tile)s: as many as make the workgroups that stay resident at once, or a multiple of that (40
+    // requests of 300 to 4,096 tokens: 107 us with 64 a KV head, 128 with 80). A request has at most twice its even share
+    // of splits and two more, which bounds the records.
     const uint64_t groups = 4 / (h.row_waves * SGLKV_TREE_SHARE(d)), count = c.request_count;
     const uint64_t resident = 256 * (d == 128 && h.row_waves == 1 ? 1 : d == 256 && h.row_waves == 1 ? 1 : 2);
     const uint64_t tiles = divide_up(mean, h.tile_queries), most_tiles = c.query_count / h.tile_queries + count;
@@ -81,7 +80,8 @@ int32_t tile_shape(const sgl_kv_attention_plan_config &c, const sgl_kv_tree_atte
     h.balanced = count <= SGLKV_TREE_BALANCED && c.query_count <= SGLKV_TREE_LISTED;
     TreeWay &w = h.tile;
     h.pairs = resident / c.kv_head_count > 1 ? resident / c.kv_head_count : 1;
-    uint64_t pieces = 2 * divide_up(h.pairs, count * tiles) + 2, numbers = divide_up(most_tiles + most_tiles / 2, h.pairs) * h.pairs;
+    uint64_t pieces = 2 * divide_up(h.pairs, count * tiles) + 2, numbers = divide_up(most_tiles, h.pairs) * h.pairs;
+    if (2 * most_tiles > h.pairs) numbers += h.pairs;
     if (!h.balanced) {
         // One length of splits for all, twice the average request's and an eighth of the longest's at least; workgroups
         // for the tiles of twice the average one.

@@ -566,11 +566,16 @@ __device__ __forceinline__ uint32_t tree_upto(uint32_t x) {
 //
 // Request r has T_r tiles of its queries and n_r tokens, cut into ceil(n_r / c) even
 // splits, with the smallest c (whole units: a block for each token group) that leaves
-// at most as many (request, split, tile)s as workgroups are resident at once, or a
-// multiple of that with half as many again as the tiles. The host does not know the
-// lengths. They are numbered without a gap, since a workgroup that finds nothing to do holds its place until the ones before it on its
+// at most as many (request, split, tile)s as w times the workgroups resident at once.
+// w is the least that holds the tiles, or one more where there are tiles for half the
+// workgroups and the longer way takes less, at 10 blocks for what a workgroup does
+// before its first and the mean share and half a split in place of a split where they
+// follow each other (64 requests of 300 to 4,096 tokens with up to 12 drafts: 161 us
+// with w = 1, 148 with 2; 30 of 300 to 2,000 with up to 120: 124 and 147). The host
+// does not know the lengths. They are numbered without a gap, since a workgroup that finds nothing to do holds its place until the ones before it on its
 // CU are done: 32 requests of 300 to 8,192 tokens took 265 us with every other
 // workgroup empty, 163 us without; with half as many pairs 209, with twice 167.
+// A request of one split has its outputs from there; the others' are merged.
 // Each workgroup finds c and its own place, a lane to a request. Past
 // SGLKV_TREE_BALANCED requests or SGLKV_TREE_LISTED queries c is the host's, and
 // tiles beyond the average request's are taken by the same workgroups.
@@ -588,31 +593,43 @@ __device__ __forceinline__ uint32_t tree_chunk(const sglkv_tree_params &p, uint3
 }
 
 // A workgroup's place: its request's queries [first, end) from tile `tile` on, every
-// tile_step-th, and the split. Queries [loose, loose_end) belong to no request.
+// tile_step-th, and the split (alone: there is one, whose outputs need no merge).
+// Queries [loose, loose_end) belong to no request.
 struct tree_place {
-    uint32_t request, split, chunk, first, end, tile, tile_step, loose, loose_end;
+    uint32_t request, split, chunk, first, end, tile, tile_step, loose, loose_end, alone;
 };
 
 // Where each request's queries begin and end, in LDS (the last entry: those of no
 // request), and whether the indices ever fall.
 __device__ __forceinline__ void tree_list(const sglkv_attn_params &a, uint32_t tid, uint32_t *begins, uint32_t *ends) {
     const uint32_t count = static_cast<uint32_t>(a.query_count), requests = static_cast<uint32_t>(a.request_count);
-    uint32_t i = tid < count ? tid : count - 1;
-    uint32_t x = a.query_request_indices[i], y = a.query_request_indices[i ? i - 1 : 0];  // (on their way over the barrier)
+    constexpr uint32_t U = 4;
+    uint32_t x[U], y[U];
+    auto load = [&](uint32_t i0) {
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) {
+            const uint32_t at = i0 + 256 * u + tid, i = at < count ? at : count - 1;
+            x[u] = a.query_request_indices[i];
+            y[u] = a.query_request_indices[i ? i - 1 : 0];
+        }
+    };
+    load(0);  // (on their way over the barrier)
     if (tid <= requests) begins[tid] = ends[tid] = 0;
     __syncthreads();
-    for (i = tid; i < count;) {
-        const uint32_t own = x < requests ? x : requests, before = y < requests ? y : requests;
-        if (i == 0 || own != before) {
-            begins[own] = i;
-            if (i) ends[before] = i;
+    for (uint32_t i0 = 0; i0 < count;) {
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) {
+            const uint32_t i = i0 + 256 * u + tid, own = x[u] < requests ? x[u] : requests, before = y[u] < requests ? y[u] : requests;
+            if (i >= count) continue;
+            if (i == 0 || own != before) {
+                begins[own] = i;
+                if (i) ends[before] = i;
+            }
+            if (i + 1 == count) ends[own] = count;
+            if (y[u] > x[u] && blockIdx.x == 0) atomicOr(a.flag, SGLKV_FLAG_ATTN_REQUEST);
         }
-        if (i + 1 == count) ends[own] = count;
-        if (y > x && blockIdx.x == 0) atomicOr(a.flag, SGLKV_FLAG_ATTN_REQUEST);
-        i += 256;
-        if (i >= count) break;
-        x = a.query_request_indices[i];
-        y = a.query_request_indices[i - 1];
+        i0 += 256 * U;
+        if (i0 < count) load(i0);
     }
     __syncthreads();
 }
@@ -639,9 +656,7 @@ __device__ __forceinline__ bool tree_balance(const sglkv_tree_params &p, uint32_
     const uint32_t tiles = end > first ? (end - first + p.tile_queries - 1) / p.tile_queries : 0;
     at->loose = __builtin_amdgcn_readfirstlane(begins[requests]);
     at->loose_end = __builtin_amdgcn_readfirstlane(ends[requests]);
-    const uint32_t least_pairs = sum(tiles), fills = (least_pairs + least_pairs / 2 + p.pairs - 1) / p.pairs;
-    const uint32_t most_pairs = p.pairs * (fills ? fills : 1);
-    // From what an even share would be (in floats: an estimate), in steps of a sixteenth.
+    const uint32_t all_tiles = sum(tiles), fills = all_tiles > p.pairs ? (all_tiles + p.pairs - 1) / p.pairs : 1;
     float work = static_cast<float>(tiles) * static_cast<float>(n);
     work += __uint_as_float(sel_join<1>(__float_as_uint(work)));
     work += __uint_as_float(sel_join<2>(__float_as_uint(work)));
@@ -652,15 +667,24 @@ __device__ __forceinline__ bool tree_balance(const sglkv_tree_params &p, uint32_
     uint32_t most = n;
     most = most > sel_join<32>(most) ? most : sel_join<32>(most);
     most = tree_most(most);
-    const uint32_t by_records = (most + a.splits - 1) / a.splits;
-    uint32_t c = static_cast<uint32_t>(work / static_cast<float>(most_pairs));
-    c = (c > by_records ? c : by_records) / unit + 1;
-    c = c > p.least ? c : p.least;
-    uint32_t own = 0, all;
-    for (;; c += c / 16 + 1) {
-        own = tiles * tree_splits(n, c * unit);
-        all = sum(own);
-        if (all <= most_pairs) break;  // (at c past the longest request: its tiles alone)
+    const uint32_t by_records = ((most + a.splits - 1) / a.splits) / unit + 1;
+    const uint32_t share = static_cast<uint32_t>(work / static_cast<float>(p.pairs)) / unit;
+    uint32_t c = 0, own = 0;
+    for (uint32_t w = fills, best = 0xFFFFFFFFu; w <= (2 * all_tiles > p.pairs ? fills + 1 : fills); ++w) {
+        // From what an even share would be, in steps of a sixteenth.
+        uint32_t d = share / w + 1, count;
+        d = d > by_records ? d : by_records;
+        d = d > p.least ? d : p.least;
+        for (;; d += d / 16 + 1) {
+            count = tiles * tree_splits(n, d * unit);
+            if (sum(count) <= p.pairs * w) break;  // (at d past the longest request: the tiles alone)
+        }
+        const uint32_t cost = (w == 1 ? d : share + d / 2) + 10 * w;
+        if (cost < best) {
+            best = cost;
+            c = d;
+            own = count;
+        }
     }
     c *= unit;
     if (number == 0 && lane == 0) *p.chunk_word = c;  // (every workgroup finds the same)
@@ -676,6 +700,7 @@ __device__ __forceinline__ bool tree_balance(const sglkv_tree_params &p, uint32_
     at->first = __builtin_amdgcn_readlane(first, l);
     at->end = __builtin_amdgcn_readlane(end, l);
     at->chunk = tree_chunk(p, __builtin_amdgcn_readlane(n, l), c);
+    at->alone = __builtin_amdgcn_readlane(n, l) <= c;
     return true;
 }
 
@@ -696,7 +721,9 @@ __device__ __forceinline__ bool tree_number(const sglkv_tree_params &p, uint32_t
     at->tile = slot;
     at->tile_step = p.tile_slots;
     const uint64_t *const range = a.request_slot_offsets + at->request;
-    at->chunk = tree_chunk(p, tree_tokens(p, range[0], range[1]), static_cast<uint32_t>(a.chunk_tokens));
+    const uint32_t n = tree_tokens(p, range[0], range[1]), c = static_cast<uint32_t>(a.chunk_tokens);
+    at->chunk = tree_chunk(p, n, c);
+    at->alone = n <= c;
     tree_find(a, lane, at->request, &at->first, &at->end);
     return true;
 }
@@ -763,7 +790,7 @@ __device__ __forceinline__ void tree_write(uint32_t w, uint32_t lane, uint8_t *l
     const uint64_t qrow = static_cast<uint64_t>(row.query) * a.query_heads + kvh * a.group + rh;
     // Value 4 i + e of the lane: dim 8 (i + OWN tw / 4) + 4 (lane / 32) + e of the wave's dims.
     const uint32_t dim = D / T::SHARE * part + 2 * T::OWN * tw + 4 * (lane >> 5);
-    if (a.splits == 1) {
+    if (__builtin_amdgcn_readfirstlane(reinterpret_cast<const uint32_t *>(lds + T::WORDS)[23])) {  // (its request is not split)
         const float linv = 1.0f / l;
         uint16_t *out = a.output + qrow * D + dim;
 #pragma unroll
@@ -842,6 +869,7 @@ __device__ __forceinline__ void tree_tile_body() {
     const uint32_t req = uniform(at.request), split = uniform(at.split), chunk = uniform(at.chunk);
     const uint32_t t0 = split * chunk;
     words[19] = chunk;
+    words[23] = uniform(at.alone);
     // Held in LDS, not in registers that the loops need; every wave writes them and reads its own.
     words[16] = uniform(at.end);
     words[17] = uniform(at.tile_step);
@@ -901,8 +929,8 @@ __device__ __forceinline__ void tree_tile_body() {
             reinterpret_cast<tree_row *>(lds + T::TABLE)[32 * w + (lane & 31)] = row;  // (the wave's own: no barrier)
             uint32_t wave = w;
             asm volatile("" : "+s"(wave));
-            if (has && !live && a.splits == 1 && wave < T::GW) {
-                // Nothing attended: zeros (with several splits the merge writes them).
+            if (has && !live && uniform(words[23]) && wave < T::GW) {
+                // Nothing attended: zeros (those of requests that are split are the merge's).
                 uint16_t *out = a.output + qrow * D + D / T::SHARE * (w % T::SHARE) + 4 * (lane >> 5);
 #pragma unroll
                 for (uint32_t i = 0; i < 4 * T::NT; ++i) *reinterpret_cast<sglkv_u16x4 *>(out + 8 * i) = sglkv_u16x4{0, 0, 0, 0};
@@ -1024,12 +1052,15 @@ extern "C" __global__ __launch_bounds__(SGLKV_ATTN_COMBINE_THREADS) void sglkv_t
     tree_query t;
     const bool any = inside && tree_metadata(p, item / a.query_heads, false, &t);
     uint64_t chunk = a.chunk_tokens;
+    bool whole = false;  // one split, which has written the output
     if (p.unit && any) {
         const uint32_t c = p.balanced ? *p.chunk_word : static_cast<uint32_t>(a.chunk_tokens);
         const uint64_t *const range = a.request_slot_offsets + a.query_request_indices[item / a.query_heads];
-        chunk = tree_chunk(p, tree_tokens(p, range[0], range[1]), c);
+        const uint32_t n = tree_tokens(p, range[0], range[1]);
+        chunk = tree_chunk(p, n, c);
+        whole = n <= c;
     }
-    uint32_t used = any ? static_cast<uint32_t>((t.reach + chunk - 1) / chunk) : 0;
+    uint32_t used = any && !whole ? static_cast<uint32_t>((t.reach + chunk - 1) / chunk) : 0;
     if (used > a.splits) used = a.splits;  // (indices that fall, which are reported: never past the records)
     const uint64_t i0 = inside ? item * a.splits : 0;
     const float2 *ml = reinterpret_cast<const float2 *>(attn_rec_ml(a, i0));
@@ -1061,7 +1092,7 @@ extern "C" __global__ __launch_bounds__(SGLKV_ATTN_COMBINE_THREADS) void sglkv_t
             }
             __syncthreads();  // (the shares are read before the next dims' are written)
         }
-        if (!inside || !place.merges) continue;
+        if (!inside || whole || !place.merges) continue;
         const float linv = any ? 1.0f / l : 0.0f;
 #pragma unroll
         for (uint32_t e = 0; e < 4; ++e)
