@@ -491,7 +491,7 @@ typedef struct sglkv_tree_params {
     uint32_t balanced;        /* tiles: the workgroups find the splits themselves */
     uint32_t unit;            /* tiles: tokens of a block for each token group (0: the generic body) */
     uint32_t least;           /* tiles: units of a split or more */
-    uint32_t *chunk_word;     /* tiles: the tokens of a split that the workgroups found */
+    uint32_t *used;           /* tiles: [query] records of each head, or SGLKV_SELECT_NONE: its outputs are there */
 } sglkv_tree_params;
 #define SGLKV_TREE_MAX_WORDS 16u
 #define SGLKV_TREE_BALANCED 64u   /* most requests whose splits are found on the device ... */

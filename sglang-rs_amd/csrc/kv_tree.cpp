@@ -28,7 +28,7 @@ struct TreeShape {
     bool tiles;
     uint32_t row_waves, tile_queries, tile_slots, unit, least;
     bool balanced;
-    uint64_t pairs;
+    uint64_t pairs, used_at;
     TreeWay tile;
 };
 
@@ -102,7 +102,8 @@ int32_t tile_shape(const sgl_kv_attention_plan_config &c, const sgl_kv_tree_atte
         h.tiles = false;
         return SGL_KV_OK;
     }
-    w.record_bytes += 64;  // the word that the workgroups leave for the merge
+    h.used_at = w.record_bytes;  // (whole records: a multiple of 4)
+    if (add_ovf(w.record_bytes, 4 * c.query_count, &w.record_bytes)) return attention_overflow();
     h.tiles = w.base <= UINT32_MAX / 256;
     return SGL_KV_OK;
 }
@@ -225,7 +226,7 @@ extern "C" int32_t sgl_rocm_kv_tree_attention(sgl_rocm_kv_ctx *ctx, const sgl_kv
         p.balanced = shape.balanced;
         p.unit = shape.unit;
         p.least = shape.least;
-        p.chunk_word = reinterpret_cast<uint32_t *>(workspace + way.record_bytes - 64);
+        p.used = reinterpret_cast<uint32_t *>(workspace + shape.used_at);
         const int dims = p.a.dk == 64 ? 0 : p.a.dk == 128 ? 1 : 2, rows = shape.row_waves == 1 ? 0 : shape.row_waves == 2 ? 1 : 2;
         rc = launch_kernel(ctx->tree_tile[dims][rows], way.base, 1, 1, 256, SGLKV_TREE_LDS_BYTES(p.a.dk, shape.row_waves), s, &p,
                            "tree attention launch");

@@ -687,7 +687,6 @@ __device__ __forceinline__ bool tree_balance(const sglkv_tree_params &p, uint32_
         }
     }
     c *= unit;
-    if (number == 0 && lane == 0) *p.chunk_word = c;  // (every workgroup finds the same)
     const uint32_t upto = tree_upto(own);
     const uint64_t here = __ballot(number < upto);
     if (!here) return false;
@@ -839,6 +838,7 @@ __device__ __forceinline__ void tree_loose(uint32_t number, uint32_t kvh, uint32
             for (uint32_t i = 0; i < p.mask_words; ++i) any |= p.masks[static_cast<uint64_t>(q) * p.mask_words + i];
             if (any) atomicOr(a.flag, SGLKV_FLAG_ATTN_REQUEST);
         }
+        if (kvh == 0 && tid == 0) p.used[q] = 0;
         if (a.splits > 1) continue;
         uint16_t *out = a.output + (static_cast<uint64_t>(q) * a.query_heads + kvh * a.group) * a.dv;
         for (uint32_t i = 4 * tid; i < a.group * a.dv; i += 1024) *reinterpret_cast<sglkv_u16x4 *>(out + i) = sglkv_u16x4{0, 0, 0, 0};
@@ -906,6 +906,8 @@ __device__ __forceinline__ void tree_tile_body() {
 #pragma unroll
             for (uint32_t c = 0; c < T::KC; ++c)
                 qf[c] = *reinterpret_cast<const sglkv_u16x8 *>(a.queries + qrow * D + 16 * c + 8 * (lane >> 5));
+            uint32_t wave = w, own = split;
+            asm volatile("" : "+s"(wave), "+s"(own));  // (no comparison of them held across the loops)
             uint32_t drafts = row.high ? 128 - __builtin_clzll(row.high) : row.low ? 64 - __builtin_clzll(row.low) : 0;
             for (uint32_t i = 2; i < p.mask_words; ++i) {
                 const uint64_t m = mask[i];
@@ -919,16 +921,17 @@ __device__ __forceinline__ void tree_tile_body() {
                 else if (from > to || to > a.sequence_slot_count || length > to - from || length + drafts > to - from ||
                          length + drafts > p.max_length)
                     bad = SGLKV_FLAG_ATTN_SEQUENCE;
-                uint32_t own = split;
-                asm volatile("" : "+s"(own));  // (no comparison of it held across the loops, nor of w below)
                 if (bad && (own | kvh) == 0) atomicOr(a.flag, bad);
             }
             const bool live = any && !bad;
+            // What the merge needs to know of each query: its records, or that its outputs are there.
+            if (has && rh == 0 && (own | kvh) == 0 && wave < T::GW)
+                tree_params().used[row.query] = uniform(words[23]) ? SGLKV_SELECT_NONE
+                                    : live             ? (static_cast<uint32_t>(length) + drafts + uniform(words[19]) - 1) / uniform(words[19])
+                                                       : 0u;
             row.context = live ? static_cast<uint32_t>(length) : 0;
             row.reach = live ? row.context + drafts : 0;
             reinterpret_cast<tree_row *>(lds + T::TABLE)[32 * w + (lane & 31)] = row;  // (the wave's own: no barrier)
-            uint32_t wave = w;
-            asm volatile("" : "+s"(wave));
             if (has && !live && uniform(words[23]) && wave < T::GW) {
                 // Nothing attended: zeros (those of requests that are split are the merge's).
                 uint16_t *out = a.output + qrow * D + D / T::SHARE * (w % T::SHARE) + 4 * (lane >> 5);
@@ -1049,19 +1052,19 @@ extern "C" __global__ __launch_bounds__(SGLKV_ATTN_COMBINE_THREADS) void sglkv_t
     const uint32_t lanes = place.lanes, per = place.per, sub = place.sub;
     const uint64_t item = static_cast<uint64_t>(blockIdx.x) * place.items + place.own;
     const bool inside = place.own < place.items && item < a.query_count * a.query_heads;
-    tree_query t;
-    const bool any = inside && tree_metadata(p, item / a.query_heads, false, &t);
-    uint64_t chunk = a.chunk_tokens;
+    uint32_t used = 0;
     bool whole = false;  // one split, which has written the output
-    if (p.unit && any) {
-        const uint32_t c = p.balanced ? *p.chunk_word : static_cast<uint32_t>(a.chunk_tokens);
-        const uint64_t *const range = a.request_slot_offsets + a.query_request_indices[item / a.query_heads];
-        const uint32_t n = tree_tokens(p, range[0], range[1]);
-        chunk = tree_chunk(p, n, c);
-        whole = n <= c;
+    if (p.unit) {
+        // (The tiles have left it: going over the query's metadata again took as long as the merge.)
+        if (inside) used = p.used[item / a.query_heads];
+        whole = used == SGLKV_SELECT_NONE;
+        if (whole) used = 0;
+        if (used > a.splits) used = a.splits;  // (indices that fall, which are reported: never past the records)
+    } else {
+        tree_query t;
+        if (inside && tree_metadata(p, item / a.query_heads, false, &t)) used = static_cast<uint32_t>((t.reach + a.chunk_tokens - 1) / a.chunk_tokens);
     }
-    uint32_t used = any && !whole ? static_cast<uint32_t>((t.reach + chunk - 1) / chunk) : 0;
-    if (used > a.splits) used = a.splits;  // (indices that fall, which are reported: never past the records)
+    const bool any = used != 0;
     const uint64_t i0 = inside ? item * a.splits : 0;
     const float2 *ml = reinterpret_cast<const float2 *>(attn_rec_ml(a, i0));
     const float *o = attn_rec_o(a, i0);
