@@ -4,7 +4,12 @@
 // Within a beam the order is that of its logits, so a row needs its K largest
 // logits, their maximum m and l = sum exp(x - m): one pass over the data. A
 // workgroup reads a split of a row into registers; the splits' results, K of them
-// each, are joined by one workgroup a request in 64 bits.
+// each, are joined by one workgroup a request in 64 bits. What can be among the K is
+// found by a bound (the K-th largest of the threads' maxima) and ranked, where K
+// rounds of maxima took 99 us for 64 requests of 4 beams, 128,256 tokens and K = 8:
+// now 16.6 (66 MB, 4.0 TB/s; loads and what is counted of each logit share the time)
+// and 5.6 for the join; 1 request of 4 beams of 32,000: 5.7 and 5.1, each a chain of
+// joins over lanes, LDS and barriers.
 
 namespace {
 
