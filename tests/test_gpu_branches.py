@@ -350,6 +350,17 @@ def test_long_tables(k):
     k.check_errors()
 
 
+@pytest.mark.parametrize("pages", [262144, 262145])
+def test_many_pages(k, pages):
+    """As many pages as one workgroup has bits for, and one more."""
+    rng = np.random.default_rng(28)
+    pool = Bytes(rng, page=2, pages=pages, layers=1, heads=1, widths=(4,))
+    case = Forks(rng, pool, [801, 500, 33, 2000], [0, 0, 1, 1], [1, 1, NONE, 3], append=3, spare=100)
+    _say(f"fork_sequences over {pages} pages")
+    _same(case.run(k), case.want())
+    k.check_errors()
+
+
 def test_a_chain_of_steps(k):
     """Steps in a row without a wait, each on the tables that the one before wrote."""
     rng = np.random.default_rng(27)
