@@ -498,8 +498,8 @@ typedef struct sglkv_tree_params {
 #define SGLKV_TREE_LISTED 4096u   /* ... and most queries */
 /* Tiles: head dims d, `rows` row waves (32 rows each) of the workgroup's four.
  * Tokens of a block; LDS: two stages of K and V rows for each token group, the
- * raw slots of two blocks a wave (2 KiB), the drafts that the tile attends, a
- * word for each wave, and each wave's rows (4 KiB). */
+ * raw slots of two blocks a wave (2 KiB), the drafts that the tile attends, 24
+ * words that the waves share, and each wave's rows (4 KiB). */
 #define SGLKV_TREE_SHARE(d) ((d) > 128u ? 2u : 1u)
 #define SGLKV_TREE_BLOCK(d, rows) ((rows) == 4u ? 64u : 32u)
 #define SGLKV_TREE_LDS_BYTES(d, rows)                                                              \
@@ -558,7 +558,7 @@ typedef struct sglkv_beam_params {
     uint32_t rounds;          /* of a split */
 } sglkv_beam_params;
 
-/* Forks. The workspace: word 0 is the plan's verdict (1: carried out), word 1 the
+/* Forks. The workspace: word 0 says whether the plan holds (1: carried out), word 1 the
  * pages taken, word 2 the copies; then each parent's lowest child and number of
  * children, each sequence's first new page's number, the copies, and a bit for
  * each page that is freed. Few sequences and pages (SGLKV_FORK_SMALL_*) are kept
