@@ -71,6 +71,10 @@ SHAPES = [
     dict(heads=2, qheads=8, contexts=(400, 3, 0, 17, 200) * 14, drafts=(7, 2, 1, 1, 61) * 14, padding=9),      # and more
     dict(heads=1, qheads=8, dk=64, contexts=(900,) + (1,) * 129, drafts=(120,) + (1,) * 129, hnd=True, spare=1),
     dict(heads=1, qheads=4, dk=256, contexts=(1,) * 99 + (700,), drafts=(1,) * 99 + (64,)),
+    dict(heads=1, qheads=128, contexts=(300, 20), drafts=(9, 40)),                            # a query to a tile
+    dict(heads=1, qheads=64, dk=256, contexts=(300, 20), drafts=(9, 40), hnd=True),
+    dict(heads=600, qheads=600, dk=64, page=1, contexts=(70, 5), drafts=(9, 3)),              # more KV heads than workgroups at once
+    dict(heads=8, qheads=32, page=64, contexts=(9000,), drafts=(3,), padding=2),              # one long request
     dict(heads=1, qheads=1, dk=64, contexts=(30, 0, 7, 64, 1), drafts=(1000, 1020, 800, 1024, 700), words=16, spare=1),  # long lists
 ]
 
