@@ -1315,11 +1315,14 @@ __device__ __forceinline__ void attn_lat_load(uint64_t src, const uint8_t *dst) 
         : "v"(src), "s"(attn_lat_lds_at(dst)));
 }
 
-// ok ? a : z per lane, as two v_cndmask_b32 (see attn_sel64x2).
+// ok ? a : z per lane, as two v_cndmask_b32 (see attn_sel64x2). gfx950 wants two
+// wait states between a vector instruction that writes VCC and one that reads it,
+// which the compiler puts between its own instructions but not into these: without
+// them a select may take the lanes that an earlier compare left in VCC.
 __device__ __forceinline__ uint64_t attn_sel64(bool ok, uint64_t a, uint64_t z) {
     const uint32_t m = ok ? 1u : 0u;
     uint32_t xl, xh;
-    asm("v_cmp_ne_u32 vcc, 0, %2\n\t"
+    asm("v_cmp_ne_u32 vcc, 0, %2\n\ts_nop 1\n\t"
         "v_cndmask_b32 %0, %3, %4, vcc\n\t"
         "v_cndmask_b32 %1, %5, %6, vcc"
         : "=&v"(xl), "=&v"(xh)
@@ -1349,7 +1352,7 @@ __device__ __forceinline__ void attn_sel64x2(bool ok, uint64_t a, uint64_t b, ui
                                              uint64_t &y) {
     const uint32_t m = ok ? 1u : 0u;
     uint32_t xl, xh, yl, yh;
-    asm("v_cmp_ne_u32 vcc, 0, %4\n\t"
+    asm("v_cmp_ne_u32 vcc, 0, %4\n\ts_nop 1\n\t"
         "v_cndmask_b32 %0, %5, %6, vcc\n\t"
         "v_cndmask_b32 %1, %7, %8, vcc\n\t"
         "v_cndmask_b32 %2, %5, %9, vcc\n\t"
