@@ -1419,9 +1419,11 @@ typedef struct sgl_kv_fork_buffers {
 /* Every old sequence ends, and sequence s goes on from sequence parents[s], whose
  * tokens it has: forked_lengths[s] = lengths[parents[s]], or 0 and a row of -1
  * where parents[s] is UINT32_MAX. Its full pages are its parent's. A last page
- * that is not full is taken over by the lowest s of that parent; the others get a
- * page of their own with its rows so far (every tensor of `layer_count` layers,
- * `pool` and layer_stride as for keep_drafts). Pages for append_tokens more tokens
+ * that is not full is taken over by the lowest s of that parent, if the parent
+ * alone holds it (page_references 1 before the call); the others, or all where
+ * another sequence or the caller holds it too, get a page of their own with its
+ * rows so far (every tensor of `layer_count` layers, `pool` and layer_stride as
+ * for keep_drafts). Pages for append_tokens more tokens
  * follow. The k-th new page of the call (by sequence, then by place in the row) is
  * free_pages[free_count - 1 - k]. page_references follow the tables; pages whose
  * count falls to 0 are appended to free_pages in ascending order, behind what is

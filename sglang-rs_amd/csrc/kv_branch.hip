@@ -119,8 +119,9 @@ struct brn_need {
     uint32_t parent, fresh;  // fresh: new pages, a copied last page first among them
     bool copies;
 };
-// `first`: the sequence is its parent's lowest child.
-__device__ __forceinline__ brn_need brn_sequence(const sglkv_fork_params &p, uint32_t parent, uint64_t length, bool first) {
+// `takes`: the sequence takes over its parent's last page, as the lowest child of a
+// parent that holds it alone.
+__device__ __forceinline__ brn_need brn_sequence(const sglkv_fork_params &p, uint32_t parent, uint64_t length, bool takes) {
     brn_need n;
     const bool live = parent != SGLKV_FORK_NONE;
     n.parent = parent;
@@ -136,9 +137,17 @@ __device__ __forceinline__ brn_need brn_sequence(const sglkv_fork_params &p, uin
         n.pages = n.full + (n.length % p.pool.page_size != 0);
         n.need = live ? end / p.pool.page_size + (end % p.pool.page_size != 0) : 0;
     }
-    n.copies = n.pages > n.full && !first;
+    n.copies = n.pages > n.full && !takes;
     n.fresh = static_cast<uint32_t>(n.need - n.pages) + (n.copies ? 1u : 0u);
     return n;
+}
+
+// Whether more than old row r holds entry `full` of it, a page that is not full:
+// other rows or the caller, by the references of before the call. No child may
+// write to it then.
+__device__ __forceinline__ bool brn_shared(const sglkv_fork_params &p, uint64_t r, uint64_t full) {
+    const uint32_t page = static_cast<uint32_t>(p.tables[r * p.table_pages + full]);
+    return page < p.page_count && p.references[page] > 1;
 }
 
 // Exclusive sums over a workgroup of 1,024 threads in their order, and the total.
@@ -188,12 +197,14 @@ __device__ __forceinline__ int32_t brn_entry(const sglkv_fork_params &p, const b
 }
 
 // Entry j of an old row of `length` tokens that `children` go on from: a row of its
-// own less, and one more for each child that shares the page. True: the page is
-// held by nothing any more. (No other row's change can follow the one that reaches
-// 0: a row that goes on holds its own reference until then.)
+// own less, and one more for each child that shares the page (its last one, if it
+// is not full: for the child that takes it over). True: the page is held by nothing
+// any more. (No other row's change can follow the one that reaches 0: a row that
+// goes on holds its own reference until then.)
 __device__ __forceinline__ bool brn_release(const sglkv_fork_params &p, uint64_t length, uint64_t j, uint32_t children, int32_t entry) {
     const uint64_t next = (j + 1) * p.pool.page_size;
-    const int32_t change = static_cast<int32_t>(next <= length ? children : children ? 1 : 0) - 1;
+    const uint32_t count = children & ~SGLKV_FORK_SHARED;
+    const int32_t change = static_cast<int32_t>(next <= length ? count : count && count == children ? 1 : 0) - 1;
     if (change == 0) return false;
     const uint32_t page = static_cast<uint32_t>(entry);
     if (page >= p.page_count) {
@@ -258,6 +269,10 @@ __device__ __forceinline__ void brn_small_body(const sglkv_fork_params &p) {
 #pragma unroll
     for (uint32_t u = 0; u < U; ++u) old[u] = parent_entry(T * u + tid);
     auto fresh = [&](uint32_t k) { return k < T ? top[k] : brn_fresh(p, free_count, k); };
+    for (uint32_t i = tid; i < p.old_sequences; i += T) {
+        const uint32_t length = lengths[i], full = length / p.pool.page_size;
+        if (length <= room && full * p.pool.page_size != length && brn_shared(p, i, full)) atomicOr(children + i, SGLKV_FORK_SHARED);
+    }
     for (uint32_t s = tid; s < p.sequences; s += T) {
         const uint32_t parent = parents[s];
         if (parent == SGLKV_FORK_NONE) continue;
@@ -277,7 +292,8 @@ __device__ __forceinline__ void brn_small_body(const sglkv_fork_params &p) {
     auto need = [&](uint32_t s) {
         const uint32_t parent = parents[s];
         const bool live = parent != SGLKV_FORK_NONE;
-        return brn_sequence(p, parent, live ? lengths[parent] : 0, !live || first[parent] == s);
+        return brn_sequence(p, parent, live ? lengths[parent] : 0,
+                            !live || (first[parent] == s && !(children[parent] & SGLKV_FORK_SHARED)));
     };
     // New pages, and copies, before each sequence's.
     uint64_t done = 0;
@@ -348,13 +364,15 @@ __device__ __forceinline__ void brn_small_body(const sglkv_fork_params &p) {
 
 // The same in three launches. One workgroup: who is whose first child, how many new
 // pages come before each sequence's, and whether all of that holds.
-__device__ __forceinline__ uint32_t brn_first(const sglkv_fork_params &p, uint32_t parent) {
-    return __hip_atomic_load(p.first + parent, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+__device__ __forceinline__ bool brn_takes(const sglkv_fork_params &p, uint32_t parent, uint32_t s) {
+    const uint32_t first = __hip_atomic_load(p.first + parent, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const uint32_t children = __hip_atomic_load(p.children + parent, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return first == s && !(children & SGLKV_FORK_SHARED);
 }
 __device__ __forceinline__ brn_need brn_sequence(const sglkv_fork_params &p, uint32_t s) {
     const uint32_t parent = p.parents[s];
     const bool live = parent != SGLKV_FORK_NONE;
-    return brn_sequence(p, parent, live ? p.lengths[parent] : 0, !live || brn_first(p, parent) == s);
+    return brn_sequence(p, parent, live ? p.lengths[parent] : 0, !live || brn_takes(p, parent, s));
 }
 __device__ __forceinline__ void brn_plan_body(const sglkv_fork_params &p) {
     constexpr uint32_t T = SGLKV_FORK_PLAN_THREADS;
@@ -366,8 +384,10 @@ __device__ __forceinline__ void brn_plan_body(const sglkv_fork_params &p) {
     if (free_count > p.page_count) bad |= SGLKV_FLAG_ATTN_SEQUENCE;
     for (uint32_t i = tid; i < p.old_sequences; i += T) {
         __hip_atomic_store(p.first + i, SGLKV_FORK_NONE, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __hip_atomic_store(p.children + i, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (p.lengths[i] > room) bad |= SGLKV_FLAG_ATTN_SEQUENCE;
+        const uint64_t length = p.lengths[i], full = length / p.pool.page_size;
+        if (length > room) bad |= SGLKV_FLAG_ATTN_SEQUENCE;
+        const bool shared = length <= room && full * p.pool.page_size != length && brn_shared(p, i, full);
+        __hip_atomic_store(p.children + i, shared ? SGLKV_FORK_SHARED : 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     for (uint32_t i = tid; i < (p.page_count + 31) / 32; i += T) p.freed[i] = 0;
     __threadfence();

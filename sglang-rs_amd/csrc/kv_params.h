@@ -567,6 +567,7 @@ typedef struct sglkv_beam_params {
 #define SGLKV_FORK_PLAN_THREADS 1024u
 #define SGLKV_FORK_HEAD_WORDS 32u
 #define SGLKV_FORK_NONE 0xFFFFFFFFu
+#define SGLKV_FORK_SHARED 0x80000000u  /* with a number of children: more than the parent holds its last page */
 #define SGLKV_FORK_SMALL_SEQUENCES 2048u  /* old or new */
 #define SGLKV_FORK_SMALL_ENTRIES 8192u    /* of the old or the new tables */
 #define SGLKV_FORK_SMALL_PAGES 262144u

@@ -1546,8 +1546,9 @@ class RocmKvPairCopyKernels:
         """The page tables of sequences that go on from `parents` (UINT32_MAX:
         none): full pages shared, last pages copied (in `layer_count` layers of
         which `pool` describes the first) for all children of a parent but the
-        lowest, pages for append_tokens more, and the pages that nothing holds
-        any more back on the free list. Asynchronous."""
+        lowest, or for all where more than the parent holds the page, pages for
+        append_tokens more, and the pages that nothing holds any more back on
+        the free list. Asynchronous."""
         _call(lib().sgl_rocm_kv_fork_sequences, self._h, ctypes.byref(plan._c), ctypes.byref(buffers._c),
               ctypes.byref(pool), layer_count, layer_stride_bytes, _stream(stream))
 
