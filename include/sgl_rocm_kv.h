@@ -1378,6 +1378,7 @@ typedef struct sgl_kv_fork_config {
     uint64_t page_size;
     uint64_t page_count;     /* pages of the pool */
     uint64_t append_tokens;  /* tokens that each sequence has to have pages for behind its own */
+    uint64_t keep_reserved;  /* 1: the old sequences have pages behind their own tokens', too (see sgl_kv_fork_buffers) */
 } sgl_kv_fork_config;
 
 typedef struct sgl_kv_fork_plan {
@@ -1393,17 +1394,25 @@ typedef struct sgl_kv_fork_plan {
     uint64_t workspace_required_bytes;
 } sgl_kv_fork_plan;
 
-/* Errors: ZeroDimension (all but append_tokens); DimensionTooLarge: "page_count"
- * past 2^31 - 1, "page_size" past 2^32 - 1, "append_tokens" past 2^32 - 1,
- * "sequence_count" or "parent_count" past 2^24, "table_pages" past 2^31,
- * "workgroups" past one dispatch. */
+/* Errors: ZeroDimension (all but append_tokens and keep_reserved);
+ * DimensionTooLarge: "page_count" past 2^31 - 1, "page_size" past 2^32 - 1,
+ * "append_tokens" past 2^32 - 1, "sequence_count" or "parent_count" past 2^24,
+ * "table_pages" past 2^31, or past 2^20 with keep_reserved, "workgroups" past one
+ * dispatch; InvalidArgument ("keep_reserved" past 1). */
 int32_t sgl_kv_fork_plan_new(const sgl_kv_fork_config *config, sgl_kv_fork_plan *out);
 
 /* A sequence of n tokens has ceil(n / page_size) pages, the first entries of its
- * table's row; entries behind them are -1 in the forked tables and not looked at
- * in the old ones. page_references counts the rows that hold a page (a caller
- * that holds pages itself, as a prefix cache does, adds its own). free_pages is a
- * stack of free_count pages that nothing holds. */
+ * table's row. A forked row has pages for append_tokens more behind these, and -1
+ * behind them all. In the old rows, what is behind a sequence's own pages is not
+ * looked at by default: its tokens are taken to have grown into all that an earlier
+ * call appended, and a page that they have not grown into is lost to the pool.
+ * Where they may not have (drafts that were not accepted, a sequence that waits),
+ * keep_reserved makes the entries behind, up to the first that is -1, pages of the
+ * sequence, too: the lowest of its children has them, and takes fewer new ones;
+ * without a child they are released.
+ * page_references counts the rows that hold a page (a caller that holds pages
+ * itself, as a prefix cache does, adds its own). free_pages is a stack of
+ * free_count pages that nothing holds. */
 typedef struct sgl_kv_fork_buffers {
     sgl_kv_device_buffer parents;         uint64_t parents_offset;
     sgl_kv_device_buffer lengths;         uint64_t lengths_offset;
@@ -1423,8 +1432,8 @@ typedef struct sgl_kv_fork_buffers {
  * alone holds it (page_references 1 before the call); the others, or all where
  * another sequence or the caller holds it too, get a page of their own with its
  * rows so far (every tensor of `layer_count` layers, `pool` and layer_stride as
- * for keep_drafts). Pages for append_tokens more tokens
- * follow. The k-th new page of the call (by sequence, then by place in the row) is
+ * for keep_drafts). Pages for append_tokens more tokens follow, reserved ones
+ * first. The k-th new page of the call (by sequence, then by place in the row) is
  * free_pages[free_count - 1 - k]. page_references follow the tables; pages whose
  * count falls to 0 are appended to free_pages in ascending order, behind what is
  * left of it.
@@ -1433,8 +1442,9 @@ typedef struct sgl_kv_fork_buffers {
  * (SEQUENCE), a free page that it would take is outside the pool (PAGE) or more
  * are wanted than there are (OUT_OF_PAGES: SGL_KV_DEVICE_OUT_OF_PAGES). A table
  * entry outside the pool is reported (PAGE) and passed on as -1; nothing is
- * counted for it, and nothing copied. forked_lengths and forked_tables overlap no
- * other buffer (InvalidArgument "in place"). */
+ * counted for it, and nothing copied (behind a sequence's own pages it ends the
+ * reserved ones). forked_lengths and forked_tables overlap no other buffer
+ * (InvalidArgument "in place"). */
 int32_t sgl_rocm_kv_fork_sequences(sgl_rocm_kv_ctx *ctx, const sgl_kv_fork_plan *plan,
                                    const sgl_kv_fork_buffers *buffers, const sgl_kv_pool_view *pool,
                                    uint32_t layer_count, uint64_t layer_stride, void *stream);

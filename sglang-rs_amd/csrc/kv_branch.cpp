@@ -12,6 +12,7 @@ using namespace sglkv;
 namespace {
 
 constexpr uint64_t kMaxSequences = 1ull << 24;
+constexpr uint64_t kMaxReservedRow = 1ull << 20;  // a thread may walk over a row's reserved pages
 
 int32_t zero_dimension(const char *what, const char *name) {
     return fail(SGL_KV_ZERO_DIMENSION, name, 0, 0, 0, "%s dimension %s must be non-zero", what, name);
@@ -115,7 +116,7 @@ namespace {
 
 // The workspace's parts, each a multiple of 64 bytes.
 struct ForkParts {
-    uint64_t first, children, before, copies, freed, bytes;
+    uint64_t first, children, held, before, copies, freed, bytes;
 };
 
 ForkParts fork_parts(const sgl_kv_fork_config &c) {
@@ -123,7 +124,8 @@ ForkParts fork_parts(const sgl_kv_fork_config &c) {
     ForkParts f;
     f.first = 4 * SGLKV_FORK_HEAD_WORDS;
     f.children = f.first + lines(c.parent_count);
-    f.before = f.children + lines(c.parent_count);
+    f.held = f.children + lines(c.parent_count);
+    f.before = f.held + lines(c.keep_reserved ? c.parent_count : 0);
     f.copies = f.before + lines(c.sequence_count);
     f.freed = f.copies + sizeof(sglkv_page_copy) / 4 * lines(c.sequence_count);
     f.bytes = f.freed + lines(divide_up(c.page_count, 32));
@@ -145,6 +147,10 @@ extern "C" int32_t sgl_kv_fork_plan_new(const sgl_kv_fork_config *config, sgl_kv
     int32_t rc = check_dims("fork", dims);
     if (rc) return rc;
     if (c.append_tokens > UINT32_MAX) return too_large_dim("append_tokens", c.append_tokens, UINT32_MAX);
+    if (c.keep_reserved > 1)
+        return fail(SGL_KV_INVALID_ARGUMENT, "keep_reserved", c.keep_reserved, 1, 0, "keep_reserved is 0 or 1, not %llu",
+                    (unsigned long long)c.keep_reserved);
+    if (c.keep_reserved && c.table_pages > kMaxReservedRow) return too_large_dim("table_pages", c.table_pages, kMaxReservedRow);
     // A workgroup to each sequence, old and new.
     const uint64_t limit = UINT32_MAX / SGLKV_FORK_THREADS;
     if (c.sequence_count + c.parent_count > limit) return too_large_dim("workgroups", c.sequence_count + c.parent_count, limit);
@@ -210,6 +216,7 @@ extern "C" int32_t sgl_rocm_kv_fork_sequences(sgl_rocm_kv_ctx *ctx, const sgl_kv
     p.head = reinterpret_cast<uint32_t *>(workspace);
     p.first = reinterpret_cast<uint32_t *>(workspace + parts.first);
     p.children = reinterpret_cast<uint32_t *>(workspace + parts.children);
+    p.held = reinterpret_cast<uint32_t *>(workspace + parts.held);
     p.before = reinterpret_cast<uint32_t *>(workspace + parts.before);
     p.copies = reinterpret_cast<sglkv_page_copy *>(workspace + parts.copies);
     p.freed = reinterpret_cast<uint32_t *>(workspace + parts.freed);
@@ -219,6 +226,7 @@ extern "C" int32_t sgl_rocm_kv_fork_sequences(sgl_rocm_kv_ctx *ctx, const sgl_kv
     p.old_sequences = (uint32_t)c.parent_count;
     p.page_count = (uint32_t)c.page_count;
     p.append = (uint32_t)c.append_tokens;
+    p.keep_reserved = (uint32_t)c.keep_reserved;
     p.tensors = pool->tensor_count;
     p.layers = layer_count;
     uint64_t bits = layer_count > 1 ? layer_stride : 0, most = 0;

@@ -113,15 +113,19 @@ __device__ __forceinline__ void brn_keep_body(const sglkv_keep_params &p) {
 // 1 request of 4 beams 8.0 us and 3.2 for the copies, 64 of 4 11.6 and 34.5 (166 MB
 // in and out, 4.8 TB/s, what a plain copy reaches).
 
-// What a sequence needs: its parent's tokens, pages of these, new pages.
+// What a sequence needs: its parent's tokens, pages of these, entries that it has
+// from its parent (`held`: these pages and, for the lowest child, reserved ones
+// behind them), new pages.
 struct brn_need {
-    uint64_t length, full, pages, need;
+    uint64_t length, full, pages, held, need;
     uint32_t parent, fresh;  // fresh: new pages, a copied last page first among them
     bool copies;
 };
 // `takes`: the sequence takes over its parent's last page, as the lowest child of a
-// parent that holds it alone.
-__device__ __forceinline__ brn_need brn_sequence(const sglkv_fork_params &p, uint32_t parent, uint64_t length, bool takes) {
+// parent that holds it alone. `reserved`: where its parent's reserved pages end, if it
+// has them (0: it has none).
+__device__ __forceinline__ brn_need brn_sequence(const sglkv_fork_params &p, uint32_t parent, uint64_t length, bool takes,
+                                                 uint32_t reserved) {
     brn_need n;
     const bool live = parent != SGLKV_FORK_NONE;
     n.parent = parent;
@@ -138,7 +142,8 @@ __device__ __forceinline__ brn_need brn_sequence(const sglkv_fork_params &p, uin
         n.need = live ? end / p.pool.page_size + (end % p.pool.page_size != 0) : 0;
     }
     n.copies = n.pages > n.full && !takes;
-    n.fresh = static_cast<uint32_t>(n.need - n.pages) + (n.copies ? 1u : 0u);
+    n.held = n.pages > reserved ? n.pages : reserved;
+    n.fresh = (n.need > n.held ? static_cast<uint32_t>(n.need - n.held) : 0u) + (n.copies ? 1u : 0u);
     return n;
 }
 
@@ -148,6 +153,19 @@ __device__ __forceinline__ brn_need brn_sequence(const sglkv_fork_params &p, uin
 __device__ __forceinline__ bool brn_shared(const sglkv_fork_params &p, uint64_t r, uint64_t full) {
     const uint32_t page = static_cast<uint32_t>(p.tables[r * p.table_pages + full]);
     return page < p.page_count && p.references[page] > 1;
+}
+
+// Entries of old row r that are pages: its own `pages` and, with keep_reserved, those
+// behind them. What ends these is -1, or reported. (A step for each reserved page:
+// few. The host bounds the row.)
+__device__ __forceinline__ uint32_t brn_held(const sglkv_fork_params &p, uint64_t r, uint64_t pages) {
+    const int32_t *row = p.tables + r * p.table_pages;
+    for (uint64_t j = pages; j < p.table_pages; ++j)
+        if (static_cast<uint32_t>(row[j]) >= p.page_count) {
+            if (row[j] != -1) atomicOr(p.flag, SGLKV_FLAG_PAGE);
+            return static_cast<uint32_t>(j);
+        }
+    return static_cast<uint32_t>(p.table_pages);
 }
 
 // Exclusive sums over a workgroup of 1,024 threads in their order, and the total.
@@ -184,13 +202,13 @@ __device__ __forceinline__ uint32_t brn_fresh(const sglkv_fork_params &p, uint64
 template <typename F>
 __device__ __forceinline__ int32_t brn_entry(const sglkv_fork_params &p, const brn_need &n, uint64_t j, int32_t old, F fresh,
                                              uint32_t before) {
-    const uint64_t begin = n.copies ? n.full : n.pages;  // new pages from here on
-    if (j >= begin && j < n.need) {
-        const uint32_t page = fresh(before + static_cast<uint32_t>(j - begin));
+    const bool behind = j >= n.held;
+    if (behind ? j < n.need : n.copies && j == n.full) {
+        const uint32_t page = fresh(before + (behind ? (n.copies ? 1u : 0u) + static_cast<uint32_t>(j - n.held) : 0u));
         p.references[page] = 1;
         return static_cast<int32_t>(page);
     }
-    if (j >= n.pages) return -1;
+    if (behind) return -1;
     if (static_cast<uint32_t>(old) < p.page_count) return old;
     atomicOr(p.flag, SGLKV_FLAG_PAGE);
     return -1;
@@ -198,13 +216,14 @@ __device__ __forceinline__ int32_t brn_entry(const sglkv_fork_params &p, const b
 
 // Entry j of an old row of `length` tokens that `children` go on from: a row of its
 // own less, and one more for each child that shares the page (its last one, if it
-// is not full: for the child that takes it over). True: the page is held by nothing
-// any more. (No other row's change can follow the one that reaches 0: a row that
-// goes on holds its own reference until then.)
+// is not full: for the child that takes it over; a reserved one: for the lowest).
+// True: the page is held by nothing any more. (No other row's change can follow the
+// one that reaches 0: a row that goes on holds its own reference until then.)
 __device__ __forceinline__ bool brn_release(const sglkv_fork_params &p, uint64_t length, uint64_t j, uint32_t children, int32_t entry) {
     const uint64_t next = (j + 1) * p.pool.page_size;
     const uint32_t count = children & ~SGLKV_FORK_SHARED;
-    const int32_t change = static_cast<int32_t>(next <= length ? count : count && count == children ? 1 : 0) - 1;
+    const bool goes_on = count && (count == children || j * p.pool.page_size >= length);
+    const int32_t change = static_cast<int32_t>(next <= length ? count : goes_on ? 1 : 0) - 1;
     if (change == 0) return false;
     const uint32_t page = static_cast<uint32_t>(entry);
     if (page >= p.page_count) {
@@ -239,7 +258,7 @@ __device__ __forceinline__ void brn_small_body(const sglkv_fork_params &p) {
     constexpr uint32_t T = SGLKV_FORK_PLAN_THREADS, N = SGLKV_FORK_SMALL_SEQUENCES, U = 4;
     extern __shared__ uint32_t brn_bits[];  // a bit for each page that is freed
     __shared__ uint64_t sums[T / 64];
-    __shared__ uint32_t parents[N], lengths[N], first[N], children[N], before[N], place[N], top[T];  // top: the first new pages
+    __shared__ uint32_t parents[N], lengths[N], first[N], children[N], held[N], before[N], place[N], top[T];  // top: the first new pages
     const uint32_t tid = threadIdx.x, words = (p.page_count + 31) / 32;
     const uint32_t width = static_cast<uint32_t>(p.table_pages), room = width * p.pool.page_size;  // (host: below 2^31)
     const uint32_t old_entries = p.old_sequences * width, new_entries = p.sequences * width;
@@ -270,8 +289,11 @@ __device__ __forceinline__ void brn_small_body(const sglkv_fork_params &p) {
     for (uint32_t u = 0; u < U; ++u) old[u] = parent_entry(T * u + tid);
     auto fresh = [&](uint32_t k) { return k < T ? top[k] : brn_fresh(p, free_count, k); };
     for (uint32_t i = tid; i < p.old_sequences; i += T) {
-        const uint32_t length = lengths[i], full = length / p.pool.page_size;
-        if (length <= room && full * p.pool.page_size != length && brn_shared(p, i, full)) atomicOr(children + i, SGLKV_FORK_SHARED);
+        const uint32_t length = lengths[i], full = length / p.pool.page_size, pages = full + (full * p.pool.page_size != length);
+        held[i] = pages;
+        if (length > room) continue;
+        if (pages != full && brn_shared(p, i, full)) atomicOr(children + i, SGLKV_FORK_SHARED);
+        if (p.keep_reserved) held[i] = brn_held(p, i, pages);
     }
     for (uint32_t s = tid; s < p.sequences; s += T) {
         const uint32_t parent = parents[s];
@@ -292,8 +314,9 @@ __device__ __forceinline__ void brn_small_body(const sglkv_fork_params &p) {
     auto need = [&](uint32_t s) {
         const uint32_t parent = parents[s];
         const bool live = parent != SGLKV_FORK_NONE;
-        return brn_sequence(p, parent, live ? lengths[parent] : 0,
-                            !live || (first[parent] == s && !(children[parent] & SGLKV_FORK_SHARED)));
+        const bool lowest = live && first[parent] == s;
+        return brn_sequence(p, parent, live ? lengths[parent] : 0, !live || (lowest && !(children[parent] & SGLKV_FORK_SHARED)),
+                            lowest ? held[parent] : 0);
     };
     // New pages, and copies, before each sequence's.
     uint64_t done = 0;
@@ -346,7 +369,7 @@ __device__ __forceinline__ void brn_small_body(const sglkv_fork_params &p) {
 #pragma unroll
         for (uint32_t u = 0; u < U; ++u) {
             const uint32_t i = i0 + T * u + tid, r = i / width, j = i - r * width;
-            if (i >= old_entries || j * p.pool.page_size >= lengths[r]) continue;
+            if (i >= old_entries || j >= held[r]) continue;
             const int32_t entry = i0 == 0 ? early[u] : p.tables[i];
             if (brn_release(p, lengths[r], j, children[r], entry)) atomicOr(brn_bits + entry / 32, 1u << (entry % 32));
         }
@@ -364,15 +387,15 @@ __device__ __forceinline__ void brn_small_body(const sglkv_fork_params &p) {
 
 // The same in three launches. One workgroup: who is whose first child, how many new
 // pages come before each sequence's, and whether all of that holds.
-__device__ __forceinline__ bool brn_takes(const sglkv_fork_params &p, uint32_t parent, uint32_t s) {
-    const uint32_t first = __hip_atomic_load(p.first + parent, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    const uint32_t children = __hip_atomic_load(p.children + parent, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    return first == s && !(children & SGLKV_FORK_SHARED);
+__device__ __forceinline__ uint32_t brn_load(const uint32_t *at) {
+    return __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 __device__ __forceinline__ brn_need brn_sequence(const sglkv_fork_params &p, uint32_t s) {
     const uint32_t parent = p.parents[s];
-    const bool live = parent != SGLKV_FORK_NONE;
-    return brn_sequence(p, parent, live ? p.lengths[parent] : 0, !live || brn_takes(p, parent, s));
+    if (parent == SGLKV_FORK_NONE) return brn_sequence(p, parent, 0, true, 0);
+    const bool lowest = brn_load(p.first + parent) == s;
+    const bool takes = lowest && !(brn_load(p.children + parent) & SGLKV_FORK_SHARED);
+    return brn_sequence(p, parent, p.lengths[parent], takes, p.keep_reserved && lowest ? brn_load(p.held + parent) : 0);
 }
 __device__ __forceinline__ void brn_plan_body(const sglkv_fork_params &p) {
     constexpr uint32_t T = SGLKV_FORK_PLAN_THREADS;
@@ -388,6 +411,9 @@ __device__ __forceinline__ void brn_plan_body(const sglkv_fork_params &p) {
         if (length > room) bad |= SGLKV_FLAG_ATTN_SEQUENCE;
         const bool shared = length <= room && full * p.pool.page_size != length && brn_shared(p, i, full);
         __hip_atomic_store(p.children + i, shared ? SGLKV_FORK_SHARED : 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (p.keep_reserved && length <= room)
+            __hip_atomic_store(p.held + i, brn_held(p, i, full + (full * p.pool.page_size != length)), __ATOMIC_RELAXED,
+                               __HIP_MEMORY_SCOPE_AGENT);
     }
     for (uint32_t i = tid; i < (p.page_count + 31) / 32; i += T) p.freed[i] = 0;
     __threadfence();
@@ -456,15 +482,15 @@ __device__ __forceinline__ void brn_tables_body(const sglkv_fork_params &p) {
         const uint64_t free_count = *p.free_count;
         if (tid == 0) p.forked_lengths[s] = n.length;
         for (uint64_t j = tid; j < p.table_pages; j += SGLKV_FORK_THREADS) {
-            const int32_t old = j < n.pages ? p.tables[n.parent * p.table_pages + j] : -1;
+            const int32_t old = j < n.held ? p.tables[n.parent * p.table_pages + j] : -1;
             p.forked_tables[s * p.table_pages + j] =
                 brn_entry(p, n, j, old, [&](uint32_t k) { return brn_fresh(p, free_count, k); }, p.before[s]);
         }
         return;
     }
     const uint32_t r = blockIdx.x - p.sequences, children = p.children[r];
-    const uint64_t length = p.lengths[r];
-    for (uint64_t j = tid; j * p.pool.page_size < length; j += SGLKV_FORK_THREADS) {
+    const uint64_t length = p.lengths[r], reserved = p.keep_reserved ? p.held[r] : 0;
+    for (uint64_t j = tid; j * p.pool.page_size < length || j < reserved; j += SGLKV_FORK_THREADS) {
         const int32_t entry = p.tables[r * p.table_pages + j];
         if (brn_release(p, length, j, children, entry)) atomicOr(p.freed + entry / 32, 1u << (entry % 32));
     }

@@ -559,9 +559,9 @@ typedef struct sglkv_beam_params {
 } sglkv_beam_params;
 
 /* Forks. The workspace: word 0 says whether the plan holds (1: carried out), word 1 the
- * pages taken, word 2 the copies; then each parent's lowest child and number of
- * children, each sequence's first new page's number, the copies, and a bit for
- * each page that is freed. Few sequences and pages (SGLKV_FORK_SMALL_*) are kept
+ * pages taken, word 2 the copies; then each parent's lowest child, number of
+ * children and pages, each sequence's first new page's number, the copies, and a
+ * bit for each page that is freed. Few sequences and pages (SGLKV_FORK_SMALL_*) are kept
  * in one workgroup's LDS instead. */
 #define SGLKV_FORK_THREADS 256u
 #define SGLKV_FORK_PLAN_THREADS 1024u
@@ -588,6 +588,7 @@ typedef struct sglkv_fork_params {
     uint32_t *head;           /* SGLKV_FORK_HEAD_WORDS */
     uint32_t *first;          /* [parent] */
     uint32_t *children;       /* [parent] */
+    uint32_t *held;           /* [parent]: with keep_reserved, the pages of a row */
     uint32_t *before;         /* [sequence] */
     sglkv_page_copy *copies;  /* [sequence] */
     uint32_t *freed;          /* [ceil(page_count / 32)] */
@@ -597,6 +598,7 @@ typedef struct sglkv_fork_params {
     uint32_t sequences, old_sequences;
     uint32_t page_count;
     uint32_t append;
+    uint32_t keep_reserved;   /* entries behind a row's pages, up to the first -1, are pages of it, too */
     uint32_t tensors;
     uint32_t heads;           /* chunks of a token's row: the heads of head-major pages, else 1 */
     uint32_t layers;

@@ -416,7 +416,7 @@ class _BeamBuffers(ctypes.Structure):
 
 class _ForkConfig(ctypes.Structure):
     _fields_ = [(n, _u64) for n in ("sequence_count", "parent_count", "table_pages", "page_size", "page_count",
-                                    "append_tokens")]
+                                    "append_tokens", "keep_reserved")]
 
 
 _FORK_BUFFERS = ("parents", "lengths", "page_tables", "forked_lengths", "forked_tables", "page_references", "free_pages",
@@ -2359,16 +2359,17 @@ class BeamBuffers:
 
 class ForkPlan:
     """What fork_sequences needs to know: sequences before and after, entries
-    of a page table's row, the pool's pages and their size, and the tokens that
-    each sequence has to have pages for behind its own."""
+    of a page table's row, the pool's pages and their size, the tokens that each
+    sequence has to have pages for behind its own, and whether the old sequences
+    have such pages, too, which they keep (keep_reserved)."""
 
     def __init__(self, c: _ForkPlan):
         self._c = c
 
     @classmethod
     def new(cls, *, sequence_count: int, parent_count: int, table_pages: int, page_size: int, page_count: int,
-            append_tokens: int = 0) -> "ForkPlan":
-        config = _ForkConfig(sequence_count, parent_count, table_pages, page_size, page_count, append_tokens)
+            append_tokens: int = 0, keep_reserved: bool = False) -> "ForkPlan":
+        config = _ForkConfig(sequence_count, parent_count, table_pages, page_size, page_count, append_tokens, keep_reserved)
         out = _ForkPlan()
         _call(lib().sgl_kv_fork_plan_new, ctypes.byref(config), ctypes.byref(out))
         return cls(out)
