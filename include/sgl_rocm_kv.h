@@ -1312,8 +1312,9 @@ typedef struct sgl_kv_draft_buffers {
 /* For every request and i in turn, the row of position length + i <- the row of
  * position length + kept[i], of every tensor and of `layer_count` layers: `pool`
  * describes the first, and each further one's tensors lie layer_stride bytes
- * behind the one before (as sgl_rocm_kv_transfer_layers). Elements of any type;
- * all other rows stay as they are. A request whose list does not ascend or
+ * behind the one before (as sgl_rocm_kv_transfer_layers); no two regions of a page
+ * overlap (InvalidArgument "layer_stride"). Elements of any type; all other rows
+ * stay as they are. A request whose list does not ascend or
  * reaches past its slots (SEQUENCE), or which has a row that moves from or to a
  * slot outside the pool (SLOT), is reported and left as it is. The positions that
  * a call moves have slots of their own: no two of them, of one request or two,

@@ -39,6 +39,20 @@ int32_t resolve_buffers(const sgl_rocm_kv_ctx *ctx, const CallBuffer (&all)[N]) 
     return SGL_KV_OK;
 }
 
+// Whether two of the regions of `layer_count` layers, each `stride` bytes behind the
+// one before, overlap inside a page: tensor t's has bytes[t] from offset[t] on.
+inline bool layers_overlap(uint32_t tensors, const uint64_t (&offset)[2], const uint64_t (&bytes)[2], uint64_t layer_count,
+                           uint64_t stride) {
+    for (uint32_t t = 0; t < tensors; ++t)
+        if (layer_count > 1 && stride < bytes[t]) return true;
+    if (tensors < 2) return false;
+    // The later tensor of a layer lies `apart` behind the earlier: behind, or inside, that of layer apart / stride after
+    // it, and before that of the layer after.
+    const uint32_t a = offset[0] <= offset[1] ? 0 : 1, b = 1 - a;
+    const uint64_t apart = offset[b] - offset[a], at = layer_count > 1 ? apart / stride : 0, rest = apart - at * stride;
+    return (at < layer_count && rest < bytes[a]) || (layer_count > 1 && at < layer_count - 1 && stride - rest < bytes[b]);
+}
+
 // The kernel side of `layer_count` layers of a pool, of which `pool` describes
 // the first; `chunks` are a row's parts that lie apart: the heads of head-major
 // pages, else one.
@@ -59,6 +73,11 @@ inline int32_t pool_layers(const sgl_rocm_kv_ctx *ctx, const sgl_kv_pool_view *p
             return fail(SGL_KV_SHAPE_OVERFLOW, nullptr, 0, 0, 0, "KV copy layers overflowed");
     }
     if (rc || (rc = check_pool_view(&last))) return rc;
+    // (A page's part of a layer lies inside the page, so that these multiply.)
+    const uint64_t bytes[2] = {pool->page_size * view_row_bytes(*pool, 0), pool->page_size * view_row_bytes(*pool, 1)};
+    if (layers_overlap(pool->tensor_count, pool->tensor_offset, bytes, layer_count, layer_stride))
+        return fail(SGL_KV_INVALID_ARGUMENT, "layer_stride", layer_stride, layer_count, 0,
+                    "the regions of %u layers that lie %llu bytes apart overlap", layer_count, (unsigned long long)layer_stride);
     const sgl_kv_device_buffer whole = {pool->base, pool->byte_len};
     if ((rc = check_device(ctx, "pool", whole))) return rc;
     side->layer_stride = layer_stride;

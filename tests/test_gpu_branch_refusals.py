@@ -1,0 +1,75 @@
+"""GPU tests of calls that keep_drafts, fork_sequences and select_beams refuse because one write would meet another or a
+read: nothing is launched, and what was there stays."""
+import numpy as np
+import pytest
+
+import sgl_rocm_kv as kv
+from sgl_rocm_kv import hip
+from test_gpu_branches import POOLS, Bytes, Drafts, _forks, _same
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def k():
+    if hip.device_count() == 0:
+        pytest.fail("no GPU visible: the gpu tests need an MI355X")
+    ctx = kv.RocmKvPairCopyKernels(0)
+    yield ctx
+    ctx.close()
+
+
+def _refused(variant, name, call):
+    with pytest.raises(kv.KvError) as e:
+        call()
+    assert (e.value.variant, e.value.name) == (variant, name)
+
+
+# Of POOLS[0], page 16, rows of 2,048 bytes: a region of 32,768 bytes, K and V side by side.
+@pytest.mark.parametrize("layers,stride", [(2, 0), (3, 1), (2, 16 * 2048 - 16), (2, 16 * 2048), (3, 16 * 2048 + 4096)])
+def test_layers_that_overlap(k, layers, stride):
+    """A row would be moved twice, or a layer's K while another's V is."""
+    rng = np.random.default_rng(71)
+    pool = Bytes(rng, pages=12, **POOLS[0])
+    case = Drafts(rng, pool, (5, 9), (12, 17), [(1, 4), (2,)], 2)
+    case.run(k)
+    after = pool.device.download()
+    plan = kv.DraftPlan.new(request_count=2, sequence_slot_count=len(case.slots), max_kept=2)
+    _refused("InvalidArgument", "layer_stride",
+             lambda: k.keep_drafts(plan, kv.DraftBuffers(**case.given), pool.view(), layer_count=layers, layer_stride_bytes=stride))
+    hip.synchronize()
+    assert np.array_equal(pool.device.download(), after)
+    forks = _forks(31, POOLS[0], [40, 40], [0, 0], [1, 1])
+    plan, buffers = forks.plan_and_buffers()
+    _refused("InvalidArgument", "layer_stride",
+             lambda: k.fork_sequences(plan, buffers, forks.pool.view(), layer_count=layers, layer_stride_bytes=stride))
+    hip.synchronize()
+    _same(forks.state(), forks.untouched())
+    k.check_errors()
+
+
+def test_layers_that_do_not(k):
+    """K of all layers, then V of all: the stride is one region. One layer has no stride."""
+    rng = np.random.default_rng(72)
+    page, row, layers, pages = 16, 64, 3, 8
+    region = page * row
+    raw = rng.integers(0, 256, pages * 2 * layers * region, dtype=np.uint8)
+    held = hip.DeviceBuffer.from_array(raw)
+    view = kv.pool_view(held.ptr, held.nbytes, page_size=page, page_stride_bytes=2 * layers * region, page_count=pages,
+                        tensor_offset=(0, layers * region), row_bytes=row, tensor_count=2, heads=1, head_layout=kv.NHD)
+    plan = kv.DraftPlan.new(request_count=1, sequence_slot_count=40, max_kept=2)
+    slots = rng.permutation(pages * page)[:40].astype(np.uint64)
+    given = dict(request_lengths=np.asarray([30], np.uint64), request_slot_offsets=np.asarray([0, 40], np.uint64),
+                 sequence_slots=slots, kept=np.asarray([3, 9], np.uint32))
+    buffers = kv.DraftBuffers(**{n: hip.DeviceBuffer.from_array(a) for n, a in given.items()})
+    k.keep_drafts(plan, buffers, view, layer_count=layers, layer_stride_bytes=region)
+    hip.synchronize()
+    k.check_errors()
+    want = raw.reshape(pages, 2 * layers, page, row).copy()
+    for i, draft in enumerate((3, 9)):
+        to, source = int(slots[30 + i]), int(slots[30 + draft])
+        want[to // page, :, to % page] = raw.reshape(want.shape)[source // page, :, source % page]
+    assert np.array_equal(held.download(), want.reshape(-1))
+    k.keep_drafts(plan, buffers, view, layer_count=1, layer_stride_bytes=0)
+    hip.synchronize()
+    k.check_errors()
