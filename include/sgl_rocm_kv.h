@@ -1444,8 +1444,8 @@ typedef struct sgl_kv_fork_buffers {
  * are wanted than there are (OUT_OF_PAGES: SGL_KV_DEVICE_OUT_OF_PAGES). A table
  * entry outside the pool is reported (PAGE) and passed on as -1; nothing is
  * counted for it, and nothing copied (behind a sequence's own pages it ends the
- * reserved ones). forked_lengths and forked_tables overlap no other buffer
- * (InvalidArgument "in place"). */
+ * reserved ones). forked_lengths and forked_tables overlap no other buffer and no
+ * page of the pool (InvalidArgument "in place"). */
 int32_t sgl_rocm_kv_fork_sequences(sgl_rocm_kv_ctx *ctx, const sgl_kv_fork_plan *plan,
                                    const sgl_kv_fork_buffers *buffers, const sgl_kv_pool_view *pool,
                                    uint32_t layer_count, uint64_t layer_stride, void *stream);

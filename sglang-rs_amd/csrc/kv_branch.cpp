@@ -204,6 +204,17 @@ extern "C" int32_t sgl_rocm_kv_fork_sequences(sgl_rocm_kv_ctx *ctx, const sgl_kv
         return fail(SGL_KV_INVALID_ARGUMENT, "pool", pool->page_size, pool->page_count, 0,
                     "the pool has %llu pages of %llu tokens, the plan %llu of %llu", (unsigned long long)pool->page_count,
                     (unsigned long long)pool->page_size, (unsigned long long)c.page_count, (unsigned long long)c.page_size);
+    // The pool's pages, from the first byte of the first to the last of the last, are copied from and to all the while.
+    uint64_t begin = UINT64_MAX, end = 0;
+    for (uint32_t t = 0; t < pool->tensor_count; ++t) {
+        const uint64_t last = p.pool.plane[t] + (c.page_count - 1) * pool->page_stride_bytes +
+                              (uint64_t)(layer_count - 1) * layer_stride + c.page_size * view_row_bytes(*pool, t);
+        begin = p.pool.plane[t] < begin ? p.pool.plane[t] : begin;
+        end = last > end ? last : end;
+    }
+    for (const CallBuffer *x : {&all[3], &all[4]})
+        if (overlap(*x->address, x->need, begin, end - begin))
+            return fail(SGL_KV_INVALID_ARGUMENT, "in place", 0, 0, 0, "%s overlaps the pool", x->name);
     const ForkParts parts = fork_parts(c);
     p.parents = reinterpret_cast<const uint32_t *>(parents);
     p.lengths = reinterpret_cast<const uint64_t *>(lengths);

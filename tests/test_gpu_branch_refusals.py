@@ -73,3 +73,32 @@ def test_layers_that_do_not(k):
     k.keep_drafts(plan, buffers, view, layer_count=1, layer_stride_bytes=0)
     hip.synchronize()
     k.check_errors()
+
+
+def test_forked_tables_in_the_pool(k):
+    """Inside the pool's pages they are refused; behind the last, in the same allocation, they are not."""
+    case = _forks(33, POOLS[1], [40, 40], [0, 0], [1, 1])
+    plan, _ = case.plan_and_buffers()
+    pool, used = case.pool, case.pool.device.nbytes
+    arena = hip.DeviceBuffer(used + 4096)
+    arena.upload(np.concatenate([pool.raw, np.full(4096, 0xA5, np.uint8)]))
+    view = pool.view()
+    view.base, view.byte_len = arena.ptr, arena.nbytes
+
+    def call(**change):
+        k.fork_sequences(plan, kv.ForkBuffers(**{**case.device, **change}), view, **pool.call())
+
+    for name in ("forked_lengths", "forked_tables"):
+        n = case.device[name].nbytes
+        for at in (0, used // 2 // 16 * 16, used - 16):
+            _refused("InvalidArgument", "in place", lambda: call(**{name: kv.device_buffer(arena.ptr + at, n)}))
+    hip.synchronize()
+    assert np.array_equal(arena.download()[:used], pool.raw)
+    tables = kv.device_buffer(arena.ptr + used, case.device["forked_tables"].nbytes)
+    call(forked_tables=tables)
+    hip.synchronize()
+    k.check_errors()
+    want = case.want()
+    got = arena.download()
+    assert np.array_equal(got[:used], want[5])
+    assert np.array_equal(got[used:used + tables.byte_len].view(np.int32).reshape(want[1].shape), want[1])
