@@ -1368,7 +1368,9 @@ typedef struct sgl_kv_beam_buffers {
  * ones go to the lower beam, then the lower token. A continuation whose score is
  * not finite is none: a beam whose score is -inf or NaN takes no part, nor does a
  * token of logit -inf, nor a beam with a logit of NaN or +inf. Fewer than max_kept
- * are followed by -inf, UINT32_MAX and UINT32_MAX. */
+ * are followed by -inf, UINT32_MAX and UINT32_MAX. best_scores may be scores itself
+ * where max_kept is beam_count; else neither the outputs nor the workspace overlap
+ * another buffer (InvalidArgument "in place"). */
 int32_t sgl_rocm_kv_select_beams(sgl_rocm_kv_ctx *ctx, const sgl_kv_beam_plan *plan,
                                  const sgl_kv_beam_buffers *buffers, void *stream);
 

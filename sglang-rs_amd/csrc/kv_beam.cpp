@@ -97,6 +97,11 @@ extern "C" int32_t sgl_rocm_kv_select_beams(sgl_rocm_kv_ctx *ctx, const sgl_kv_b
         {"best_tokens", &b->best_tokens, b->best_tokens_offset, f.best_tokens_required_bytes, &best_tokens, 4, true},
         {"workspace", &b->workspace, b->workspace_offset, f.workspace_required_bytes, &workspace, 16, true}};
     if ((rc = resolve_buffers(ctx, all))) return rc;
+    // In place: a workgroup has read its request's scores before it writes the best ones to the same places.
+    const bool in_place = best_scores == scores && c.max_kept == c.beam_count;
+    if ((rc = refuse_overlaps(all, 2, in_place ? 1 : 2)) || (rc = refuse_overlaps(all, 3)) || (rc = refuse_overlaps(all, 4)) ||
+        (rc = refuse_overlaps(all, 5)))
+        return rc;
     sglkv_beam_params p;
     memset(&p, 0, sizeof p);
     p.logits = reinterpret_cast<const void *>(logits);

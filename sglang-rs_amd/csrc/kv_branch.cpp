@@ -132,8 +132,6 @@ ForkParts fork_parts(const sgl_kv_fork_config &c) {
     return f;
 }
 
-bool overlap(uint64_t a, uint64_t an, uint64_t b, uint64_t bn) { return an && bn && a < b + bn && b < a + an; }
-
 }  // namespace
 
 extern "C" int32_t sgl_kv_fork_plan_new(const sgl_kv_fork_config *config, sgl_kv_fork_plan *out) {
@@ -193,10 +191,7 @@ extern "C" int32_t sgl_rocm_kv_fork_sequences(sgl_rocm_kv_ctx *ctx, const sgl_kv
         {"workspace", &b->workspace, b->workspace_offset, f.workspace_required_bytes, &workspace, 16, true}};
     if ((rc = resolve_buffers(ctx, all))) return rc;
     // The new lengths and tables are written while the old ones are read.
-    for (const CallBuffer *x : {&all[3], &all[4]})
-        for (const CallBuffer &y : all)
-            if (x != &y && overlap(*x->address, x->need, *y.address, y.need))
-                return fail(SGL_KV_INVALID_ARGUMENT, "in place", 0, 0, 0, "%s overlaps %s", x->name, y.name);
+    if ((rc = refuse_overlaps(all, 3)) || (rc = refuse_overlaps(all, 4))) return rc;
     sglkv_fork_params p;
     memset(&p, 0, sizeof p);
     if ((rc = pool_layers(ctx, pool, layer_count, layer_stride, &p.pool, &p.heads))) return rc;

@@ -39,6 +39,18 @@ int32_t resolve_buffers(const sgl_rocm_kv_ctx *ctx, const CallBuffer (&all)[N]) 
     return SGL_KV_OK;
 }
 
+inline bool overlap(uint64_t a, uint64_t an, uint64_t b, uint64_t bn) { return an && bn && a < b + bn && b < a + an; }
+
+// Buffer `written` of a call against all others but `same`, if any: it is written while these are read, or written, too.
+template <size_t N>
+int32_t refuse_overlaps(const CallBuffer (&all)[N], size_t written, size_t same = N) {
+    const CallBuffer &x = all[written];
+    for (const CallBuffer &y : all)
+        if (&x != &y && &y != all + same && x.used && y.used && overlap(*x.address, x.need, *y.address, y.need))
+            return fail(SGL_KV_INVALID_ARGUMENT, "in place", 0, 0, 0, "%s overlaps %s", x.name, y.name);
+    return SGL_KV_OK;
+}
+
 // Whether two of the regions of `layer_count` layers, each `stride` bytes behind the
 // one before, overlap inside a page: tensor t's has bytes[t] from offset[t] on.
 inline bool layers_overlap(uint32_t tensors, const uint64_t (&offset)[2], const uint64_t (&bytes)[2], uint64_t layer_count,

@@ -5,6 +5,7 @@ import pytest
 
 import sgl_rocm_kv as kv
 from sgl_rocm_kv import hip
+from test_gpu_beams import _random
 from test_gpu_branches import POOLS, Bytes, Drafts, _forks, _same
 
 pytestmark = pytest.mark.gpu
@@ -102,3 +103,38 @@ def test_forked_tables_in_the_pool(k):
     got = arena.download()
     assert np.array_equal(got[:used], want[5])
     assert np.array_equal(got[used:used + tables.byte_len].view(np.int32).reshape(want[1].shape), want[1])
+
+
+@pytest.mark.parametrize("beams,vocab", [(4, 9000), (1, 50), (20, 700)])  # (20 x 20 continuations: the merge by lists)
+def test_scores_in_place(k, beams, vocab):
+    """As many continuations as beams: the best scores may take the scores' places."""
+    case = _random(73, 40, beams, vocab, beams, "bf16")
+    want = [a.copy() for a in case.run(k)]
+    scores = np.concatenate([case.scores.reshape(-1).view(np.uint8), np.full(64, 0xA5, np.uint8)])
+    case.given["scores"] = case.given["best_scores"] = hip.DeviceBuffer.from_array(scores)
+    got = case.run(k)
+    k.check_errors()
+    assert all(np.array_equal(a, b) for a, b in zip(got, want))
+
+
+def test_outputs_over_inputs(k):
+    case = _random(74, 3, 4, 600, 8, "f32")
+    shared = hip.DeviceBuffer(1 << 20)
+
+    def call(**change):
+        k.select_beams(case.plan, kv.BeamBuffers(**{**case.given, **change}))
+
+    for written in ("best_scores", "best_parents", "best_tokens", "workspace"):
+        for other in case.given:
+            if other.endswith("_offset") or other == written:
+                continue
+            nbytes = getattr(case.plan, other + "_required_bytes")
+            _refused("InvalidArgument", "in place", lambda: call(**{
+                other: shared, written: kv.device_buffer(shared.ptr + nbytes // 16 * 16 - (16 if nbytes % 16 == 0 else 0), 1 << 19)}))
+    _refused("InvalidArgument", "in place", lambda: call(scores=shared, best_scores=shared))  # (8 kept of 4 beams)
+    square = _random(75, 3, 4, 600, 4, "f32")
+    _refused("InvalidArgument", "in place", lambda: k.select_beams(square.plan, kv.BeamBuffers(**{
+        **square.given, "logits": shared, "scores": shared, "best_scores": shared})))
+    call()
+    hip.synchronize()
+    k.check_errors()
