@@ -1276,7 +1276,8 @@ typedef struct sgl_kv_tree_attention_buffers {
  * that a query does not attend never reach its output, whatever they hold. An
  * infinite value that it does attend gives an infinity or NaN (a weight's lo part
  * may be 0 or negative). Softmax statistics and sums are held in 32 bits; the
- * output is rounded to bf16. */
+ * output is rounded to bf16. The output and the workspace overlap no other buffer
+ * (InvalidArgument "in place"). */
 int32_t sgl_rocm_kv_tree_attention(sgl_rocm_kv_ctx *ctx, const sgl_kv_tree_attention_plan *plan,
                                    const sgl_kv_tree_attention_buffers *buffers, void *stream);
 

@@ -188,6 +188,8 @@ extern "C" int32_t sgl_rocm_kv_tree_attention(sgl_rocm_kv_ctx *ctx, const sgl_kv
         {"workspace", &b->workspace, b->workspace_offset, fresh.workspace_required_bytes, &workspace, 16,
          fresh.workspace_required_bytes > 0}};
     if ((rc = resolve_buffers(ctx, all))) return rc;
+    // (A query's row is read by a workgroup of its own for every 128 value dims, in the generic body.)
+    if ((rc = refuse_overlaps(all, 6)) || (rc = refuse_overlaps(all, 8))) return rc;
     if ((lay.key_in_page_offset | lay.value_in_page_offset | lay.page_stride_bytes) & 1)
         return fail(SGL_KV_INVALID_ARGUMENT, "alignment", 0, 0, 0, "pool rows must be aligned to their element size");
     sglkv_tree_params p;

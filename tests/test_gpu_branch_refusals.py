@@ -1,4 +1,4 @@
-"""GPU tests of calls that keep_drafts, fork_sequences and select_beams refuse because one write would meet another or a
+"""GPU tests of calls that the operators for several continuations refuse because one write would meet another or a
 read: nothing is launched, and what was there stays."""
 import numpy as np
 import pytest
@@ -7,6 +7,8 @@ import sgl_rocm_kv as kv
 from sgl_rocm_kv import hip
 from test_gpu_beams import _random
 from test_gpu_branches import POOLS, Bytes, Drafts, _forks, _same
+from test_gpu_selection import _filled
+from test_gpu_tree import _make
 
 pytestmark = pytest.mark.gpu
 
@@ -136,5 +138,28 @@ def test_outputs_over_inputs(k):
     _refused("InvalidArgument", "in place", lambda: k.select_beams(square.plan, kv.BeamBuffers(**{
         **square.given, "logits": shared, "scores": shared, "best_scores": shared})))
     call()
+    hip.synchronize()
+    k.check_errors()
+
+
+@pytest.mark.parametrize("dk", [128, 40])
+def test_attention_over_its_inputs(k, dk):
+    _, trees = _make(9, dk=dk, contexts=(50, 900), drafts=(10, 7))
+    plan = trees.plan()
+    sizes = {n: getattr(plan.attention, n + "_required_bytes") for n in (
+        "query_request_indices", "query_sequence_lengths", "request_slot_offsets", "sequence_slots", "pool", "output")}
+    sizes.update(queries=plan.attention.query_required_bytes, masks=plan.masks_required_bytes,
+                 workspace=plan.workspace_required_bytes)
+    given = dict(**trees.upload(), pool=trees.pool.buffer, output=_filled(sizes["output"]), workspace=_filled(sizes["workspace"]))
+    assert set(sizes) == set(given) and all(sizes.values())
+    shared = hip.DeviceBuffer(max(sizes.values()) + (1 << 22))
+    for written in ("output", "workspace"):
+        for other in given:
+            if other == written:
+                continue
+            at = (sizes[other] - 1) // 16 * 16
+            _refused("InvalidArgument", "in place", lambda: k.tree_attention(plan, kv.TreeAttentionBuffers(**{
+                **given, other: shared, written: kv.device_buffer(shared.ptr + at, 1 << 21)})))
+    k.tree_attention(plan, kv.TreeAttentionBuffers(**given))
     hip.synchronize()
     k.check_errors()
