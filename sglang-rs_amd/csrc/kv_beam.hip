@@ -137,7 +137,9 @@ __device__ __forceinline__ void beam_rows_body(const sglkv_beam_params &p) {
     if (tid == 0) lanes = count = 0;
     const float log2e = 1.4426950408889634f;
     // (At 0 where there is no maximum yet: its terms are 0, or NaN if it is +inf. A NaN stays in the sum.)
-    float m = odd, l = __builtin_amdgcn_exp2f((odd - (odd > -INFINITY ? odd : 0.0f)) * log2e);
+    float m = odd;
+    // (Of the rounds' sums: up to 64 of 32 logits, whose running sum in 32 bits would be off by a rounding for each logit.)
+    double total = __builtin_amdgcn_exp2f((odd - (odd > -INFINITY ? odd : 0.0f)) * log2e);
     auto work = [&](uint32_t round, sglkv_v4u (&raw)[VECTORS]) {
         if (begin + (round + 1) * ROUND > vectors) {
             const uint32_t none = sizeof(E) == 2 ? 0xFF80FF80u : 0xFF800000u;  // -inf
@@ -153,15 +155,17 @@ __device__ __forceinline__ void beam_rows_body(const sglkv_beam_params &p) {
                 higher = attn_max3(higher, beam_element(E(), raw[v], e), beam_element(E(), raw[v], e + 1));
         }
         const float top = higher > -INFINITY ? higher : 0.0f;
-        l *= __builtin_amdgcn_exp2f((m > -INFINITY ? m - top : 0.0f) * log2e);
+        const float scale = __builtin_amdgcn_exp2f((m > -INFINITY ? m - top : 0.0f) * log2e);
         m = higher;
+        float sum = 0.0f;
         // (The floats are made anew from the 16 bytes: kept, they would take as many registers again.)
 #pragma unroll
         for (uint32_t v = 0; v < VECTORS; ++v) {
             asm volatile("" : "+v"(raw[v]));
 #pragma unroll
-            for (uint32_t e = 0; e < PER; ++e) l += __builtin_amdgcn_exp2f((beam_element(E(), raw[v], e) - top) * log2e);
+            for (uint32_t e = 0; e < PER; ++e) sum += __builtin_amdgcn_exp2f((beam_element(E(), raw[v], e) - top) * log2e);
         }
+        total = __builtin_fma(total, static_cast<double>(scale), static_cast<double>(sum));
     };
     if (rounds) {
         // The next round's loads are in flight while one is worked on.
@@ -176,6 +180,7 @@ __device__ __forceinline__ void beam_rows_body(const sglkv_beam_params &p) {
         }
         work(round, raw);
     }
+    float l = static_cast<float>(total);
     const uint32_t mine = beam_order32(m);
     uint32_t bound = 0;
     if (kept <= 64) {

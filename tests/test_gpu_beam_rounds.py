@@ -127,3 +127,21 @@ def test_what_takes_no_part_in_a_later_round(k, dtype):
     scores[5] = (-np.inf, np.nan)
     got = _check(k, logits, scores, 171, 12, dtype, 4)
     assert (got[1][:, 5] == NONE).all() and (got[1][:, 0] == NONE).all()
+
+
+def test_a_long_sum_of_equal_terms(k):
+    """32 rounds in which each thread has one 1 and terms a little below it: added to one running sum in 32 bits, each
+    would be rounded up to 1 from 512 terms on, 2^-16.1 of the sum in all."""
+    vocab, rows = 32 * CHUNK, 2048
+    assert _rounds(rows, vocab) == 32
+    near = bf16(np.float32([-2.75e-5]))[0]
+    row = np.full((1, 1, vocab), near, np.uint16)
+    row[0, 0, :2048:8] = 0  # the first of each thread's first eight
+    _say("select_beams: 32 rounds of nearly equal logits")
+    got = _select(k, row, np.zeros((1, 1)), rows, 3, "bf16")
+    x = f64(np.asarray([near]))[0]
+    total = -np.log(256.0 + (vocab - 256) * np.exp(x))
+    assert (got[2] == np.asarray([0, 8, 16], np.uint32)).all()
+    error = np.abs(got[0] - total)
+    _say(f"beams: largest error {error.max():.3g}, bound {2.0 ** -17 + 2.0 ** -24 * abs(total):.3g}")
+    assert (error <= 2.0 ** -17 + 2.0 ** -24 * abs(total)).all()
