@@ -113,7 +113,6 @@ extern "C" int32_t sgl_rocm_kv_select_beams(sgl_rocm_kv_ctx *ctx, const sgl_kv_b
     p.candidates = reinterpret_cast<uint64_t *>(workspace + h.partial_bytes);
     p.lists = reinterpret_cast<uint64_t *>(workspace + h.partial_bytes + h.candidate_bytes);
     p.row_stride = h.stride;
-    p.requests = (uint32_t)c.request_count;
     p.beams = (uint32_t)c.beam_count;
     p.vocab = (uint32_t)c.vocab_size;
     p.kept = (uint32_t)c.max_kept;

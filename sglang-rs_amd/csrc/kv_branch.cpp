@@ -80,11 +80,9 @@ extern "C" int32_t sgl_rocm_kv_keep_drafts(sgl_rocm_kv_ctx *ctx, const sgl_kv_dr
     p.sequence_slots = reinterpret_cast<const uint64_t *>(slots);
     p.kept = reinterpret_cast<const uint32_t *>(kept);
     p.flag = ctx->attn_flag;
-    p.request_count = c.request_count;
     p.sequence_slot_count = c.sequence_slot_count;
     p.max_kept = (uint32_t)c.max_kept;
     p.tensors = pool->tensor_count;
-    p.layers = layer_count;
     // The widest of 16, 4 and 1 bytes that divides every address and chunk.
     uint64_t bits = layer_count > 1 ? layer_stride : 0, chunk[2] = {0, 0};
     for (uint32_t t = 0; t < p.tensors; ++t) {

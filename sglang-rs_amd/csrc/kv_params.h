@@ -517,13 +517,11 @@ typedef struct sglkv_keep_params {
     const uint64_t *sequence_slots;
     const uint32_t *kept;     /* [request][max_kept] */
     uint32_t *flag;
-    uint64_t request_count;
     uint64_t sequence_slot_count;
     sglkv_side pool;          /* layer_stride: between layers */
     uint32_t max_kept;
     uint32_t tensors;
     uint32_t heads;           /* chunks of a row: the heads of head-major pages, else 1 */
-    uint32_t layers;
     uint32_t chunk_pieces[2]; /* access-sized pieces of tensor t's chunk */
     uint32_t pieces;          /* of a row, all tensors and chunks */
     uint32_t groups;          /* workgroups of a (request, layer) */
@@ -551,7 +549,7 @@ typedef struct sglkv_beam_params {
     uint64_t *candidates;     /* [row][split][kept]: ordered logit and inverted token, descending; 0: none */
     uint64_t *lists;          /* [row][kept]: a row's, joined */
     uint64_t row_stride;
-    uint32_t requests, beams;
+    uint32_t beams;
     uint32_t vocab;
     uint32_t kept;
     uint32_t splits;

@@ -77,6 +77,7 @@ int32_t tile_shape(const sgl_kv_attention_plan_config &c, const sgl_kv_tree_atte
     const uint64_t tiles = divide_up(mean, h.tile_queries), most_tiles = c.query_count / h.tile_queries + count;
     h.unit = (uint32_t)(groups * SGLKV_TREE_BLOCK(d, h.row_waves));
     h.least = 2;
+    h.tile_slots = 0;
     h.balanced = count <= SGLKV_TREE_BALANCED && c.query_count <= SGLKV_TREE_LISTED;
     TreeWay &w = h.tile;
     h.pairs = resident / c.kv_head_count > 1 ? resident / c.kv_head_count : 1;

@@ -586,9 +586,10 @@ __device__ __forceinline__ uint32_t tree_upto(uint32_t x) {
 // before its first and the mean share and half a split in place of a split where they
 // follow each other (64 requests of 300 to 4,096 tokens with up to 12 drafts: 161 us
 // with w = 1, 148 with 2; 30 of 300 to 2,000 with up to 120: 124 and 147). The host
-// does not know the lengths. They are numbered without a gap, since a workgroup that finds nothing to do holds its place until the ones before it on its
-// CU are done: 32 requests of 300 to 8,192 tokens took 265 us with every other
-// workgroup empty, 163 us without; with half as many pairs 209, with twice 167.
+// does not know the lengths. They are numbered without a gap, since a workgroup that
+// finds nothing to do holds its place until the ones before it on its CU are done:
+// 32 requests of 300 to 8,192 tokens took 265 us with every other workgroup empty,
+// 163 us without; with half as many pairs 209, with twice 167.
 // A request of one split has its outputs from there; the others' are merged.
 // Each workgroup finds c and its own place, a lane to a request. Past
 // SGLKV_TREE_BALANCED requests or SGLKV_TREE_LISTED queries c is the host's, and
