@@ -1366,7 +1366,8 @@ typedef struct sgl_kv_beam_buffers {
  * that goes on (a parent, as fork_sequences takes it) and the token. Continuations
  * of one beam are ordered by their logits, those of two by this score in 64 bits
  * (of a sum of exponentials held in 32 bits for 32 logits of a thread and across a
- * workgroup's threads, in 64 bits otherwise: off by less than 2^-16); equal
+ * workgroup's threads, in 64 bits otherwise: off by less than 2^-15 of itself);
+ * equal
  * ones go to the lower beam, then the lower token. A continuation whose score is
  * not finite is none: a beam whose score is -inf or NaN takes no part, nor does a
  * token of logit -inf, nor a beam with a logit of NaN or +inf. Fewer than max_kept

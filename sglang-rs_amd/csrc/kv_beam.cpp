@@ -40,7 +40,8 @@ int32_t beam_shape(const sgl_kv_beam_config &c, BeamShape *out) {
     h.rows = c.request_count * c.beam_count;  // (below 2^42)
     h.stride = c.row_stride ? c.row_stride : c.vocab_size;
     // Several rounds a workgroup where there are more than fill the card: what a workgroup does once is shared by them (64
-    // requests of 4 beams, 128,256 tokens: 27.3 us at a round each, 21.3 at 2,048 workgroups and 22.0 at 1,024).
+    // requests of 4 beams, 128,256 tokens: 28.8 us at a round each, 24.6 at 2,048 workgroups, 24.0 at 1,024 and 25.0 at 512;
+    // 256 requests of 50,257 tokens: 35.9, 34.7, 35.0 and 34.9).
     const uint64_t chunks = divide_up(c.vocab_size, SGLKV_BEAM_CHUNK);
     h.rounds = h.rows * chunks / 2048;
     h.rounds = h.rounds < 1 ? 1 : h.rounds > chunks ? chunks : h.rounds;

@@ -7,9 +7,10 @@
 // each, are joined by one workgroup a request in 64 bits. What can be among the K is
 // found by a bound (the K-th largest of the threads' maxima) and ranked, where K
 // rounds of maxima took 99 us for 64 requests of 4 beams, 128,256 tokens and K = 8:
-// now 16.6 (66 MB, 4.0 TB/s; loads and what is counted of each logit share the time)
-// and 5.6 for the join; 1 request of 4 beams of 32,000: 5.7 and 5.1, each a chain of
-// joins over lanes, LDS and barriers.
+// now 16.8 (66 MB, 3.9 TB/s; loads and what is counted of each logit share the time)
+// and 5.7 for the join; 1 request of 4 beams of 32,000: 5.7 and 5.2, each a chain of
+// joins over lanes, LDS and barriers. Many kept have no such bound: with K = 64 the
+// first batch takes 1,150 us, with 128 2,150.
 
 namespace {
 

@@ -246,7 +246,8 @@ extern "C" int32_t sgl_rocm_kv_fork_sequences(sgl_rocm_kv_ctx *ctx, const sgl_kv
     const uint64_t groups = (uint64_t)p.sequences * p.layers * p.tensors, limit = UINT32_MAX / SGLKV_FORK_THREADS;
     if (groups > limit) return too_large_dim("workgroups", groups, limit);
     // One workgroup takes as long as the other way's three launches where it goes through some 8,000 entries (256
-    // sequences with their copies, 4,352 entries: 49 us, with three launches 56; 16,384: 62 and 50; 65,536: 146 and 57).
+    // sequences with their copies, 4,352 entries: 48 us, with three launches 54; 8,192: 53 and 54; 16,384: 67 and 54;
+    // 65,536: 133 and 54).
     const bool small = c.sequence_count <= SGLKV_FORK_SMALL_SEQUENCES && c.parent_count <= SGLKV_FORK_SMALL_SEQUENCES &&
                        c.table_pages <= SGLKV_FORK_SMALL_ENTRIES && c.page_count <= SGLKV_FORK_SMALL_PAGES &&
                        c.sequence_count * c.table_pages <= SGLKV_FORK_SMALL_ENTRIES &&

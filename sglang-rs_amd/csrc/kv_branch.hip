@@ -20,9 +20,10 @@ __device__ __forceinline__ uint64_t brn_row(const sglkv_side &s, uint32_t tensor
 // owns the same piece of every row and takes the rows in the list's order, a few
 // at a time (all read before any is written), so nothing is written before it is
 // read and no thread waits for another. Bytes bound it where there are many (64
-// requests of 8 rows, 32 layers, 57 MB in and out: 15.6 us, 3.7 TB/s, three quarters
-// of the waves' time waiting for rows of 2 KiB), else three loads one after another:
-// list, slots, rows (3 requests, 24 layers: 4.9 us, 7.0 with its launch).
+// requests of 8 rows, 32 layers, 57 MB in and out: 15.7 us, 3.7 TB/s, three quarters
+// of the waves' time waiting for rows of 2 KiB; packed rows of 649 bytes, which go
+// byte by byte: 28.9 for 21 MB), else three loads one after another: list, slots,
+// rows (3 requests, 24 layers: 4.9 us, 7.1 with its launch).
 
 template <typename V>
 __device__ __forceinline__ void brn_keep_body(const sglkv_keep_params &p) {
@@ -110,8 +111,9 @@ __device__ __forceinline__ void brn_keep_body(const sglkv_keep_params &p) {
 // pages come before each sequence's (a sum), the tables, the references, the freed
 // pages in order. Few sequences take one workgroup, which has all of it in LDS;
 // many take three launches. The copies are a launch of their own: bytes. Measured:
-// 1 request of 4 beams 8.0 us and 3.2 for the copies, 64 of 4 11.6 and 34.5 (166 MB
-// in and out, 4.8 TB/s, what a plain copy reaches).
+// 1 request of 4 beams 9.2 us and 3.1 for the copies, 64 of 4 11.8 and 34.4 (166 MB
+// in and out, 4.8 TB/s, 0.82 of this library's stream copy: waves wait to issue for
+// 0.71 of their time, each vector with a 64-bit address of its own).
 
 // What a sequence needs: its parent's tokens, pages of these, entries that it has
 // from its parent (`held`: these pages and, for the lowest child, reserved ones

@@ -40,7 +40,7 @@ __device__ __forceinline__ bool tree_metadata(const sglkv_tree_params &p, uint64
 }
 
 // Any head dims, page size and alignment (32 requests of 300 to 8,192 tokens whose
-// rows the tiles could read: 2,254 us, in tiles 146): a wave to 16 query heads and
+// rows the tiles could read: 2,254 us, in tiles 147): a wave to 16 query heads and
 // SGLKV_ATTN_DV value dims of one query, 32 tokens a step, as the generic body of
 // paged attention (attn_body), whose layouts of the matrix products it shares.
 template <bool VEC>
@@ -150,9 +150,9 @@ __device__ __forceinline__ void tree_body(const sglkv_tree_params &p) {
 // registers; rows go straight to LDS a block ahead. The weights enter as hi + lo
 // bf16 pairs, which costs half as many products again and 6 vector instructions a
 // pair of weights. Measured with 32 query heads on 8 KV heads of 128 dims:
-// - 32 requests of 300 to 8,192 tokens with up to 24 drafts: 146 us, 4.0 TB/s of
+// - 32 requests of 300 to 8,192 tokens with up to 24 drafts: 147 us, 4.0 TB/s of
 //   rows, bound by waits for them and by how evenly splits fall on workgroups;
-// - 6 of 9,000 to 32,768 with up to 120: 380 us, 560 TFLOP/s not counting the lo
+// - 6 of 9,000 to 32,768 with up to 120: 377 to 390 us, 550 TFLOP/s not counting the lo
 //   halves, bound by vector and matrix instructions, which follow each other in a
 //   wave (the matrix pipes are busy 41 % of the time);
 // - one of 2,048 with 16: 16.7 us, of which the merge's launch takes 4 and what a
