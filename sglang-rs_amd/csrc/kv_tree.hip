@@ -152,9 +152,9 @@ __device__ __forceinline__ void tree_body(const sglkv_tree_params &p) {
 // pair of weights. Measured with 32 query heads on 8 KV heads of 128 dims:
 // - 32 requests of 300 to 8,192 tokens with up to 24 drafts: 147 us, 4.0 TB/s of
 //   rows, bound by waits for them and by how evenly splits fall on workgroups;
-// - 6 of 9,000 to 32,768 with up to 120: 377 to 390 us, 550 TFLOP/s not counting the lo
-//   halves, bound by vector and matrix instructions, which follow each other in a
-//   wave (the matrix pipes are busy 41 % of the time);
+// - 6 of 9,000 to 32,768 with up to 120: 377 to 401 us, 534 to 568 TFLOP/s not
+//   counting the lo halves, bound by vector and matrix instructions, which follow
+//   each other in a wave (the matrix pipes are busy 41 % of the time);
 // - one of 2,048 with 16: 16.7 us, of which the merge's launch takes 4 and what a
 //   workgroup does before its first block and behind its last 7.
 
